@@ -94,7 +94,7 @@ def _lengths(case: dict, top: int, least: int = 0) -> list[int]:
     b = case["batch"]
     if not case["ragged"] or b == 1:
         return [top] * b
-    return [least + round((top - least) * ((7 * i + 3) % b) / (b - 1)) for i in range(b)]
+    return [least + round((top - least) * ((37 * i + 3) % b) / (b - 1)) for i in range(b)]
 
 
 def work(case: dict) -> dict:
