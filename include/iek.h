@@ -39,8 +39,17 @@ typedef enum iek_status {
 } iek_status;
 
 /* Tensor dtypes: the reference's TensorType (src/core/tensor.rs:13-23); IEK_F16 is the device KV
- * cache's element type (iek_dev_attention_decode). */
-typedef enum iek_dtype { IEK_F32 = 0, IEK_Q4K = 1, IEK_Q6K = 2, IEK_Q8_0 = 3, IEK_F16 = 4 } iek_dtype;
+ * cache's element type (iek_dev_attention_decode); IEK_I8 and IEK_E4M3 (one sign, four exponent and
+ * three mantissa bits, no infinities, largest value 448) are those of the 8-bit cache (iek_kv8). */
+typedef enum iek_dtype {
+  IEK_F32 = 0,
+  IEK_Q4K = 1,
+  IEK_Q6K = 2,
+  IEK_Q8_0 = 3,
+  IEK_F16 = 4,
+  IEK_I8 = 5,
+  IEK_E4M3 = 6
+} iek_dtype;
 
 typedef struct iek_model iek_model;
 typedef struct iek_session iek_session;
@@ -287,6 +296,76 @@ iek_status iek_dev_attention_decode_noalloc(const float* q, const void* k_cache,
                                             size_t n_heads, size_t n_kv_heads, size_t head_dim, size_t max_seq_len,
                                             size_t total_pos, size_t sliding_window, float scale, float* out,
                                             void* stream);
+
+/* ---- 8-bit KV cache, device pointers (asynchronous on `stream`) ------------------------------
+ * No counterpart in the reference, whose KVCache (src/layers/attention.rs:16-24) is f32. A batch of
+ * sequences' keys and values as 8-bit codes with one scale per block of IEK_KV8_BLOCK slots of a
+ * head; a row's values are code * scale. Scales are powers of two: for the block's largest |value| a,
+ * the smallest 2^e >= 2^-100 with a <= M * 2^e, M = 127 (IEK_I8) or 448 (IEK_E4M3), so that a value
+ * is off by at most half a step of its scale (and by less than a whole one after later appends or
+ * evictions have brought its block to a larger scale).
+ *
+ * The buffers are the caller's, in HBM, the codes 16-byte aligned; nothing needs to be cleared. All
+ * entries are asynchronous, allocate nothing, wait for nothing and may be captured into a graph; what
+ * changes from step to step (lengths, positions) is read from device memory. `stream` NULL is the
+ * current device's null stream. Calls that share a workspace must be ordered by the caller; calls
+ * with workspaces and outputs of their own may overlap. IEK_ERR_OP for null or misaligned pointers
+ * and unsupported shapes: head_dim 64, 128, 256 or 512, n_heads / n_kv_heads <= 8, row strides in
+ * floats, multiples of 4 and not below a row; f32 rows and workspaces 16-byte aligned. A batch, n or
+ * n_q of 0 does nothing. */
+#define IEK_KV8_BLOCK 32
+typedef struct iek_kv8 {
+  int32_t dtype; /* IEK_I8 or IEK_E4M3 */
+  uint64_t batch, n_kv_heads, capacity, head_dim;
+  void *k, *v;              /* codes [batch][n_kv_heads][capacity][head_dim] */
+  float *k_scale, *v_scale; /* [batch][n_kv_heads][ceil(capacity / IEK_KV8_BLOCK)] */
+} iek_kv8;
+/* Rows i < count[b] (count NULL: n; at most n) of sequence b, k and v [batch][n] rows of
+ * n_kv_heads * head_dim floats, row_stride floats from one row to the next (a slice of fused rows),
+ * go to slots start[b] + i (start NULL: 0). Rows past the capacity are dropped, and all rows of a
+ * sequence whose start is negative or past it. The slots behind the new rows no longer hold anything,
+ * those before start in the same block keep their values (their codes are rounded again when the
+ * block's scale grows). An infinity or NaN makes its block's scale NaN, and so whatever attends to
+ * the block. len_out (or NULL): the lengths after the append; may be start itself, and must not
+ * overlap it otherwise. weights (or NULL): [batch][n_kv_heads][capacity] running attention weights,
+ * set to 0 for the new rows. IEK_ERR_KV_CACHE when n > capacity. */
+iek_status iek_dev_kv8_append(const iek_kv8* cache, const float* k, const float* v, size_t n, size_t row_stride,
+                              const int32_t* start, const int32_t* count, int32_t* len_out, float* weights,
+                              void* stream);
+/* The values of slots start[b] + i, i < count[b], as f32 rows (arguments as above; what
+ * iek_session_kv is for a session): e.g. a cached prefix for iek_dev_attention_prefill. Rows from
+ * count[b] on, and those of slots that do not exist, are left as they were. */
+iek_status iek_dev_kv8_load(const iek_kv8* cache, size_t n, size_t row_stride, const int32_t* start,
+                            const int32_t* count, float* k, float* v, void* stream);
+/* Attention of the last n_q (at most 64) tokens of every sequence, their rows already appended.
+ * q: [batch][n_q] rows of n_heads * head_dim floats, q_stride floats apart; len[b] entries in
+ * sequence b, at most max_len (<= capacity; IEK_ERR_KV_CACHE otherwise), which sizes the launch.
+ * Query token t sees the entries [lo, hi), hi = len[b] - (n_q - 1 - t), lo = hi - sliding_window if
+ * that is positive and there is a window (0: none; in a cache that has been evicted from it counts
+ * entries, not positions). out[b][t][h] = softmax(scale * q . K[j]) . V[j] over them, h's KV head
+ * being h / (n_heads / n_kv_heads); zeros where there are none. Entries from len[b] on may hold
+ * anything. weights_out (or NULL): [batch][n_kv_heads][capacity], for j < len[b]
+ * weights_out[j] = weights_in[j] + the attention weight of entry j summed over the KV head's query
+ * heads and the n_q tokens; weights_in may be weights_out itself, or NULL for zeros. workspace:
+ * iek_kv8_attention_workspace bytes for the same arguments, its contents of no matter. */
+iek_status iek_kv8_attention_workspace(const iek_kv8* cache, size_t n_heads, size_t n_q, size_t max_len,
+                                       int with_weights, size_t* bytes);
+iek_status iek_dev_kv8_attention(const iek_kv8* cache, const float* q, size_t n_heads, size_t n_q, size_t q_stride,
+                                 const int32_t* len, size_t max_len, size_t sliding_window, float scale, float* out,
+                                 const float* weights_in, float* weights_out, void* workspace,
+                                 size_t workspace_bytes, void* stream);
+/* Cuts every sequence of more than `keep` entries down to `keep`, for each KV head by itself: the
+ * first `first`, the last `last` and, of those between, the ones of the largest weight (equal
+ * weights: the earlier ones; NaN counts as the largest), in their order. len[b] <= max_len as above.
+ * src and dst are two caches of the same dtype, batch and heads (dst.capacity >= keep, IEK_ERR_KV_CACHE
+ * otherwise) that share nothing (nor do weights and weights_out), or twice the same one, with
+ * weights_out = weights: an eviction in place. Sequences of up to `keep` entries are copied, or left
+ * as they are. A block's new scale is the largest of its rows' old ones. len_out[b] = min(len[b],
+ * keep); it may be len itself, and must not overlap it otherwise. index_out (or NULL): [batch][n_kv_heads][keep], the old slots of the entries kept. */
+iek_status iek_kv8_evict_workspace(const iek_kv8* src, size_t max_len, size_t keep, size_t* bytes);
+iek_status iek_dev_kv8_evict(const iek_kv8* src, const iek_kv8* dst, const float* weights, float* weights_out,
+                             const int32_t* len, int32_t* len_out, size_t max_len, size_t keep, size_t first,
+                             size_t last, int32_t* index_out, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- device memory helpers for FFI callers without a HIP binding ---------------------------- */
 iek_status iek_device_alloc(size_t bytes, void** out);

@@ -47,6 +47,8 @@ SOURCES = [
     "kernels/chain.hip",
     "kernels/noalloc.hip",
     "kernels/sampling.hip",
+    "kernels/kv8.hip",
+    "kernels/kv8_attention.hip",
     "model.cpp",
     "session.cpp",
     "api.cpp",

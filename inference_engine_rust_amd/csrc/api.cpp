@@ -6,6 +6,7 @@
 #include <vector>
 
 #include "../../include/iek.h"
+#include "kernels/kv8.h"
 #include "session.h"
 
 namespace iek {
@@ -627,6 +628,219 @@ iek_status iek_dev_attention_decode_noalloc(const float* q, const void* k_cache,
     float* part = reinterpret_cast<float*>(base + NOALLOC_COUNTER_BYTES);
     attention_launch(q, k_cache, v_cache, kv_dtype == IEK_F32, n_heads, n_kv_heads, head_dim, max_seq_len, total_pos,
                      sliding_window, scale, out, part, cnt, true, as_stream(stream));
+  })
+}
+
+// ---- 8-bit KV cache ----
+static_assert(KV8_BLOCK == IEK_KV8_BLOCK && (int)DT_I8 == IEK_I8 && (int)DT_E4M3 == IEK_E4M3, "iek.h");
+
+// Work on a stream is launched with the stream's device current (the null stream: the current device).
+class OnDeviceOf {
+ public:
+  explicit OnDeviceOf(hipStream_t st) {
+    if (!st) return;
+    int dev = 0;
+    IEK_HIP(hipGetDevice(&was_));
+    IEK_HIP(hipStreamGetDevice(st, &dev));
+    if (dev == was_) was_ = -1;
+    else IEK_HIP(hipSetDevice(dev));
+  }
+  ~OnDeviceOf() {
+    if (was_ >= 0) (void)hipSetDevice(was_);
+  }
+
+ private:
+  int was_ = -1;
+};
+
+static void aligned(const void* p, size_t to, const char* what) {
+  if (!p) fail(ST_OP, std::string("kv8: null ") + what);
+  if (reinterpret_cast<uintptr_t>(p) % to)
+    fail(ST_OP, std::string("kv8: ") + what + " is not " + std::to_string(to) + "-byte aligned");
+}
+static void optional_aligned(const void* p, size_t to, const char* what) {
+  if (p) aligned(p, to, what);
+}
+// a and b are one array, or do not overlap; returns whether they are one
+static bool same_or_apart(const void* a, size_t a_bytes, const void* b, size_t b_bytes, const char* what) {
+  if (!a || !b) return false;
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  if (x != y && x < y + b_bytes && y < x + a_bytes) fail(ST_OP, std::string("kv8: ") + what + " overlap");
+  return x == y;
+}
+
+// Checks of the cache's shape (and, with `buffers`, of its pointers).
+static Kv8 kv8_view(const iek_kv8* c, bool buffers = true) {
+  if (!c) fail(ST_OP, "kv8: null cache");
+  if (c->dtype != IEK_I8 && c->dtype != IEK_E4M3) fail(ST_OP, "kv8: the cache dtype must be I8 or E4M3");
+  if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256 && c->head_dim != 512)
+    fail(ST_OP, "kv8: head_dim must be 64, 128, 256 or 512");
+  if (c->n_kv_heads == 0 || c->capacity == 0) fail(ST_OP, "kv8: no KV heads or no capacity");
+  if (c->n_kv_heads > 4096 || c->batch > 65536 || c->capacity > (1u << 30) || c->batch * c->n_kv_heads > (1u << 20))
+    fail(ST_OP, "kv8: dims too large");
+  if (buffers) {
+    aligned(c->k, 16, "k");
+    aligned(c->v, 16, "v");
+    aligned(c->k_scale, 4, "k_scale");
+    aligned(c->v_scale, 4, "v_scale");
+  }
+  Kv8 o;
+  o.k = static_cast<uint8_t*>(c->k);
+  o.v = static_cast<uint8_t*>(c->v);
+  o.ks = c->k_scale;
+  o.vs = c->v_scale;
+  o.batch = (int)c->batch;
+  o.n_kv = (int)c->n_kv_heads;
+  o.cap = (int)c->capacity;
+  o.hd = (int)c->head_dim;
+  o.nblk = (o.cap + KV8_BLOCK - 1) / KV8_BLOCK;
+  o.e4m3 = c->dtype == IEK_E4M3;
+  return o;
+}
+static void kv8_rows(size_t stride, size_t width, const char* what) {
+  if (stride % 4 || stride < width)
+    fail(ST_OP, std::string("kv8: ") + what + " must be a multiple of 4 and at least a row");
+  if (stride > (1u << 30)) fail(ST_OP, "kv8: dims too large");
+}
+static void kv8_length(const Kv8& c, size_t max_len) {
+  if (max_len > (size_t)c.cap)
+    fail(ST_KVCACHE, "KV cache position " + std::to_string(max_len - 1) + " is out of bounds (max_seq_len is " +
+                         std::to_string(c.cap) + ")");
+}
+static void kv8_heads(const Kv8& c, size_t n_heads, size_t n_q) {
+  if (n_heads == 0 || n_heads % c.n_kv != 0 || n_heads / c.n_kv > 8)
+    fail(ST_OP, "kv8: GQA group must divide the heads and be at most 8");
+  if (n_q > 64) fail(ST_OP, "kv8: at most 64 query tokens");
+}
+
+iek_status iek_dev_kv8_append(const iek_kv8* cache, const float* k, const float* v, size_t n, size_t row_stride,
+                              const int32_t* start, const int32_t* count, int32_t* len_out, float* weights,
+                              void* stream) {
+  IEK_API_TRY({
+    const Kv8 c = kv8_view(cache);
+    kv8_rows(row_stride, (size_t)c.n_kv * c.hd, "row_stride");
+    if (n > (size_t)c.cap) fail(ST_KVCACHE, "KVCache is Full: max len is " + std::to_string(c.cap) + ".");
+    if (n == 0 || c.batch == 0) return IEK_OK;
+    aligned(k, 16, "k rows");
+    aligned(v, 16, "v rows");
+    optional_aligned(start, 4, "start");
+    optional_aligned(count, 4, "count");
+    optional_aligned(len_out, 4, "len_out");
+    optional_aligned(weights, 4, "weights");
+    const size_t lens = (size_t)c.batch * 4;
+    same_or_apart(start, lens, len_out, lens, "start and len_out");
+    if (same_or_apart(count, lens, len_out, lens, "count and len_out"))
+      fail(ST_OP, "kv8: count and len_out overlap");
+    OnDeviceOf on(as_stream(stream));
+    launch_kv8_append(c, k, v, (int)n, row_stride, start, count, len_out, weights, as_stream(stream));
+    after_launch();
+  })
+}
+
+iek_status iek_dev_kv8_load(const iek_kv8* cache, size_t n, size_t row_stride, const int32_t* start,
+                            const int32_t* count, float* k, float* v, void* stream) {
+  IEK_API_TRY({
+    const Kv8 c = kv8_view(cache);
+    kv8_rows(row_stride, (size_t)c.n_kv * c.hd, "row_stride");
+    kv8_length(c, n);
+    if (n == 0 || c.batch == 0) return IEK_OK;
+    aligned(k, 16, "k rows");
+    aligned(v, 16, "v rows");
+    optional_aligned(start, 4, "start");
+    optional_aligned(count, 4, "count");
+    OnDeviceOf on(as_stream(stream));
+    launch_kv8_load(c, (int)n, row_stride, start, count, k, v, as_stream(stream));
+    after_launch();
+  })
+}
+
+iek_status iek_kv8_attention_workspace(const iek_kv8* cache, size_t n_heads, size_t n_q, size_t max_len,
+                                       int with_weights, size_t* bytes) {
+  IEK_API_TRY({
+    const Kv8 c = kv8_view(cache, false);
+    kv8_heads(c, n_heads, n_q);
+    kv8_length(c, max_len);
+    if (!bytes) fail(ST_OP, "null argument");
+    *bytes = kv8_attention_workspace(c, (int)n_heads, (int)n_q, (int)max_len, with_weights != 0);
+  })
+}
+
+iek_status iek_dev_kv8_attention(const iek_kv8* cache, const float* q, size_t n_heads, size_t n_q, size_t q_stride,
+                                 const int32_t* len, size_t max_len, size_t sliding_window, float scale, float* out,
+                                 const float* weights_in, float* weights_out, void* workspace,
+                                 size_t workspace_bytes, void* stream) {
+  IEK_API_TRY({
+    const Kv8 c = kv8_view(cache);
+    kv8_heads(c, n_heads, n_q);
+    kv8_rows(q_stride, n_heads * c.hd, "q_stride");
+    kv8_length(c, max_len);
+    if (n_q == 0 || c.batch == 0) return IEK_OK;
+    aligned(q, 16, "q");
+    aligned(len, 4, "len");
+    aligned(out, 16, "out");
+    optional_aligned(weights_in, 4, "weights_in");
+    optional_aligned(weights_out, 4, "weights_out");
+    if (weights_in && !weights_out) fail(ST_OP, "kv8: weights_in without weights_out");
+    const size_t w_bytes = (size_t)c.batch * c.n_kv * c.cap * 4;
+    same_or_apart(weights_in, w_bytes, weights_out, w_bytes, "weights_in and weights_out");
+    if (workspace_bytes < kv8_attention_workspace(c, (int)n_heads, (int)n_q, (int)max_len, weights_out != nullptr))
+      fail(ST_OP, "kv8: the workspace is too small");
+    if (workspace_bytes) aligned(workspace, 16, "workspace");
+    OnDeviceOf on(as_stream(stream));
+    const Kv8Attn a{q, q_stride, (int)n_heads, (int)n_q, len, (int)max_len,
+                    sliding_window >= max_len ? 0 : (int)sliding_window, scale, out, weights_in, weights_out};
+    launch_kv8_attention(c, a, workspace, as_stream(stream));
+    after_launch();
+  })
+}
+
+iek_status iek_kv8_evict_workspace(const iek_kv8* src, size_t max_len, size_t keep, size_t* bytes) {
+  IEK_API_TRY({
+    const Kv8 c = kv8_view(src, false);
+    kv8_length(c, max_len);
+    if (keep > (1u << 30)) fail(ST_OP, "kv8: dims too large");
+    if (!bytes) fail(ST_OP, "null argument");
+    *bytes = kv8_evict_workspace(c, (int)max_len, (int)keep);
+  })
+}
+
+iek_status iek_dev_kv8_evict(const iek_kv8* src, const iek_kv8* dst, const float* weights, float* weights_out,
+                             const int32_t* len, int32_t* len_out, size_t max_len, size_t keep, size_t first,
+                             size_t last, int32_t* index_out, void* workspace, size_t workspace_bytes, void* stream) {
+  IEK_API_TRY({
+    const Kv8 s = kv8_view(src);
+    const Kv8 d = kv8_view(dst);
+    if (s.e4m3 != d.e4m3 || s.batch != d.batch || s.n_kv != d.n_kv || s.hd != d.hd)
+      fail(ST_OP, "kv8: the caches differ in dtype, batch or heads");
+    kv8_length(s, max_len);
+    if (keep > (size_t)d.cap) fail(ST_KVCACHE, "KVCache is Full: max len is " + std::to_string(d.cap) + ".");
+    if (first > keep || last > keep - first) fail(ST_OP, "kv8: first + last exceed keep");
+    if (s.batch == 0) return IEK_OK;
+    aligned(weights, 4, "weights");
+    aligned(weights_out, 4, "weights_out");
+    aligned(len, 4, "len");
+    aligned(len_out, 4, "len_out");
+    optional_aligned(index_out, 4, "index_out");
+    // one cache throughout, or two that share nothing
+    const size_t heads = (size_t)s.batch * s.n_kv;
+    const size_t sw = heads * s.cap;
+    const size_t dw = heads * d.cap;
+    const size_t sb = heads * s.nblk * 4;
+    const size_t db = heads * d.nblk * 4;
+    const int same = same_or_apart(s.k, sw * s.hd, d.k, dw * s.hd, "the caches' k") +
+                     same_or_apart(s.v, sw * s.hd, d.v, dw * s.hd, "the caches' v") +
+                     same_or_apart(s.ks, sb, d.ks, db, "the caches' k_scale") +
+                     same_or_apart(s.vs, sb, d.vs, db, "the caches' v_scale") +
+                     same_or_apart(weights, sw * 4, weights_out, dw * 4, "weights and weights_out");
+    if (same != 0 && (same != 5 || s.cap != d.cap)) fail(ST_OP, "kv8: the caches share some of their buffers");
+    same_or_apart(len, (size_t)s.batch * 4, len_out, (size_t)s.batch * 4, "len and len_out");
+    if (workspace_bytes < kv8_evict_workspace(s, (int)max_len, (int)keep))
+      fail(ST_OP, "kv8: the workspace is too small");
+    if (workspace_bytes) aligned(workspace, 16, "workspace");
+    OnDeviceOf on(as_stream(stream));
+    const Kv8Evict a{weights, weights_out, len, len_out, (int)max_len, (int)keep, (int)first, (int)last, index_out};
+    launch_kv8_evict(s, d, a, workspace, as_stream(stream));
+    after_launch();
   })
 }
 

@@ -25,7 +25,7 @@ LIB_PATH = os.path.join(_HERE, "libiek.so")
 KINDS = {1: "Io", 2: "Utf8", 3: "Gguf", 4: "Tensor", 5: "MatMul", 6: "Model", 7: "Tokenizer", 8: "KvCache",
          9: "Sampling", 10: "Op", 11: "Device"}
 
-F32, Q4K, Q6K, Q8_0, F16 = 0, 1, 2, 3, 4
+F32, Q4K, Q6K, Q8_0, F16, I8, E4M3 = 0, 1, 2, 3, 4, 5, 6
 GGML_TO_DTYPE = {0: F32, 12: Q4K, 14: Q6K, 8: Q8_0}
 BLOCK = {Q4K: (256, 144), Q6K: (256, 210), Q8_0: (32, 34)}
 
@@ -45,6 +45,16 @@ class Weight(ctypes.Structure):
                 ("on_device", ctypes.c_int32)]
 
 
+class KV8Cache(ctypes.Structure):
+    """iek_kv8: an 8-bit KV cache (dtype I8 or E4M3) over the caller's device buffers (addresses): codes
+    k, v [batch][n_kv_heads][capacity][head_dim] and f32 scales [batch][n_kv_heads][ceil(capacity / 32)].
+    The buffers must outlive it."""
+    _fields_ = [("dtype", ctypes.c_int32), ("batch", ctypes.c_uint64), ("n_kv_heads", ctypes.c_uint64),
+                ("capacity", ctypes.c_uint64), ("head_dim", ctypes.c_uint64), ("k", ctypes.c_void_p),
+                ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p)]
+    BLOCK = 32
+
+
 class TokenizerPrompt(ctypes.Structure):
     """TokenizerPromptConfig (src/model_config.rs:8-60)."""
     _fields_ = [("add_bos_token", ctypes.c_int32), ("add_eos_token", ctypes.c_int32),
@@ -62,6 +72,7 @@ class ModelConfig(ctypes.Structure):
 
 _P = ctypes.c_void_p
 _SZ = ctypes.c_size_t
+_PKV8 = ctypes.POINTER(KV8Cache)
 EXPORTS = {
     "iek_last_error": ([], ctypes.c_char_p),
     "iek_model_load": ([ctypes.c_char_p, ctypes.c_int, ctypes.POINTER(_P)], ctypes.c_int),
@@ -129,6 +140,13 @@ EXPORTS = {
     "iek_dev_attention_decode_noalloc": ([_P, _P, _P, ctypes.c_int, _SZ, _SZ, _SZ, _SZ, _SZ, _SZ, ctypes.c_float, _P,
                                           _P], ctypes.c_int),
     "iek_dev_attention_prefill": ([_P, _P, _P, _SZ, _SZ, _SZ, _SZ, _SZ, ctypes.c_float, _P, _P], ctypes.c_int),
+    "iek_dev_kv8_append": ([_PKV8, _P, _P, _SZ, _SZ, _P, _P, _P, _P, _P], ctypes.c_int),
+    "iek_dev_kv8_load": ([_PKV8, _SZ, _SZ, _P, _P, _P, _P, _P], ctypes.c_int),
+    "iek_kv8_attention_workspace": ([_PKV8, _SZ, _SZ, _SZ, ctypes.c_int, ctypes.POINTER(_SZ)], ctypes.c_int),
+    "iek_dev_kv8_attention": ([_PKV8, _P, _SZ, _SZ, _SZ, _P, _SZ, _SZ, ctypes.c_float, _P, _P, _P, _P, _SZ, _P],
+                              ctypes.c_int),
+    "iek_kv8_evict_workspace": ([_PKV8, _SZ, _SZ, ctypes.POINTER(_SZ)], ctypes.c_int),
+    "iek_dev_kv8_evict": ([_PKV8, _PKV8, _P, _P, _P, _P, _SZ, _SZ, _SZ, _SZ, _P, _P, _SZ, _P], ctypes.c_int),
     "iek_device_alloc": ([_SZ, ctypes.POINTER(_P)], ctypes.c_int),
     "iek_device_free": ([_P], ctypes.c_int),
     "iek_memcpy_h2d": ([_P, _P, _SZ], ctypes.c_int),
@@ -525,6 +543,53 @@ def attention_prefill(q_ptr: int, k_ptr: int, v_ptr: int, seq: int, n_heads: int
     """Prefill attention over the layer's own q / k / v rows (device pointers, f32)."""
     _check(lib().iek_dev_attention_prefill(q_ptr, k_ptr, v_ptr, seq, n_heads, n_kv_heads, head_dim, sliding_window,
                                            scale, out_ptr, stream or None))
+
+
+# ---- 8-bit KV cache (include/iek.h): device pointers, asynchronous; a pointer of 0 is NULL ----
+
+def kv8_append(cache: KV8Cache, k_ptr: int, v_ptr: int, n: int, row_stride: int, start_ptr: int = 0, count_ptr: int = 0,
+               len_out_ptr: int = 0, weights_ptr: int = 0, stream: int = 0) -> None:
+    """f32 rows [batch][n] (row_stride floats apart) into slots start[b] + i, i < count[b]."""
+    _check(lib().iek_dev_kv8_append(cache, k_ptr, v_ptr, n, row_stride, start_ptr or None, count_ptr or None,
+                                    len_out_ptr or None, weights_ptr or None, stream or None))
+
+
+def kv8_load(cache: KV8Cache, n: int, row_stride: int, start_ptr: int, count_ptr: int, k_ptr: int, v_ptr: int,
+             stream: int = 0) -> None:
+    """The values of slots start[b] + i, i < count[b], as f32 rows [batch][n] (row_stride floats apart)."""
+    _check(lib().iek_dev_kv8_load(cache, n, row_stride, start_ptr or None, count_ptr or None, k_ptr, v_ptr,
+                                  stream or None))
+
+
+def kv8_attention_workspace(cache: KV8Cache, n_heads: int, n_q: int, max_len: int, with_weights: bool) -> int:
+    """Bytes of the workspace of kv8_attention (with_weights: with a weights_out)."""
+    v = ctypes.c_size_t()
+    _check(lib().iek_kv8_attention_workspace(cache, n_heads, n_q, max_len, int(with_weights), ctypes.byref(v)))
+    return v.value
+
+
+def kv8_attention(cache: KV8Cache, q_ptr: int, n_heads: int, n_q: int, q_stride: int, len_ptr: int, max_len: int,
+                  sliding_window: int, scale: float, out_ptr: int, weights_in_ptr: int, weights_out_ptr: int,
+                  workspace_ptr: int, workspace_bytes: int, stream: int = 0) -> None:
+    """Attention of the last n_q tokens of every sequence; weights_out = weights_in + each entry's weight."""
+    _check(lib().iek_dev_kv8_attention(cache, q_ptr, n_heads, n_q, q_stride, len_ptr, max_len, sliding_window, scale,
+                                       out_ptr, weights_in_ptr or None, weights_out_ptr or None, workspace_ptr or None,
+                                       workspace_bytes, stream or None))
+
+
+def kv8_evict_workspace(src: KV8Cache, max_len: int, keep: int) -> int:
+    """Bytes of the workspace of kv8_evict."""
+    v = ctypes.c_size_t()
+    _check(lib().iek_kv8_evict_workspace(src, max_len, keep, ctypes.byref(v)))
+    return v.value
+
+
+def kv8_evict(src: KV8Cache, dst: KV8Cache, weights_ptr: int, weights_out_ptr: int, len_ptr: int, len_out_ptr: int,
+              max_len: int, keep: int, first: int, last: int, index_out_ptr: int, workspace_ptr: int,
+              workspace_bytes: int, stream: int = 0) -> None:
+    """Sequences of more than `keep` entries cut down to the first, the last and the ones of the largest weight."""
+    _check(lib().iek_dev_kv8_evict(src, dst, weights_ptr, weights_out_ptr, len_ptr, len_out_ptr, max_len, keep, first,
+                                   last, index_out_ptr or None, workspace_ptr or None, workspace_bytes, stream or None))
 
 
 def synchronize() -> None:
