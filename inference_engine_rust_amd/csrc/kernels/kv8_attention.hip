@@ -1,10 +1,19 @@
 // Attention of one or several new tokens per sequence over the 8-bit KV cache (kv8.h).
 //
 // Column c = t * G + g of a KV head is query token t, query head g of its group of G. It sees the
-// entries [lo, hi): hi = len - (n_q - 1 - t), lo = hi - window with a window, else 0. A chunk's
-// partial of a column is (m, l, o): m the largest score in base 2, l = sum 2^(s - m),
-// o = sum 2^(s - m) v; the second launch joins the chunks and, with weights, adds each entry's
-// share 2^(s - m) / l, summed over the KV head's columns, from the stored scores.
+// entries [lo, hi): hi = len - (n_q - 1 - t), lo = hi - window with a window, else 0. With scores s in
+// base 2, out = (sum 2^(s - m) v) / (sum 2^(s - m)).
+//
+// The work is reading the codes once. A wave takes 32 slots (one block, one scale) at a time, both
+// products on the matrix cores in fp16, which holds every code exactly, with 16 columns a product: eight
+// query columns, each as two halves of an fp16 (hi, lo) pair that carries 22 bits (the sums are f32).
+//   S^T[slot][column] = K q: K's bytes are a lane's own row, converted in registers;
+//   O^T[dim][column] += V^T P: P comes out of the first product in the layout the second one takes
+//     (slots 4 kg .. 4 kg + 3 of both halves of the block are the eight terms of lane group kg), V's bytes
+//     are loaded as rows and transposed in registers, 2 x 2 values at a time.
+// Nothing is staged in LDS before the end of a chunk. q is scaled by a power of two into fp16's range,
+// P by 2^14 relative to its block's largest score of the column, so that neither can leave it: the
+// factor between the block's and the running maximum, and V's scale, are applied to the f32 products.
 #include "common.cuh"
 #include "kv8.h"
 #include "kv8_codes.cuh"
@@ -13,157 +22,520 @@ namespace iek {
 
 namespace {
 
+typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
+typedef float f4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
+
+constexpr int TILE = KV8_BLOCK;
+constexpr int WAVES = 4;
+constexpr int MAX_SPLIT = 256;
+
 struct Plan {
-  int cols, chunk, nsplit, spad;  // columns of a KV head, slots a chunk, chunks, stored scores a column
-  float* ml;                      // [batch * n_kv][cols][nsplit][2]
-  float* o;                       // [batch * n_kv][cols][nsplit][hd]
-  float* s;                       // [batch * n_kv][cols][spad] or null
+  int cols, cblocks;       // columns of a KV head, workgroups they are spread over
+  int tiles, nsplit;       // tiles a chunk, chunks a sequence at most
+  int spad;                // stored scores a column
+  float* ml;               // [batch * n_kv][cols][nsplit] pairs (m, l)
+  float* o;                // [batch * n_kv][cols][nsplit][hd]
+  float* s;                // [batch * n_kv][cols][spad], base 2, or null
 };
 
-IEK_DEV void col_range(const Kv8Attn& a, int n, int t, int& lo, int& hi) {
-  hi = n - (a.n_q - 1 - t);
-  lo = a.window > 0 ? max(0, hi - a.window) : 0;
+// The slots that the columns of query token t see, and tile range [t0, t1) that any column sees.
+IEK_DEV int col_hi(const Kv8Attn& a, int n, int t) { return n - (a.n_q - 1 - t); }
+IEK_DEV int col_lo(const Kv8Attn& a, int hi) { return a.window > 0 ? max(0, hi - a.window) : 0; }
+IEK_DEV void tile_range(const Kv8Attn& a, int n, int& t0, int& t1) {
+  t0 = col_lo(a, max(0, col_hi(a, n, 0))) / TILE;
+  t1 = (n + TILE - 1) / TILE;
 }
 
-// One wave per (column, chunk).
-template <int HD, bool E4M3>
-__global__ __launch_bounds__(64) void part_kernel(Kv8 c, Kv8Attn a, Plan p) {
-  constexpr int DPL = HD / 64;
-  const int lane = threadIdx.x;
-  int id = blockIdx.x;
-  const int cp = id % p.nsplit;
-  id /= p.nsplit;
-  const int col = id % p.cols, bh = id / p.cols;
-  const int b = bh / c.n_kv, h = bh % c.n_kv, G = a.n_heads / c.n_kv, t = col / G;
+// v over the wave's four groups of 16 lanes
+IEK_DEV float groups_max(float v) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+IEK_DEV float groups_sum(float v) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+// v plus the value of the lane eight further in its row of 16: the hi and lo columns
+IEK_DEV float pair_sum(float v) { return v + dpp_f<0x128>(0.f, v); }  // row_ror:8
+
+// Four codes as fp16: pairs (0, 1) and (2, 3). int8: as 1024 + (code + 128), whose fp16 bits are
+// 0x6400 | byte, minus 1152.
+template <bool E4M3>
+IEK_DEV void codes_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (E4M3) {
+    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.0f, false));
+    hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.0f, true));
+  } else {
+    w ^= 0x80808080u;
+    const h2_t k = {(_Float16)-1152.f, (_Float16)-1152.f};
+    lo = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2_t, __builtin_amdgcn_perm(0x64646464u, w, 0x04010400u)) + k);
+    hi = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2_t, __builtin_amdgcn_perm(0x64646464u, w, 0x04030402u)) + k);
+  }
+}
+
+IEK_DEV f4_t mfma(u4_t a, u4_t b, f4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, a), __builtin_bit_cast(h8_t, b), c, 0, 0, 0);
+}
+
+// Raw bytes of a tile: K, two sets of 16 rows, 16 bytes per 64 dims; V, eight rows of hd / 16 bytes.
+template <int HD>
+struct Tile {
+  static constexpr int KC = HD / 64, VW = HD / 64;  // 16-byte pieces of K a row, dwords of V a row
+  u4_t k[2][KC];
+  uint32_t v[8][VW];
+  float ks, vs;
+};
+
+template <int HD>
+IEK_DEV void load_k(Tile<HD>& T, const uint8_t* base, const float* ks, int tile, int n, int lane) {
+  const uint8_t* p = base + (size_t)tile * (TILE * HD);
+  const int lim = n - 1 - tile * TILE;
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const int off = min(16 * s + (lane & 15), lim) * HD + 16 * (lane >> 4);  // (rows past the last repeat it)
+#pragma unroll
+    for (int i = 0; i < Tile<HD>::KC; ++i) T.k[s][i] = *reinterpret_cast<const u4_t*>(p + off + 64 * i);
+  }
+  T.ks = ks[tile];
+}
+
+template <int HD>
+IEK_DEV void load_v(Tile<HD>& T, const uint8_t* base, const float* vs, int tile, int n, int lane) {
+  constexpr int VW = Tile<HD>::VW;
+  const uint8_t* p = base + (size_t)tile * (TILE * HD);
+  const int lim = n - 1 - tile * TILE;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int off = min(16 * (j >> 2) + 4 * (lane >> 4) + (j & 3), lim) * HD + (HD / 16) * (lane & 15);
+    if constexpr (VW == 1) {
+      T.v[j][0] = *reinterpret_cast<const uint32_t*>(p + off);
+    } else if constexpr (VW == 2) {
+      const uint2 x = *reinterpret_cast<const uint2*>(p + off);
+      T.v[j][0] = x.x;
+      T.v[j][1] = x.y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < VW / 4; ++i) {
+        const u4_t x = *reinterpret_cast<const u4_t*>(p + off + 16 * i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) T.v[j][4 * i + e] = x[e];
+      }
+    }
+  }
+  T.vs = vs[tile];
+}
+
+// One workgroup: CG * 8 columns of a KV head over a chunk, its waves every fourth tile.
+template <int HD, bool E4M3, int CG>
+__global__ __launch_bounds__(64 * WAVES) void part_kernel(Kv8 c, Kv8Attn a, Plan p) {
+  constexpr int NS = HD / 32;   // steps of the first product
+  constexpr int ND = HD / 16;   // dims of a lane in the second: (HD / 16) r + i of row r
+  constexpr int VW = Tile<HD>::VW;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kg = lane >> 4, c8 = lane & 7;
+  const bool lo_half = lane & 8;
+  // the workgroups of a chunk's columns on one XCD (consecutive ones go to the eight XCDs in turn)
+  const int slot = blockIdx.x >> 3;
+  const int cb = slot % p.cblocks, unit = (slot / p.cblocks) * 8 + (blockIdx.x & 7);
+  const int cp = unit % p.nsplit, bh = unit / p.nsplit;
+  if (bh >= c.batch * c.n_kv) return;
+  const int b = bh / c.n_kv, h = bh - b * c.n_kv, G = a.n_heads / c.n_kv;
   const int n = max(0, min(a.len[b], a.max_len));
-  int lo, hi;
-  col_range(a, n, t, lo, hi);
-  const int c0 = cp * p.chunk, c1 = min(n, c0 + p.chunk);
-  const size_t pi = ((size_t)bh * p.cols + col) * p.nsplit + cp;
-  __shared__ __align__(16) float q[HD];
-  __shared__ float ps[64];
-  const float* qr = a.q + ((size_t)b * a.n_q + t) * a.q_stride + (size_t)(h * G + col % G) * HD;
-  for (int d = lane; d < HD; d += 64) q[d] = qr[d];
-  __syncthreads();
+  int t0, t1;
+  tile_range(a, n, t0, t1);
+  const int live = (t1 - t0 + p.tiles - 1) / p.tiles;
+  const bool direct = p.nsplit == 1;
+  if (cp >= live && !(direct && live <= 0)) return;  // (an empty sequence's only chunk writes zeros)
+  t0 += cp * p.tiles;
+  t1 = min(t1, t0 + p.tiles);
   const uint8_t* K = c.k + (size_t)bh * c.cap * HD;
   const uint8_t* V = c.v + (size_t)bh * c.cap * HD;
-  float m = -INFINITY, l = 0.f, o[DPL] = {};
-  for (int j0 = c0; j0 < c1; j0 += 64) {
-    const int j = j0 + lane;
-    float s = -INFINITY;
-    if (j < c1 && j >= lo && j < hi) {
-      float dot = 0.f;
-      for (int d = 0; d < HD; d += 4) {
-        const float4 k4 = kv8_unpack<E4M3>(*reinterpret_cast<const uint32_t*>(K + (size_t)j * HD + d));
-        dot += q[d] * k4.x + q[d + 1] * k4.y + q[d + 2] * k4.z + q[d + 3] * k4.w;
-      }
-      s = dot * (c.ks[(size_t)bh * c.nblk + j / KV8_BLOCK] * (a.scale * 1.44269504088896340736f));
-    }
-    if (p.s && j < c1) p.s[((size_t)bh * p.cols + col) * p.spad + j] = s;
-    const bool in = j < c1 && j >= lo && j < hi;
-    const float mn = fmaxf(m, wave_max(s));
-    const float corr = m == -INFINITY ? 1.f : exp2f(m - mn);
-    const float e = in ? exp2f(s - mn) : 0.f;
-    l = l * corr + wave_sum(e);
-    m = mn;
-    ps[lane] = e;
-    __syncthreads();
-    for (int i = 0; i < DPL; ++i) o[i] *= corr;
-    for (int i = 0; i < 64 && j0 + i < c1; ++i) {
-      if (j0 + i < lo || j0 + i >= hi) continue;
-      const float w = ps[i] * c.vs[(size_t)bh * c.nblk + (j0 + i) / KV8_BLOCK];
-      for (int d = 0; d < DPL; ++d) {
-        const uint32_t by = V[(size_t)(j0 + i) * HD + lane + 64 * d];
-        o[d] += w * kv8_unpack<E4M3>(by).x;
-      }
-    }
-    __syncthreads();
+  const float* KS = c.ks + (size_t)bh * c.nblk;
+  const float* VS = c.vs + (size_t)bh * c.nblk;
+  Tile<HD> T;
+  int tile = t0 + wave;
+  if (tile < t1) {
+    load_k(T, K, KS, tile, n, lane);
+    load_v(T, V, VS, tile, n, lane);
   }
-  if (lane == 0) {
-    p.ml[2 * pi] = isnan(l) ? l : m;  // (a NaN reaches the output: the maximum passes it over)
-    p.ml[2 * pi + 1] = l;
+  // this lane's columns and its part of their q: dims 64 i + 16 kg + [0, 16) as steps 2 i and 2 i + 1
+  u4_t q[CG][NS];
+  float qs[CG];
+  int hi[CG], lo[CG];
+  int lo_max = 0, hi_min = n;
+#pragma unroll
+  for (int u = 0; u < CG; ++u) {
+    const int col = (cb * CG + u) * 8 + c8;
+    const int cc = min(col, p.cols - 1), t = cc / G;
+    hi[u] = col_hi(a, n, t);
+    lo[u] = col_lo(a, hi[u]);
+    const float* row = a.q + ((size_t)b * a.n_q + t) * a.q_stride + (size_t)(h * G + cc - t * G) * HD + 16 * kg;
+    float x[HD / 4];
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < HD / 64; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const f4_t v = *reinterpret_cast<const f4_t*>(row + 64 * i + 4 * e);
+#pragma unroll
+        for (int f = 0; f < 4; ++f) {
+          x[16 * i + 4 * e + f] = v[f];
+          top = fmaxf(top, fabsf(v[f]));
+        }
+      }
+    top = groups_max(top);
+    // into [2^13, 2^14) by a power of two (an infinity or NaN, or a row of zeros, stays what it is)
+    int ex = (int)(__float_as_uint(top) >> 23) - 127;
+    ex = ex == 128 ? 0 : max(13 - ex, -127 + 13);
+    ex = min(ex, 126);
+    const float up = __builtin_amdgcn_ldexpf(1.f, ex);
+    qs[u] = __builtin_amdgcn_ldexpf(a.scale * 1.44269504088896340736f, -ex);
+#pragma unroll
+    for (int i = 0; i < NS; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float y0 = x[8 * i + 2 * e] * up, y1 = x[8 * i + 2 * e + 1] * up;
+        const h2_t w = {(_Float16)y0, (_Float16)y1};
+        const h2_t z = {(_Float16)(y0 - (float)w[0]), (_Float16)(y1 - (float)w[1])};
+        q[u][i][e] = __builtin_bit_cast(uint32_t, lo_half ? z : w);
+      }
+    lo_max = max(lo_max, lo[u]);
+    hi_min = min(hi_min, hi[u]);
   }
-  for (int d = 0; d < DPL; ++d) p.o[pi * HD + lane + 64 * d] = o[d];
+  // (over the workgroup's columns, which are in ascending order of t)
+  lo_max = __builtin_amdgcn_readlane(lo_max, 7);
+  hi_min = __builtin_amdgcn_readlane(hi_min, 0);
+  float m[CG], l[CG];
+  f4_t o[CG][ND];
+#pragma unroll
+  for (int u = 0; u < CG; ++u) {
+    m[u] = -INFINITY;
+    l[u] = 0.f;
+#pragma unroll
+    for (int i = 0; i < ND; ++i) o[u][i] = f4_t{0.f, 0.f, 0.f, 0.f};
+  }
+  // P's column of this lane: e's fp16, or 2^11 times what that cuts off (applied to o at the end)
+  const float cut = lo_half ? -2048.f : 0.f, keep = lo_half ? 2048.f : 1.f;
+
+  for (; tile < t1; tile += WAVES) {
+    const bool inner = tile * TILE >= lo_max && (tile + 1) * TILE <= hi_min;  // every column sees all of it
+    const bool more = tile + WAVES < t1;
+    f4_t d[CG][2];
+#pragma unroll
+    for (int u = 0; u < CG; ++u) d[u][0] = d[u][1] = f4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        u4_t k;
+        uint32_t x, y;
+        codes_f16<E4M3>(T.k[s][i >> 1][2 * (i & 1)], x, y);
+        k[0] = x;
+        k[1] = y;
+        codes_f16<E4M3>(T.k[s][i >> 1][2 * (i & 1) + 1], x, y);
+        k[2] = x;
+        k[3] = y;
+#pragma unroll
+        for (int u = 0; u < CG; ++u) d[u][s] = mfma(k, q[u][i], d[u][s]);
+      }
+    const float ks = T.ks;
+    if (more) load_k(T, K, KS, tile + WAVES, n, lane);
+    u4_t pr[CG];
+    float fac[CG];
+#pragma unroll
+    for (int u = 0; u < CG; ++u) {
+      const float f = qs[u] * ks;
+      float s[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[i] = pair_sum(d[u][i >> 2][i & 3]) * f;
+      if (!inner) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int j = tile * TILE + 16 * (i >> 2) + 4 * kg + (i & 3);
+          if (j < lo[u] || j >= hi[u]) s[i] = -INFINITY;
+        }
+      }
+      if (p.s) {
+        const int col = (cb * CG + u) * 8 + c8;
+        float* to = p.s + ((size_t)bh * p.cols + col) * p.spad + tile * TILE + 4 * kg + (lo_half ? 16 : 0);
+        const f4_t v = lo_half ? f4_t{s[4], s[5], s[6], s[7]} : f4_t{s[0], s[1], s[2], s[3]};
+        if (col < p.cols) *reinterpret_cast<f4_t*>(to) = v;
+      }
+      float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+      top = groups_max(top);
+      // The running maximum is only a reference: it moves when a block's is 2^30 above it.
+      if (__any(top > m[u] + 30.f || (m[u] == -INFINITY && top > m[u]))) {
+        const bool up = top > m[u] + 30.f || m[u] == -INFINITY;
+        const float corr = up && m[u] != -INFINITY ? __builtin_amdgcn_exp2f(m[u] - top) : 1.f;  // (all is 0 before)
+        if (up) m[u] = top;
+        l[u] *= corr;
+#pragma unroll
+        for (int i = 0; i < ND; ++i) o[u][i] *= corr;
+      }
+      const float ref = top == -INFINITY ? 0.f : top;
+      fac[u] = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - m[u] - 14.f);
+      float sum = 0.f, x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[i] = __builtin_amdgcn_exp2f(s[i] - ref + 14.f);
+        sum += x[i];
+      }
+      l[u] += sum * fac[u];
+      fac[u] *= T.vs;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const h2_t e = __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_pkrtz(x[2 * i], x[2 * i + 1]));
+        pr[u][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(fmaf((float)e[0], cut, x[2 * i] * keep),
+                                                                           fmaf((float)e[1], cut, x[2 * i + 1] * keep)));
+      }
+    }
+#pragma unroll
+    for (int w = 0; w < VW; ++w) {
+      uint32_t x[8][2];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) codes_f16<E4M3>(T.v[j][w], x[j][0], x[j][1]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        u4_t v;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          v[j] = __builtin_amdgcn_perm(x[2 * j + 1][e >> 1], x[2 * j][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+        for (int u = 0; u < CG; ++u) {
+          const f4_t t = mfma(v, pr[u], f4_t{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+          for (int r = 0; r < 4; ++r) o[u][4 * w + e][r] += t[r] * fac[u];
+        }
+      }
+    }
+    if (more) load_v(T, V, VS, tile + WAVES, n, lane);
+  }
+
+  // The waves' parts: to a common maximum, then summed through LDS, one wave after the other's columns.
+  __shared__ float sm[WAVES][8 * CG], sl[WAVES][8 * CG];
+  __shared__ __align__(16) float so[WAVES][8][HD];
+#pragma unroll
+  for (int u = 0; u < CG; ++u) {
+    l[u] = groups_sum(l[u]);
+    if (lane < 8) {
+      sm[wave][8 * u + lane] = m[u];
+      sl[wave][8 * u + lane] = l[u];
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < CG; ++u) {
+    float top = sm[0][8 * u + c8];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) top = fmaxf(top, sm[w][8 * u + c8]);
+    const float mine = m[u] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[u] - top - (lo_half ? 11.f : 0.f));
+    if (u > 0) __syncthreads();
+    // dims (HD / 16) (4 kg + r) + i: for each r the lane has ND of them in a row, stored by the hi lanes for
+    // r = 0, 1 and the lo lanes for r = 2, 3
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      float y[ND];
+#pragma unroll
+      for (int i = 0; i < ND; ++i) y[i] = pair_sum(o[u][i][r] * mine);
+      if (lo_half == (r >= 2)) {
+#pragma unroll
+        for (int i = 0; i < ND; i += 4)
+          *reinterpret_cast<f4_t*>(&so[wave][c8][ND * (4 * kg + r) + i]) = f4_t{y[i], y[i + 1], y[i + 2], y[i + 3]};
+      }
+    }
+    __syncthreads();
+    const int c0 = (cb * CG + u) * 8;
+    for (int i = threadIdx.x; i < 8 * HD / 4; i += 64 * WAVES) {
+      const int col = i / (HD / 4), dim = 4 * (i % (HD / 4));
+      if (c0 + col >= p.cols) continue;
+      f4_t y = *reinterpret_cast<const f4_t*>(&so[0][col][dim]);
+#pragma unroll
+      for (int w = 1; w < WAVES; ++w) y += *reinterpret_cast<const f4_t*>(&so[w][col][dim]);
+      float mm = sm[0][8 * u + col];
+#pragma unroll
+      for (int w = 1; w < WAVES; ++w) mm = fmaxf(mm, sm[w][8 * u + col]);
+      float ll = 0.f;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w)
+        ll += sl[w][8 * u + col] * (sm[w][8 * u + col] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(sm[w][8 * u + col] - mm));
+      const size_t row = (size_t)bh * p.cols + c0 + col;
+      if (direct) {
+        const int t = (c0 + col) / G, g = (c0 + col) - t * G;
+        float* out = a.out + (((size_t)b * a.n_q + t) * a.n_heads + h * G + g) * HD + dim;
+        *reinterpret_cast<f4_t*>(out) = ll == 0.f ? f4_t{0.f, 0.f, 0.f, 0.f} : y / ll;
+      } else {
+        *reinterpret_cast<f4_t*>(p.o + (row * p.nsplit + cp) * HD + dim) = y;
+      }
+      if (dim == 0) {
+        p.ml[2 * (row * p.nsplit + cp)] = isnan(ll) ? ll : mm;  // (a NaN: the maxima pass it over)
+        p.ml[2 * (row * p.nsplit + cp) + 1] = ll;
+      }
+    }
+  }
 }
 
-// Workgroups [0, batch * n_kv * cols): the output of a column; those behind them: weights of 256 entries.
+// Workgroups [0, batch * n_kv * cols), unless the chunks have written the output themselves: one
+// column each. Those behind them: the weights of 1024 entries of a KV head.
 template <int HD>
-__global__ __launch_bounds__(256) void join_kernel(Kv8 c, Kv8Attn a, Plan p, int wblocks) {
-  const int t = threadIdx.x, ncol = c.batch * c.n_kv * p.cols, G = a.n_heads / c.n_kv;
+__global__ __launch_bounds__(256) void join_kernel(Kv8 c, Kv8Attn a, Plan p, int ncol, int wblocks) {
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, G = a.n_heads / c.n_kv;
   if ((int)blockIdx.x < ncol) {
-    const int bh = blockIdx.x / p.cols, col = blockIdx.x % p.cols, b = bh / c.n_kv, h = bh % c.n_kv;
-    const float* ml = p.ml + (size_t)blockIdx.x * p.nsplit * 2;
-    const float* o = p.o + (size_t)blockIdx.x * p.nsplit * HD;
+    constexpr int TPR = HD / 4, GRP = 256 / TPR;
+    __shared__ float w[MAX_SPLIT];
+    __shared__ float red[2][4];
+    __shared__ __align__(16) float acc[GRP][HD];
+    const int bh = blockIdx.x / p.cols, col = blockIdx.x - bh * p.cols, b = bh / c.n_kv, h = bh - b * c.n_kv;
+    const int n = max(0, min(a.len[b], a.max_len));
+    int t0, t1;
+    tile_range(a, n, t0, t1);
+    const int live = (t1 - t0 + p.tiles - 1) / p.tiles;
+    const size_t row = (size_t)blockIdx.x * p.nsplit;
     float m = -INFINITY, l = 0.f;
-    for (int i = 0; i < p.nsplit; ++i) m = fmaxf(m, ml[2 * i]);
-    for (int i = 0; i < p.nsplit; ++i) l += ml[2 * i] == -INFINITY ? 0.f : ml[2 * i + 1] * exp2f(ml[2 * i] - m);
-    for (int d = t; d < HD; d += 256) {
-      float x = 0.f;
-      for (int i = 0; i < p.nsplit; ++i)
-        if (ml[2 * i] != -INFINITY) x += o[(size_t)i * HD + d] * exp2f(ml[2 * i] - m);
-      a.out[(((size_t)b * a.n_q + col / G) * a.n_heads + h * G + col % G) * HD + d] = m == -INFINITY && l == 0.f ? 0.f : x / l;
+    if (t < live) {
+      m = p.ml[2 * (row + t)];
+      l = p.ml[2 * (row + t) + 1];
+    }
+    float top = wave_max(m);
+    if (lane == 0) red[0][wave] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+    const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+    if (t < live) w[t] = f;
+    l = wave_sum(l * f);
+    if (lane == 0) red[1][wave] = l;
+    __syncthreads();
+    l = red[1][0] + red[1][1] + red[1][2] + red[1][3];
+    const int g = t / TPR, d = 4 * (t % TPR);
+    f4_t y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int i = g; i < live; i += GRP) y += *reinterpret_cast<const f4_t*>(p.o + (row + i) * HD + d) * w[i];
+    *reinterpret_cast<f4_t*>(&acc[g][d]) = y;
+    __syncthreads();
+    if (t < TPR) {
+#pragma unroll
+      for (int i = 1; i < GRP; ++i) y += *reinterpret_cast<const f4_t*>(&acc[i][d]);
+      const int tq = col / G;
+      float* out = a.out + (((size_t)b * a.n_q + tq) * a.n_heads + h * G + col - tq * G) * HD + d;
+      *reinterpret_cast<f4_t*>(out) = l == 0.f ? f4_t{0.f, 0.f, 0.f, 0.f} : y / l;
     }
     return;
   }
-  const int id = blockIdx.x - ncol, bh = id / wblocks, j = (id % wblocks) * 256 + t, b = bh / c.n_kv;
+  constexpr int COLS = 64 * 8;  // n_q <= 64, groups of at most 8
+  __shared__ float cm[COLS], cl[COLS];
+  const int id = blockIdx.x - ncol, bh = id / wblocks, b = bh / c.n_kv;
   const int n = max(0, min(a.len[b], a.max_len));
-  if (j >= n) return;
-  float w = 0.f;
-  for (int col = 0; col < p.cols; ++col) {
-    int lo, hi;
-    col_range(a, n, col / G, lo, hi);
+  const int j = (id - bh * wblocks) * 1024 + 4 * t;
+  if (j - 4 * t >= n) return;  // uniform
+  int t0, t1;
+  tile_range(a, n, t0, t1);
+  const int live = (t1 - t0 + p.tiles - 1) / p.tiles;
+  for (int col = wave; col < p.cols; col += 4) {
     const float* ml = p.ml + ((size_t)bh * p.cols + col) * p.nsplit * 2;
-    float m = -INFINITY, l = 0.f;
-    for (int i = 0; i < p.nsplit; ++i) m = fmaxf(m, ml[2 * i]);
-    for (int i = 0; i < p.nsplit; ++i) l += ml[2 * i] == -INFINITY ? 0.f : ml[2 * i + 1] * exp2f(ml[2 * i] - m);
-    if (j >= lo && j < hi) w += exp2f(p.s[((size_t)bh * p.cols + col) * p.spad + j] - m) / l;
+    float m = -INFINITY;
+    for (int i = lane; i < live; i += 64) m = fmaxf(m, ml[2 * i]);
+    m = wave_max(m);
+    float l = 0.f;
+    for (int i = lane; i < live; i += 64) l += ml[2 * i] == -INFINITY ? 0.f : ml[2 * i + 1] * __builtin_amdgcn_exp2f(ml[2 * i] - m);
+    l = wave_sum(l);
+    if (lane == 0) {
+      cm[col] = m == -INFINITY ? 0.f : m;  // (a column that sees nothing has only scores of -inf)
+      cl[col] = l == 0.f ? 0.f : 1.f / l;
+    }
+  }
+  __syncthreads();
+  if (j >= n) return;
+  f4_t w = {0.f, 0.f, 0.f, 0.f};
+  if (j >= t0 * TILE) {
+    const float* s = p.s + (size_t)bh * p.cols * p.spad + j;
+#pragma unroll 4
+    for (int col = 0; col < p.cols; ++col) {
+      const f4_t v = *reinterpret_cast<const f4_t*>(s + (size_t)col * p.spad);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] += __builtin_amdgcn_exp2f(v[i] - cm[col]) * cl[col];
+    }
   }
   const size_t at = (size_t)bh * c.cap + j;
-  a.w_out[at] = (a.w_in ? a.w_in[at] : 0.f) + w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (j + i < n) a.w_out[at + i] = (a.w_in ? a.w_in[at + i] : 0.f) + w[i];
 }
 
 size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
-Plan make_plan(const Kv8& c, int n_heads, int n_q, int max_len, bool weights, void* ws, size_t* bytes) {
+// Column groups of eight per workgroup: two where there are more than eight columns, whose accumulators
+// leave room for two waves a SIMD (head_dim up to 256).
+int col_groups(int cols, int hd) { return cols > 8 && hd <= 256 ? 2 : 1; }
+
+// What the plan and the workspace's size share: the chunks that a sequence is cut into at most.
+int most_chunks(const Kv8& c, int cblocks) {
+  const long long units = std::max<long long>(1, (long long)c.batch * c.n_kv * cblocks);
+  return (int)std::max<long long>(1, std::min<long long>(MAX_SPLIT, 1024 / units));
+}
+
+struct Sizes {
+  size_t ml, o, s;
+};
+Sizes sizes(const Kv8& c, int cols, int nsplit, int spad, bool weights) {
+  const size_t rows = (size_t)c.batch * c.n_kv * cols;
+  return {up256(rows * nsplit * 8), nsplit > 1 ? up256(rows * nsplit * c.hd * 4) : 0, weights ? up256(rows * spad * 4) : 0};
+}
+
+Plan make_plan(const Kv8& c, const Kv8Attn& a, void* ws) {
   Plan p{};
-  p.cols = n_heads / c.n_kv * n_q;
-  p.chunk = std::max(256, (max_len + 63) / 64);
-  p.nsplit = std::max(1, (max_len + p.chunk - 1) / p.chunk);
-  p.spad = (max_len + 31) / 32 * 32;
-  const size_t rows = (size_t)c.batch * c.n_kv * p.cols;
-  const size_t ml = up256(rows * p.nsplit * 8), o = up256(rows * p.nsplit * c.hd * 4);
+  p.cols = a.n_heads / c.n_kv * a.n_q;
+  const int per = 8 * col_groups(p.cols, c.hd);
+  p.cblocks = (p.cols + per - 1) / per;
+  // the tiles that a sequence's columns see at most, as chunks of whole rounds of the waves
+  const long long span = a.window > 0 ? std::min<long long>(a.max_len, (long long)a.window + a.n_q + TILE - 2) : a.max_len;
+  const int tiles = (int)((span + TILE - 1) / TILE), want = most_chunks(c, p.cblocks);
+  p.tiles = std::max(1, ((tiles + want - 1) / want + WAVES - 1) / WAVES) * WAVES;
+  p.nsplit = std::max(1, (tiles + p.tiles - 1) / p.tiles);
+  p.spad = (a.max_len + TILE - 1) / TILE * TILE;
+  const Sizes z = sizes(c, p.cols, p.nsplit, p.spad, a.w_out != nullptr);
   char* base = static_cast<char*>(ws);
   p.ml = reinterpret_cast<float*>(base);
-  p.o = reinterpret_cast<float*>(base + ml);
-  p.s = weights ? reinterpret_cast<float*>(base + ml + o) : nullptr;
-  if (bytes) *bytes = ml + o + (weights ? up256(rows * p.spad * 4) : 0);
+  p.o = reinterpret_cast<float*>(base + z.ml);
+  p.s = a.w_out ? reinterpret_cast<float*>(base + z.ml + z.o) : nullptr;
   return p;
 }
 
-template <int HD>
-void launch_hd(const Kv8& c, const Kv8Attn& a, const Plan& p, hipStream_t st) {
-  const int rows = c.batch * c.n_kv * p.cols, wblocks = a.w_out ? (a.max_len + 255) / 256 : 0;
-  auto fn = c.e4m3 ? part_kernel<HD, true> : part_kernel<HD, false>;
-  hipLaunchKernelGGL(fn, dim3((unsigned)rows * p.nsplit), dim3(64), 0, st, c, a, p);
-  hipLaunchKernelGGL(join_kernel<HD>, dim3((unsigned)rows + c.batch * c.n_kv * wblocks), dim3(256), 0, st, c, a, p,
-                     wblocks);
+template <int HD, int CG>
+void launch_cg(const Kv8& c, const Kv8Attn& a, const Plan& p, hipStream_t st) {
+  const long long units = ((long long)c.batch * c.n_kv * p.nsplit + 7) / 8 * 8 * p.cblocks;
+  const long long ncol = p.nsplit > 1 ? (long long)c.batch * c.n_kv * p.cols : 0;
+  const int wblocks = a.w_out ? (a.max_len + 1023) / 1024 : 0;
+  const long long join = ncol + (long long)c.batch * c.n_kv * wblocks;
+  if (units > INT32_MAX || join > INT32_MAX) fail(ST_OP, "kv8: dims too large");
+  auto fn = c.e4m3 ? part_kernel<HD, true, CG> : part_kernel<HD, false, CG>;
+  hipLaunchKernelGGL(fn, dim3((unsigned)units), dim3(64 * WAVES), 0, st, c, a, p);
+  if (join)
+    hipLaunchKernelGGL(join_kernel<HD>, dim3((unsigned)join), dim3(256), 0, st, c, a, p, (int)ncol, wblocks);
 }
 
 }  // namespace
 
+// For any window: whatever its chunks, there are at most most_chunks of at least WAVES tiles.
 size_t kv8_attention_workspace(const Kv8& c, int n_heads, int n_q, int max_len, bool weights) {
-  size_t bytes = 0;
-  make_plan(c, n_heads, n_q, max_len, weights, nullptr, &bytes);
-  return bytes;
+  const int cols = n_heads / c.n_kv * n_q, per = 8 * col_groups(cols, c.hd), spad = (max_len + TILE - 1) / TILE * TILE;
+  const int rounds = (spad / TILE + WAVES - 1) / WAVES;
+  const Sizes z = sizes(c, cols, std::max(1, std::min(rounds, most_chunks(c, (cols + per - 1) / per))), spad, weights);
+  return z.ml + z.o + z.s;
 }
 
 void launch_kv8_attention(const Kv8& c, const Kv8Attn& a, void* ws, hipStream_t st) {
-  const Plan p = make_plan(c, a.n_heads, a.n_q, a.max_len, a.w_out != nullptr, ws, nullptr);
+  const Plan p = make_plan(c, a, ws);
+  const bool two = col_groups(p.cols, c.hd) == 2;
   switch (c.hd) {
-    case 64: launch_hd<64>(c, a, p, st); break;
-    case 128: launch_hd<128>(c, a, p, st); break;
-    case 256: launch_hd<256>(c, a, p, st); break;
-    default: launch_hd<512>(c, a, p, st); break;
+    case 64: two ? launch_cg<64, 2>(c, a, p, st) : launch_cg<64, 1>(c, a, p, st); break;
+    case 128: two ? launch_cg<128, 2>(c, a, p, st) : launch_cg<128, 1>(c, a, p, st); break;
+    case 256: two ? launch_cg<256, 2>(c, a, p, st) : launch_cg<256, 1>(c, a, p, st); break;
+    default: launch_cg<512, 1>(c, a, p, st); break;
   }
 }
 

@@ -94,7 +94,11 @@ class Cache:
                     # 32 at a time, then over tiles, waves and at most 256 chunks.
                     size = scale * (np.abs(qq) @ np.abs(keys[lo:hi]).T).max(1, keepdims=True)
                     rel = (2 * (hd + 16) * size + 32 + n / 32 + 300) * 2.0 ** -24
-                    bound[b, t, h * group:(h + 1) * group] = rel * (p @ np.abs(vals[lo:hi]))
+                    # A share may be held in fixed point relative to the largest of its block: as a pair of
+                    # fp16, of 2^14 p and of 2^11 times the rest, it is off by at most half of fp16's smallest
+                    # step, 2^-25 2^-11 2^-14 = 2^-50, of the largest share (2^-49 for a cut rest).
+                    fixed = (hi - lo) * 2.0 ** -49 * np.abs(vals[lo:hi]).max(0)
+                    bound[b, t, h * group:(h + 1) * group] = rel * (p @ np.abs(vals[lo:hi])) + fixed
         return out, weights, bound
 
     def kept(self, w, n, keep, first, last):
