@@ -32,7 +32,7 @@ constexpr int WAVES = 4;
 constexpr int MAX_SPLIT = 256;
 
 struct Plan {
-  int cols, cblocks;       // columns of a KV head, workgroups they are spread over
+  int group, cols, cblocks;  // query heads and columns of a KV head, workgroups the columns are spread over
   int tiles, nsplit;       // tiles a chunk, chunks a sequence at most
   int spad;                // stored scores a column
   float* ml;               // [batch * n_kv][cols][nsplit] pairs (m, l)
@@ -92,37 +92,43 @@ struct Tile {
   float ks, vs;
 };
 
+// Buffer accesses end at the last live row of the tile: the rows behind it read as zero codes, whatever
+// they hold (a NaN code would reach O through a weight of 0).
 template <int HD>
-IEK_DEV void load_k(Tile<HD>& T, const uint8_t* base, const float* ks, int tile, int n, int lane) {
-  const uint8_t* p = base + (size_t)tile * (TILE * HD);
-  const int lim = n - 1 - tile * TILE;
+IEK_DEV __amdgpu_buffer_rsrc_t tile_rsrc(const uint8_t* codes, int tile, int n) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(codes) + (size_t)tile * (TILE * HD), (short)0,
+                                           min(TILE, n - tile * TILE) * HD, 0x00020000);
+}
+
+template <int HD>
+IEK_DEV void load_k(Tile<HD>& T, const uint8_t* codes, const float* ks, int tile, int n, int lane) {
+  const auto rs = tile_rsrc<HD>(codes, tile, n);
 #pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    const int off = min(16 * s + (lane & 15), lim) * HD + 16 * (lane >> 4);  // (rows past the last repeat it)
+  for (int s = 0; s < 2; ++s)
 #pragma unroll
-    for (int i = 0; i < Tile<HD>::KC; ++i) T.k[s][i] = *reinterpret_cast<const u4_t*>(p + off + 64 * i);
-  }
+    for (int i = 0; i < Tile<HD>::KC; ++i)
+      T.k[s][i] = __builtin_amdgcn_raw_buffer_load_b128(rs, (lane & 15) * HD + 16 * (lane >> 4), 16 * s * HD + 64 * i, 0);
   T.ks = ks[tile];
 }
 
 template <int HD>
-IEK_DEV void load_v(Tile<HD>& T, const uint8_t* base, const float* vs, int tile, int n, int lane) {
+IEK_DEV void load_v(Tile<HD>& T, const uint8_t* codes, const float* vs, int tile, int n, int lane) {
   constexpr int VW = Tile<HD>::VW;
-  const uint8_t* p = base + (size_t)tile * (TILE * HD);
-  const int lim = n - 1 - tile * TILE;
+  const auto rs = tile_rsrc<HD>(codes, tile, n);
+  const int off = 4 * (lane >> 4) * HD + (HD / 16) * (lane & 15);
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const int off = min(16 * (j >> 2) + 4 * (lane >> 4) + (j & 3), lim) * HD + (HD / 16) * (lane & 15);
+    const int row = (16 * (j >> 2) + (j & 3)) * HD;
     if constexpr (VW == 1) {
-      T.v[j][0] = *reinterpret_cast<const uint32_t*>(p + off);
+      T.v[j][0] = __builtin_amdgcn_raw_buffer_load_b32(rs, off, row, 0);
     } else if constexpr (VW == 2) {
-      const uint2 x = *reinterpret_cast<const uint2*>(p + off);
-      T.v[j][0] = x.x;
-      T.v[j][1] = x.y;
+      const auto x = __builtin_amdgcn_raw_buffer_load_b64(rs, off, row, 0);
+      T.v[j][0] = x[0];
+      T.v[j][1] = x[1];
     } else {
 #pragma unroll
       for (int i = 0; i < VW / 4; ++i) {
-        const u4_t x = *reinterpret_cast<const u4_t*>(p + off + 16 * i);
+        const auto x = __builtin_amdgcn_raw_buffer_load_b128(rs, off, row + 16 * i, 0);
 #pragma unroll
         for (int e = 0; e < 4; ++e) T.v[j][4 * i + e] = x[e];
       }
@@ -133,19 +139,25 @@ IEK_DEV void load_v(Tile<HD>& T, const uint8_t* base, const float* vs, int tile,
 
 // One workgroup: CG * 8 columns of a KV head over a chunk, its waves every fourth tile.
 template <int HD, bool E4M3, int CG>
-__global__ __launch_bounds__(64 * WAVES) void part_kernel(Kv8 c, Kv8Attn a, Plan p) {
+__global__ __launch_bounds__(64 * WAVES, HD * CG <= 256 ? 2 : 1) void part_kernel(Kv8 c, Kv8Attn a, Plan p) {
   constexpr int NS = HD / 32;   // steps of the first product
   constexpr int ND = HD / 16;   // dims of a lane in the second: (HD / 16) r + i of row r
   constexpr int VW = Tile<HD>::VW;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kg = lane >> 4, c8 = lane & 7;
   const bool lo_half = lane & 8;
-  // the workgroups of a chunk's columns on one XCD (consecutive ones go to the eight XCDs in turn)
-  const int slot = blockIdx.x >> 3;
-  const int cb = slot % p.cblocks, unit = (slot / p.cblocks) * 8 + (blockIdx.x & 7);
-  const int cp = unit % p.nsplit, bh = unit / p.nsplit;
-  if (bh >= c.batch * c.n_kv) return;
-  const int b = bh / c.n_kv, h = bh - b * c.n_kv, G = a.n_heads / c.n_kv;
+  // several workgroups for a chunk's columns: on one XCD (consecutive ones go to the eight XCDs in turn)
+  int cp = blockIdx.x, h = blockIdx.y, b = blockIdx.z, cb = 0;
+  if (p.cblocks > 1) {
+    const int slot = blockIdx.x >> 3, unit = (slot / p.cblocks) * 8 + (blockIdx.x & 7);
+    cb = slot % p.cblocks;
+    cp = unit % p.nsplit;
+    h = unit / p.nsplit;
+    b = h / c.n_kv;
+    h -= b * c.n_kv;
+    if (b >= c.batch) return;
+  }
+  const int bh = b * c.n_kv + h, G = p.group;
   const int n = max(0, min(a.len[b], a.max_len));
   int t0, t1;
   tile_range(a, n, t0, t1);
@@ -172,7 +184,7 @@ __global__ __launch_bounds__(64 * WAVES) void part_kernel(Kv8 c, Kv8Attn a, Plan
 #pragma unroll
   for (int u = 0; u < CG; ++u) {
     const int col = (cb * CG + u) * 8 + c8;
-    const int cc = min(col, p.cols - 1), t = cc / G;
+    const int cc = min(col, p.cols - 1), t = a.n_q == 1 ? 0 : cc / G;
     hi[u] = col_hi(a, n, t);
     lo[u] = col_lo(a, hi[u]);
     const float* row = a.q + ((size_t)b * a.n_q + t) * a.q_stride + (size_t)(h * G + cc - t * G) * HD + 16 * kg;
@@ -223,7 +235,7 @@ __global__ __launch_bounds__(64 * WAVES) void part_kernel(Kv8 c, Kv8Attn a, Plan
   // P's column of this lane: e's fp16, or 2^11 times what that cuts off (applied to o at the end)
   const float cut = lo_half ? -2048.f : 0.f, keep = lo_half ? 2048.f : 1.f;
 
-  for (; tile < t1; tile += WAVES) {
+  for (; tile < t1; tile = __builtin_amdgcn_readfirstlane(tile + WAVES)) {
     const bool inner = tile * TILE >= lo_max && (tile + 1) * TILE <= hi_min;  // every column sees all of it
     const bool more = tile + WAVES < t1;
     f4_t d[CG][2];
@@ -384,7 +396,7 @@ __global__ __launch_bounds__(64 * WAVES) void part_kernel(Kv8 c, Kv8Attn a, Plan
 // column each. Those behind them: the weights of 1024 entries of a KV head.
 template <int HD>
 __global__ __launch_bounds__(256) void join_kernel(Kv8 c, Kv8Attn a, Plan p, int ncol, int wblocks) {
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, G = a.n_heads / c.n_kv;
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, G = p.group;
   if ((int)blockIdx.x < ncol) {
     constexpr int TPR = HD / 4, GRP = 256 / TPR;
     __shared__ float w[MAX_SPLIT];
@@ -488,7 +500,8 @@ Sizes sizes(const Kv8& c, int cols, int nsplit, int spad, bool weights) {
 
 Plan make_plan(const Kv8& c, const Kv8Attn& a, void* ws) {
   Plan p{};
-  p.cols = a.n_heads / c.n_kv * a.n_q;
+  p.group = a.n_heads / c.n_kv;
+  p.cols = p.group * a.n_q;
   const int per = 8 * col_groups(p.cols, c.hd);
   p.cblocks = (p.cols + per - 1) / per;
   // the tiles that a sequence's columns see at most, as chunks of whole rounds of the waves
@@ -507,13 +520,14 @@ Plan make_plan(const Kv8& c, const Kv8Attn& a, void* ws) {
 
 template <int HD, int CG>
 void launch_cg(const Kv8& c, const Kv8Attn& a, const Plan& p, hipStream_t st) {
-  const long long units = ((long long)c.batch * c.n_kv * p.nsplit + 7) / 8 * 8 * p.cblocks;
+  const long long units = p.cblocks == 1 ? p.nsplit : ((long long)c.batch * c.n_kv * p.nsplit + 7) / 8 * 8 * p.cblocks;
+  const dim3 grid = p.cblocks == 1 ? dim3((unsigned)units, (unsigned)c.n_kv, (unsigned)c.batch) : dim3((unsigned)units);
   const long long ncol = p.nsplit > 1 ? (long long)c.batch * c.n_kv * p.cols : 0;
   const int wblocks = a.w_out ? (a.max_len + 1023) / 1024 : 0;
   const long long join = ncol + (long long)c.batch * c.n_kv * wblocks;
   if (units > INT32_MAX || join > INT32_MAX) fail(ST_OP, "kv8: dims too large");
   auto fn = c.e4m3 ? part_kernel<HD, true, CG> : part_kernel<HD, false, CG>;
-  hipLaunchKernelGGL(fn, dim3((unsigned)units), dim3(64 * WAVES), 0, st, c, a, p);
+  hipLaunchKernelGGL(fn, grid, dim3(64 * WAVES), 0, st, c, a, p);
   if (join)
     hipLaunchKernelGGL(join_kernel<HD>, dim3((unsigned)join), dim3(256), 0, st, c, a, p, (int)ncol, wblocks);
 }
