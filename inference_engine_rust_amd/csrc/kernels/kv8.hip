@@ -133,20 +133,6 @@ IEK_DEV uint32_t weight_key(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Inclusive prefix sum over the wave's lanes.
-template <int CTRL, int ROWS = 0xF>
-IEK_DEV int dpp_up(int v) {
-  return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
-}
-IEK_DEV int wave_scan(int v) {
-  v += dpp_up<0x111>(v);  // row_shr 1, 2, 4, 8
-  v += dpp_up<0x112>(v);
-  v += dpp_up<0x114>(v);
-  v += dpp_up<0x118>(v);
-  v += dpp_up<DPP_BCAST15, 0xA>(v);
-  return v + dpp_up<DPP_BCAST31, 0xC>(v);
-}
-
 // The bin in which the running sum from the top of `hist` passes `need` (> 0, at most the sum); need
 // becomes what is left of it in that bin. Wave w sums the w-th part of the bins, then every wave looks
 // through the part that holds it (sums: NW ints).

@@ -31,21 +31,78 @@ constexpr int TILE = KV8_BLOCK;
 constexpr int WAVES = 4;
 constexpr int MAX_SPLIT = 256;
 
+// A sequence's tiles are cut into chunks, whole rounds of a workgroup's waves, one workgroup and one
+// partial result each. Up to SHARED_BATCH sequences the chunk's size is found on the device from the
+// lengths themselves (a launch is sized for max_len, and may be a captured one): the total over the
+// sequences by the chunks that fill the chip (half of one a sequence is lost to its last chunk), then
+// each sequence evenly into as many as that takes: a batch of ragged lengths is spread evenly, and a
+// short sequence in a large cache finely (16 sequences up to 8223 keys, cut by max_len 48 us, so 38).
+// Chunk x of a KV head is chunk cp of sequence b by the running sum of
+// their counts; a sequence without entries has one, which writes zeros. Larger batches are cut by max_len.
+constexpr int SHARED_BATCH = 64;
+
 struct Plan {
   int group, cols, cblocks;  // query heads and columns of a KV head, workgroups the columns are spread over
-  int tiles, nsplit;       // tiles a chunk, chunks a sequence at most
-  int spad;                // stored scores a column
-  float* ml;               // [batch * n_kv][cols][nsplit] pairs (m, l)
-  float* o;                // [batch * n_kv][cols][nsplit][hd]
-  float* s;                // [batch * n_kv][cols][spad], base 2, or null
+  int share;                 // chunks of a KV head to aim at; 0: sequences are cut by `tiles`
+  int tiles, nsplit;         // share 0: tiles a chunk, chunks a sequence at most; else the smallest chunk
+  int chunks;                // of a KV head at most
+  bool direct;               // every sequence is one chunk
+  int spad;                  // stored scores a column
+  float* ml;                 // [chunks][n_kv][cols] pairs (m, l)
+  float* o;                  // [chunks][n_kv][cols][hd]
+  float* s;                  // [batch][n_kv][cols][spad], base 2, or null
 };
 
-// The slots that the columns of query token t see, and tile range [t0, t1) that any column sees.
+// The slots that the columns of query token t see, and the tile range [t0, t1) that any column sees.
 IEK_DEV int col_hi(const Kv8Attn& a, int n, int t) { return n - (a.n_q - 1 - t); }
 IEK_DEV int col_lo(const Kv8Attn& a, int hi) { return a.window > 0 ? max(0, hi - a.window) : 0; }
+IEK_DEV int entries(const Kv8Attn& a, int b) { return max(0, min(a.len[b], a.max_len)); }
 IEK_DEV void tile_range(const Kv8Attn& a, int n, int& t0, int& t1) {
   t0 = col_lo(a, max(0, col_hi(a, n, 0))) / TILE;
   t1 = (n + TILE - 1) / TILE;
+}
+
+// Chunk x of a KV head (FIND), or the chunks of sequence b: its entries n, tiles a chunk, number of
+// chunks (0 with FIND: there is no chunk x) and first chunk.
+struct Cut {
+  int b, n, tiles, count, first;
+};
+IEK_DEV int ceil_div(int a, int b) { return (int)(((unsigned)a + b - 1) / (unsigned)b); }
+template <bool FIND>
+IEK_DEV Cut cut(const Kv8& c, const Kv8Attn& a, const Plan& p, int x, int b) {
+  Cut r{b, 0, p.tiles, 0, 0};
+  int t0, t1;
+  if (p.share == 0 || c.batch == 1) {
+    if (FIND) r.b = c.batch == 1 ? 0 : min(x / p.nsplit, c.batch - 1);  // (the grid may be rounded up)
+    r.n = entries(a, r.b);
+    tile_range(a, r.n, t0, t1);
+    if (p.share != 0)
+      r.tiles = max(p.tiles, ceil_div(ceil_div(t1 - t0, min(p.share, MAX_SPLIT)), WAVES) * WAVES);
+    r.count = max(1, ceil_div(t1 - t0, r.tiles));
+    r.first = r.b * p.nsplit;
+    if (FIND && x - r.first >= r.count) r.count = 0;
+    return r;
+  }
+  const int lane = threadIdx.x & 63;
+  const int n = lane < c.batch ? entries(a, lane) : 0;
+  tile_range(a, n, t0, t1);
+  const int each = lane < c.batch ? t1 - t0 : 0;
+  const int total = __builtin_amdgcn_readlane(wave_scan(each), 63);
+  int most = each;
+#pragma unroll
+  for (int o = 32; o; o >>= 1) most = max(most, __shfl_xor(most, o));
+  most = __builtin_amdgcn_readfirstlane(most);
+  const int aim = max(p.share - c.batch / 2, (p.share + 1) / 2);
+  const int size = max(p.tiles, ceil_div(max(ceil_div(total, aim), ceil_div(most, MAX_SPLIT)), WAVES) * WAVES);
+  const int even = max(p.tiles, ceil_div(ceil_div(each, max(1, ceil_div(each, size))), WAVES) * WAVES);
+  const int mine = lane < c.batch ? max(1, ceil_div(each, even)) : 0, upto = wave_scan(mine);
+  if (FIND) r.b = __popcll(__ballot(lane < c.batch && upto - mine <= x)) - 1;
+  r.n = __builtin_amdgcn_readlane(n, r.b);
+  r.tiles = __builtin_amdgcn_readlane(even, r.b);
+  r.count = __builtin_amdgcn_readlane(mine, r.b);
+  r.first = __builtin_amdgcn_readlane(upto, r.b) - r.count;
+  if (FIND && x - r.first >= r.count) r.count = 0;
+  return r;
 }
 
 // v over the wave's four groups of 16 lanes
@@ -146,26 +203,33 @@ __global__ __launch_bounds__(64 * WAVES, HD * CG <= 256 ? 2 : 1) void part_kerne
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kg = lane >> 4, c8 = lane & 7;
   const bool lo_half = lane & 8;
-  // several workgroups for a chunk's columns: on one XCD (consecutive ones go to the eight XCDs in turn)
-  int cp = blockIdx.x, h = blockIdx.y, b = blockIdx.z, cb = 0;
-  if (p.cblocks > 1) {
-    const int slot = blockIdx.x >> 3, unit = (slot / p.cblocks) * 8 + (blockIdx.x & 7);
-    cb = slot % p.cblocks;
-    cp = unit % p.nsplit;
-    h = unit / p.nsplit;
-    b = h / c.n_kv;
-    h -= b * c.n_kv;
-    if (b >= c.batch) return;
+  // The chunks that do not exist are the last workgroups, so that the others spread evenly over the CUs (between
+  // them they left some with three and some with one: 16 x 4096 keys of 8 heads 34 us instead of 29).
+  int h = blockIdx.x, x = blockIdx.y, cb = 0;
+  if (p.cblocks > 1) {  // the workgroups of a chunk's columns on one XCD: consecutive ones go to the eight in turn
+    const int unit = (h >> 3) / p.cblocks * 8 + (h & 7);
+    cb = (h >> 3) % p.cblocks;
+    x = unit / c.n_kv;
+    h = unit - x * c.n_kv;
   }
-  const int bh = b * c.n_kv + h, G = p.group;
-  const int n = max(0, min(a.len[b], a.max_len));
+  const Cut ct = cut<true>(c, a, p, x, 0);
+  const int b = ct.b, n = ct.n, bh = b * c.n_kv + h, G = p.group;
+  // this lane's columns, and its part of their q: dims 64 i + 16 kg + [0, 16) as steps 2 i and 2 i + 1
+  f4_t qr[CG][HD / 16];
+#pragma unroll
+  for (int u = 0; u < CG; ++u) {
+    const int cc = min((cb * CG + u) * 8 + c8, p.cols - 1), t = a.n_q == 1 ? 0 : cc / G;
+    const float* row = a.q + ((size_t)b * a.n_q + t) * a.q_stride + (size_t)(h * G + cc - t * G) * HD + 16 * kg;
+#pragma unroll
+    for (int i = 0; i < HD / 64; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) qr[u][4 * i + e] = *reinterpret_cast<const f4_t*>(row + 64 * i + 4 * e);
+  }
+  if (ct.count == 0) return;  // uniform
   int t0, t1;
   tile_range(a, n, t0, t1);
-  const int live = (t1 - t0 + p.tiles - 1) / p.tiles;
-  const bool direct = p.nsplit == 1;
-  if (cp >= live && !(direct && live <= 0)) return;  // (an empty sequence's only chunk writes zeros)
-  t0 += cp * p.tiles;
-  t1 = min(t1, t0 + p.tiles);
+  t0 += (x - ct.first) * ct.tiles;
+  t1 = min(t1, t0 + ct.tiles);
   const uint8_t* K = c.k + (size_t)bh * c.cap * HD;
   const uint8_t* V = c.v + (size_t)bh * c.cap * HD;
   const float* KS = c.ks + (size_t)bh * c.nblk;
@@ -176,43 +240,32 @@ __global__ __launch_bounds__(64 * WAVES, HD * CG <= 256 ? 2 : 1) void part_kerne
     load_k(T, K, KS, tile, n, lane);
     load_v(T, V, VS, tile, n, lane);
   }
-  // this lane's columns and its part of their q: dims 64 i + 16 kg + [0, 16) as steps 2 i and 2 i + 1
   u4_t q[CG][NS];
   float qs[CG];
   int hi[CG], lo[CG];
   int lo_max = 0, hi_min = n;
 #pragma unroll
   for (int u = 0; u < CG; ++u) {
-    const int col = (cb * CG + u) * 8 + c8;
-    const int cc = min(col, p.cols - 1), t = a.n_q == 1 ? 0 : cc / G;
-    hi[u] = col_hi(a, n, t);
+    const int cc = min((cb * CG + u) * 8 + c8, p.cols - 1);
+    hi[u] = col_hi(a, n, a.n_q == 1 ? 0 : cc / G);
     lo[u] = col_lo(a, hi[u]);
-    const float* row = a.q + ((size_t)b * a.n_q + t) * a.q_stride + (size_t)(h * G + cc - t * G) * HD + 16 * kg;
-    float x[HD / 4];
     float top = 0.f;
 #pragma unroll
-    for (int i = 0; i < HD / 64; ++i)
+    for (int i = 0; i < HD / 16; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const f4_t v = *reinterpret_cast<const f4_t*>(row + 64 * i + 4 * e);
-#pragma unroll
-        for (int f = 0; f < 4; ++f) {
-          x[16 * i + 4 * e + f] = v[f];
-          top = fmaxf(top, fabsf(v[f]));
-        }
-      }
+      for (int f = 0; f < 4; ++f) top = fmaxf(top, fabsf(qr[u][i][f]));
     top = groups_max(top);
     // into [2^13, 2^14) by a power of two (an infinity or NaN, or a row of zeros, stays what it is)
     int ex = (int)(__float_as_uint(top) >> 23) - 127;
-    ex = ex == 128 ? 0 : max(13 - ex, -127 + 13);
-    ex = min(ex, 126);
+    ex = ex == 128 ? 0 : min(13 - ex, 126);
     const float up = __builtin_amdgcn_ldexpf(1.f, ex);
     qs[u] = __builtin_amdgcn_ldexpf(a.scale * 1.44269504088896340736f, -ex);
 #pragma unroll
     for (int i = 0; i < NS; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float y0 = x[8 * i + 2 * e] * up, y1 = x[8 * i + 2 * e + 1] * up;
+        const f4_t v = qr[u][2 * i + (e >> 1)];
+        const float y0 = v[2 * (e & 1)] * up, y1 = v[2 * (e & 1) + 1] * up;
         const h2_t w = {(_Float16)y0, (_Float16)y1};
         const h2_t z = {(_Float16)(y0 - (float)w[0]), (_Float16)(y1 - (float)w[1])};
         q[u][i][e] = __builtin_bit_cast(uint32_t, lo_half ? z : w);
@@ -376,17 +429,17 @@ __global__ __launch_bounds__(64 * WAVES, HD * CG <= 256 ? 2 : 1) void part_kerne
 #pragma unroll
       for (int w = 0; w < WAVES; ++w)
         ll += sl[w][8 * u + col] * (sm[w][8 * u + col] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(sm[w][8 * u + col] - mm));
-      const size_t row = (size_t)bh * p.cols + c0 + col;
-      if (direct) {
+      const size_t row = ((size_t)x * c.n_kv + h) * p.cols + c0 + col;
+      if (p.direct) {
         const int t = (c0 + col) / G, g = (c0 + col) - t * G;
         float* out = a.out + (((size_t)b * a.n_q + t) * a.n_heads + h * G + g) * HD + dim;
         *reinterpret_cast<f4_t*>(out) = ll == 0.f ? f4_t{0.f, 0.f, 0.f, 0.f} : y / ll;
       } else {
-        *reinterpret_cast<f4_t*>(p.o + (row * p.nsplit + cp) * HD + dim) = y;
+        *reinterpret_cast<f4_t*>(p.o + row * HD + dim) = y;
       }
       if (dim == 0) {
-        p.ml[2 * (row * p.nsplit + cp)] = isnan(ll) ? ll : mm;  // (a NaN: the maxima pass it over)
-        p.ml[2 * (row * p.nsplit + cp) + 1] = ll;
+        p.ml[2 * row] = isnan(ll) ? ll : mm;  // (a NaN: the maxima pass it over)
+        p.ml[2 * row + 1] = ll;
       }
     }
   }
@@ -403,15 +456,23 @@ __global__ __launch_bounds__(256) void join_kernel(Kv8 c, Kv8Attn a, Plan p, int
     __shared__ float red[2][4];
     __shared__ __align__(16) float acc[GRP][HD];
     const int bh = blockIdx.x / p.cols, col = blockIdx.x - bh * p.cols, b = bh / c.n_kv, h = bh - b * c.n_kv;
-    const int n = max(0, min(a.len[b], a.max_len));
-    int t0, t1;
-    tile_range(a, n, t0, t1);
-    const int live = (t1 - t0 + p.tiles - 1) / p.tiles;
-    const size_t row = (size_t)blockIdx.x * p.nsplit;
+    // of a single sequence the first parts, without waiting for its length
+    constexpr int PRE = 4;
+    const size_t step = (size_t)c.n_kv * p.cols;
+    const int g = t / TPR, d = 4 * (t % TPR);
+    f4_t pre[PRE];
+    if (c.batch == 1) {
+#pragma unroll
+      for (int k = 0; k < PRE; ++k)
+        pre[k] = *reinterpret_cast<const f4_t*>(p.o + (min(g + GRP * k, p.chunks - 1) * step + blockIdx.x) * HD + d);
+    }
+    const Cut ct = cut<false>(c, a, p, 0, b);
+    const int live = ct.count;
+    const size_t row = (size_t)ct.first * step + (size_t)h * p.cols + col;
     float m = -INFINITY, l = 0.f;
     if (t < live) {
-      m = p.ml[2 * (row + t)];
-      l = p.ml[2 * (row + t) + 1];
+      m = p.ml[2 * (row + t * step)];
+      l = p.ml[2 * (row + t * step) + 1];
     }
     float top = wave_max(m);
     if (lane == 0) red[0][wave] = top;
@@ -423,10 +484,15 @@ __global__ __launch_bounds__(256) void join_kernel(Kv8 c, Kv8Attn a, Plan p, int
     if (lane == 0) red[1][wave] = l;
     __syncthreads();
     l = red[1][0] + red[1][1] + red[1][2] + red[1][3];
-    const int g = t / TPR, d = 4 * (t % TPR);
     f4_t y = {0.f, 0.f, 0.f, 0.f};
+    int i0 = g;
+    if (c.batch == 1) {
+#pragma unroll
+      for (int k = 0; k < PRE; ++k, i0 += GRP)
+        if (i0 < live) y += pre[k] * w[i0];
+    }
 #pragma unroll 4
-    for (int i = g; i < live; i += GRP) y += *reinterpret_cast<const f4_t*>(p.o + (row + i) * HD + d) * w[i];
+    for (int i = i0; i < live; i += GRP) y += *reinterpret_cast<const f4_t*>(p.o + (row + i * step) * HD + d) * w[i];
     *reinterpret_cast<f4_t*>(&acc[g][d]) = y;
     __syncthreads();
     if (t < TPR) {
@@ -440,42 +506,69 @@ __global__ __launch_bounds__(256) void join_kernel(Kv8 c, Kv8Attn a, Plan p, int
   }
   constexpr int COLS = 64 * 8;  // n_q <= 64, groups of at most 8
   __shared__ float cm[COLS], cl[COLS];
-  const int id = blockIdx.x - ncol, bh = id / wblocks, b = bh / c.n_kv;
-  const int n = max(0, min(a.len[b], a.max_len));
+  const int id = blockIdx.x - ncol, bh = id / wblocks, b = bh / c.n_kv, h = bh - b * c.n_kv;
   const int j = (id - bh * wblocks) * 1024 + 4 * t;
+  // what does not wait for the lengths: the first columns' scores (`spad` of them are there) and the old sums
+  constexpr int PRE = 8;
+  const float* s = p.s + (size_t)bh * p.cols * p.spad + min(j, p.spad - 4);
+  const size_t at = (size_t)bh * c.cap + j;
+  f4_t v[PRE], w = {0.f, 0.f, 0.f, 0.f}, old = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int col = 0; col < PRE; ++col) v[col] = *reinterpret_cast<const f4_t*>(s + (size_t)min(col, p.cols - 1) * p.spad);
+  if (a.w_in) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (j + i < a.max_len) old[i] = a.w_in[at + i];
+  }
+  const Cut ct = cut<false>(c, a, p, 0, b);
+  const int n = ct.n;
   if (j - 4 * t >= n) return;  // uniform
   int t0, t1;
   tile_range(a, n, t0, t1);
-  const int live = (t1 - t0 + p.tiles - 1) / p.tiles;
+  const size_t step = (size_t)c.n_kv * p.cols;
   for (int col = wave; col < p.cols; col += 4) {
-    const float* ml = p.ml + ((size_t)bh * p.cols + col) * p.nsplit * 2;
-    float m = -INFINITY;
-    for (int i = lane; i < live; i += 64) m = fmaxf(m, ml[2 * i]);
-    m = wave_max(m);
-    float l = 0.f;
-    for (int i = lane; i < live; i += 64) l += ml[2 * i] == -INFINITY ? 0.f : ml[2 * i + 1] * __builtin_amdgcn_exp2f(ml[2 * i] - m);
-    l = wave_sum(l);
+    const float* ml = p.ml + 2 * ((size_t)ct.first * step + (size_t)h * p.cols + col);
+    float m[MAX_SPLIT / 64], l[MAX_SPLIT / 64], top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < MAX_SPLIT / 64; ++i) {
+      const int k = lane + 64 * i;
+      m[i] = -INFINITY;
+      l[i] = 0.f;
+      if (64 * i < ct.count && k < ct.count) {
+        m[i] = ml[2 * k * step];
+        l[i] = ml[2 * k * step + 1];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < MAX_SPLIT / 64; ++i) top = fmaxf(top, m[i]);
+    top = wave_max(top);
+#pragma unroll
+    for (int i = 0; i < MAX_SPLIT / 64; ++i) sum += m[i] == -INFINITY ? 0.f : l[i] * __builtin_amdgcn_exp2f(m[i] - top);
+    sum = wave_sum(sum);
     if (lane == 0) {
-      cm[col] = m == -INFINITY ? 0.f : m;  // (a column that sees nothing has only scores of -inf)
-      cl[col] = l == 0.f ? 0.f : 1.f / l;
+      cm[col] = top == -INFINITY ? 0.f : top;  // (a column that sees nothing has only scores of -inf)
+      cl[col] = sum == 0.f ? 0.f : 1.f / sum;
     }
   }
   __syncthreads();
   if (j >= n) return;
-  f4_t w = {0.f, 0.f, 0.f, 0.f};
   if (j >= t0 * TILE) {
-    const float* s = p.s + (size_t)bh * p.cols * p.spad + j;
-#pragma unroll 4
-    for (int col = 0; col < p.cols; ++col) {
-      const f4_t v = *reinterpret_cast<const f4_t*>(s + (size_t)col * p.spad);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] += __builtin_amdgcn_exp2f(v[i] - cm[col]) * cl[col];
+    for (int col = 0; col < PRE; ++col) {
+      if (col >= p.cols) break;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] += __builtin_amdgcn_exp2f(v[col][i] - cm[col]) * cl[col];
+    }
+#pragma unroll 4
+    for (int col = PRE; col < p.cols; ++col) {
+      const f4_t z = *reinterpret_cast<const f4_t*>(s + (size_t)col * p.spad);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] += __builtin_amdgcn_exp2f(z[i] - cm[col]) * cl[col];
     }
   }
-  const size_t at = (size_t)bh * c.cap + j;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    if (j + i < n) a.w_out[at + i] = (a.w_in ? a.w_in[at + i] : 0.f) + w[i];
+    if (j + i < n) a.w_out[at + i] = old[i] + w[i];
 }
 
 size_t up256(size_t x) { return (x + 255) / 256 * 256; }
@@ -484,48 +577,51 @@ size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 // leave room for two waves a SIMD (head_dim up to 256).
 int col_groups(int cols, int hd) { return cols > 8 && hd <= 256 ? 2 : 1; }
 
-// What the plan and the workspace's size share: the chunks that a sequence is cut into at most.
-int most_chunks(const Kv8& c, int cblocks) {
-  const long long units = std::max<long long>(1, (long long)c.batch * c.n_kv * cblocks);
-  return (int)std::max<long long>(1, std::min<long long>(MAX_SPLIT, 1024 / units));
+// The plan for sequences whose columns see at most `tiles` tiles; more of them never need less.
+Plan make_plan(const Kv8& c, int n_heads, int n_q, int tiles) {
+  Plan p{};
+  p.group = n_heads / c.n_kv;
+  p.cols = p.group * n_q;
+  const int cg = col_groups(p.cols, c.hd), per = 8 * cg;
+  p.cblocks = (p.cols + per - 1) / per;
+  // Chunks that fill the chip once: two workgroups a CU, one where the accumulators leave a wave a SIMD. Up to
+  // eight tiles a second round of the waves costs less than the joining of two chunks.
+  const int target = c.hd * cg <= 256 ? 512 : 256;
+  p.tiles = tiles <= 2 * WAVES ? 2 * WAVES : WAVES;
+  p.direct = tiles <= p.tiles;
+  if (c.batch <= SHARED_BATCH) {
+    p.share = std::max(1, target / (c.n_kv * p.cblocks));
+    p.nsplit = 0;
+    // (sum of ceil(tiles / size) <= total / size + batch, size >= total / share)
+    p.chunks = (int)std::min<long long>(p.share + c.batch, (long long)c.batch * std::max(1, (tiles + p.tiles - 1) / p.tiles));
+  } else {
+    const long long units = (long long)c.batch * c.n_kv * p.cblocks;
+    const int want = (int)std::max<long long>(1, std::min<long long>(MAX_SPLIT, 2 * target / units));
+    p.nsplit = std::max(1, std::min(want, (tiles + p.tiles - 1) / p.tiles));
+    p.tiles = std::max(p.tiles, ((tiles + p.nsplit - 1) / p.nsplit + WAVES - 1) / WAVES * WAVES);
+    p.chunks = c.batch * p.nsplit;
+    p.direct = p.nsplit == 1;
+  }
+  return p;
 }
 
 struct Sizes {
   size_t ml, o, s;
 };
-Sizes sizes(const Kv8& c, int cols, int nsplit, int spad, bool weights) {
-  const size_t rows = (size_t)c.batch * c.n_kv * cols;
-  return {up256(rows * nsplit * 8), nsplit > 1 ? up256(rows * nsplit * c.hd * 4) : 0, weights ? up256(rows * spad * 4) : 0};
-}
-
-Plan make_plan(const Kv8& c, const Kv8Attn& a, void* ws) {
-  Plan p{};
-  p.group = a.n_heads / c.n_kv;
-  p.cols = p.group * a.n_q;
-  const int per = 8 * col_groups(p.cols, c.hd);
-  p.cblocks = (p.cols + per - 1) / per;
-  // the tiles that a sequence's columns see at most, as chunks of whole rounds of the waves
-  const long long span = a.window > 0 ? std::min<long long>(a.max_len, (long long)a.window + a.n_q + TILE - 2) : a.max_len;
-  const int tiles = (int)((span + TILE - 1) / TILE), want = most_chunks(c, p.cblocks);
-  p.tiles = std::max(1, ((tiles + want - 1) / want + WAVES - 1) / WAVES) * WAVES;
-  p.nsplit = std::max(1, (tiles + p.tiles - 1) / p.tiles);
-  p.spad = (a.max_len + TILE - 1) / TILE * TILE;
-  const Sizes z = sizes(c, p.cols, p.nsplit, p.spad, a.w_out != nullptr);
-  char* base = static_cast<char*>(ws);
-  p.ml = reinterpret_cast<float*>(base);
-  p.o = reinterpret_cast<float*>(base + z.ml);
-  p.s = a.w_out ? reinterpret_cast<float*>(base + z.ml + z.o) : nullptr;
-  return p;
+Sizes sizes(const Kv8& c, const Plan& p, int spad, bool weights) {
+  const size_t rows = (size_t)p.chunks * c.n_kv * p.cols;
+  return {up256(rows * 8), p.direct ? 0 : up256(rows * c.hd * 4),
+          weights ? up256((size_t)c.batch * c.n_kv * p.cols * spad * 4) : 0};
 }
 
 template <int HD, int CG>
 void launch_cg(const Kv8& c, const Kv8Attn& a, const Plan& p, hipStream_t st) {
-  const long long units = p.cblocks == 1 ? p.nsplit : ((long long)c.batch * c.n_kv * p.nsplit + 7) / 8 * 8 * p.cblocks;
-  const dim3 grid = p.cblocks == 1 ? dim3((unsigned)units, (unsigned)c.n_kv, (unsigned)c.batch) : dim3((unsigned)units);
-  const long long ncol = p.nsplit > 1 ? (long long)c.batch * c.n_kv * p.cols : 0;
+  const long long part = ((long long)p.chunks * c.n_kv + 7) / 8 * 8 * p.cblocks;
+  const dim3 grid = p.cblocks == 1 ? dim3((unsigned)c.n_kv, (unsigned)p.chunks) : dim3((unsigned)part);
+  const long long ncol = p.direct ? 0 : (long long)c.batch * c.n_kv * p.cols;
   const int wblocks = a.w_out ? (a.max_len + 1023) / 1024 : 0;
   const long long join = ncol + (long long)c.batch * c.n_kv * wblocks;
-  if (units > INT32_MAX || join > INT32_MAX) fail(ST_OP, "kv8: dims too large");
+  if (part > INT32_MAX || join > INT32_MAX) fail(ST_OP, "kv8: dims too large");
   auto fn = c.e4m3 ? part_kernel<HD, true, CG> : part_kernel<HD, false, CG>;
   hipLaunchKernelGGL(fn, grid, dim3(64 * WAVES), 0, st, c, a, p);
   if (join)
@@ -534,16 +630,24 @@ void launch_cg(const Kv8& c, const Kv8Attn& a, const Plan& p, hipStream_t st) {
 
 }  // namespace
 
-// For any window: whatever its chunks, there are at most most_chunks of at least WAVES tiles.
+// For any window: fewer tiles do not take more chunks.
 size_t kv8_attention_workspace(const Kv8& c, int n_heads, int n_q, int max_len, bool weights) {
-  const int cols = n_heads / c.n_kv * n_q, per = 8 * col_groups(cols, c.hd), spad = (max_len + TILE - 1) / TILE * TILE;
-  const int rounds = (spad / TILE + WAVES - 1) / WAVES;
-  const Sizes z = sizes(c, cols, std::max(1, std::min(rounds, most_chunks(c, (cols + per - 1) / per))), spad, weights);
+  const int tiles = (max_len + TILE - 1) / TILE;
+  Plan p = make_plan(c, n_heads, n_q, tiles);
+  const Sizes z = sizes(c, p, tiles * TILE, weights);
   return z.ml + z.o + z.s;
 }
 
 void launch_kv8_attention(const Kv8& c, const Kv8Attn& a, void* ws, hipStream_t st) {
-  const Plan p = make_plan(c, a, ws);
+  // the slots that a sequence's columns see at most, wherever they begin in their tile
+  const long long span = a.window > 0 ? std::min<long long>(a.max_len, (long long)a.window + a.n_q + TILE - 2) : a.max_len;
+  Plan p = make_plan(c, a.n_heads, a.n_q, (int)((span + TILE - 1) / TILE));
+  p.spad = (a.max_len + TILE - 1) / TILE * TILE;
+  const Sizes z = sizes(c, p, p.spad, a.w_out != nullptr);
+  char* base = static_cast<char*>(ws);
+  p.ml = reinterpret_cast<float*>(base);
+  p.o = reinterpret_cast<float*>(base + z.ml);
+  p.s = a.w_out ? reinterpret_cast<float*>(base + z.ml + z.o) : nullptr;
   const bool two = col_groups(p.cols, c.hd) == 2;
   switch (c.hd) {
     case 64: two ? launch_cg<64, 2>(c, a, p, st) : launch_cg<64, 1>(c, a, p, st); break;

@@ -1,10 +1,24 @@
-// Codes and scales of the 8-bit KV cache: int8 (-127 .. 127) or e4m3 (|value| <= 448, finite).
+// Codes and scales of the 8-bit KV cache: int8 (-127 .. 127) or e4m3 (|value| <= 448, finite); a wave's prefix sum.
 #pragma once
 #include "common.cuh"
 
 namespace iek {
 
 IEK_DEV uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
+
+// Inclusive prefix sum over the wave's lanes.
+template <int CTRL, int ROWS = 0xF>
+IEK_DEV int dpp_up(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
+}
+IEK_DEV int wave_scan(int v) {
+  v += dpp_up<0x111>(v);  // row_shr 1, 2, 4, 8
+  v += dpp_up<0x112>(v);
+  v += dpp_up<0x114>(v);
+  v += dpp_up<0x118>(v);
+  v += dpp_up<DPP_BCAST15, 0xA>(v);
+  return v + dpp_up<DPP_BCAST31, 0xC>(v);
+}
 
 // The smallest power of two s >= 2^-100 with amax <= M * s (M = 127 or 448) for the bits of a
 // non-negative amax; NaN for infinities and NaN. With amax = (1 + f) 2^x: M = (1 + F) 2^X, so

@@ -265,6 +265,13 @@ def test_attention_long(gpu, dtype, hd, kv, group):
     check_attention(5, dtype, kv, group, hd, 1, [20011, 9000], 0)
 
 
+@pytest.mark.parametrize("batch", [63, 64, 65, 200])
+@pytest.mark.parametrize("hd,kv,group,n_q,window", [(64, 1, 8, 1, 0), (64, 2, 8, 3, 0), (128, 1, 2, 1, 300)])
+def test_attention_many_sequences(gpu, batch, hd, kv, group, n_q, window):
+    lens = [(37 * i * i + 5) % 1200 if i % 7 else 0 for i in range(batch)]
+    check_attention(batch, "e4m3", kv, group, hd, n_q, lens, window)
+
+
 def test_attention_max_len_beyond_and_below_the_lengths(gpu):
     check_attention(6, "i8", 2, 4, 128, 1, [40, 700], 0, cap=3000, max_len=3000)
     # lengths above max_len count as max_len
