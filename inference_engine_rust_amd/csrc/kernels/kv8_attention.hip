@@ -31,6 +31,13 @@ constexpr int TILE = KV8_BLOCK;
 constexpr int WAVES = 4;
 constexpr int MAX_SPLIT = 256;
 
+// A wave takes DIMS of a row: up to head_dim 128 all of them, and the four waves four tiles at a time;
+// of wider rows two or four waves take 128 each of one tile, so that a tile's work, and the registers of q
+// and o, are no larger (one wave a row had 256 accumulators and more at 512: 8223 keys of one KV head
+// 26 us, so TODO).
+constexpr int dims_of(int hd) { return hd < 128 ? hd : 128; }
+constexpr int tile_waves(int hd) { return WAVES * dims_of(hd) / hd; }
+
 // A sequence's tiles are cut into chunks, whole rounds of a workgroup's waves, one workgroup and one
 // partial result each. Up to SHARED_BATCH sequences the chunk's size is found on the device from the
 // lengths themselves (a launch is sized for max_len, and may be a captured one): the total over the
@@ -68,8 +75,9 @@ struct Cut {
   int b, n, tiles, count, first;
 };
 IEK_DEV int ceil_div(int a, int b) { return (int)(((unsigned)a + b - 1) / (unsigned)b); }
-template <bool FIND>
+template <bool FIND, int HD>
 IEK_DEV Cut cut(const Kv8& c, const Kv8Attn& a, const Plan& p, int x, int b) {
+  constexpr int TW = tile_waves(HD);
   Cut r{b, 0, p.tiles, 0, 0};
   int t0, t1;
   if (p.share == 0 || c.batch == 1) {
@@ -77,7 +85,7 @@ IEK_DEV Cut cut(const Kv8& c, const Kv8Attn& a, const Plan& p, int x, int b) {
     r.n = entries(a, r.b);
     tile_range(a, r.n, t0, t1);
     if (p.share != 0)
-      r.tiles = max(p.tiles, ceil_div(ceil_div(t1 - t0, min(p.share, MAX_SPLIT)), WAVES) * WAVES);
+      r.tiles = max(p.tiles, ceil_div(ceil_div(t1 - t0, min(p.share, MAX_SPLIT)), TW) * TW);
     r.count = max(1, ceil_div(t1 - t0, r.tiles));
     r.first = r.b * p.nsplit;
     if (FIND && x - r.first >= r.count) r.count = 0;
@@ -93,8 +101,8 @@ IEK_DEV Cut cut(const Kv8& c, const Kv8Attn& a, const Plan& p, int x, int b) {
   for (int o = 32; o; o >>= 1) most = max(most, __shfl_xor(most, o));
   most = __builtin_amdgcn_readfirstlane(most);
   const int aim = max(p.share - c.batch / 2, (p.share + 1) / 2);
-  const int size = max(p.tiles, ceil_div(max(ceil_div(total, aim), ceil_div(most, MAX_SPLIT)), WAVES) * WAVES);
-  const int even = max(p.tiles, ceil_div(ceil_div(each, max(1, ceil_div(each, size))), WAVES) * WAVES);
+  const int size = max(p.tiles, ceil_div(max(ceil_div(total, aim), ceil_div(most, MAX_SPLIT)), TW) * TW);
+  const int even = max(p.tiles, ceil_div(ceil_div(each, max(1, ceil_div(each, size))), TW) * TW);
   const int mine = lane < c.batch ? max(1, ceil_div(each, even)) : 0, upto = wave_scan(mine);
   if (FIND) r.b = __popcll(__ballot(lane < c.batch && upto - mine <= x)) - 1;
   r.n = __builtin_amdgcn_readlane(n, r.b);
@@ -140,10 +148,11 @@ IEK_DEV f4_t mfma(u4_t a, u4_t b, f4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, a), __builtin_bit_cast(h8_t, b), c, 0, 0, 0);
 }
 
-// Raw bytes of a tile: K, two sets of 16 rows, 16 bytes per 64 dims; V, eight rows of hd / 16 bytes.
-template <int HD>
+// Raw bytes of a wave's part of a tile: K, two sets of 16 rows, 16 bytes per 64 dims; V, eight rows of
+// DIMS / 16 bytes.
+template <int DIMS>
 struct Tile {
-  static constexpr int KC = HD / 64, VW = HD / 64;  // 16-byte pieces of K a row, dwords of V a row
+  static constexpr int KC = DIMS / 64, VW = DIMS / 64;  // 16-byte pieces of K a row, dwords of V a row
   u4_t k[2][KC];
   uint32_t v[8][VW];
   float ks, vs;
@@ -157,52 +166,49 @@ IEK_DEV __amdgpu_buffer_rsrc_t tile_rsrc(const uint8_t* codes, int tile, int n) 
                                            min(TILE, n - tile * TILE) * HD, 0x00020000);
 }
 
-template <int HD>
-IEK_DEV void load_k(Tile<HD>& T, const uint8_t* codes, const float* ks, int tile, int n, int lane) {
+// (dim0: the wave's first dim)
+template <int HD, int DIMS>
+IEK_DEV void load_k(Tile<DIMS>& T, const uint8_t* codes, const float* ks, int tile, int n, int dim0, int lane) {
   const auto rs = tile_rsrc<HD>(codes, tile, n);
 #pragma unroll
   for (int s = 0; s < 2; ++s)
 #pragma unroll
-    for (int i = 0; i < Tile<HD>::KC; ++i)
-      T.k[s][i] = __builtin_amdgcn_raw_buffer_load_b128(rs, (lane & 15) * HD + 16 * (lane >> 4), 16 * s * HD + 64 * i, 0);
+    for (int i = 0; i < Tile<DIMS>::KC; ++i)
+      T.k[s][i] = __builtin_amdgcn_raw_buffer_load_b128(rs, (lane & 15) * HD + 16 * (lane >> 4), dim0 + 16 * s * HD + 64 * i, 0);
   T.ks = ks[tile];
 }
 
-template <int HD>
-IEK_DEV void load_v(Tile<HD>& T, const uint8_t* codes, const float* vs, int tile, int n, int lane) {
-  constexpr int VW = Tile<HD>::VW;
+template <int HD, int DIMS>
+IEK_DEV void load_v(Tile<DIMS>& T, const uint8_t* codes, const float* vs, int tile, int n, int dim0, int lane) {
+  constexpr int VW = Tile<DIMS>::VW;
+  static_assert(VW == 1 || VW == 2, "dims of a lane");
   const auto rs = tile_rsrc<HD>(codes, tile, n);
-  const int off = 4 * (lane >> 4) * HD + (HD / 16) * (lane & 15);
+  const int off = 4 * (lane >> 4) * HD + (DIMS / 16) * (lane & 15);
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const int row = (16 * (j >> 2) + (j & 3)) * HD;
+    const int row = dim0 + (16 * (j >> 2) + (j & 3)) * HD;
     if constexpr (VW == 1) {
       T.v[j][0] = __builtin_amdgcn_raw_buffer_load_b32(rs, off, row, 0);
-    } else if constexpr (VW == 2) {
+    } else {
       const auto x = __builtin_amdgcn_raw_buffer_load_b64(rs, off, row, 0);
       T.v[j][0] = x[0];
       T.v[j][1] = x[1];
-    } else {
-#pragma unroll
-      for (int i = 0; i < VW / 4; ++i) {
-        const auto x = __builtin_amdgcn_raw_buffer_load_b128(rs, off, row + 16 * i, 0);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) T.v[j][4 * i + e] = x[e];
-      }
     }
   }
   T.vs = vs[tile];
 }
 
-// One workgroup: CG * 8 columns of a KV head over a chunk, its waves every fourth tile.
+// One workgroup: CG * 8 columns of a KV head over a chunk.
 template <int HD, bool E4M3, int CG>
-__global__ __launch_bounds__(64 * WAVES, HD * CG <= 256 ? 2 : 1) void part_kernel(Kv8 c, Kv8Attn a, Plan p) {
-  constexpr int NS = HD / 32;   // steps of the first product
-  constexpr int ND = HD / 16;   // dims of a lane in the second: (HD / 16) r + i of row r
-  constexpr int VW = Tile<HD>::VW;
+__global__ __launch_bounds__(64 * WAVES, 2) void part_kernel(Kv8 c, Kv8Attn a, Plan p) {
+  constexpr int DIMS = dims_of(HD), TW = tile_waves(HD), DW = WAVES / TW;
+  constexpr int NS = DIMS / 32;  // steps of the first product
+  constexpr int ND = DIMS / 16;  // dims of a lane in the second: ND r + i of row r
+  constexpr int VW = Tile<DIMS>::VW;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kg = lane >> 4, c8 = lane & 7;
   const bool lo_half = lane & 8;
+  const int tw = wave / DW, dim0 = (wave % DW) * DIMS;
   // The chunks that do not exist are the last workgroups, so that the others spread evenly over the CUs (between
   // them they left some with three and some with one: 16 x 4096 keys of 8 heads 34 us instead of 29).
   int h = blockIdx.x, x = blockIdx.y, cb = 0;
@@ -212,16 +218,16 @@ __global__ __launch_bounds__(64 * WAVES, HD * CG <= 256 ? 2 : 1) void part_kerne
     x = unit / c.n_kv;
     h = unit - x * c.n_kv;
   }
-  const Cut ct = cut<true>(c, a, p, x, 0);
+  const Cut ct = cut<true, HD>(c, a, p, x, 0);
   const int b = ct.b, n = ct.n, bh = b * c.n_kv + h, G = p.group;
   // this lane's columns, and its part of their q: dims 64 i + 16 kg + [0, 16) as steps 2 i and 2 i + 1
-  f4_t qr[CG][HD / 16];
+  f4_t qr[CG][DIMS / 16];
 #pragma unroll
   for (int u = 0; u < CG; ++u) {
     const int cc = min((cb * CG + u) * 8 + c8, p.cols - 1), t = a.n_q == 1 ? 0 : cc / G;
-    const float* row = a.q + ((size_t)b * a.n_q + t) * a.q_stride + (size_t)(h * G + cc - t * G) * HD + 16 * kg;
+    const float* row = a.q + ((size_t)b * a.n_q + t) * a.q_stride + (size_t)(h * G + cc - t * G) * HD + dim0 + 16 * kg;
 #pragma unroll
-    for (int i = 0; i < HD / 64; ++i)
+    for (int i = 0; i < DIMS / 64; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) qr[u][4 * i + e] = *reinterpret_cast<const f4_t*>(row + 64 * i + 4 * e);
   }
@@ -234,13 +240,14 @@ __global__ __launch_bounds__(64 * WAVES, HD * CG <= 256 ? 2 : 1) void part_kerne
   const uint8_t* V = c.v + (size_t)bh * c.cap * HD;
   const float* KS = c.ks + (size_t)bh * c.nblk;
   const float* VS = c.vs + (size_t)bh * c.nblk;
-  Tile<HD> T;
-  int tile = t0 + wave;
+  Tile<DIMS> T;
+  int tile = t0 + tw;
   if (tile < t1) {
-    load_k(T, K, KS, tile, n, lane);
-    load_v(T, V, VS, tile, n, lane);
+    load_k<HD>(T, K, KS, tile, n, dim0, lane);
+    load_v<HD>(T, V, VS, tile, n, dim0, lane);
   }
   u4_t q[CG][NS];
+  const float less = lo_half ? -1.f : 0.f;
   float qs[CG];
   int hi[CG], lo[CG];
   int lo_max = 0, hi_min = n;
@@ -251,7 +258,7 @@ __global__ __launch_bounds__(64 * WAVES, HD * CG <= 256 ? 2 : 1) void part_kerne
     lo[u] = col_lo(a, hi[u]);
     float top = 0.f;
 #pragma unroll
-    for (int i = 0; i < HD / 16; ++i)
+    for (int i = 0; i < DIMS / 16; ++i)
 #pragma unroll
       for (int f = 0; f < 4; ++f) top = fmaxf(top, fabsf(qr[u][i][f]));
     top = groups_max(top);
@@ -266,9 +273,9 @@ __global__ __launch_bounds__(64 * WAVES, HD * CG <= 256 ? 2 : 1) void part_kerne
       for (int e = 0; e < 4; ++e) {
         const f4_t v = qr[u][2 * i + (e >> 1)];
         const float y0 = v[2 * (e & 1)] * up, y1 = v[2 * (e & 1) + 1] * up;
-        const h2_t w = {(_Float16)y0, (_Float16)y1};
-        const h2_t z = {(_Float16)(y0 - (float)w[0]), (_Float16)(y1 - (float)w[1])};
-        q[u][i][e] = __builtin_bit_cast(uint32_t, lo_half ? z : w);
+        const h2_t w = {(_Float16)y0, (_Float16)y1};  // hi, or what that rounds off
+        const h2_t z = {(_Float16)fmaf((float)w[0], less, y0), (_Float16)fmaf((float)w[1], less, y1)};
+        q[u][i][e] = __builtin_bit_cast(uint32_t, z);
       }
     lo_max = max(lo_max, lo[u]);
     hi_min = min(hi_min, hi[u]);
@@ -285,54 +292,84 @@ __global__ __launch_bounds__(64 * WAVES, HD * CG <= 256 ? 2 : 1) void part_kerne
 #pragma unroll
     for (int i = 0; i < ND; ++i) o[u][i] = f4_t{0.f, 0.f, 0.f, 0.f};
   }
-  // P's column of this lane: e's fp16, or 2^11 times what that cuts off (applied to o at the end)
-  const float cut = lo_half ? -2048.f : 0.f, keep = lo_half ? 2048.f : 1.f;
+  // P's column of this lane: e's fp16, or 2^11 times what that rounds off (taken back from o at the end)
+  const float rest = lo_half ? -2048.f : 0.f, keep = lo_half ? 2048.f : 1.f;
 
-  for (; tile < t1; tile = __builtin_amdgcn_readfirstlane(tile + WAVES)) {
+  __shared__ __align__(16) f4_t parts[DW > 1 ? 2 : 1][DW > 1 ? WAVES : 1][CG][64];  // a tile's scores from each wave's dims
+  const int t_end = DW > 1 ? t0 + ceil_div(t1 - t0, TW) * TW : t1;  // (all waves go through the barriers)
+  for (int turn = 0; tile < t_end; tile = __builtin_amdgcn_readfirstlane(tile + TW), turn ^= 1) {
+    const bool have = DW == 1 || tile < t1;
     const bool inner = tile * TILE >= lo_max && (tile + 1) * TILE <= hi_min;  // every column sees all of it
-    const bool more = tile + WAVES < t1;
-    f4_t d[CG][2];
+    const bool more = tile + TW < t1;
+    float s[CG][8], ks = 0.f;
+    if (have) {
+      f4_t d[CG][2];
 #pragma unroll
-    for (int u = 0; u < CG; ++u) d[u][0] = d[u][1] = f4_t{0.f, 0.f, 0.f, 0.f};
+      for (int u = 0; u < CG; ++u) d[u][0] = d[u][1] = f4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
+      for (int r = 0; r < 2; ++r)
 #pragma unroll
-      for (int i = 0; i < NS; ++i) {
-        u4_t k;
-        uint32_t x, y;
-        codes_f16<E4M3>(T.k[s][i >> 1][2 * (i & 1)], x, y);
-        k[0] = x;
-        k[1] = y;
-        codes_f16<E4M3>(T.k[s][i >> 1][2 * (i & 1) + 1], x, y);
-        k[2] = x;
-        k[3] = y;
+        for (int i = 0; i < NS; ++i) {
+          u4_t k;
+          uint32_t y, z;
+          codes_f16<E4M3>(T.k[r][i >> 1][2 * (i & 1)], y, z);
+          k[0] = y;
+          k[1] = z;
+          codes_f16<E4M3>(T.k[r][i >> 1][2 * (i & 1) + 1], y, z);
+          k[2] = y;
+          k[3] = z;
 #pragma unroll
-        for (int u = 0; u < CG; ++u) d[u][s] = mfma(k, q[u][i], d[u][s]);
+          for (int u = 0; u < CG; ++u) d[u][r] = mfma(k, q[u][i], d[u][r]);
+        }
+      ks = T.ks;
+      if (more) load_k<HD>(T, K, KS, tile + TW, n, dim0, lane);
+#pragma unroll
+      for (int u = 0; u < CG; ++u) {
+        const float f = DW == 1 ? qs[u] * ks : qs[u];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[u][i] = pair_sum(d[u][i >> 2][i & 3]) * f;
+        if (DW > 1)  // both halves of a row of lanes have all eight: four each
+          parts[turn][wave][u][lane] = lo_half ? f4_t{s[u][4], s[u][5], s[u][6], s[u][7]} : f4_t{s[u][0], s[u][1], s[u][2], s[u][3]};
       }
-    const float ks = T.ks;
-    if (more) load_k(T, K, KS, tile + WAVES, n, lane);
+    }
+    if constexpr (DW > 1) {
+      __syncthreads();
+      if (!have) continue;
+#pragma unroll
+      for (int u = 0; u < CG; ++u) {
+        f4_t y = parts[turn][tw * DW][u][lane & ~8], z = parts[turn][tw * DW][u][lane | 8];
+#pragma unroll
+        for (int w = 1; w < DW; ++w) {  // (in the same order in every wave: their maxima are the same)
+          y += parts[turn][tw * DW + w][u][lane & ~8];
+          z += parts[turn][tw * DW + w][u][lane | 8];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s[u][i] = y[i] * ks;
+          s[u][4 + i] = z[i] * ks;
+        }
+      }
+    }
     u4_t pr[CG];
     float fac[CG];
 #pragma unroll
     for (int u = 0; u < CG; ++u) {
-      const float f = qs[u] * ks;
-      float s[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) s[i] = pair_sum(d[u][i >> 2][i & 3]) * f;
       if (!inner) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int j = tile * TILE + 16 * (i >> 2) + 4 * kg + (i & 3);
-          if (j < lo[u] || j >= hi[u]) s[i] = -INFINITY;
+          if (j < lo[u] || j >= hi[u]) s[u][i] = -INFINITY;
         }
       }
-      if (p.s) {
+      if (p.s && dim0 == 0) {
         const int col = (cb * CG + u) * 8 + c8;
         float* to = p.s + ((size_t)bh * p.cols + col) * p.spad + tile * TILE + 4 * kg + (lo_half ? 16 : 0);
-        const f4_t v = lo_half ? f4_t{s[4], s[5], s[6], s[7]} : f4_t{s[0], s[1], s[2], s[3]};
+        const f4_t v = lo_half ? f4_t{s[u][4], s[u][5], s[u][6], s[u][7]} : f4_t{s[u][0], s[u][1], s[u][2], s[u][3]};
         if (col < p.cols) *reinterpret_cast<f4_t*>(to) = v;
       }
-      float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+      float top = s[u][0];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) top = fmaxf(top, s[u][i]);
       top = groups_max(top);
       // The running maximum is only a reference: it moves when a block's is 2^30 above it.
       if (__any(top > m[u] + 30.f || (m[u] == -INFINITY && top > m[u]))) {
@@ -348,16 +385,16 @@ __global__ __launch_bounds__(64 * WAVES, HD * CG <= 256 ? 2 : 1) void part_kerne
       float sum = 0.f, x[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        x[i] = __builtin_amdgcn_exp2f(s[i] - ref + 14.f);
+        x[i] = __builtin_amdgcn_exp2f(s[u][i] - ref + 14.f);
         sum += x[i];
       }
       l[u] += sum * fac[u];
       fac[u] *= T.vs;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const h2_t e = __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_pkrtz(x[2 * i], x[2 * i + 1]));
-        pr[u][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(fmaf((float)e[0], cut, x[2 * i] * keep),
-                                                                           fmaf((float)e[1], cut, x[2 * i + 1] * keep)));
+        const h2_t e = {(_Float16)x[2 * i], (_Float16)x[2 * i + 1]};
+        const h2_t f = {(_Float16)fmaf((float)e[0], rest, x[2 * i] * keep), (_Float16)fmaf((float)e[1], rest, x[2 * i + 1] * keep)};
+        pr[u][i] = __builtin_bit_cast(uint32_t, f);
       }
     }
 #pragma unroll
@@ -379,18 +416,18 @@ __global__ __launch_bounds__(64 * WAVES, HD * CG <= 256 ? 2 : 1) void part_kerne
         }
       }
     }
-    if (more) load_v(T, V, VS, tile + WAVES, n, lane);
+    if (more) load_v<HD>(T, V, VS, tile + TW, n, dim0, lane);
   }
 
   // The waves' parts: to a common maximum, then summed through LDS, one wave after the other's columns.
-  __shared__ float sm[WAVES][8 * CG], sl[WAVES][8 * CG];
-  __shared__ __align__(16) float so[WAVES][8][HD];
+  __shared__ float sm[TW][8 * CG], sl[TW][8 * CG];
+  __shared__ __align__(16) float so[TW][8][HD];
 #pragma unroll
   for (int u = 0; u < CG; ++u) {
     l[u] = groups_sum(l[u]);
-    if (lane < 8) {
-      sm[wave][8 * u + lane] = m[u];
-      sl[wave][8 * u + lane] = l[u];
+    if (lane < 8 && dim0 == 0) {
+      sm[tw][8 * u + lane] = m[u];
+      sl[tw][8 * u + lane] = l[u];
     }
   }
   __syncthreads();
@@ -398,10 +435,10 @@ __global__ __launch_bounds__(64 * WAVES, HD * CG <= 256 ? 2 : 1) void part_kerne
   for (int u = 0; u < CG; ++u) {
     float top = sm[0][8 * u + c8];
 #pragma unroll
-    for (int w = 1; w < WAVES; ++w) top = fmaxf(top, sm[w][8 * u + c8]);
+    for (int w = 1; w < TW; ++w) top = fmaxf(top, sm[w][8 * u + c8]);
     const float mine = m[u] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[u] - top - (lo_half ? 11.f : 0.f));
     if (u > 0) __syncthreads();
-    // dims (HD / 16) (4 kg + r) + i: for each r the lane has ND of them in a row, stored by the hi lanes for
+    // dims dim0 + ND (4 kg + r) + i: for each r the lane has ND of them in a row, stored by the hi lanes for
     // r = 0, 1 and the lo lanes for r = 2, 3
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -411,7 +448,7 @@ __global__ __launch_bounds__(64 * WAVES, HD * CG <= 256 ? 2 : 1) void part_kerne
       if (lo_half == (r >= 2)) {
 #pragma unroll
         for (int i = 0; i < ND; i += 4)
-          *reinterpret_cast<f4_t*>(&so[wave][c8][ND * (4 * kg + r) + i]) = f4_t{y[i], y[i + 1], y[i + 2], y[i + 3]};
+          *reinterpret_cast<f4_t*>(&so[tw][c8][dim0 + ND * (4 * kg + r) + i]) = f4_t{y[i], y[i + 1], y[i + 2], y[i + 3]};
       }
     }
     __syncthreads();
@@ -421,13 +458,13 @@ __global__ __launch_bounds__(64 * WAVES, HD * CG <= 256 ? 2 : 1) void part_kerne
       if (c0 + col >= p.cols) continue;
       f4_t y = *reinterpret_cast<const f4_t*>(&so[0][col][dim]);
 #pragma unroll
-      for (int w = 1; w < WAVES; ++w) y += *reinterpret_cast<const f4_t*>(&so[w][col][dim]);
+      for (int w = 1; w < TW; ++w) y += *reinterpret_cast<const f4_t*>(&so[w][col][dim]);
       float mm = sm[0][8 * u + col];
 #pragma unroll
-      for (int w = 1; w < WAVES; ++w) mm = fmaxf(mm, sm[w][8 * u + col]);
+      for (int w = 1; w < TW; ++w) mm = fmaxf(mm, sm[w][8 * u + col]);
       float ll = 0.f;
 #pragma unroll
-      for (int w = 0; w < WAVES; ++w)
+      for (int w = 0; w < TW; ++w)
         ll += sl[w][8 * u + col] * (sm[w][8 * u + col] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(sm[w][8 * u + col] - mm));
       const size_t row = ((size_t)x * c.n_kv + h) * p.cols + c0 + col;
       if (p.direct) {
@@ -445,28 +482,28 @@ __global__ __launch_bounds__(64 * WAVES, HD * CG <= 256 ? 2 : 1) void part_kerne
   }
 }
 
-// Workgroups [0, batch * n_kv * cols), unless the chunks have written the output themselves: one
-// column each. Those behind them: the weights of 1024 entries of a KV head.
+// Workgroups [0, ncol), unless the chunks have written the output themselves: 64 dims of a column
+// each, sixteen chunks at a time. Those behind them: the weights of 1024 entries of a KV head.
 template <int HD>
 __global__ __launch_bounds__(256) void join_kernel(Kv8 c, Kv8Attn a, Plan p, int ncol, int wblocks) {
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, G = p.group;
   if ((int)blockIdx.x < ncol) {
-    constexpr int TPR = HD / 4, GRP = 256 / TPR;
+    constexpr int SD = 64, TPR = SD / 4, GRP = 256 / TPR;
     __shared__ float w[MAX_SPLIT];
     __shared__ float red[2][4];
-    __shared__ __align__(16) float acc[GRP][HD];
-    const int bh = blockIdx.x / p.cols, col = blockIdx.x - bh * p.cols, b = bh / c.n_kv, h = bh - b * c.n_kv;
+    __shared__ __align__(16) float acc[GRP][SD];
+    const int bc = blockIdx.x / (HD / SD), bh = bc / p.cols, col = bc - bh * p.cols, b = bh / c.n_kv, h = bh - b * c.n_kv;
     // of a single sequence the first parts, without waiting for its length
     constexpr int PRE = 4;
     const size_t step = (size_t)c.n_kv * p.cols;
-    const int g = t / TPR, d = 4 * (t % TPR);
+    const int g = t / TPR, ds = 4 * (t % TPR), d = (blockIdx.x % (HD / SD)) * SD + ds;
     f4_t pre[PRE];
     if (c.batch == 1) {
 #pragma unroll
       for (int k = 0; k < PRE; ++k)
-        pre[k] = *reinterpret_cast<const f4_t*>(p.o + (min(g + GRP * k, p.chunks - 1) * step + blockIdx.x) * HD + d);
+        pre[k] = *reinterpret_cast<const f4_t*>(p.o + (min(g + GRP * k, p.chunks - 1) * step + bc) * HD + d);
     }
-    const Cut ct = cut<false>(c, a, p, 0, b);
+    const Cut ct = cut<false, HD>(c, a, p, 0, b);
     const int live = ct.count;
     const size_t row = (size_t)ct.first * step + (size_t)h * p.cols + col;
     float m = -INFINITY, l = 0.f;
@@ -493,11 +530,11 @@ __global__ __launch_bounds__(256) void join_kernel(Kv8 c, Kv8Attn a, Plan p, int
     }
 #pragma unroll 4
     for (int i = i0; i < live; i += GRP) y += *reinterpret_cast<const f4_t*>(p.o + (row + i * step) * HD + d) * w[i];
-    *reinterpret_cast<f4_t*>(&acc[g][d]) = y;
+    *reinterpret_cast<f4_t*>(&acc[g][ds]) = y;
     __syncthreads();
     if (t < TPR) {
 #pragma unroll
-      for (int i = 1; i < GRP; ++i) y += *reinterpret_cast<const f4_t*>(&acc[i][d]);
+      for (int i = 1; i < GRP; ++i) y += *reinterpret_cast<const f4_t*>(&acc[i][ds]);
       const int tq = col / G;
       float* out = a.out + (((size_t)b * a.n_q + tq) * a.n_heads + h * G + col - tq * G) * HD + d;
       *reinterpret_cast<f4_t*>(out) = l == 0.f ? f4_t{0.f, 0.f, 0.f, 0.f} : y / l;
@@ -520,7 +557,7 @@ __global__ __launch_bounds__(256) void join_kernel(Kv8 c, Kv8Attn a, Plan p, int
     for (int i = 0; i < 4; ++i)
       if (j + i < a.max_len) old[i] = a.w_in[at + i];
   }
-  const Cut ct = cut<false>(c, a, p, 0, b);
+  const Cut ct = cut<false, HD>(c, a, p, 0, b);
   const int n = ct.n;
   if (j - 4 * t >= n) return;  // uniform
   int t0, t1;
@@ -573,21 +610,20 @@ __global__ __launch_bounds__(256) void join_kernel(Kv8 c, Kv8Attn a, Plan p, int
 
 size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
-// Column groups of eight per workgroup: two where there are more than eight columns, whose accumulators
-// leave room for two waves a SIMD (head_dim up to 256).
-int col_groups(int cols, int hd) { return cols > 8 && hd <= 256 ? 2 : 1; }
+// Column groups of eight per workgroup: two where there are more than eight columns.
+int col_groups(int cols) { return cols > 8 ? 2 : 1; }
 
 // The plan for sequences whose columns see at most `tiles` tiles; more of them never need less.
 Plan make_plan(const Kv8& c, int n_heads, int n_q, int tiles) {
   Plan p{};
   p.group = n_heads / c.n_kv;
   p.cols = p.group * n_q;
-  const int cg = col_groups(p.cols, c.hd), per = 8 * cg;
+  const int per = 8 * col_groups(p.cols), tw = tile_waves(c.hd);
   p.cblocks = (p.cols + per - 1) / per;
-  // Chunks that fill the chip once: two workgroups a CU, one where the accumulators leave a wave a SIMD. Up to
-  // eight tiles a second round of the waves costs less than the joining of two chunks.
-  const int target = c.hd * cg <= 256 ? 512 : 256;
-  p.tiles = tiles <= 2 * WAVES ? 2 * WAVES : WAVES;
+  // Chunks that fill the chip once, two workgroups a CU. Up to two rounds of the waves the second one costs
+  // less than the joining of two chunks.
+  constexpr int target = 512;
+  p.tiles = tiles <= 2 * tw ? 2 * tw : tw;
   p.direct = tiles <= p.tiles;
   if (c.batch <= SHARED_BATCH) {
     p.share = std::max(1, target / (c.n_kv * p.cblocks));
@@ -598,7 +634,7 @@ Plan make_plan(const Kv8& c, int n_heads, int n_q, int tiles) {
     const long long units = (long long)c.batch * c.n_kv * p.cblocks;
     const int want = (int)std::max<long long>(1, std::min<long long>(MAX_SPLIT, 2 * target / units));
     p.nsplit = std::max(1, std::min(want, (tiles + p.tiles - 1) / p.tiles));
-    p.tiles = std::max(p.tiles, ((tiles + p.nsplit - 1) / p.nsplit + WAVES - 1) / WAVES * WAVES);
+    p.tiles = std::max(p.tiles, ((tiles + p.nsplit - 1) / p.nsplit + tw - 1) / tw * tw);
     p.chunks = c.batch * p.nsplit;
     p.direct = p.nsplit == 1;
   }
@@ -618,7 +654,7 @@ template <int HD, int CG>
 void launch_cg(const Kv8& c, const Kv8Attn& a, const Plan& p, hipStream_t st) {
   const long long part = ((long long)p.chunks * c.n_kv + 7) / 8 * 8 * p.cblocks;
   const dim3 grid = p.cblocks == 1 ? dim3((unsigned)c.n_kv, (unsigned)p.chunks) : dim3((unsigned)part);
-  const long long ncol = p.direct ? 0 : (long long)c.batch * c.n_kv * p.cols;
+  const long long ncol = p.direct ? 0 : (long long)c.batch * c.n_kv * p.cols * (HD / 64);
   const int wblocks = a.w_out ? (a.max_len + 1023) / 1024 : 0;
   const long long join = ncol + (long long)c.batch * c.n_kv * wblocks;
   if (part > INT32_MAX || join > INT32_MAX) fail(ST_OP, "kv8: dims too large");
@@ -648,12 +684,12 @@ void launch_kv8_attention(const Kv8& c, const Kv8Attn& a, void* ws, hipStream_t 
   p.ml = reinterpret_cast<float*>(base);
   p.o = reinterpret_cast<float*>(base + z.ml);
   p.s = a.w_out ? reinterpret_cast<float*>(base + z.ml + z.o) : nullptr;
-  const bool two = col_groups(p.cols, c.hd) == 2;
+  const bool two = col_groups(p.cols) == 2;
   switch (c.hd) {
     case 64: two ? launch_cg<64, 2>(c, a, p, st) : launch_cg<64, 1>(c, a, p, st); break;
     case 128: two ? launch_cg<128, 2>(c, a, p, st) : launch_cg<128, 1>(c, a, p, st); break;
     case 256: two ? launch_cg<256, 2>(c, a, p, st) : launch_cg<256, 1>(c, a, p, st); break;
-    default: launch_cg<512, 1>(c, a, p, st); break;
+    default: two ? launch_cg<512, 2>(c, a, p, st) : launch_cg<512, 1>(c, a, p, st); break;
   }
 }
 
