@@ -28,17 +28,12 @@ template <int HD, bool E4M3>
 __global__ __launch_bounds__(AT) void append_kernel(Kv8 c, const float* __restrict__ kin, const float* __restrict__ vin,
                                                     int n, size_t stride, const int* __restrict__ start_p,
                                                     const int* __restrict__ count_p, int* __restrict__ len_out,
-                                                    float* __restrict__ weights, int nspan) {
+                                                    float* __restrict__ weights) {
   constexpr int TPR = HD / 4;          // threads per row (four values each)
   constexpr int RPP = AT / TPR;        // rows per pass
   constexpr int NP = (KV8_BLOCK + RPP - 1) / RPP;
   const int t = threadIdx.x;
-  int id = blockIdx.x;
-  const int which = id & 1;
-  id >>= 1;
-  const int h = id % c.n_kv;
-  id /= c.n_kv;
-  const int span = id % nspan, b = id / nspan;
+  const int which = blockIdx.x & 1, span = blockIdx.x >> 1, h = blockIdx.y, b = blockIdx.z;
   const int start = start_p ? start_p[b] : 0;
   int count = count_p ? min(count_p[b], n) : n;
   if (start < 0 || start > c.cap) count = 0;  // (nothing is written)
@@ -100,21 +95,23 @@ __global__ void advance_kernel(int batch, int cap, const int* count, int n, int*
 }
 
 // ---- load ----------------------------------------------------------------------------------------
+// One workgroup per (32 rows, KV head, sequence): 4 codes of K and of V to 16 bytes of f32 a lane. Bound by the
+// stores.
 template <int HD, bool E4M3>
 __global__ __launch_bounds__(256) void load_kernel(Kv8 c, int n, size_t stride, const int* __restrict__ start_p,
                                                    const int* __restrict__ count_p, float* __restrict__ k,
-                                                   float* __restrict__ v, size_t total) {
-  constexpr int TPR = HD / 4;
-  for (size_t i = blockIdx.x * (size_t)256 + threadIdx.x; i < total; i += (size_t)gridDim.x * 256) {
-    const int d = 4 * (int)(i % TPR);
-    size_t row = i / TPR;
-    const int h = (int)(row % c.n_kv);
-    row /= c.n_kv;
-    const int j = (int)(row % n), b = (int)(row / n);
-    const int start = start_p ? start_p[b] : 0, count = count_p ? min(count_p[b], n) : n;
+                                                   float* __restrict__ v) {
+  constexpr int TPR = HD / 4, RPP = 256 / TPR, NP = 32 / RPP;
+  const int h = blockIdx.y, b = blockIdx.z, d = 4 * (threadIdx.x % TPR);
+  const int start = start_p ? start_p[b] : 0, count = count_p ? min(count_p[b], n) : n;
+  const size_t head = (size_t)b * c.n_kv + h;
+  const int j0 = 32 * blockIdx.x + threadIdx.x / TPR;
+  if (32 * (int)blockIdx.x >= count) return;
+#pragma unroll 4
+  for (int p = 0; p < NP; ++p) {
+    const int j = j0 + RPP * p;
     const long long slot = (long long)start + j;
     if (j >= count || slot < 0 || slot >= c.cap) continue;
-    const size_t head = (size_t)b * c.n_kv + h;
     const size_t src = (head * c.cap + slot) * HD + d, dst = ((size_t)b * n + j) * stride + (size_t)h * HD + d;
     const size_t sc = head * c.nblk + slot / KV8_BLOCK;
     const float4 a = kv8_unpack<E4M3>(*reinterpret_cast<const uint32_t*>(c.k + src));
@@ -432,14 +429,12 @@ __global__ __launch_bounds__(IN_PLACE ? 1024 : 256) void move_kernel(Kv8 src, Kv
 
 void launch_kv8_append(const Kv8& c, const float* k, const float* v, int n, size_t stride, const int* start,
                        const int* count, int* len_out, float* weights, hipStream_t st) {
-  const int nspan = (n + 2 * KV8_BLOCK - 2) / KV8_BLOCK;  // blocks that n rows can touch
-  const size_t grid = (size_t)2 * c.n_kv * nspan * c.batch;
-  if (grid > INT32_MAX) fail(ST_OP, "kv8 append: too many rows");
+  const unsigned nspan = (unsigned)((n + 2 * KV8_BLOCK - 2) / KV8_BLOCK);  // blocks that n rows can touch
+  const dim3 grid(2 * nspan, (unsigned)c.n_kv, (unsigned)c.batch);
   const bool over = len_out && len_out == start;
   KV8_HD(c.hd, {
     auto fn = c.e4m3 ? append_kernel<HD, true> : append_kernel<HD, false>;
-    hipLaunchKernelGGL(fn, dim3((unsigned)grid), dim3(AT), 0, st, c, k, v, n, stride, start, count,
-                       over ? nullptr : len_out, weights, nspan);
+    hipLaunchKernelGGL(fn, grid, dim3(AT), 0, st, c, k, v, n, stride, start, count, over ? nullptr : len_out, weights);
   })
   if (over)
     hipLaunchKernelGGL(advance_kernel, dim3((c.batch + 63) / 64), dim3(64), 0, st, c.batch, c.cap, count, n, len_out);
@@ -447,11 +442,10 @@ void launch_kv8_append(const Kv8& c, const float* k, const float* v, int n, size
 
 void launch_kv8_load(const Kv8& c, int n, size_t stride, const int* start, const int* count, float* k, float* v,
                      hipStream_t st) {
-  const size_t total = (size_t)c.batch * n * c.n_kv * (c.hd / 4);
-  const unsigned grid = (unsigned)std::min<size_t>((total + 255) / 256, 256 * 32);
+  const dim3 grid((unsigned)(n + 31) / 32, (unsigned)c.n_kv, (unsigned)c.batch);
   KV8_HD(c.hd, {
     auto fn = c.e4m3 ? load_kernel<HD, true> : load_kernel<HD, false>;
-    hipLaunchKernelGGL(fn, dim3(grid), dim3(256), 0, st, c, n, stride, start, count, k, v, total);
+    hipLaunchKernelGGL(fn, grid, dim3(256), 0, st, c, n, stride, start, count, k, v);
   })
 }
 
