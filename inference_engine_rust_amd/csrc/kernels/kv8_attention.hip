@@ -482,13 +482,68 @@ __global__ __launch_bounds__(64 * WAVES, 2) void part_kernel(Kv8 c, Kv8Attn a, P
   }
 }
 
-// Workgroups [0, ncol), unless the chunks have written the output themselves: 64 dims of a column
-// each, sixteen chunks at a time. Those behind them: the weights of 1024 entries of a KV head.
-template <int HD>
+// Largest m and sum of l 2^(m - top) over the chunks of a column, by one wave: ml the first chunk's pair, `step`
+// columns apart. m and l are left in the lanes, chunk lane + 64 i.
+IEK_DEV void column_sum(const float* ml, size_t step, int count, float (&m)[MAX_SPLIT / 64], float& top, float& sum) {
+  const int lane = threadIdx.x & 63;
+  float l[MAX_SPLIT / 64];
+  top = -INFINITY;
+  sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < MAX_SPLIT / 64; ++i) {
+    const int k = lane + 64 * i;
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+    if (64 * i < count && k < count) {
+      m[i] = ml[2 * k * step];
+      l[i] = ml[2 * k * step + 1];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < MAX_SPLIT / 64; ++i) top = fmaxf(top, m[i]);
+  top = wave_max(top);
+#pragma unroll
+  for (int i = 0; i < MAX_SPLIT / 64; ++i) sum += m[i] == -INFINITY ? 0.f : l[i] * __builtin_amdgcn_exp2f(m[i] - top);
+  sum = wave_sum(sum);
+}
+
+// The join. Workgroups [0, ncol), unless the chunks have written the output themselves: 64 dims of a
+// column, sixteen chunks at a time; those behind them: the weights of 1024 entries of a KV head. MANY
+// (several query tokens: many columns of few chunks, where workgroups are what costs): 64 dims of four
+// columns, a wave each; the weights of 256 entries, a quarter of the columns a wave (22 sequences up to
+// 451 keys of 512, eleven tokens: 69 us before, TODO so).
+template <int HD, bool MANY>
 __global__ __launch_bounds__(256) void join_kernel(Kv8 c, Kv8Attn a, Plan p, int ncol, int wblocks) {
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, G = p.group;
-  if ((int)blockIdx.x < ncol) {
-    constexpr int SD = 64, TPR = SD / 4, GRP = 256 / TPR;
+  constexpr int SD = 64, TPR = SD / 4, GRP = 256 / TPR;
+  if (MANY && (int)blockIdx.x < ncol) {
+    __shared__ float wc[4][MAX_SPLIT];
+    const int quads = (p.cols + 3) / 4, id = blockIdx.x / (HD / SD), bh = id / quads;
+    const int col = (id - bh * quads) * 4 + wave, b = bh / c.n_kv, h = bh - b * c.n_kv;
+    if (col >= p.cols) return;  // (uniform in the wave; there is no barrier)
+    const Cut ct = cut<false, HD>(c, a, p, 0, b);
+    const int d = (blockIdx.x % (HD / SD)) * SD + 4 * (lane & 15);
+    const size_t step = (size_t)c.n_kv * p.cols, row = (size_t)ct.first * step + (size_t)h * p.cols + col;
+    float m[MAX_SPLIT / 64], top, sum;
+    column_sum(p.ml + 2 * row, step, ct.count, m, top, sum);
+#pragma unroll
+    for (int i = 0; i < MAX_SPLIT / 64; ++i)
+      if (64 * i < ct.count) wc[wave][lane + 64 * i] = m[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[i] - top);
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    f4_t y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int i = lane >> 4; i < ct.count; i += 4)
+      y += *reinterpret_cast<const f4_t*>(p.o + (row + i * step) * HD + d) * wc[wave][i];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = groups_sum(y[i]);
+    const int tq = col / G;
+    float* out = a.out + (((size_t)b * a.n_q + tq) * a.n_heads + h * G + col - tq * G) * HD + d;
+    if (lane < 16) *reinterpret_cast<f4_t*>(out) = sum == 0.f ? f4_t{0.f, 0.f, 0.f, 0.f} : y / sum;
+    return;
+  }
+  if (!MANY && (int)blockIdx.x < ncol) {
     __shared__ float w[MAX_SPLIT];
     __shared__ float red[2][4];
     __shared__ __align__(16) float acc[GRP][SD];
@@ -544,14 +599,15 @@ __global__ __launch_bounds__(256) void join_kernel(Kv8 c, Kv8Attn a, Plan p, int
   constexpr int COLS = 64 * 8;  // n_q <= 64, groups of at most 8
   __shared__ float cm[COLS], cl[COLS];
   const int id = blockIdx.x - ncol, bh = id / wblocks, b = bh / c.n_kv, h = bh - b * c.n_kv;
-  const int j = (id - bh * wblocks) * 1024 + 4 * t;
+  const int j0 = (id - bh * wblocks) * (MANY ? 256 : 1024), j = j0 + 4 * (MANY ? lane : t);
   // what does not wait for the lengths: the first columns' scores (`spad` of them are there) and the old sums
-  constexpr int PRE = 8;
+  constexpr int PRE = 8, CS = MANY ? 4 : 1;  // (column c0 + CS k)
+  const int c0 = MANY ? wave : 0;
   const float* s = p.s + (size_t)bh * p.cols * p.spad + min(j, p.spad - 4);
   const size_t at = (size_t)bh * c.cap + j;
   f4_t v[PRE], w = {0.f, 0.f, 0.f, 0.f}, old = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int col = 0; col < PRE; ++col) v[col] = *reinterpret_cast<const f4_t*>(s + (size_t)min(col, p.cols - 1) * p.spad);
+  for (int col = 0; col < PRE; ++col) v[col] = *reinterpret_cast<const f4_t*>(s + (size_t)min(c0 + CS * col, p.cols - 1) * p.spad);
   if (a.w_in) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -559,49 +615,58 @@ __global__ __launch_bounds__(256) void join_kernel(Kv8 c, Kv8Attn a, Plan p, int
   }
   const Cut ct = cut<false, HD>(c, a, p, 0, b);
   const int n = ct.n;
-  if (j - 4 * t >= n) return;  // uniform
+  if (j0 >= n) return;  // uniform
   int t0, t1;
   tile_range(a, n, t0, t1);
   const size_t step = (size_t)c.n_kv * p.cols;
-  for (int col = wave; col < p.cols; col += 4) {
-    const float* ml = p.ml + 2 * ((size_t)ct.first * step + (size_t)h * p.cols + col);
-    float m[MAX_SPLIT / 64], l[MAX_SPLIT / 64], top = -INFINITY, sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < MAX_SPLIT / 64; ++i) {
-      const int k = lane + 64 * i;
-      m[i] = -INFINITY;
-      l[i] = 0.f;
-      if (64 * i < ct.count && k < ct.count) {
-        m[i] = ml[2 * k * step];
-        l[i] = ml[2 * k * step + 1];
+  // a wave a column, or, of many columns with few chunks, a thread
+  const float* ml0 = p.ml + 2 * ((size_t)ct.first * step + (size_t)h * p.cols);
+  if (!MANY || p.cols <= ct.count) {
+    for (int col = wave; col < p.cols; col += 4) {
+      float m[MAX_SPLIT / 64], top, sum;
+      column_sum(ml0 + 2 * col, step, ct.count, m, top, sum);
+      if (lane == 0) {
+        cm[col] = top == -INFINITY ? 0.f : top;  // (a column that sees nothing has only scores of -inf)
+        cl[col] = sum == 0.f ? 0.f : 1.f / sum;
       }
     }
-#pragma unroll
-    for (int i = 0; i < MAX_SPLIT / 64; ++i) top = fmaxf(top, m[i]);
-    top = wave_max(top);
-#pragma unroll
-    for (int i = 0; i < MAX_SPLIT / 64; ++i) sum += m[i] == -INFINITY ? 0.f : l[i] * __builtin_amdgcn_exp2f(m[i] - top);
-    sum = wave_sum(sum);
-    if (lane == 0) {
-      cm[col] = top == -INFINITY ? 0.f : top;  // (a column that sees nothing has only scores of -inf)
+  } else {
+    for (int col = t; col < p.cols; col += 256) {
+      float top = -INFINITY, sum = 0.f;
+#pragma unroll 4
+      for (int k = 0; k < ct.count; ++k) top = fmaxf(top, ml0[2 * (k * step + col)]);
+#pragma unroll 4
+      for (int k = 0; k < ct.count; ++k) {
+        const float m = ml0[2 * (k * step + col)], l = ml0[2 * (k * step + col) + 1];
+        sum += m == -INFINITY ? 0.f : l * __builtin_amdgcn_exp2f(m - top);
+      }
+      cm[col] = top == -INFINITY ? 0.f : top;
       cl[col] = sum == 0.f ? 0.f : 1.f / sum;
     }
   }
   __syncthreads();
-  if (j >= n) return;
-  if (j >= t0 * TILE) {
+  if (!MANY && j >= n) return;
+  if (j < n && j >= t0 * TILE) {
 #pragma unroll
-    for (int col = 0; col < PRE; ++col) {
+    for (int k = 0; k < PRE; ++k) {
+      const int col = c0 + CS * k;
       if (col >= p.cols) break;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] += __builtin_amdgcn_exp2f(v[col][i] - cm[col]) * cl[col];
+      for (int i = 0; i < 4; ++i) w[i] += __builtin_amdgcn_exp2f(v[k][i] - cm[col]) * cl[col];
     }
-#pragma unroll 4
-    for (int col = PRE; col < p.cols; ++col) {
+#pragma unroll 8
+    for (int col = c0 + CS * PRE; col < p.cols; col += CS) {
       const f4_t z = *reinterpret_cast<const f4_t*>(s + (size_t)col * p.spad);
 #pragma unroll
       for (int i = 0; i < 4; ++i) w[i] += __builtin_amdgcn_exp2f(z[i] - cm[col]) * cl[col];
     }
+  }
+  if constexpr (MANY) {
+    __shared__ f4_t part[4][64];
+    part[wave][lane] = w;
+    __syncthreads();
+    if (wave != 0 || j >= n) return;
+    w = part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane];
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i)
@@ -654,14 +719,15 @@ template <int HD, int CG>
 void launch_cg(const Kv8& c, const Kv8Attn& a, const Plan& p, hipStream_t st) {
   const long long part = ((long long)p.chunks * c.n_kv + 7) / 8 * 8 * p.cblocks;
   const dim3 grid = p.cblocks == 1 ? dim3((unsigned)c.n_kv, (unsigned)p.chunks) : dim3((unsigned)part);
-  const long long ncol = p.direct ? 0 : (long long)c.batch * c.n_kv * p.cols * (HD / 64);
-  const int wblocks = a.w_out ? (a.max_len + 1023) / 1024 : 0;
+  const bool many = CG > 1;  // (more than eight columns)
+  const long long ncol = p.direct ? 0 : (long long)c.batch * c.n_kv * (HD / 64) * (many ? (p.cols + 3) / 4 : p.cols);
+  const int wblocks = a.w_out ? (a.max_len + (many ? 255 : 1023)) / (many ? 256 : 1024) : 0;
   const long long join = ncol + (long long)c.batch * c.n_kv * wblocks;
   if (part > INT32_MAX || join > INT32_MAX) fail(ST_OP, "kv8: dims too large");
   auto fn = c.e4m3 ? part_kernel<HD, true, CG> : part_kernel<HD, false, CG>;
   hipLaunchKernelGGL(fn, grid, dim3(64 * WAVES), 0, st, c, a, p);
   if (join)
-    hipLaunchKernelGGL(join_kernel<HD>, dim3((unsigned)join), dim3(256), 0, st, c, a, p, (int)ncol, wblocks);
+    hipLaunchKernelGGL((join_kernel<HD, (CG > 1)>), dim3((unsigned)join), dim3(256), 0, st, c, a, p, (int)ncol, wblocks);
 }
 
 }  // namespace
