@@ -676,7 +676,8 @@ static Kv8 kv8_view(const iek_kv8* c, bool buffers = true) {
   if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256 && c->head_dim != 512)
     fail(ST_OP, "kv8: head_dim must be 64, 128, 256 or 512");
   if (c->n_kv_heads == 0 || c->capacity == 0) fail(ST_OP, "kv8: no KV heads or no capacity");
-  if (c->n_kv_heads > 4096 || c->batch > 65535 || c->capacity > (1u << 30) || c->batch * c->n_kv_heads > (1u << 20))
+  // (so that every grid is within 2^32 threads a dimension)
+  if (c->n_kv_heads > 4096 || c->batch > 65535 || c->capacity > (1u << 26) || c->batch * c->n_kv_heads > (1u << 16))
     fail(ST_OP, "kv8: dims too large");
   if (buffers) {
     aligned(c->k, 16, "k");

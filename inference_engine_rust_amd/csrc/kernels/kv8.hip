@@ -477,7 +477,7 @@ void launch_kv8_evict(const Kv8& src, const Kv8& dst, const Kv8Evict& a, void* w
   const int sw = in_place || src.hd == 64 ? 64 : 128, slices = 2 * src.hd / sw;
   const int nb = (std::min(a.keep, a.max_len) + KV8_BLOCK - 1) / KV8_BLOCK;
   const int mb = in_place || (long long)heads * slices * nb > 8192 ? 2 : 1;
-  const int parts = in_place ? 1 : std::max(1, std::min((nb + 4 * mb - 1) / (4 * mb), INT32_MAX / (heads * slices)));
+  const int parts = in_place ? 1 : std::max(1, std::min((nb + 4 * mb - 1) / (4 * mb), ((1 << 24) - 1) / (heads * slices)));
   void (*fn)(Kv8, Kv8, Kv8Evict, const int*, const int*, const float*, int);
   if (in_place) fn = src.e4m3 ? move_kernel<true, 64, true, 2> : move_kernel<false, 64, true, 2>;
   else if (sw == 64 && mb == 1) fn = src.e4m3 ? move_kernel<true, 64, false, 1> : move_kernel<false, 64, false, 1>;

@@ -371,9 +371,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void part_kernel(Kv8 c, Kv8Attn a, P
 #pragma unroll
       for (int i = 1; i < 8; ++i) top = fmaxf(top, s[u][i]);
       top = groups_max(top);
-      // The running maximum is only a reference: it moves when a block's is 2^30 above it.
-      if (__any(top > m[u] + 30.f || (m[u] == -INFINITY && top > m[u]))) {
-        const bool up = top > m[u] + 30.f || m[u] == -INFINITY;
+      // The running maximum is only a reference: it moves when a block's is more than 2^8 above it.
+      if (__any(top > m[u] + 8.f || (m[u] == -INFINITY && top > m[u]))) {
+        const bool up = top > m[u] + 8.f || m[u] == -INFINITY;
         const float corr = up && m[u] != -INFINITY ? __builtin_amdgcn_exp2f(m[u] - top) : 1.f;  // (all is 0 before)
         if (up) m[u] = top;
         l[u] *= corr;
@@ -723,7 +723,7 @@ void launch_cg(const Kv8& c, const Kv8Attn& a, const Plan& p, hipStream_t st) {
   const long long ncol = p.direct ? 0 : (long long)c.batch * c.n_kv * (HD / 64) * (many ? (p.cols + 3) / 4 : p.cols);
   const int wblocks = a.w_out ? (a.max_len + (many ? 255 : 1023)) / (many ? 256 : 1024) : 0;
   const long long join = ncol + (long long)c.batch * c.n_kv * wblocks;
-  if (part > INT32_MAX || join > INT32_MAX) fail(ST_OP, "kv8: dims too large");
+  if (part >= 1 << 24 || join >= 1 << 24) fail(ST_OP, "kv8: dims too large");  // (2^32 threads)
   auto fn = c.e4m3 ? part_kernel<HD, true, CG> : part_kernel<HD, false, CG>;
   hipLaunchKernelGGL(fn, grid, dim3(64 * WAVES), 0, st, c, a, p);
   if (join)
@@ -734,6 +734,7 @@ void launch_cg(const Kv8& c, const Kv8Attn& a, const Plan& p, hipStream_t st) {
 
 // For any window: fewer tiles do not take more chunks.
 size_t kv8_attention_workspace(const Kv8& c, int n_heads, int n_q, int max_len, bool weights) {
+  if (c.batch == 0 || n_q == 0) return 0;
   const int tiles = (max_len + TILE - 1) / TILE;
   Plan p = make_plan(c, n_heads, n_q, tiles);
   const Sizes z = sizes(c, p, tiles * TILE, weights);

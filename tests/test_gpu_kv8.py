@@ -515,6 +515,34 @@ def test_captured_step_replays(gpu):
             assert torch.equal(a["c"].scale[j][:, :, :2], b["c"].scale[j][:, :, :2])
 
 
+@pytest.mark.parametrize("batch", [1, 3])
+def test_captured_attention_follows_the_lengths(gpu, batch):
+    """One captured attention with weights, launched for the whole capacity, replayed at lengths from none to all of it."""
+    cap, kv, group, hd = 5000, 2, 4, 64
+    ref = filled(12, batch, kv, cap, hd, "i8", [cap] * batch)
+    d, lens = Dev(batch, kv, cap, hd, "i8", ref), ints([cap] * batch)
+    q = np.random.default_rng(3).standard_normal((batch, 1, kv * group, hd)).astype(np.float32)
+    dq, out, w = dev(q), torch.zeros((batch, kv * group * hd), device="cuda"), torch.zeros((batch, kv, cap), device="cuda")
+    size = E.kv8_attention_workspace(d.h, kv * group, 1, cap, True)
+    ws = torch.full((size,), 255, dtype=torch.uint8, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        E.kv8_attention(d.h, dq.data_ptr(), kv * group, 1, kv * group * hd, lens.data_ptr(), cap, 0, 0.125, out.data_ptr(), 0,
+                        w.data_ptr(), ws.data_ptr(), size, stream())
+    for n in (1, 40, 0, 531, 5000, 33, 2049):
+        now = [max(0, n - 7 * b) for b in range(batch)]
+        lens.copy_(torch.tensor(now, dtype=torch.int32))
+        out.fill_(9)
+        w.fill_(-4)
+        graph.replay()
+        want, want_w, bound = ref.attention(q, now, 0, 0.125)
+        assert (np.abs(host(out).reshape(q.shape) - want) <= bound).all(), n
+        got = host(w)
+        for b in range(batch):
+            assert np.allclose(got[b, :, :now[b]], want_w[b, :, :now[b]], rtol=1e-4, atol=1e-9) and (got[b, :, now[b]:] == -4).all()
+
+
 def test_two_streams_at_once(gpu):
     """Calls on two streams, each with its own workspace and outputs over one cache, give what they give alone."""
     ref = filled(6, 2, 4, 1500, 128, "i8", [1500, 900])

@@ -125,6 +125,8 @@ def test_workspaces_grow_with_what_they_hold():
     assert E.kv8_attention_workspace(c, 64, 64, 70000, True) >= 3 * 64 * 64 * 70000 * 4
     assert E.kv8_evict_workspace(c, 70000, 60000) >= 3 * 8 * 60000 * 4
     refused("KvCache", "70000", E.kv8_attention_workspace, c, 32, 1, 70001, True)
+    assert E.kv8_attention_workspace(c, 32, 0, 70000, True) == 0
+    assert E.kv8_attention_workspace(cache(batch=0), 4, 1, 100, True) == 0 == E.kv8_evict_workspace(cache(batch=0), 100, 50)
     refused("KvCache", "70000", E.kv8_evict_workspace, c, 70001, 5)
 
 
