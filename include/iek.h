@@ -362,7 +362,9 @@ iek_status iek_dev_kv8_attention(const iek_kv8* cache, const float* q, size_t n_
  * otherwise) that share nothing (nor do weights and weights_out), or twice the same one, with
  * weights_out = weights: an eviction in place. Sequences of up to `keep` entries are copied, or left
  * as they are. A block's new scale is the largest of its rows' old ones. len_out[b] = min(len[b],
- * keep); it may be len itself, and must not overlap it otherwise. index_out (or NULL): [batch][n_kv_heads][keep], the old slots of the entries kept. */
+ * keep); it may be len itself, and must not overlap it otherwise. index_out (or NULL):
+ * [batch][n_kv_heads][keep], the old slots of the entries kept (places past the new length are left
+ * as they were). */
 iek_status iek_kv8_evict_workspace(const iek_kv8* src, size_t max_len, size_t keep, size_t* bytes);
 iek_status iek_dev_kv8_evict(const iek_kv8* src, const iek_kv8* dst, const float* weights, float* weights_out,
                              const int32_t* len, int32_t* len_out, size_t max_len, size_t keep, size_t first,
