@@ -281,14 +281,16 @@ __global__ __launch_bounds__(ST) void select_kernel(Kv8 src, Kv8Evict a, int* __
         }
         if (all == 0) return;
         const int bin = key >> SHIFT & ((1 << BITS) - 1);
-        const int bin0 = __builtin_amdgcn_readlane(bin, __ffsll(all) - 1);
-        const int same = __popcll(__ballot(bin == bin0) & all);
-        if (same >= 8) {
-          if (in && bin != bin0) atomicAdd(&h[bin], 1);
-          if (lane == 0) atomicAdd(&h[bin0], same);
-        } else if (in) {
-          atomicAdd(&h[bin], 1);
+        if (__popcll(all) >= 8) {
+          const int bin0 = __builtin_amdgcn_readlane(bin, __ffsll(all) - 1);
+          const int same = __popcll(__ballot(bin == bin0) & all);
+          if (same >= 8) {
+            if (in && bin != bin0) atomicAdd(&h[bin], 1);
+            if (lane == 0) atomicAdd(&h[bin0], same);
+            return;
+          }
         }
+        if (in) atomicAdd(&h[bin], 1);
       });
       __syncthreads();
       prefix |= (uint32_t)pick_bin<NW, 1 << BITS>(h, part_sums, need) << SHIFT;
