@@ -219,8 +219,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void part_kernel(Kv8 c, Kv8Attn a, P
     x = unit / c.n_kv;
     h = unit - x * c.n_kv;
   }
-  const Cut ct = cut<true, HD>(c, a, p, x, 0);
-  const int b = ct.b, n = ct.n, bh = b * c.n_kv + h, G = p.group;
+  // (a single sequence's queries are under way before its length is there)
+  Cut ct{};
+  if (c.batch != 1) ct = cut<true, HD>(c, a, p, x, 0);
+  const int b = ct.b, bh = b * c.n_kv + h, G = p.group;
   // this lane's columns, and its part of their q: dims 64 i + 16 kg + [0, 16) as steps 2 i and 2 i + 1
   f4_t qr[CG][DIMS / 16];
 #pragma unroll
@@ -232,7 +234,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void part_kernel(Kv8 c, Kv8Attn a, P
 #pragma unroll
       for (int e = 0; e < 4; ++e) qr[u][4 * i + e] = *reinterpret_cast<const f4_t*>(row + 64 * i + 4 * e);
   }
+  if (c.batch == 1) ct = cut<true, HD>(c, a, p, x, 0);
   if (ct.count == 0) return;  // uniform
+  const int n = ct.n;
   int t0, t1;
   tile_range(a, n, t0, t1);
   t0 += (x - ct.first) * ct.tiles;

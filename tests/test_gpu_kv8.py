@@ -413,6 +413,11 @@ def test_evict_long(gpu):
         check_evict(4, "i8", 2, 64, [40000, 33001], 20011, 4, 1024, w, in_place)
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+def test_evict_of_many_blocks(gpu, hd):
+    check_evict(5, "e4m3", 4, hd, [20000, 17001], 16500, 0, 100, some_weights(5, (2, 4, 20007)), False)
+
+
 def test_evict_keeps_a_poisoned_block_poisoned(gpu):
     ref = filled(1, 1, 1, 128, 64, "i8", [128])
     ref.scale[0][0, 0, 1] = np.nan
