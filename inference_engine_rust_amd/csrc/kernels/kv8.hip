@@ -187,12 +187,11 @@ IEK_DEV int pick_bin(const int* hist, int* sums, int& need) {
 // sign, exponent and three bits more, spread weights over many bins and so the LDS atomics; entries that
 // share the bin of their wave's first are added at once if there are many); then an entry's place is the number of
 // larger ones before it plus those of that very key, of which the first ones stay. A wave has a run of
-// entries to itself, their keys in LDS (HELD; of more than CAP entries they are read anew in every
-// pass). Bound by one workgroup's latency and instructions, so few of both: a barrier per pass, none in
-// the search of the bins, four rows of 64 entries at a time, the ends of [first, n - last) apart.
+// entries to itself, their keys in LDS. Bound by one workgroup's latency and instructions, so few of both:
+// two barriers per digit, four rows of 64 entries at a time, the ends of [first, n - last) apart.
 // counts[head] = the entries that the sequence has. In place (olds given) the scales, which the move
 // overwrites, are put by.
-template <int ST, int CAP, bool HELD>
+template <int ST, int CAP>
 __global__ __launch_bounds__(ST) void select_kernel(Kv8 src, Kv8Evict a, int* __restrict__ index,
                                                     int* __restrict__ counts, float* __restrict__ olds) {
   constexpr int NW = ST / 64, RU = 4;
@@ -206,24 +205,22 @@ __global__ __launch_bounds__(ST) void select_kernel(Kv8 src, Kv8Evict a, int* __
     for (int i = t; i < n; i += ST) idx[i] = i;
     return;
   }
-  __shared__ uint32_t keys[HELD ? CAP : 1];
+  __shared__ uint32_t keys[CAP];  // (max_len <= CAP)
   __shared__ __align__(16) int hist[4096 + 1024 + 1024];
   __shared__ int wsum[NW][2], sums[3][NW];
   const int lo = a.first, hi = n - a.last;
   const int rows = (n + ST * RU - 1) / (ST * RU) * RU;  // of 64 entries, a wave
   const int j0 = wave * rows * 64;                      // the wave's first entry
-  if (HELD) {
-    // sixteen rows in flight, those that do not exist as the last entry (keys are read again by the
-    // lane that wrote them)
-    constexpr int LU = 16;
-    for (int i = 0; i < rows; i += LU) {
-      float x[LU];
+  // sixteen rows in flight, those that do not exist as the last entry (keys are read again by the
+  // lane that wrote them)
+  constexpr int LU = 16;
+  for (int i = 0; i < rows; i += LU) {
+    float x[LU];
 #pragma unroll
-      for (int r = 0; r < LU; ++r) x[r] = w[min(j0 + 64 * (i + r) + lane, n - 1)];
+    for (int r = 0; r < LU; ++r) x[r] = w[min(j0 + 64 * (i + r) + lane, n - 1)];
 #pragma unroll
-      for (int r = 0; r < LU; ++r)
-        if (i + r < rows) keys[j0 + 64 * (i + r) + lane] = weight_key(x[r]);
-    }
+    for (int r = 0; r < LU; ++r)
+      if (i + r < rows) keys[j0 + 64 * (i + r) + lane] = weight_key(x[r]);
   }
   for (int i = t; i < 6144 / 4; i += ST) reinterpret_cast<int4*>(hist)[i] = make_int4(0, 0, 0, 0);
   if (olds) {
@@ -240,14 +237,7 @@ __global__ __launch_bounds__(ST) void select_kernel(Kv8 src, Kv8Evict a, int* __
       if (jb >= n) break;
       uint32_t k[RU];
 #pragma unroll
-      for (int r = 0; r < RU; ++r) {
-        const int j = jb + 64 * r + lane;
-        if constexpr (HELD) {
-          k[r] = keys[j];
-        } else {
-          k[r] = weight_key(w[min(j, n - 1)]);
-        }
-      }
+      for (int r = 0; r < RU; ++r) k[r] = keys[jb + 64 * r + lane];
       if (jb >= lo && jb + 64 * RU <= hi) {
 #pragma unroll
         for (int r = 0; r < RU; ++r) f(jb + 64 * r, k[r], std::true_type{});
@@ -269,13 +259,13 @@ __global__ __launch_bounds__(ST) void select_kernel(Kv8 src, Kv8Evict a, int* __
     auto digit = [&](auto shift_, auto bits_, int* h, int* part_sums) {
       constexpr int SHIFT = decltype(shift_)::value, BITS = decltype(bits_)::value;
       constexpr bool TOP = SHIFT + BITS == 32, LAST = SHIFT == 0;
-      if (HELD && LAST) unsure = 0;
+      if (LAST) unsure = 0;
       each_row([&](int j, uint32_t key, auto inner) {
         bool in = open(j, inner);
         const bool o = in;
         if constexpr (!TOP) in = in && (key ^ prefix) >> (SHIFT + BITS) == 0;
         const unsigned long long all = __ballot(in);
-        if (HELD && LAST) {
+        if (LAST) {
           if (all != 0) unsure |= 1u << ((j - j0) >> 6);
           else larger += __popcll(__ballot(o ? key > prefix : j + lane < n));
         }
@@ -306,14 +296,10 @@ __global__ __launch_bounds__(ST) void select_kernel(Kv8 src, Kv8Evict a, int* __
     larger += __popcll(__ballot(o ? key > prefix : j + lane < n));
     equal += __popcll(__ballot(o && key == prefix));
   };
-  if (HELD) {
-    for (; unsure != 0; unsure &= unsure - 1) {
-      const int i = __ffs(unsure) - 1, j = j0 + 64 * i;
-      if (i >= rows || j >= n) break;
-      count(j, keys[j + lane], std::false_type{});
-    }
-  } else {
-    each_row(count);
+  for (; unsure != 0; unsure &= unsure - 1) {
+    const int i = __ffs(unsure) - 1, j = j0 + 64 * i;
+    if (i >= rows || j >= n) break;
+    count(j, keys[j + lane], std::false_type{});
   }
   if (lane == 0) {
     wsum[wave][0] = larger;
@@ -338,6 +324,254 @@ __global__ __launch_bounds__(ST) void select_kernel(Kv8 src, Kv8Evict a, int* __
     }
     larger += __popcll(mg);
   });
+}
+
+// The same selection of long sequences by several workgroups a head, one per segment of its entries: the
+// histogram of the upper twelve bits (survey), the keys that share those of the smallest key that stays, and how many are
+// surely larger (gather), then that key from the gathered ones and the segment's places (place). Each launch
+// waits for the one before it, so this pays where one workgroup's time over the entries is more than theirs.
+constexpr int MAX_SEGS = 32, SEG_CHUNK = 4096, SEG_ROWS = SEG_CHUNK / 256;
+
+struct Segs {
+  int n, size;     // segments a head, entries a segment (whole chunks)
+  int* hist;       // [heads][n][4096]
+  uint32_t* keys;  // [heads][n][size]
+  int* found;      // [heads][n] gathered keys, then [heads][n] surely larger ones
+  int* state;      // [heads] prefix, then [heads] need
+};
+
+// The wave's sixteen rows of 64 entries of a chunk, the ones past the last as the last.
+IEK_DEV void segment_keys(const float* w, int j0, int n, uint32_t (&key)[SEG_ROWS]) {
+  float x[SEG_ROWS];
+#pragma unroll
+  for (int r = 0; r < SEG_ROWS; ++r) x[r] = w[min(j0 + 64 * r + (int)(threadIdx.x & 63), n - 1)];
+#pragma unroll
+  for (int r = 0; r < SEG_ROWS; ++r) key[r] = weight_key(x[r]);
+}
+
+__global__ __launch_bounds__(256) void survey_kernel(Kv8 src, Kv8Evict a, Segs g, int* __restrict__ counts,
+                                                     float* __restrict__ olds) {
+  const int head = blockIdx.y, s = blockIdx.x, t = threadIdx.x, lane = t & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int n = max(0, min(a.len[head / src.n_kv], a.max_len));
+  const int e0 = s * g.size, e1 = min(n, e0 + g.size), lo = a.first, hi = n - a.last;
+  if (s == 0 && t == 0) counts[head] = n;
+  if (n <= a.keep || e0 >= n) return;
+  if (olds) {
+    const int b0 = e0 / KV8_BLOCK, b1 = (e1 + KV8_BLOCK - 1) / KV8_BLOCK;
+    for (int i = b0 + t; i < b1; i += 256) {
+      olds[(size_t)head * 2 * src.nblk + i] = src.ks[(size_t)head * src.nblk + i];
+      olds[((size_t)head * 2 + 1) * src.nblk + i] = src.vs[(size_t)head * src.nblk + i];
+    }
+  }
+  if (a.keep - a.first - a.last == 0) return;
+  __shared__ __align__(16) int h[4096];
+  const float* w = a.w + (size_t)head * src.cap;
+  for (int i = t; i < 1024; i += 256) reinterpret_cast<int4*>(h)[i] = make_int4(0, 0, 0, 0);
+  __syncthreads();
+  for (int c0 = e0; c0 < e1; c0 += SEG_CHUNK) {
+    const int j0 = c0 + wave * 64 * SEG_ROWS;
+    uint32_t key[SEG_ROWS];
+    segment_keys(w, j0, n, key);
+#pragma unroll
+    for (int r = 0; r < SEG_ROWS; ++r) {
+      const int j = j0 + 64 * r + lane, bin = key[r] >> 20;
+      const bool in = j >= lo && j < hi;
+      const unsigned long long all = __ballot(in);
+      if (all == 0) continue;
+      const int bin0 = __builtin_amdgcn_readlane(bin, __ffsll(all) - 1);
+      const int same = __popcll(__ballot(bin == bin0) & all);
+      if (same >= 8) {
+        if (in && bin != bin0) atomicAdd(&h[bin], 1);
+        if (lane == 0) atomicAdd(&h[bin0], same);
+      } else if (in) {
+        atomicAdd(&h[bin], 1);
+      }
+    }
+  }
+  __syncthreads();
+  int4* out = reinterpret_cast<int4*>(g.hist + ((size_t)head * g.n + s) * 4096);
+  for (int i = t; i < 1024; i += 256) out[i] = reinterpret_cast<const int4*>(h)[i];
+}
+
+__global__ __launch_bounds__(256) void gather_kernel(Kv8 src, Kv8Evict a, Segs g) {
+  const int head = blockIdx.y, s = blockIdx.x, t = threadIdx.x, lane = t & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int n = max(0, min(a.len[head / src.n_kv], a.max_len));
+  const int e0 = s * g.size, e1 = min(n, e0 + g.size), lo = a.first, hi = n - a.last;
+  if (n <= a.keep || e0 >= n) return;
+  __shared__ __align__(16) int h[4096];
+  __shared__ int sums[4], wsum[2][4], gsum[4];
+  const float* w = a.w + (size_t)head * src.cap;
+  int need = a.keep - a.first - a.last;
+  uint32_t prefix = 0xFFFFFFFFu;
+  const bool any = need > 0;  // (else only the protected ones stay)
+  if (any) {
+    const int live = (n + g.size - 1) / g.size;
+    const int4* in = reinterpret_cast<const int4*>(g.hist + (size_t)head * g.n * 4096) + t;
+    int4 x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = make_int4(0, 0, 0, 0);
+#pragma unroll 4
+    for (int k = 0; k < live; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int4 y = in[k * 1024 + 256 * i];
+        x[i].x += y.x, x[i].y += y.y, x[i].z += y.z, x[i].w += y.w;
+      }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) reinterpret_cast<int4*>(h)[t + 256 * i] = x[i];
+    __syncthreads();
+    prefix = (uint32_t)pick_bin<4, 4096>(h, sums, need) << 20;
+  }
+  if (s == 0 && t == 0) {
+    g.state[head] = (int)prefix;
+    g.state[gridDim.y + head] = need;
+  }
+  int run = 0, larger = 0, turn = 0;
+  uint32_t* out = g.keys + ((size_t)head * g.n + s) * g.size;
+  for (int c0 = e0; c0 < e1; c0 += SEG_CHUNK, turn ^= 1) {
+    const int j0 = c0 + wave * 64 * SEG_ROWS;
+    uint32_t key[SEG_ROWS];
+    segment_keys(w, j0, n, key);
+    int mine = 0;
+#pragma unroll
+    for (int r = 0; r < SEG_ROWS; ++r) {
+      const int j = j0 + 64 * r + lane;
+      const bool o = j >= lo && j < hi;
+      mine += __popcll(__ballot(any && o && (key[r] ^ prefix) >> 20 == 0));
+      larger += __popcll(__ballot(o ? any && key[r] >> 20 > prefix >> 20 : j < n));
+    }
+    if (lane == 0) wsum[turn][wave] = mine;
+    __syncthreads();
+    int at = run;
+    for (int i = 0; i < wave; ++i) at += wsum[turn][i];
+    run += wsum[turn][0] + wsum[turn][1] + wsum[turn][2] + wsum[turn][3];
+#pragma unroll
+    for (int r = 0; r < SEG_ROWS; ++r) {
+      const int j = j0 + 64 * r + lane;
+      const bool in = any && j >= lo && j < hi && (key[r] ^ prefix) >> 20 == 0;
+      const unsigned long long m = __ballot(in);
+      if (in) out[at + __popcll(m & ((1ull << lane) - 1))] = key[r];
+      at += __popcll(m);
+    }
+  }
+  if (lane == 0) gsum[wave] = larger;
+  __syncthreads();
+  if (t == 0) {
+    const size_t at = (size_t)head * g.n + s;
+    g.found[at] = run;
+    g.found[(size_t)gridDim.y * g.n + at] = gsum[0] + gsum[1] + gsum[2] + gsum[3];
+  }
+}
+
+__global__ __launch_bounds__(256) void place_kernel(Kv8 src, Kv8Evict a, Segs g, int* __restrict__ index) {
+  const int head = blockIdx.y, s = blockIdx.x, t = threadIdx.x, lane = t & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int n = max(0, min(a.len[head / src.n_kv], a.max_len));
+  const int e0 = s * g.size, e1 = min(n, e0 + g.size), lo = a.first, hi = n - a.last;
+  int* idx = index + (size_t)head * a.keep;
+  if (n <= a.keep) {
+    for (int i = e0 + t; i < e1; i += 256) idx[i] = i;
+    return;
+  }
+  if (e0 >= n) return;
+  constexpr int LIST = 4096;
+  __shared__ __align__(16) int h[2][1024];
+  __shared__ uint32_t list[LIST];
+  __shared__ int first[MAX_SEGS], sums[2][4], wsum[2][4][2], before[4][2];
+  const float* w = a.w + (size_t)head * src.cap;
+  const int live = (n + g.size - 1) / g.size;
+  // the segments' gathered keys as one list, and what lies before this segment
+  const int mine = lane < live ? g.found[(size_t)head * g.n + lane] : 0, upto = wave_scan(mine);
+  const int sure = lane < s ? g.found[(size_t)gridDim.y * g.n + (size_t)head * g.n + lane] : 0;
+  const int listed = __builtin_amdgcn_readlane(upto, 63), own = __builtin_amdgcn_readlane(upto - mine, s);
+  int larger = __builtin_amdgcn_readlane(wave_scan(sure), 63), equal = 0;
+  uint32_t prefix = (uint32_t)g.state[head];
+  int need = g.state[gridDim.y + head];
+  for (int i = t; i < 512; i += 256) reinterpret_cast<int4*>(h[0])[i] = make_int4(0, 0, 0, 0);
+  if (t < MAX_SEGS) first[t] = upto - mine;  // (segments behind the last one: the list's end)
+  __syncthreads();
+  auto gathered = [&](int i) {  // the i-th: in the last segment that begins at or before it
+    int k = 0;
+#pragma unroll
+    for (int step = MAX_SEGS / 2; step; step >>= 1)
+      if (first[k + step] <= i) k += step;
+    return g.keys[((size_t)head * g.n + k) * g.size + i - first[k]];
+  };
+  const bool held = listed <= LIST;
+  if (held) {
+    for (int i = t; i < listed; i += 256) list[i] = gathered(i);
+    __syncthreads();
+  }
+  auto each = [&](auto f) {
+    for (int i = t; i < listed; i += 256) f(i, held ? list[i] : gathered(i));
+  };
+  if (need > 0) {
+    each([&](int, uint32_t key) { atomicAdd(&h[0][key >> 10 & 1023], 1); });
+    __syncthreads();
+    prefix |= (uint32_t)pick_bin<4, 1024>(h[0], sums[0], need) << 10;
+    each([&](int, uint32_t key) {
+      if ((key ^ prefix) >> 10 == 0) atomicAdd(&h[1][key & 1023], 1);
+    });
+    __syncthreads();
+    prefix |= (uint32_t)pick_bin<4, 1024>(h[1], sums[1], need);
+    int gb = 0, eb = 0;
+    each([&](int i, uint32_t key) {
+      gb += i < own && key > prefix;
+      eb += i < own && key == prefix;
+    });
+    gb = wave_scan(gb);
+    eb = wave_scan(eb);
+    if (lane == 63) {
+      before[wave][0] = gb;
+      before[wave][1] = eb;
+    }
+    __syncthreads();
+    for (int i = 0; i < 4; ++i) {
+      larger += before[i][0];
+      equal += before[i][1];
+    }
+  }
+  // `need` of the entries with the key `prefix` stay
+  int turn = 0;
+  for (int c0 = e0; c0 < e1; c0 += SEG_CHUNK, turn ^= 1) {
+    const int j0 = c0 + wave * 64 * SEG_ROWS;
+    uint32_t key[SEG_ROWS];
+    segment_keys(w, j0, n, key);
+    int gr = 0, er = 0;
+#pragma unroll
+    for (int r = 0; r < SEG_ROWS; ++r) {
+      const int j = j0 + 64 * r + lane;
+      const bool o = j >= lo && j < hi;
+      gr += __popcll(__ballot(o ? key[r] > prefix : j < n));
+      er += __popcll(__ballot(o && key[r] == prefix));
+    }
+    if (lane == 0) {
+      wsum[turn][wave][0] = gr;
+      wsum[turn][wave][1] = er;
+    }
+    __syncthreads();
+    int gl = larger, eq = equal;
+    for (int i = 0; i < 4; ++i) {
+      if (i < wave) {
+        gl += wsum[turn][i][0];
+        eq += wsum[turn][i][1];
+      }
+      larger += wsum[turn][i][0];
+      equal += wsum[turn][i][1];
+    }
+#pragma unroll
+    for (int r = 0; r < SEG_ROWS; ++r) {
+      const int j = j0 + 64 * r + lane;
+      const bool o = j >= lo && j < hi, gt = o ? key[r] > prefix : j < n, e = o && key[r] == prefix;
+      const unsigned long long mg = __ballot(gt), me = __ballot(e), below = (1ull << lane) - 1;
+      const int eb = eq + __popcll(me & below);
+      if (gt || (e && eb < need)) idx[gl + __popcll(mg & below) + min(eb, need)] = j;
+      gl += __popcll(mg);
+      eq += __popcll(me);
+    }
+  }
 }
 
 // Row r of the result is row idx[r] >= r of the source, its codes rounded to the block's new scale, the
@@ -452,28 +686,65 @@ void launch_kv8_load(const Kv8& c, int n, size_t stride, const int* start, const
   })
 }
 
-// [entries of each head: ints][scales put by: 2 * nblk floats a head][kept slots: keep ints a head]
+// One workgroup a head selects from up to SELECT_MOST entries, several from more: an eviction of 8 heads of 128 takes
+// 33 us either way at 32768 (of 128 heads 76 against 102), 37 against 64 at 65536, 41 against 111 at 131072.
+constexpr int SELECT_MOST = 32768;
+
 static size_t up256(size_t x) { return (x + 255) / 256 * 256; }
-static size_t evict_counts_bytes(const Kv8& c) { return up256((size_t)c.batch * c.n_kv * 4); }
-static size_t evict_scales_bytes(const Kv8& c) { return up256((size_t)c.batch * c.n_kv * 2 * c.nblk * 4); }
-size_t kv8_evict_workspace(const Kv8& src, int, int keep) {
-  return evict_counts_bytes(src) + evict_scales_bytes(src) + up256((size_t)src.batch * src.n_kv * keep * 4);
+namespace {
+// [entries of each head][scales put by: 2 * nblk floats a head][kept slots: keep ints a head][segments]
+struct EvictWs {
+  int *counts, *index;
+  float* olds;
+  bool spread;
+  Segs g;
+  size_t bytes;
+};
+EvictWs evict_ws(const Kv8& c, int max_len, int keep, void* ws) {
+  const size_t heads = (size_t)c.batch * c.n_kv;
+  char* const base = static_cast<char*>(ws);
+  EvictWs o{};
+  size_t at = 0;
+  auto part = [&](auto*& p, size_t n) {
+    p = reinterpret_cast<std::remove_reference_t<decltype(p)>>(base + at);
+    at += up256(n * 4);
+  };
+  part(o.counts, heads);
+  part(o.olds, heads * 2 * c.nblk);
+  part(o.index, heads * keep);
+  o.spread = max_len > SELECT_MOST;
+  if (o.spread) {
+    const int chunks = (max_len + SEG_CHUNK - 1) / SEG_CHUNK;
+    o.g.size = (chunks + MAX_SEGS - 1) / MAX_SEGS * SEG_CHUNK;
+    o.g.n = (max_len + o.g.size - 1) / o.g.size;
+    part(o.g.hist, heads * o.g.n * 4096);
+    part(o.g.keys, heads * o.g.n * o.g.size);
+    part(o.g.found, heads * o.g.n * 2);
+    part(o.g.state, heads * 2);
+  }
+  o.bytes = at;
+  return o;
 }
+}  // namespace
+size_t kv8_evict_workspace(const Kv8& src, int max_len, int keep) { return evict_ws(src, max_len, keep, nullptr).bytes; }
 
 void launch_kv8_evict(const Kv8& src, const Kv8& dst, const Kv8Evict& a, void* ws, hipStream_t st) {
   const int heads = src.batch * src.n_kv;
   const bool in_place = src.k == dst.k;
-  char* base = static_cast<char*>(ws);
-  int* counts = reinterpret_cast<int*>(base);
-  float* olds = reinterpret_cast<float*>(base + evict_counts_bytes(src));
-  int* index = a.index_out;
-  if (!index) index = reinterpret_cast<int*>(base + evict_counts_bytes(src) + evict_scales_bytes(src));
+  const EvictWs o = evict_ws(src, a.max_len, a.keep, ws);
+  int* const index = a.index_out ? a.index_out : o.index;
+  float* const put_by = in_place ? o.olds : nullptr;
   // Four waves up to 1024 entries, whose barriers are cheaper, sixteen above: an eviction from 8 heads of 128
   // takes 16.9 us against 17.6 at 1000 entries, 21.8 against 21.1 at 2000, 27.8 against 24.3 at 4000.
-  auto select = a.max_len <= 1024 ? select_kernel<256, 1024, true>
-                : a.max_len <= 32768 ? select_kernel<1024, 32768, true> : select_kernel<1024, 32768, false>;
-  hipLaunchKernelGGL(select, dim3(heads), dim3(a.max_len <= 1024 ? 256 : 1024), 0, st, src, a, index, counts,
-                     in_place ? olds : nullptr);
+  auto select = a.max_len <= 1024 ? select_kernel<256, 1024> : select_kernel<1024, SELECT_MOST>;
+  if (o.spread) {
+    const dim3 grid((unsigned)o.g.n, (unsigned)heads);
+    hipLaunchKernelGGL(survey_kernel, grid, dim3(256), 0, st, src, a, o.g, o.counts, put_by);
+    hipLaunchKernelGGL(gather_kernel, grid, dim3(256), 0, st, src, a, o.g);
+    hipLaunchKernelGGL(place_kernel, grid, dim3(256), 0, st, src, a, o.g, index);
+  } else {
+    hipLaunchKernelGGL(select, dim3(heads), dim3(a.max_len <= 1024 ? 256 : 1024), 0, st, src, a, index, o.counts, put_by);
+  }
   // Not in place a wave takes 128 bytes a row (the lines of L2), one block where all waves fit the chip at once
   // (1024 entries of 8 heads of 128: 18.9 us against 20.0 for the eviction), else two (8192 of 24 heads: 102 against 104).
   const int sw = in_place || src.hd == 64 ? 64 : 128, slices = 2 * src.hd / sw;
@@ -487,7 +758,7 @@ void launch_kv8_evict(const Kv8& src, const Kv8& dst, const Kv8Evict& a, void* w
   else if (mb == 1) fn = src.e4m3 ? move_kernel<true, 128, false, 1> : move_kernel<false, 128, false, 1>;
   else fn = src.e4m3 ? move_kernel<true, 128, false, 2> : move_kernel<false, 128, false, 2>;
   hipLaunchKernelGGL(fn, dim3((unsigned)heads * slices * parts), dim3(in_place ? 1024 : 256), 0, st, src, dst,
-                     a, index, counts, olds, parts);
+                     a, index, o.counts, o.olds, parts);
 }
 
 }  // namespace iek

@@ -413,6 +413,15 @@ def test_evict_long(gpu):
         check_evict(4, "i8", 2, 64, [40000, 33001], 20011, 4, 1024, w, in_place)
 
 
+@pytest.mark.parametrize("in_place", [False, True])
+def test_evict_very_long(gpu, in_place):
+    """Segments of more than one piece; the smallest weight that stays is one of very many, or one of few."""
+    w = some_weights(7, (2, 1, 140008))
+    w[1] = np.exp(np.random.default_rng(8).standard_normal(140008)).astype(np.float32)
+    check_evict(4, "i8", 1, 64, [140001, 131000], 70001, 3, 50, w, in_place)
+    check_evict(4, "i8", 1, 64, [33000, 0, 900, 32769], 1000, 1000, 0, some_weights(9, (4, 1, 33007)), in_place)
+
+
 @pytest.mark.parametrize("hd", [64, 128])
 def test_evict_of_many_blocks(gpu, hd):
     check_evict(5, "e4m3", 4, hd, [20000, 17001], 16500, 0, 100, some_weights(5, (2, 4, 20007)), False)
