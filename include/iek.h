@@ -312,7 +312,7 @@ iek_status iek_dev_attention_decode_noalloc(const float* q, const void* k_cache,
  * with workspaces and outputs of their own may overlap. IEK_ERR_OP for null or misaligned pointers
  * and unsupported shapes: head_dim 64, 128, 256 or 512, n_heads / n_kv_heads <= 8, row strides in
  * floats, multiples of 4 and not below a row; f32 rows and workspaces 16-byte aligned; at most 2^26
- * slots, 65535 sequences and 65536 KV heads in all. What a call writes must not overlap what it reads,
+ * slots and 65535 sequences times KV heads. What a call writes must not overlap what it reads,
  * but where this says so. A batch, n or n_q of 0 does nothing. */
 #define IEK_KV8_BLOCK 32
 typedef struct iek_kv8 {

@@ -677,7 +677,7 @@ static Kv8 kv8_view(const iek_kv8* c, bool buffers = true) {
     fail(ST_OP, "kv8: head_dim must be 64, 128, 256 or 512");
   if (c->n_kv_heads == 0 || c->capacity == 0) fail(ST_OP, "kv8: no KV heads or no capacity");
   // (so that every grid is within 2^32 threads a dimension)
-  if (c->n_kv_heads > 4096 || c->batch > 65535 || c->capacity > (1u << 26) || c->batch * c->n_kv_heads > (1u << 16))
+  if (c->n_kv_heads > 4096 || c->batch > 65535 || c->capacity > (1u << 26) || c->batch * c->n_kv_heads > 65535)
     fail(ST_OP, "kv8: dims too large");
   if (buffers) {
     aligned(c->k, 16, "k");

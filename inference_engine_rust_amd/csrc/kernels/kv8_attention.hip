@@ -50,6 +50,7 @@ constexpr int SHARED_BATCH = 64;
 
 struct Plan {
   int group, cols, cblocks;  // query heads and columns of a KV head, workgroups the columns are spread over
+  int groups;                // of eight columns a workgroup
   int share;                 // chunks of a KV head to aim at; 0: sequences are cut by `tiles`
   int tiles, nsplit;         // share 0: tiles a chunk, chunks a sequence at most; else the smallest chunk
   int chunks;                // of a KV head at most
@@ -682,15 +683,23 @@ __global__ __launch_bounds__(256) void join_kernel(Kv8 c, Kv8Attn a, Plan p, int
 
 size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
-// Column groups of eight per workgroup: two where there are more than eight columns.
-int col_groups(int cols) { return cols > 8 ? 2 : 1; }
+// Column groups of eight per workgroup. Two share the reading and the conversion of the codes, and take twice
+// the registers and twice as long over a tile: they pay where the workgroups of one group each would go
+// through more than ten times the chip (five tokens, 8 sequences of 4000 keys of 8 heads of 128: 38 us against 41;
+// sixteen, 16 of 4000 of 256: 69 against 96; but five, 4 of 3001 of 64: 12.0 against 10.8).
+int col_groups(const Kv8& c, int cols, int tiles) {
+  const int tw = tile_waves(c.hd);
+  const long long turns = (long long)c.batch * c.n_kv * ((cols + 7) / 8) * ((tiles + tw - 1) / tw);
+  return cols > 8 && turns > 10 * 512 ? 2 : 1;
+}
 
 // The plan for sequences whose columns see at most `tiles` tiles; more of them never need less.
 Plan make_plan(const Kv8& c, int n_heads, int n_q, int tiles) {
   Plan p{};
   p.group = n_heads / c.n_kv;
   p.cols = p.group * n_q;
-  const int per = 8 * col_groups(p.cols), tw = tile_waves(c.hd);
+  p.groups = col_groups(c, p.cols, tiles);
+  const int per = 8 * p.groups, tw = tile_waves(c.hd);
   p.cblocks = (p.cols + per - 1) / per;
   // Chunks that fill the chip once, two workgroups a CU. Up to two rounds of the waves the second one costs
   // less than the joining of two chunks.
@@ -726,7 +735,7 @@ template <int HD, int CG>
 void launch_cg(const Kv8& c, const Kv8Attn& a, const Plan& p, hipStream_t st) {
   const long long part = ((long long)p.chunks * c.n_kv + 7) / 8 * 8 * p.cblocks;
   const dim3 grid = p.cblocks == 1 ? dim3((unsigned)c.n_kv, (unsigned)p.chunks) : dim3((unsigned)part);
-  const bool many = CG > 1;  // (more than eight columns)
+  const bool many = p.cols > 8;
   const long long ncol = p.direct ? 0 : (long long)c.batch * c.n_kv * (HD / 64) * (many ? (p.cols + 3) / 4 : p.cols);
   const int wblocks = a.w_out ? (a.max_len + (many ? 255 : 1023)) / (many ? 256 : 1024) : 0;
   const long long join = ncol + (long long)c.batch * c.n_kv * wblocks;
@@ -734,12 +743,12 @@ void launch_cg(const Kv8& c, const Kv8Attn& a, const Plan& p, hipStream_t st) {
   auto fn = c.e4m3 ? part_kernel<HD, true, CG> : part_kernel<HD, false, CG>;
   hipLaunchKernelGGL(fn, grid, dim3(64 * WAVES), 0, st, c, a, p);
   if (join)
-    hipLaunchKernelGGL((join_kernel<HD, (CG > 1)>), dim3((unsigned)join), dim3(256), 0, st, c, a, p, (int)ncol, wblocks);
+    hipLaunchKernelGGL((many ? join_kernel<HD, true> : join_kernel<HD, false>), dim3((unsigned)join), dim3(256), 0, st, c, a, p, (int)ncol, wblocks);
 }
 
 }  // namespace
 
-// For any window: fewer tiles do not take more chunks.
+// For any window: fewer tiles do not take more chunks, nor do smaller column groups.
 size_t kv8_attention_workspace(const Kv8& c, int n_heads, int n_q, int max_len, bool weights) {
   if (c.batch == 0 || n_q == 0) return 0;
   const int tiles = (max_len + TILE - 1) / TILE;
@@ -758,7 +767,7 @@ void launch_kv8_attention(const Kv8& c, const Kv8Attn& a, void* ws, hipStream_t 
   p.ml = reinterpret_cast<float*>(base);
   p.o = reinterpret_cast<float*>(base + z.ml);
   p.s = a.w_out ? reinterpret_cast<float*>(base + z.ml + z.o) : nullptr;
-  const bool two = col_groups(p.cols) == 2;
+  const bool two = p.groups == 2;
   switch (c.hd) {
     case 64: two ? launch_cg<64, 2>(c, a, p, st) : launch_cg<64, 1>(c, a, p, st); break;
     case 128: two ? launch_cg<128, 2>(c, a, p, st) : launch_cg<128, 1>(c, a, p, st); break;

@@ -253,6 +253,14 @@ def test_attention_several_tokens(gpu, dtype, window, hd, kv, group, n_q):
     check_attention(n_q, dtype, kv, group, hd, n_q, [0, 1, n_q - 1, n_q, 40, 300], window)
 
 
+@pytest.mark.parametrize("hd,kv,group,n_q,lens", [(64, 2, 8, 9, [4000, 0, 3111]), (128, 1, 8, 33, [5000, 40, 1701]),
+                                                  (256, 1, 5, 21, [3000, 1, 2222]), (512, 1, 8, 16, [1500, 700, 15])])
+@pytest.mark.parametrize("window", [0, 40, 1400])
+def test_attention_several_tokens_long(gpu, hd, kv, group, n_q, lens, window):
+    """Enough work for the workgroups that take sixteen columns (without a window and with a long one)."""
+    check_attention(hd + window, "e4m3" if window else "i8", kv, group, hd, n_q, lens * 8, window)
+
+
 @pytest.mark.parametrize("window", [1, 31, 32, 33, 512, 513])
 @pytest.mark.parametrize("hd", [64, 256])
 def test_attention_window(gpu, window, hd):
