@@ -76,6 +76,12 @@ struct Cut {
   int b, n, tiles, count, first;
 };
 IEK_DEV int ceil_div(int a, int b) { return (int)(((unsigned)a + b - 1) / (unsigned)b); }
+// the same for tiles of one sequence (below 2^22, so that the product with the reciprocal is off by less than one)
+IEK_DEV int ceil_div_tiles(int a, int b) {
+  const int up = a + b - 1, q = (int)((float)up * __builtin_amdgcn_rcpf((float)b)), r = up - q * b;
+  return q + (r >= b ? 1 : 0) - (r < 0 ? 1 : 0);
+}
+IEK_DEV int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 template <bool FIND, int HD>
 IEK_DEV Cut cut(const Kv8& c, const Kv8Attn& a, const Plan& p, int x, int b) {
   constexpr int TW = tile_waves(HD);
@@ -86,8 +92,8 @@ IEK_DEV Cut cut(const Kv8& c, const Kv8Attn& a, const Plan& p, int x, int b) {
     r.n = entries(a, r.b);
     tile_range(a, r.n, t0, t1);
     if (p.share != 0)
-      r.tiles = max(p.tiles, ceil_div(ceil_div(t1 - t0, min(p.share, MAX_SPLIT)), TW) * TW);
-    r.count = max(1, ceil_div(t1 - t0, r.tiles));
+      r.tiles = max(p.tiles, ceil_div(uniform(ceil_div_tiles(t1 - t0, min(p.share, MAX_SPLIT))), TW) * TW);
+    r.count = max(1, uniform(ceil_div_tiles(t1 - t0, r.tiles)));
     r.first = r.b * p.nsplit;
     if (FIND && x - r.first >= r.count) r.count = 0;
     return r;
@@ -97,14 +103,11 @@ IEK_DEV Cut cut(const Kv8& c, const Kv8Attn& a, const Plan& p, int x, int b) {
   tile_range(a, n, t0, t1);
   const int each = lane < c.batch ? t1 - t0 : 0;
   const int total = __builtin_amdgcn_readlane(wave_scan(each), 63);
-  int most = each;
-#pragma unroll
-  for (int o = 32; o; o >>= 1) most = max(most, __shfl_xor(most, o));
-  most = __builtin_amdgcn_readfirstlane(most);
+  const int most = (int)wave_max((float)each);  // (exact: a sequence has at most 2^21 tiles)
   const int aim = max(p.share - c.batch / 2, (p.share + 1) / 2);
   const int size = max(p.tiles, ceil_div(max(ceil_div(total, aim), ceil_div(most, MAX_SPLIT)), TW) * TW);
-  const int even = max(p.tiles, ceil_div(ceil_div(each, max(1, ceil_div(each, size))), TW) * TW);
-  const int mine = lane < c.batch ? max(1, ceil_div(each, even)) : 0, upto = wave_scan(mine);
+  const int even = max(p.tiles, ceil_div(ceil_div_tiles(each, max(1, ceil_div_tiles(each, size))), TW) * TW);
+  const int mine = lane < c.batch ? max(1, ceil_div_tiles(each, even)) : 0, upto = wave_scan(mine);
   if (FIND) r.b = __popcll(__ballot(lane < c.batch && upto - mine <= x)) - 1;
   r.n = __builtin_amdgcn_readlane(n, r.b);
   r.tiles = __builtin_amdgcn_readlane(even, r.b);
