@@ -43,9 +43,9 @@ constexpr int tile_waves(int hd) { return WAVES * dims_of(hd) / hd; }
 // lengths themselves (a launch is sized for max_len, and may be a captured one): the total over the
 // sequences by the chunks that fill the chip (half of one a sequence is lost to its last chunk), then
 // each sequence evenly into as many as that takes: a batch of ragged lengths is spread evenly, and a
-// short sequence in a large cache finely (16 sequences up to 8223 keys, cut by max_len 48 us, so 38).
-// Chunk x of a KV head is chunk cp of sequence b by the running sum of
-// their counts; a sequence without entries has one, which writes zeros. Larger batches are cut by max_len.
+// short sequence in a large cache finely (16 sequences up to 8223 keys, cut by max_len 48 us, so 36). A
+// chunk's number is its place in the running sum of the sequences' counts; a sequence without entries has
+// one chunk, which writes zeros. Larger batches are cut by max_len.
 constexpr int SHARED_BATCH = 64;
 
 struct Plan {
