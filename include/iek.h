@@ -326,8 +326,9 @@ typedef struct iek_kv8 {
  * go to slots start[b] + i (start NULL: 0). Rows past the capacity are dropped, and all rows of a
  * sequence whose start is negative or past it. The slots behind the new rows no longer hold anything,
  * those before start in the same block keep their values (their codes are rounded again when the
- * block's scale grows). An infinity or NaN makes its block's scale NaN, and so whatever attends to
- * the block. len_out (or NULL): the lengths after the append; may be start itself, and must not
+ * block's scale grows). An infinity or NaN makes its block's scale NaN, and so all its rows, until
+ * the block's first slot is written again: queries that see one of them get NaN, the others nothing of
+ * it. (Codes are what these entries write: an E4M3 code that is NaN belongs to a NaN scale.) len_out (or NULL): the lengths after the append; may be start itself, and must not
  * overlap it otherwise. weights (or NULL): [batch][n_kv_heads][capacity] running attention weights,
  * set to 0 for the new rows. IEK_ERR_KV_CACHE when n > capacity. */
 iek_status iek_dev_kv8_append(const iek_kv8* cache, const float* k, const float* v, size_t n, size_t row_stride,

@@ -398,8 +398,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void part_kernel(Kv8 c, Kv8Attn a, P
         x[i] = __builtin_amdgcn_exp2f(s[u][i] - ref + 14.f);
         sum += x[i];
       }
-      l[u] += sum * fac[u];
-      fac[u] *= T.vs;
+      l[u] += sum * fac[u];  // (NaN with a NaN among the scores, also if the largest of the others is -inf)
+      fac[u] = top == -INFINITY ? 0.f : fac[u] * T.vs;  // (a column that sees none of the block takes no NaN from it)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const h2_t e = {(_Float16)x[2 * i], (_Float16)x[2 * i + 1]};
@@ -407,6 +407,13 @@ __global__ __launch_bounds__(64 * WAVES, 2) void part_kernel(Kv8 c, Kv8Attn a, P
                         (_Float16)fmaf((float)e[1], rest, x[2 * i + 1] * keep)};
         pr[u][i] = __builtin_bit_cast(uint32_t, f);
       }
+    }
+    // Codes of a block with a NaN scale may be NaN (e4m3), times a weight of 0 too: the scale alone is to tell.
+    if (E4M3 && isnan(__uint_as_float(uniform(__float_as_uint(T.vs))))) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int w = 0; w < VW; ++w) T.v[j][w] = 0;
     }
 #pragma unroll
     for (int w = 0; w < VW; ++w) {

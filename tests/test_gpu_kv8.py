@@ -618,3 +618,51 @@ def test_offsets_beyond_32_bits(gpu):
     want, _, bound = ref.attention(q, [0, 64, 64], 0, 0.04)
     got = host(res).reshape(batch, 1, 8, hd)
     assert (np.abs(got - want) <= bound).all()
+
+
+# ---- blocks that hold an infinity or NaN, and queries that see none of them ----
+
+def poisoned(seed, dtype, kv, group, hd, n_q, lens, at, which, window):
+    """A cache whose slot at[b] of KV head kv - 1 (None: none) was appended with an infinity in K or V; queries; the reference."""
+    rng = np.random.default_rng(seed)
+    batch, cap = len(lens), max(lens) + 5
+    ref, d = kv8_ref.Cache(batch, kv, cap, hd, dtype), Dev(batch, kv, cap, hd, dtype)
+    x = rng.standard_normal((2, batch, cap, kv, hd)).astype(np.float32)
+    for b, j in enumerate(at):
+        if j is not None:
+            x[which, b, j, kv - 1, 3] = np.inf
+    k, v = dev(x[0]), dev(x[1])
+    E.kv8_append(d.h, k.data_ptr(), v.data_ptr(), cap, kv * hd, 0, ints(lens).data_ptr(), 0, 0, stream())
+    ref.append(x[0], x[1], [0] * batch, lens)
+    q = rng.standard_normal((batch, n_q, kv * group, hd)).astype(np.float32)
+    return ref, d, q, ref.attention(q, lens, window, 0.1)
+
+
+def same_nan_and_near(got, want, bound):
+    assert np.array_equal(np.isnan(got), np.isnan(want)), np.argwhere(np.isnan(got) != np.isnan(want))[:5]
+    ok = ~np.isnan(want)
+    assert (np.abs(got - want) <= bound)[ok].all()
+    return ok
+
+
+BLIND = [  # (KV heads, group, head_dim, query tokens, lengths, the poisoned slots, window)
+    # a block that begins with the last two of three tokens: the first sees none of it; in one chunk, and joined
+    *[(2, 2, hd, 3, [32 * m + 2], [32 * m], 0) for hd in (64, 128, 256, 512) for m in (1, 70)],
+    # a block whose last slot is the first that the first token's window holds: the others see none of it
+    *[(1, 4, hd, 3, [32 * 9 - 1 + w + 2], [32 * 8 + 5], w) for hd in (64, 128, 256, 512) for w in (40, 1400)],
+    # sequences beside it, tokens with no entries at all, a poisoned block that is everything
+    (2, 4, 128, 5, [0, 3, 34, 35, 700, 33], [None, 1, 32, 32, 672, 0], 0),
+    # sixteen columns a workgroup
+    (2, 8, 64, 9, [4001, 0, 3113] * 8, [4000, None, 3104] * 8, 0),
+    (1, 8, 128, 33, [4015, 41, 2975] * 8, [4000, 32, 2944] * 8, 0),
+]
+
+
+@pytest.mark.parametrize("dtype", ["i8", "e4m3"])
+@pytest.mark.parametrize("which", [0, 1], ids=["k", "v"])
+@pytest.mark.parametrize("kv,group,hd,n_q,lens,at,window", BLIND)
+def test_attention_of_tokens_that_see_none_of_a_poisoned_block(gpu, kv, group, hd, n_q, lens, at, window, which, dtype):
+    ref, d, q, (want, _, bound) = poisoned(hd, dtype, kv, group, hd, n_q, lens, at, which, window)
+    got, _ = attend(d, q, lens, window, 0.1)
+    ok = same_nan_and_near(got, want, bound)
+    assert not ok.all() and ok.any()
