@@ -348,7 +348,7 @@ iek_status iek_dev_kv8_load(const iek_kv8* cache, size_t n, size_t row_stride, c
  * being h / (n_heads / n_kv_heads); zeros where there are none. Entries from len[b] on may hold
  * anything. weights_out (or NULL): [batch][n_kv_heads][capacity], for j < len[b]
  * weights_out[j] = weights_in[j] + the attention weight of entry j summed over the KV head's query
- * heads and the n_q tokens; weights_in may be weights_out itself, or NULL for zeros. workspace:
+ * heads and the n_q tokens (a token with a NaN score: NaN for the entries it sees); weights_in may be weights_out itself, or NULL for zeros. workspace:
  * iek_kv8_attention_workspace bytes for the same arguments, its contents of no matter. */
 iek_status iek_kv8_attention_workspace(const iek_kv8* cache, size_t n_heads, size_t n_q, size_t max_len,
                                        int with_weights, size_t* bytes);

@@ -14,6 +14,8 @@
 // Nothing is staged in LDS before the end of a chunk. q is scaled by a power of two into fp16's range,
 // P by 2^14 relative to its block's largest score of the column, so that neither can leave it: the
 // factor between the block's and the running maximum, and V's scale, are applied to the f32 products.
+#include <cfloat>
+
 #include "common.cuh"
 #include "kv8.h"
 #include "kv8_codes.cuh"
@@ -525,6 +527,13 @@ IEK_DEV void column_sum(const float* ml, size_t step, int count, float (&m)[MAX_
   sum = wave_sum(sum);
 }
 
+// A column's largest score and sum as m and r, with which an entry's weight is 2^(score - m) r. Out of the column's
+// sight scores are -inf and weights 0; a NaN sum makes NaN (infinity times 0) of all others and of them nothing.
+IEK_DEV void share_terms(float top, float sum, float& m, float& r) {
+  m = isnan(sum) ? -FLT_MAX : top == -INFINITY ? 0.f : top;
+  r = isnan(sum) || sum == 0.f ? 0.f : 1.f / sum;
+}
+
 // The join. Workgroups [0, ncol), unless the chunks have written the output themselves: 64 dims of a
 // column, sixteen chunks at a time; those behind them: the weights of 1024 entries of a KV head. MANY
 // (several query tokens: many columns of few chunks, where workgroups are what costs): 64 dims of four
@@ -643,10 +652,7 @@ __global__ __launch_bounds__(256) void join_kernel(Kv8 c, Kv8Attn a, Plan p, int
     for (int col = wave; col < p.cols; col += 4) {
       float m[MAX_SPLIT / 64], top, sum;
       column_sum(ml0 + 2 * col, step, ct.count, m, top, sum);
-      if (lane == 0) {
-        cm[col] = top == -INFINITY ? 0.f : top;  // (a column that sees nothing has only scores of -inf)
-        cl[col] = sum == 0.f ? 0.f : 1.f / sum;
-      }
+      if (lane == 0) share_terms(top, sum, cm[col], cl[col]);
     }
   } else {
     for (int col = t; col < p.cols; col += 256) {
@@ -658,8 +664,7 @@ __global__ __launch_bounds__(256) void join_kernel(Kv8 c, Kv8Attn a, Plan p, int
         const float m = ml0[2 * (k * step + col)], l = ml0[2 * (k * step + col) + 1];
         sum += m == -INFINITY ? 0.f : l * __builtin_amdgcn_exp2f(m - top);
       }
-      cm[col] = top == -INFINITY ? 0.f : top;
-      cl[col] = sum == 0.f ? 0.f : 1.f / sum;
+      share_terms(top, sum, cm[col], cl[col]);
     }
   }
   __syncthreads();

@@ -666,3 +666,29 @@ def test_attention_of_tokens_that_see_none_of_a_poisoned_block(gpu, kv, group, h
     got, _ = attend(d, q, lens, window, 0.1)
     ok = same_nan_and_near(got, want, bound)
     assert not ok.all() and ok.any()
+
+
+@pytest.mark.parametrize("dtype", ["i8", "e4m3"])
+@pytest.mark.parametrize("where", ["k", "v", "q"])
+@pytest.mark.parametrize("kv,group,hd,n_q,lens,at,window", BLIND)
+def test_weights_of_entries_that_a_nan_token_does_not_see(gpu, kv, group, hd, n_q, lens, at, window, where, dtype):
+    """A token whose scores are NaN (a NaN in its query, or in a key it sees) gives NaN to the entries it sees and
+    nothing to the others; a NaN value gives none."""
+    ref, d, q, (want, w, bound) = poisoned(hd, dtype, kv, group, hd, n_q, lens, at if where != "q" else [None] * len(lens),
+                                           int(where == "v"), window)
+    if where == "q":
+        q[:, 0, 1, 5] = np.nan  # (the first token of a draft does not see the last entries, nor with a window all the first)
+        want, w, bound = ref.attention(q, lens, window, 0.1)
+    w_out = torch.full(w.shape, -4.0, device="cuda")
+    got, _ = attend(d, q, lens, window, 0.1, None, w_out)
+    same_nan_and_near(got, want, bound)
+    got = host(w_out)
+    for b, n in enumerate(lens):
+        assert (got[b, :, n:] == -4).all()
+        a, z = got[b, :, :n], w[b, :, :n]
+        assert np.array_equal(np.isnan(a), np.isnan(z)), (b, np.argwhere(np.isnan(a) != np.isnan(z))[:4])
+        ok = ~np.isnan(z)
+        # (relative error of a share as in check_attention)
+        keys = max([np.nanmax(np.abs(ref.value(0, b, h, n)), initial=0) for h in range(kv)])
+        rel = (2 * (hd + 16) * 0.1 * np.nanmax(np.abs(q[b]).sum(-1)) * keys + 32 + n / 32 + 300 + group * n_q) * 2.0 ** -24
+        assert (np.abs(a - z) <= rel * z + 1e-30)[ok].all()
