@@ -182,6 +182,20 @@ IEK_DEV int pick_bin(const int* hist, int* sums, int& need) {
   return bin;
 }
 
+// Adds the wave's lanes with `in` to their bins, those that share the first one's bin at once if there are many.
+IEK_DEV void add_bins(int* hist, int bin, bool in) {
+  const unsigned long long all = __ballot(in);
+  if (all == 0) return;
+  const int bin0 = __builtin_amdgcn_readlane(bin, __ffsll(all) - 1);
+  const int same = __popcll(__ballot(bin == bin0) & all);
+  if (same >= 8) {
+    if (in && bin != bin0) atomicAdd(&hist[bin], 1);
+    if ((threadIdx.x & 63) == 0) atomicAdd(&hist[bin0], same);
+  } else if (in) {
+    atomicAdd(&hist[bin], 1);
+  }
+}
+
 // One workgroup per (sequence, KV head): the slots of the entries that stay, in order. The smallest
 // key that stays is found by histograms of its bits from the top, 12, 10 and 10 at a time (12 at first,
 // sign, exponent and three bits more, spread weights over many bins and so the LDS atomics; entries that
@@ -327,14 +341,17 @@ __global__ __launch_bounds__(ST) void select_kernel(Kv8 src, Kv8Evict a, int* __
 }
 
 // The same selection of long sequences by several workgroups a head, one per segment of its entries: the
-// histogram of the upper twelve bits (survey), the keys that share those of the smallest key that stays, and how many are
-// surely larger (gather), then that key from the gathered ones and the segment's places (place). Each launch
+// histogram of the upper twelve bits (survey), the keys that share those of the smallest key that stays, a histogram of
+// their next ten, and how many are surely larger (gather), then that key from the gathered ones and the segment's places
+// (place). There every workgroup goes through all gathered keys, which are most of the entries where most weights are equal
+// (those of fresh entries are zeros): once only, and those of a common value are counted in registers. Each launch
 // waits for the one before it, so this pays where one workgroup's time over the entries is more than theirs.
 constexpr int MAX_SEGS = 32, SEG_CHUNK = 4096, SEG_ROWS = SEG_CHUNK / 256;
 
 struct Segs {
   int n, size;     // segments a head, entries a segment (whole chunks)
   int* hist;       // [heads][n][4096]
+  int* next;       // [heads][n][1024], of the gathered keys
   uint32_t* keys;  // [heads][n][size]
   int* found;      // [heads][n] gathered keys, then [heads][n] surely larger ones
   int* state;      // [heads] prefix, then [heads] need
@@ -375,18 +392,8 @@ __global__ __launch_bounds__(256) void survey_kernel(Kv8 src, Kv8Evict a, Segs g
     segment_keys(w, j0, n, key);
 #pragma unroll
     for (int r = 0; r < SEG_ROWS; ++r) {
-      const int j = j0 + 64 * r + lane, bin = key[r] >> 20;
-      const bool in = j >= lo && j < hi;
-      const unsigned long long all = __ballot(in);
-      if (all == 0) continue;
-      const int bin0 = __builtin_amdgcn_readlane(bin, __ffsll(all) - 1);
-      const int same = __popcll(__ballot(bin == bin0) & all);
-      if (same >= 8) {
-        if (in && bin != bin0) atomicAdd(&h[bin], 1);
-        if (lane == 0) atomicAdd(&h[bin0], same);
-      } else if (in) {
-        atomicAdd(&h[bin], 1);
-      }
+      const int j = j0 + 64 * r + lane;
+      add_bins(h, key[r] >> 20, j >= lo && j < hi);
     }
   }
   __syncthreads();
@@ -401,6 +408,7 @@ __global__ __launch_bounds__(256) void gather_kernel(Kv8 src, Kv8Evict a, Segs g
   const int e0 = s * g.size, e1 = min(n, e0 + g.size), lo = a.first, hi = n - a.last;
   if (n <= a.keep || e0 >= n) return;
   __shared__ __align__(16) int h[4096];
+  __shared__ __align__(16) int h2[1024];
   __shared__ int sums[4], wsum[2][4], gsum[4];
   const float* w = a.w + (size_t)head * src.cap;
   int need = a.keep - a.first - a.last;
@@ -421,6 +429,7 @@ __global__ __launch_bounds__(256) void gather_kernel(Kv8 src, Kv8Evict a, Segs g
       }
 #pragma unroll
     for (int i = 0; i < 4; ++i) reinterpret_cast<int4*>(h)[t + 256 * i] = x[i];
+    reinterpret_cast<int4*>(h2)[t] = make_int4(0, 0, 0, 0);
     __syncthreads();
     prefix = (uint32_t)pick_bin<4, 4096>(h, sums, need) << 20;
   }
@@ -447,6 +456,7 @@ __global__ __launch_bounds__(256) void gather_kernel(Kv8 src, Kv8Evict a, Segs g
     int at = run;
     for (int i = 0; i < wave; ++i) at += wsum[turn][i];
     run += wsum[turn][0] + wsum[turn][1] + wsum[turn][2] + wsum[turn][3];
+    const bool few = mine <= 64;  // (of the wave's 1024)
 #pragma unroll
     for (int r = 0; r < SEG_ROWS; ++r) {
       const int j = j0 + 64 * r + lane;
@@ -454,10 +464,14 @@ __global__ __launch_bounds__(256) void gather_kernel(Kv8 src, Kv8Evict a, Segs g
       const unsigned long long m = __ballot(in);
       if (in) out[at + __popcll(m & ((1ull << lane) - 1))] = key[r];
       at += __popcll(m);
+      const int bin = key[r] >> 10 & 1023;
+      if (!few) add_bins(h2, bin, in);
+      else if (in) atomicAdd(&h2[bin], 1);
     }
   }
   if (lane == 0) gsum[wave] = larger;
   __syncthreads();
+  if (any) reinterpret_cast<int4*>(g.next + ((size_t)head * g.n + s) * 1024)[t] = reinterpret_cast<const int4*>(h2)[t];
   if (t == 0) {
     const size_t at = (size_t)head * g.n + s;
     g.found[at] = run;
@@ -476,62 +490,112 @@ __global__ __launch_bounds__(256) void place_kernel(Kv8 src, Kv8Evict a, Segs g,
     return;
   }
   if (e0 >= n) return;
-  constexpr int LIST = 4096;
-  __shared__ __align__(16) int h[2][1024];
-  __shared__ uint32_t list[LIST];
-  __shared__ int first[MAX_SEGS], sums[2][4], wsum[2][4][2], before[4][2];
+  constexpr int BATCH = 4096;  // keys at a time
+  __shared__ __align__(16) int h[2][2][1024];
+  __shared__ int first[MAX_SEGS + 1], sums[2][4], wsum[2][4][2], before[4];
   const float* w = a.w + (size_t)head * src.cap;
   const int live = (n + g.size - 1) / g.size;
   // the segments' gathered keys as one list, and what lies before this segment
   const int mine = lane < live ? g.found[(size_t)head * g.n + lane] : 0, upto = wave_scan(mine);
   const int sure = lane < s ? g.found[(size_t)gridDim.y * g.n + (size_t)head * g.n + lane] : 0;
-  const int listed = __builtin_amdgcn_readlane(upto, 63), own = __builtin_amdgcn_readlane(upto - mine, s);
+  const int listed = __builtin_amdgcn_readlane(upto, 63);
   int larger = __builtin_amdgcn_readlane(wave_scan(sure), 63), equal = 0;
   uint32_t prefix = (uint32_t)g.state[head];
   int need = g.state[gridDim.y + head];
-  for (int i = t; i < 512; i += 256) reinterpret_cast<int4*>(h[0])[i] = make_int4(0, 0, 0, 0);
-  if (t < MAX_SEGS) first[t] = upto - mine;  // (segments behind the last one: the list's end)
+  for (int i = t; i < 1024; i += 256) reinterpret_cast<int4*>(h[0][0])[i] = make_int4(0, 0, 0, 0);
+  if (t <= MAX_SEGS) first[t] = upto - mine;  // (segments behind the last one: the list's end)
   __syncthreads();
-  auto gathered = [&](int i) {  // the i-th: in the last segment that begins at or before it
-    int k = 0;
-#pragma unroll
-    for (int step = MAX_SEGS / 2; step; step >>= 1)
-      if (first[k + step] <= i) k += step;
-    return g.keys[((size_t)head * g.n + k) * g.size + i - first[k]];
-  };
-  const bool held = listed <= LIST;
-  if (held) {
-    for (int i = t; i < listed; i += 256) list[i] = gathered(i);
-    __syncthreads();
-  }
-  auto each = [&](auto f) {
-    for (int i = t; i < listed; i += 256) f(i, held ? list[i] : gathered(i));
-  };
   if (need > 0) {
-    each([&](int, uint32_t key) { atomicAdd(&h[0][key >> 10 & 1023], 1); });
+    // Sixteen keys a lane, of which those that share the digits above are added to the bins of the digit at `shift`, of
+    // all and of those before this segment. A value that many have is counted in registers.
+    auto place = [&](int i0, int q) { return i0 + 1024 * (q >> 2) + 4 * t + (q & 3); };
+    auto add = [&](const uint32_t(&key)[16], int i0, int end, int prior_end, int shift, int(&bins)[2][1024]) {
+      auto in = [&](int q) { return place(i0, q) < end && (key[q] ^ prefix) >> shift >> 10 == 0; };
+      int some = -1;
+#pragma unroll
+      for (int q = 0; q < 16; ++q) {
+        if (i0 + 1024 * (q >> 2) >= end) break;  // uniform
+        if (in(q)) some = key[q] >> shift & 1023;
+      }
+      const unsigned long long any = __ballot(some >= 0);
+      if (any == 0) return;
+      const int common = __builtin_amdgcn_readlane(some, __ffsll(any) - 1);
+      int many = 0;  // and those before this segment, from bit 16 on
+#pragma unroll
+      for (int q = 0; q < 16; ++q) {
+        if (i0 + 1024 * (q >> 2) >= end) break;
+        if (!in(q)) continue;
+        const int bin = key[q] >> shift & 1023;
+        const bool prior = place(i0, q) < prior_end;
+        if (bin == common) {
+          many += prior ? 0x10001 : 1;
+        } else {
+          atomicAdd(&bins[0][bin], 1);
+          if (prior) atomicAdd(&bins[1][bin], 1);
+        }
+      }
+      many = wave_scan(many);
+      if (lane == 63) {
+        atomicAdd(&bins[0][common], many & 0xFFFF);
+        atomicAdd(&bins[1][common], many >> 16);
+      }
+    };
+    uint32_t key[16];
+    const bool held = listed <= BATCH;
+    if (held) {  // the second digit of a short list, whose keys stay in registers for the third
+#pragma unroll
+      for (int q = 0; q < 16; ++q) {
+        if (1024 * (q >> 2) >= listed) break;
+        const int i = min(place(0, q), listed - 1);  // the i-th: in the last segment that begins at or before it
+        int k = 0;
+#pragma unroll
+        for (int step = MAX_SEGS / 2; step; step >>= 1)
+          if (first[k + step] <= i) k += step;
+        key[q] = g.keys[((size_t)head * g.n + k) * g.size + i - first[k]];
+      }
+      add(key, 0, listed, first[s], 10, h[0]);
+    } else {  // and of a long one
+      const int4* in = reinterpret_cast<const int4*>(g.next + (size_t)head * g.n * 1024) + t;
+      int4 x = make_int4(0, 0, 0, 0), y = x;
+#pragma unroll 8
+      for (int k = 0; k < live; ++k) {
+        const int4 z = in[k * 256];
+        x.x += z.x, x.y += z.y, x.z += z.z, x.w += z.w;
+        if (k < s) y = x;
+      }
+      reinterpret_cast<int4*>(h[0][0])[t] = x;
+      reinterpret_cast<int4*>(h[0][1])[t] = y;
+    }
     __syncthreads();
-    prefix |= (uint32_t)pick_bin<4, 1024>(h[0], sums[0], need) << 10;
-    each([&](int, uint32_t key) {
-      if ((key ^ prefix) >> 10 == 0) atomicAdd(&h[1][key & 1023], 1);
-    });
+    const int second = pick_bin<4, 1024>(h[0][0], sums[0], need);
+    prefix |= (uint32_t)second << 10;
+    if (held) {
+      add(key, 0, listed, first[s], 0, h[1]);
+    } else {
+      for (int k = 0; k < live; ++k) {
+        const uint32_t* from = g.keys + ((size_t)head * g.n + k) * g.size;
+        const int here = first[k + 1] - first[k];
+        for (int i0 = 0; i0 < here; i0 += BATCH) {
+#pragma unroll
+          for (int q = 0; q < 16; q += 4) {  // (a segment has room for whole fours)
+            const int i = place(i0, q);
+            const uint4 x = i < here ? *reinterpret_cast<const uint4*>(from + i) : make_uint4(0, 0, 0, 0);
+            key[q] = x.x, key[q + 1] = x.y, key[q + 2] = x.z, key[q + 3] = x.w;
+          }
+          add(key, i0, here, k < s ? here : 0, 0, h[1]);
+        }
+      }
+    }
     __syncthreads();
-    prefix |= (uint32_t)pick_bin<4, 1024>(h[1], sums[1], need);
-    int gb = 0, eb = 0;
-    each([&](int i, uint32_t key) {
-      gb += i < own && key > prefix;
-      eb += i < own && key == prefix;
-    });
+    const int third = pick_bin<4, 1024>(h[1][0], sums[1], need);
+    prefix |= (uint32_t)third;
+    int gb = 0;
+    for (int i = t; i < 1024; i += 256) gb += (i > second ? h[0][1][i] : 0) + (i > third ? h[1][1][i] : 0);
     gb = wave_scan(gb);
-    eb = wave_scan(eb);
-    if (lane == 63) {
-      before[wave][0] = gb;
-      before[wave][1] = eb;
-    }
+    if (lane == 63) before[wave] = gb;
     __syncthreads();
-    for (int i = 0; i < 4; ++i) {
-      larger += before[i][0];
-      equal += before[i][1];
-    }
+    larger += before[0] + before[1] + before[2] + before[3];
+    equal = h[1][1][third];
   }
   // `need` of the entries with the key `prefix` stay
   int turn = 0;
@@ -687,7 +751,8 @@ void launch_kv8_load(const Kv8& c, int n, size_t stride, const int* start, const
 }
 
 // One workgroup a head selects from up to SELECT_MOST entries, several from more: an eviction of 8 heads of 128 takes
-// 33 us either way at 32768 (of 128 heads 76 against 102), 37 against 64 at 65536, 41 against 111 at 131072.
+// 33 us either way at 32768 (of 128 heads 76 against 102), 37 against 63 at 65536, 42 against 111 at 131072; with all
+// weights equal 56 either way at 40000, 67 against 82 at 65536, 103 against 151 at 131072.
 constexpr int SELECT_MOST = 32768;
 
 static size_t up256(size_t x) { return (x + 255) / 256 * 256; }
@@ -718,6 +783,7 @@ EvictWs evict_ws(const Kv8& c, int max_len, int keep, void* ws) {
     o.g.size = (chunks + MAX_SEGS - 1) / MAX_SEGS * SEG_CHUNK;
     o.g.n = (max_len + o.g.size - 1) / o.g.size;
     part(o.g.hist, heads * o.g.n * 4096);
+    part(o.g.next, heads * o.g.n * 1024);
     part(o.g.keys, heads * o.g.n * o.g.size);
     part(o.g.found, heads * o.g.n * 2);
     part(o.g.state, heads * 2);

@@ -692,3 +692,31 @@ def test_weights_of_entries_that_a_nan_token_does_not_see(gpu, kv, group, hd, n_
         keys = max([np.nanmax(np.abs(ref.value(0, b, h, n)), initial=0) for h in range(kv)])
         rel = (2 * (hd + 16) * 0.1 * np.nanmax(np.abs(q[b]).sum(-1)) * keys + 32 + n / 32 + 300 + group * n_q) * 2.0 ** -24
         assert (np.abs(a - z) <= rel * z + 1e-30)[ok].all()
+
+
+# ---- evictions of more than 32768 entries, which several workgroups a head select ----
+
+def many_weights(n):
+    """Rows of n weights whose smallest kept one is hard to place: signs, infinities and NaN; all equal; equal but for a few;
+    equal in all but the last bits; one size with many different last bits; NaN only."""
+    rng = np.random.default_rng(n)
+    w = np.zeros((7, 1, n), np.float32)
+    w[0, 0] = rng.choice(np.array([np.inf, -np.inf, np.nan, 0.0, -0.0, 1e-45, -1e-45, -3, 7], np.float32), n)
+    w[1, 0] = 1.0
+    w[2, 0, rng.integers(0, n, 900)] = rng.uniform(0, 1, 900)
+    w[3, 0] = (np.float32(1).view(np.int32) + rng.integers(0, 40, n)).astype(np.int32).view(np.float32)
+    w[4, 0] = rng.uniform(1, 1.12, n)
+    w[5, 0] = np.nan
+    w[6, 0] = -np.arange(n)
+    return w
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("n,keep,first,last", [(40001, 1000, 0, 0), (33000, 32000, 4, 500), (70003, 20011, 1, 0), (70003, 1, 0, 0),
+                                               (40001, 600, 100, 500), (135000, 90001, 0, 77)])
+def test_evict_order_of_many_weights(gpu, n, keep, first, last, in_place):
+    w = many_weights(n)
+    if keep == first + last:  # (only what the caller names stays, whatever the weights)
+        w[6] = np.nan
+    lens = [n, n - 1, n - 300, n, n, n, 32769]
+    check_evict(3, "i8", 1, 64, lens, keep, first, last, w, in_place, cap=n)
