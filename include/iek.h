@@ -312,8 +312,10 @@ iek_status iek_dev_attention_decode_noalloc(const float* q, const void* k_cache,
  * with workspaces and outputs of their own may overlap. IEK_ERR_OP for null or misaligned pointers
  * and unsupported shapes: head_dim 64, 128, 256 or 512, n_heads / n_kv_heads <= 8, row strides in
  * floats, multiples of 4 and not below a row; f32 rows and workspaces 16-byte aligned; at most 2^26
- * slots and 65535 sequences times KV heads. What a call writes must not overlap what it reads,
- * but where this says so. A batch, n or n_q of 0 does nothing. */
+ * slots, 4096 KV heads and 65535 sequences times KV heads. An attention of 2^29 floats of q or 2^31
+ * running weights and more may be refused too, then by its workspace query as by the call. What a
+ * call writes must not overlap what it reads, but where this says so. A batch, n or n_q of 0 does
+ * nothing. */
 #define IEK_KV8_BLOCK 32
 typedef struct iek_kv8 {
   int32_t dtype; /* IEK_I8 or IEK_E4M3 */
@@ -348,8 +350,9 @@ iek_status iek_dev_kv8_load(const iek_kv8* cache, size_t n, size_t row_stride, c
  * being h / (n_heads / n_kv_heads); zeros where there are none. Entries from len[b] on may hold
  * anything. weights_out (or NULL): [batch][n_kv_heads][capacity], for j < len[b]
  * weights_out[j] = weights_in[j] + the attention weight of entry j summed over the KV head's query
- * heads and the n_q tokens (a token with a NaN score: NaN for the entries it sees); weights_in may be weights_out itself, or NULL for zeros. workspace:
- * iek_kv8_attention_workspace bytes for the same arguments, its contents of no matter. */
+ * heads and the n_q tokens (of a token with a NaN score: NaN for the entries it sees); weights_in may
+ * be weights_out itself, or NULL for zeros. workspace: iek_kv8_attention_workspace bytes for the same
+ * arguments, its contents of no matter. */
 iek_status iek_kv8_attention_workspace(const iek_kv8* cache, size_t n_heads, size_t n_q, size_t max_len,
                                        int with_weights, size_t* bytes);
 iek_status iek_dev_kv8_attention(const iek_kv8* cache, const float* q, size_t n_heads, size_t n_q, size_t q_stride,

@@ -746,28 +746,42 @@ Sizes sizes(const Kv8& c, const Plan& p, int spad, bool weights) {
           weights ? up256((size_t)c.batch * c.n_kv * p.cols * spad * 4) : 0};
 }
 
+// Workgroups of the join: `ncol` for columns, then `wblocks` a KV head for weights.
+struct JoinGrid {
+  int ncol, wblocks, all;
+};
+JoinGrid join_grid(const Kv8& c, const Plan& p, int max_len, bool weights) {
+  const bool many = p.cols > 8;
+  const long long heads = (long long)c.batch * c.n_kv;
+  const long long ncol = p.direct ? 0 : heads * (c.hd / 64) * (many ? (p.cols + 3) / 4 : p.cols);
+  const int wblocks = weights ? (max_len + (many ? 255 : 1023)) / (many ? 256 : 1024) : 0;
+  const long long all = ncol + heads * wblocks;
+  if (all >= 1 << 24) fail(ST_OP, "kv8: dims too large");  // (2^32 threads)
+  return {(int)ncol, wblocks, (int)all};
+}
+
 template <int HD, int CG>
 void launch_cg(const Kv8& c, const Kv8Attn& a, const Plan& p, hipStream_t st) {
+  // (at most 65535 KV heads of 64 workgroups' columns each, or chunks that fill the chip: below 2^24 workgroups)
   const long long part = ((long long)p.chunks * c.n_kv + 7) / 8 * 8 * p.cblocks;
   const dim3 grid = p.cblocks == 1 ? dim3((unsigned)c.n_kv, (unsigned)p.chunks) : dim3((unsigned)part);
   const bool many = p.cols > 8;
-  const long long ncol = p.direct ? 0 : (long long)c.batch * c.n_kv * (HD / 64) * (many ? (p.cols + 3) / 4 : p.cols);
-  const int wblocks = a.w_out ? (a.max_len + (many ? 255 : 1023)) / (many ? 256 : 1024) : 0;
-  const long long join = ncol + (long long)c.batch * c.n_kv * wblocks;
-  if (part >= 1 << 24 || join >= 1 << 24) fail(ST_OP, "kv8: dims too large");  // (2^32 threads)
+  const JoinGrid join = join_grid(c, p, a.max_len, a.w_out != nullptr);
   auto fn = c.e4m3 ? part_kernel<HD, true, CG> : part_kernel<HD, false, CG>;
   hipLaunchKernelGGL(fn, grid, dim3(64 * WAVES), 0, st, c, a, p);
-  if (join)
-    hipLaunchKernelGGL((many ? join_kernel<HD, true> : join_kernel<HD, false>), dim3((unsigned)join), dim3(256), 0, st, c, a, p, (int)ncol, wblocks);
+  if (join.all)
+    hipLaunchKernelGGL((many ? join_kernel<HD, true> : join_kernel<HD, false>), dim3((unsigned)join.all), dim3(256), 0, st, c, a, p,
+                       join.ncol, join.wblocks);
 }
 
 }  // namespace
 
-// For any window: fewer tiles do not take more chunks, nor do smaller column groups.
+// For any window: fewer tiles do not take more chunks, nor do smaller column groups; nor more workgroups in the join.
 size_t kv8_attention_workspace(const Kv8& c, int n_heads, int n_q, int max_len, bool weights) {
   if (c.batch == 0 || n_q == 0) return 0;
   const int tiles = (max_len + TILE - 1) / TILE;
   Plan p = make_plan(c, n_heads, n_q, tiles);
+  join_grid(c, p, max_len, weights);  // (refuses)
   const Sizes z = sizes(c, p, tiles * TILE, weights);
   return z.ml + z.o + z.s;
 }

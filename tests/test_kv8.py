@@ -142,3 +142,14 @@ def test_row_by_row_rounding_stays_under_a_step(dtype):
     step = s if dtype == "i8" else np.maximum(2.0 ** (np.floor(np.log2(np.maximum(np.abs(x[0, :, 0]) / s, 2 ** -6))) - 3) * s, s * 2.0 ** -9)
     assert (np.abs(got - x[0, :, 0]) < step).all()
     assert np.abs(x).max() <= kv8_ref.TOP[dtype] * s and np.abs(x).max() > kv8_ref.TOP[dtype] * s / 2
+
+
+def test_what_a_launch_cannot_hold_the_workspace_query_refuses_too():
+    """A join of 2^24 workgroups and more: 65520 KV heads of 512 with 136 columns each; and what lies below."""
+    c = cache(batch=16, kv=4095, cap=4000, hd=512)
+    refused("Op", "too large", E.kv8_attention_workspace, c, 8 * 4095, 17, 4000, False)
+    refused("Op", "too large", attention, c, heads=8 * 4095, n_q=17, stride=512 * 8 * 4095, max_len=4000, size=1 << 62)
+    # (2^29 floats of q, and 2^31 weights)
+    assert E.kv8_attention_workspace(cache(batch=16, kv=4096 // 2, cap=4000, hd=512), 8 * 2048, 4, 4000, False) > 0
+    assert E.kv8_attention_workspace(cache(batch=512, kv=8, cap=1 << 19, hd=64), 8, 1, 1 << 19, True) > 0
+    refused("Op", "too large", E.kv8_attention_workspace, cache(kv=4097), 4097, 1, 100, False)
