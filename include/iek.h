@@ -337,8 +337,9 @@ iek_status iek_dev_kv8_append(const iek_kv8* cache, const float* k, const float*
                               const int32_t* start, const int32_t* count, int32_t* len_out, float* weights,
                               void* stream);
 /* The values of slots start[b] + i, i < count[b], as f32 rows (arguments as above; what
- * iek_session_kv is for a session): e.g. a cached prefix for iek_dev_attention_prefill. Rows from
- * count[b] on, and those of slots that do not exist, are left as they were. */
+ * iek_session_kv is for a session; those of one sequence, n_kv_heads * head_dim floats apart, are the
+ * caches of iek_attention_decode). Rows from count[b] on, and those of slots that do not exist, are
+ * left as they were. IEK_ERR_KV_CACHE when n > capacity. */
 iek_status iek_dev_kv8_load(const iek_kv8* cache, size_t n, size_t row_stride, const int32_t* start,
                             const int32_t* count, float* k, float* v, void* stream);
 /* Attention of the last n_q (at most 64) tokens of every sequence, their rows already appended.

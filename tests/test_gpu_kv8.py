@@ -720,3 +720,22 @@ def test_evict_order_of_many_weights(gpu, n, keep, first, last, in_place):
         w[6] = np.nan
     lens = [n, n - 1, n - 300, n, n, n, 32769]
     check_evict(3, "i8", 1, 64, lens, keep, first, last, w, in_place, cap=n)
+
+
+# ---- uses that the documentation names ----
+
+@pytest.mark.parametrize("dtype", ["i8", "e4m3"])
+def test_loaded_rows_are_the_caches_of_attention_decode(gpu, dtype):
+    """Rows of one sequence read back are the f32 caches that iek_attention_decode takes: the same attention."""
+    kv, group, hd, n = 2, 4, 128, 301
+    ref = filled(21, 1, kv, 320, hd, dtype, [n])
+    d = Dev(1, kv, 320, hd, dtype, ref)
+    d.stale_from([n])
+    q = np.random.default_rng(2).standard_normal((1, 1, kv * group, hd)).astype(np.float32)
+    rows = [torch.full((n, kv, hd), 7.0, device="cuda") for _ in range(2)]
+    E.kv8_load(d.h, n, kv * hd, 0, ints([n]).data_ptr(), rows[0].data_ptr(), rows[1].data_ptr(), stream())
+    out = E.host_attention_decode(q.reshape(-1), host(rows[0]).reshape(-1), host(rows[1]).reshape(-1), kv * group, kv, hd, n, 0, 0.09)
+    want, _, bound = ref.attention(q, [n], 0, 0.09)
+    got, _ = attend(d, q, [n], 0, 0.09)
+    # (bound is of f32 sums in any order: the plain kernel's too)
+    assert (np.abs(np.asarray(out).reshape(q.shape) - want) <= bound).all() and (np.abs(got - want) <= bound).all()
