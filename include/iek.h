@@ -302,8 +302,8 @@ iek_status iek_dev_attention_decode_noalloc(const float* q, const void* k_cache,
  * sequences' keys and values as 8-bit codes with one scale per block of IEK_KV8_BLOCK slots of a
  * head; a row's values are code * scale. Scales are powers of two: for the block's largest |value| a,
  * the smallest 2^e >= 2^-100 with a <= M * 2^e, M = 127 (IEK_I8) or 448 (IEK_E4M3), so that a value
- * is off by at most half a step of its scale (and by less than a whole one after later appends or
- * evictions have brought its block to a larger scale).
+ * is off by at most half a step between its neighbouring codes (and by less than a whole one after
+ * later appends or evictions have brought its block to a larger scale).
  *
  * The buffers are the caller's, in HBM, the codes 16-byte aligned; nothing needs to be cleared. All
  * entries are asynchronous, allocate nothing, wait for nothing and may be captured into a graph; what
@@ -330,9 +330,10 @@ typedef struct iek_kv8 {
  * those before start in the same block keep their values (their codes are rounded again when the
  * block's scale grows). An infinity or NaN makes its block's scale NaN, and so all its rows, until
  * the block's first slot is written again: queries that see one of them get NaN, the others nothing of
- * it. (Codes are what these entries write: an E4M3 code that is NaN belongs to a NaN scale.) len_out (or NULL): the lengths after the append; may be start itself, and must not
- * overlap it otherwise. weights (or NULL): [batch][n_kv_heads][capacity] running attention weights,
- * set to 0 for the new rows. IEK_ERR_KV_CACHE when n > capacity. */
+ * it. (Codes are what these entries write: an E4M3 code that is NaN belongs to a NaN scale.) len_out
+ * (or NULL): the lengths after the append; may be start itself (not where several layers' appends read
+ * the same start), and must not overlap it otherwise. weights (or NULL): [batch][n_kv_heads][capacity]
+ * running attention weights, set to 0 for the new rows. IEK_ERR_KV_CACHE when n > capacity. */
 iek_status iek_dev_kv8_append(const iek_kv8* cache, const float* k, const float* v, size_t n, size_t row_stride,
                               const int32_t* start, const int32_t* count, int32_t* len_out, float* weights,
                               void* stream);

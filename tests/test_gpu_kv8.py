@@ -739,3 +739,42 @@ def test_loaded_rows_are_the_caches_of_attention_decode(gpu, dtype):
     got, _ = attend(d, q, [n], 0, 0.09)
     # (bound is of f32 sums in any order: the plain kernel's too)
     assert (np.abs(np.asarray(out).reshape(q.shape) - want) <= bound).all() and (np.abs(got - want) <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", ["i8", "e4m3"])
+def test_layers_share_their_lengths(gpu, dtype):
+    """Three layers' caches of two sequences: each append reads the lengths before the step and writes those after it, which
+    the attentions take; at the end of the step the latter become the former, by a copy or by the layers' evictions."""
+    rng = np.random.default_rng(17)
+    layers, kv, group, hd, cap, keep = 3, 2, 4, 64, 96, 60
+    ref = [kv8_ref.Cache(2, kv, cap, hd, dtype) for _ in range(layers)]
+    d = [Dev(2, kv, cap, hd, dtype) for _ in range(layers)]
+    length, after, lens = ints([0, 0]), ints([-1, -1]), [0, 0]
+    es = torch.empty(E.kv8_evict_workspace(d[0].h, cap, keep), dtype=torch.uint8, device="cuda")
+    for step in range(40):
+        n, count = (50, [50, 33]) if step == 0 else (1, [1, 1])
+        for x, c in zip(ref, d):
+            r = rng.standard_normal((2, 2, n, kv, hd)).astype(np.float32)
+            k, v, q = dev(r[0]), dev(r[1]), rng.standard_normal((2, 1, kv * group, hd)).astype(np.float32)
+            E.kv8_append(c.h, k.data_ptr(), v.data_ptr(), n, kv * hd, length.data_ptr(), ints(count).data_ptr(), after.data_ptr(),
+                         c.w.data_ptr(), stream())
+            now = x.append(r[0], r[1], lens, count)
+            assert host(after).tolist() == now
+            got, _ = attend(c, q, now, 0, 0.125, c.w, c.w, max_len=cap)
+            want, _, bound = x.attention(q, now, 0, 0.125)
+            assert (np.abs(got - want) <= bound).all()
+        if max(now) > 80:
+            for i, c in enumerate(d):
+                w = host(c.w)
+                E.kv8_evict(c.h, c.h, c.w.data_ptr(), c.w.data_ptr(), after.data_ptr(), length.data_ptr(), cap, keep, 2, 16, 0,
+                            es.data_ptr(), es.numel(), stream())
+                ref[i], _, now_left, _ = ref[i].evict(w, now, keep, 2, 16)
+            now = now_left
+        else:
+            length.copy_(after)
+        lens = now
+        assert host(length).tolist() == lens
+        HELD[2:] = []
+    for x, c in zip(ref, d):
+        c.stale_from(lens)
+        c.check(x, lens)
