@@ -778,3 +778,34 @@ def test_layers_share_their_lengths(gpu, dtype):
     for x, c in zip(ref, d):
         c.stale_from(lens)
         c.check(x, lens)
+
+
+def test_offsets_beyond_31_bits_within_a_head(gpu):
+    """One head of 2.5 GiB of K and of V: rows appended, read back, attended to and moved from beyond 2^31 bytes of its start."""
+    cap, hd, n = 5 * 2 ** 20, 512, 64
+    code = [torch.empty((1, 1, cap, hd), dtype=torch.uint8, device="cuda") for _ in range(2)]
+    scale = [torch.empty((1, 1, cap // 32), device="cuda") for _ in range(2)]
+    w = torch.zeros((1, 1, cap), device="cuda")
+    h = E.KV8Cache(E.I8, 1, 1, cap, hd, *(x.data_ptr() for x in code + scale))
+    rng = np.random.default_rng(1)
+    x = rng.standard_normal((2, 1, n, 1, hd)).astype(np.float32)
+    k, v, start, end = dev(x[0]), dev(x[1]), ints([cap - n]), ints([0])
+    E.kv8_append(h, k.data_ptr(), v.data_ptr(), n, hd, start.data_ptr(), 0, end.data_ptr(), 0, stream())
+    ref = kv8_ref.Cache(1, 1, n, hd, "i8")
+    ref.append(x[0], x[1], [0], [n])
+    to = Dev(1, 1, n, hd, "i8")
+    len_out, ws = ints([0]), torch.empty(E.kv8_evict_workspace(h, cap, n), dtype=torch.uint8, device="cuda")
+    E.kv8_evict(h, to.h, w.data_ptr(), to.w.data_ptr(), end.data_ptr(), len_out.data_ptr(), cap, n, 0, n, 0, ws.data_ptr(),
+                ws.numel(), stream())
+    assert host(end).tolist() == [cap] and host(len_out).tolist() == [n]
+    to.check(ref, [n])
+    out = [torch.zeros((n, hd), device="cuda") for _ in range(2)]
+    E.kv8_load(h, n, hd, start.data_ptr(), 0, out[0].data_ptr(), out[1].data_ptr(), stream())
+    for i in range(2):
+        assert np.array_equal(host(out[i]), ref.value(i, 0, 0, n).astype(np.float32))
+    q = rng.standard_normal((1, 1, 8, hd)).astype(np.float32)
+    size = E.kv8_attention_workspace(h, 8, 1, cap, False)
+    ws, res, dq = torch.empty(size, dtype=torch.uint8, device="cuda"), torch.zeros((8, hd), device="cuda"), dev(q)
+    E.kv8_attention(h, dq.data_ptr(), 8, 1, 8 * hd, end.data_ptr(), cap, n, 0.04, res.data_ptr(), 0, 0, ws.data_ptr(), size, stream())
+    want, _, bound = ref.attention(q, [n], 0, 0.04)
+    assert (np.abs(host(res).reshape(q.shape) - want) <= bound).all()
