@@ -95,8 +95,9 @@ __global__ void advance_kernel(int batch, int cap, const int* count, int n, int*
 }
 
 // ---- load ----------------------------------------------------------------------------------------
-// One workgroup per (32 rows, KV head, sequence): 4 codes of K and of V to 16 bytes of f32 a lane. Bound by the
-// stores, which do not stay in L2 (24576 rows of 8 heads of 128: 39 us, and 31 with nontemporal stores).
+// One workgroup per (32 rows, KV head, sequence): 4 codes of K and of V to 16 bytes of f32 a lane. Bound by HBM
+// (24576 rows of 8 heads of 128, 252 MB: 47 us). Nontemporal stores, so that the rows leave the caches to what comes next:
+// this kernel takes as long without, but the move of the eviction that follows 33 us instead of 21.5.
 typedef float kf4_t __attribute__((ext_vector_type(4)));
 template <int HD, bool E4M3>
 __global__ __launch_bounds__(256) void load_kernel(Kv8 c, int n, size_t stride, const int* __restrict__ start_p,
@@ -800,8 +801,9 @@ void launch_kv8_evict(const Kv8& src, const Kv8& dst, const Kv8Evict& a, void* w
   const EvictWs o = evict_ws(src, a.max_len, a.keep, ws);
   int* const index = a.index_out ? a.index_out : o.index;
   float* const put_by = in_place ? o.olds : nullptr;
-  // Four waves up to 1024 entries, whose barriers are cheaper, sixteen above: an eviction from 8 heads of 128
-  // takes 16.9 us against 17.6 at 1000 entries, 21.8 against 21.1 at 2000, 27.8 against 24.3 at 4000.
+  // Four waves up to 1024 entries, whose barriers are cheaper, sixteen above: an eviction from 8 heads of 128 takes with
+  // four, eight and sixteen 16.9, 17.3 and 17.6 us at 1000 entries, 21.8, 20.7 and 21.1 at 2000, 27.8, 25.0 and 24.3 at 4000
+  // (eight would gain 2 % around 2000 alone).
   auto select = a.max_len <= 1024 ? select_kernel<256, 1024> : select_kernel<1024, SELECT_MOST>;
   if (o.spread) {
     const dim3 grid((unsigned)o.g.n, (unsigned)heads);
