@@ -350,7 +350,8 @@ iek_status iek_dev_kv8_load(const iek_kv8* cache, size_t n, size_t row_stride, c
  * that is positive and there is a window (0: none; in a cache that has been evicted from it counts
  * entries, not positions). out[b][t][h] = softmax(scale * q . K[j]) . V[j] over them, h's KV head
  * being h / (n_heads / n_kv_heads); zeros where there are none. Entries from len[b] on may hold
- * anything. weights_out (or NULL): [batch][n_kv_heads][capacity], for j < len[b]
+ * anything. Sums are f32, of shares relative to a maximum that may lag by 2^8: the entries times the
+ * largest |V| must stay below 2^119. weights_out (or NULL): [batch][n_kv_heads][capacity], for j < len[b]
  * weights_out[j] = weights_in[j] + the attention weight of entry j summed over the KV head's query
  * heads and the n_q tokens (of a token with a NaN score: NaN for the entries it sees); weights_in may
  * be weights_out itself, or NULL for zeros. workspace: iek_kv8_attention_workspace bytes for the same

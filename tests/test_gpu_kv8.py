@@ -809,3 +809,23 @@ def test_offsets_beyond_31_bits_within_a_head(gpu):
     E.kv8_attention(h, dq.data_ptr(), 8, 1, 8 * hd, end.data_ptr(), cap, n, 0.04, res.data_ptr(), 0, 0, ws.data_ptr(), size, stream())
     want, _, bound = ref.attention(q, [n], 0, 0.04)
     assert (np.abs(host(res).reshape(q.shape) - want) <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", ["i8", "e4m3"])
+def test_attention_of_values_up_to_the_stated_limit(gpu, dtype):
+    """300 entries of up to 2^110 (below 2^119 in all), the scores rising slowly from entry to entry, so that the running
+    maximum is behind the largest one most of the time."""
+    n, hd = 300, 64
+    rng = np.random.default_rng(5)
+    ref, d = kv8_ref.Cache(1, 1, n, hd, dtype), Dev(1, 1, n, hd, dtype)
+    k = np.zeros((1, n, 1, hd), np.float32)
+    k[0, :, 0, 0] = np.arange(n) / 8
+    v = (rng.uniform(0.5, 1, (1, n, 1, hd)) * 2.0 ** 110).astype(np.float32)
+    dk, dv = dev(k), dev(v)
+    E.kv8_append(d.h, dk.data_ptr(), dv.data_ptr(), n, hd, 0, 0, 0, 0, stream())
+    ref.append(k, v, [0], [n])
+    q = np.zeros((1, 1, 8, hd), np.float32)
+    q[..., 0] = np.arange(8)[None, None]
+    want, _, bound = ref.attention(q, [n], 0, 0.3)
+    got, _ = attend(d, q, [n], 0, 0.3)
+    assert (np.abs(got - want) <= bound).all()
