@@ -133,6 +133,10 @@ iek_status iek_greedy_next_token(iek_session* s, uint32_t* out_token);
  * IEK_ERR_OP for r outside [0, 1). NaN or +inf among the scaled logits gives the last index, as
  * the reference's NaN probabilities do. */
 iek_status iek_session_sample_temperature(iek_session* s, float temperature, float r, uint32_t* out_token);
+/* iek_sample on the session's last-token logits: temperature, top-k, top-p and min-p (the reference has
+ * sample_temperature alone). Errors as iek_sample. */
+iek_status iek_session_sample(iek_session* s, float temperature, int32_t top_k, float top_p, float min_p, float r,
+                              uint32_t* out_token);
 /* n iterations of { id = greedy_next_token; decode_token(id) } — the loop of src/main.rs:100-116
  * and EngineBench::run_decode_throughput (src/bench_metrics.rs:178-182) — replayed as one
  * captured decode-step graph; token ids never leave the device until the end. */
@@ -234,6 +238,11 @@ iek_status iek_argmax(const float* logits, size_t n, uint32_t* out_index);
 /* sample_temperature (src/engine/sampling.rs:54-79) over host logits; r is the caller's uniform
  * draw in [0, 1). Errors as iek_session_sample_temperature. */
 iek_status iek_sample_temperature(const float* logits, size_t n, float temperature, float r, uint32_t* out_index);
+/* iek_dev_sample of one row of host logits; out_prob may be NULL. IEK_ERR_SAMPLING for no logits, a temperature that
+ * is negative or not finite and for a row that iek_dev_sample has no token for, IEK_ERR_OP for r outside [0, 1) or a
+ * NaN among the filters. */
+iek_status iek_sample(const float* logits, size_t n, float temperature, int32_t top_k, float top_p, float min_p, float r,
+                      uint32_t* out_index, float* out_prob);
 /* The attention of decode_attention_layer (src/layers/attention.rs:608-650) for one new token,
  * its K/V already appended: for every query head h (KV head h / (n_heads / n_kv_heads)),
  * out[h] = softmax(scale * q[h] . K[j]) . V[j] over positions j in [j_min, total_pos), j_min =
@@ -376,6 +385,87 @@ iek_status iek_kv8_evict_workspace(const iek_kv8* src, size_t max_len, size_t ke
 iek_status iek_dev_kv8_evict(const iek_kv8* src, const iek_kv8* dst, const float* weights, float* weights_out,
                              const int32_t* len, int32_t* len_out, size_t max_len, size_t keep, size_t first,
                              size_t last, int32_t* index_out, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- paged KV cache, device pointers (asynchronous on `stream`) -------------------------------
+ * No counterpart in the reference, whose KVCache (src/layers/attention.rs:16-24) is contiguous. Keys and values of a
+ * batch of sequences in a pool of pages, f32 (the reference's element type) or fp16: entry j of sequence b is slot
+ * j % page_size of page table[b][j / page_size], so that sequences grow page by page and can share pages. The
+ * capacity of a sequence is max_pages * page_size entries. A number outside [0, n_pages) is no page: rows appended to
+ * it are dropped, and no query sees its entries.
+ *
+ * The conventions are those of the 8-bit cache above: the caller's buffers in HBM, the pools 16-byte aligned, nothing
+ * cleared beforehand, nothing allocated or waited for, capturable; lengths, starts and page numbers are read from
+ * device memory when a call runs. IEK_ERR_OP for null or misaligned pointers and unsupported shapes: head_dim 64, 128,
+ * 256 or 512, page_size a power of two from 16 to 1024, row strides in floats, multiples of 4 and not below a row,
+ * f32 rows and workspaces 16-byte aligned; at most 2^26 entries a sequence, 4096 KV heads and 65535 sequences. What a
+ * call writes must not overlap what it reads, but where this says so. A batch, n or n_q of 0 does nothing. */
+typedef struct iek_paged_kv {
+  int32_t dtype; /* IEK_F32 or IEK_F16 */
+  uint64_t n_pages, n_kv_heads, page_size, head_dim;
+  void *k, *v; /* [n_pages][n_kv_heads][page_size][head_dim] */
+  uint64_t batch, max_pages;
+  const int32_t* table; /* page numbers [batch][max_pages] */
+} iek_paged_kv;
+/* The (cos, sin) rows of rope (src/ops/rope.rs:11-59) for the positions 0 .. n - 1, as a session holds them:
+ * out[n][rotary_dim / 2][2], HOST memory; freq_factors may be NULL. Errors as iek_rope. */
+iek_status iek_rope_table(uint32_t head_dim, uint32_t rotary_dim, float base, size_t n, const float* freq_factors,
+                          size_t ff_len, float* out);
+/* Rows i < count[b] (count NULL: n; at most n) of sequence b, q, k and v [batch][n] rows of n_heads or n_kv_heads times
+ * head_dim floats, row_stride floats from one row to the next (slices of fused rows), are the tokens at the positions
+ * start[b] + i (start NULL: 0). The first rotary_dim dims of every query and key head are rotated to their position as
+ * iek_rope does, with the row of rope ([rope_rows][rotary_dim / 2][2] in HBM, rope_rows not below the capacity); keys
+ * and values go to their entries, queries to q_out ([batch][n] rows, q_out_stride floats apart; q itself is allowed
+ * with q_out_stride = row_stride). q NULL: keys and values alone; rope NULL (rotary_dim 0, no q): keys as they come. fp16
+ * entries are rounded to nearest, to an infinity beyond fp16's range. Rows past the capacity are dropped, and all rows
+ * of a sequence whose start is negative or past it; their q_out and that of rows from count[b] on is left as it was.
+ * len_out (or NULL): the lengths after the append; may be start itself, and must not overlap it otherwise. The entry of
+ * two rows of a call (one page twice in the tables) holds values of either. IEK_ERR_KV_CACHE when n > capacity. */
+iek_status iek_dev_paged_append(const iek_paged_kv* cache, const float* q, const float* k, const float* v, size_t n_heads,
+                                size_t n, size_t row_stride, const float* rope, size_t rope_rows, size_t rotary_dim,
+                                const int32_t* start, const int32_t* count, int32_t* len_out, float* q_out,
+                                size_t q_out_stride, void* stream);
+/* Attention of the last n_q (at most 64) tokens of every sequence, their rows already appended; n_heads / n_kv_heads
+ * <= 8. q: [batch][n_q] rows of n_heads * head_dim floats, q_stride floats apart; len[b] entries in sequence b, at most
+ * max_len (<= capacity; IEK_ERR_KV_CACHE otherwise), which sizes the launch. Query token t sees the entries [lo, hi),
+ * hi = len[b] - (n_q - 1 - t), lo = hi - sliding_window if that is positive and there is a window (0: none). out[b][t][h]
+ * = softmax(scale * q . K[j]) . V[j] over them, h's KV head being h / (n_heads / n_kv_heads); zeros where there are none.
+ * Entries that no query sees may hold anything. An infinity or NaN reaches the queries that see it alone, as NaN or (of
+ * an infinity in V) as an infinity.
+ * The first *shared entries of every sequence (a word in HBM, at most max_shared <= max_len, which sizes the launch) are
+ * the same ones, in the pages shared_pages[j / page_size] (ceil(max_shared / page_size) numbers): they are read from
+ * there, once for the whole batch, whatever the tables say, and the answer is that of tables that begin with them. *shared
+ * need not be a multiple of page_size. max_shared 0 (both NULL): nothing is shared. Sums are f32, of shares relative to a
+ * maximum that may lag by 2^8: the entries times the largest |V| must stay below 2^119. Of fp16 caches, products are
+ * those of 22 bits of q and of the weights. workspace: iek_paged_attention_workspace bytes for the same arguments, its
+ * contents of no matter. */
+iek_status iek_paged_attention_workspace(const iek_paged_kv* cache, size_t n_heads, size_t n_q, size_t max_len,
+                                         size_t max_shared, size_t* bytes);
+iek_status iek_dev_paged_attention(const iek_paged_kv* cache, const float* q, size_t n_heads, size_t n_q, size_t q_stride,
+                                   const int32_t* len, size_t max_len, const int32_t* shared_pages, const int32_t* shared,
+                                   size_t max_shared, size_t sliding_window, float scale, float* out, void* workspace,
+                                   size_t workspace_bytes, void* stream);
+
+/* ---- sampling of a batch, device pointers (asynchronous on `stream`) --------------------------
+ * The reference has sample_temperature alone (src/engine/sampling.rs:54-79: iek_sample_temperature, one row in its f32
+ * steps). The next token of every row of logits [rows][n], row_stride floats apart, with filters of its own (arrays of
+ * `rows` in HBM). With the row's maximum M, token i has the weight w_i = exp((l_i - M) / temperature), 0 for -inf;
+ * in descending order (equal logits: the lower index first) the filters keep
+ *   top_k (<= 0, >= n or NULL: none): the first top_k;
+ *   top_p (>= 1 or NULL: none): of those the ones before which the weights sum to less than top_p times the total of
+ *     those (the first one always);
+ *   min_p (<= 0 or NULL: none): of those the ones with w_i >= min_p (with w_i = 1 always).
+ * out_index: the first token in index order up to which the kept weights sum to more than r (in [0, 1)) times their
+ * total; out_prob (or NULL): its weight over that total. Sums are exact ones of weights that are off by 2^-44 of the
+ * largest at most up to 2^19 tokens, so a row's token does not depend on the order of anything. temperature 0: the
+ * largest logit, the lowest index of equal ones, with probability 1. A row with a NaN or +inf, or with -inf alone, and
+ * one whose temperature is negative or not finite, whose r is outside [0, 1) or which has a NaN among its filters gets
+ * the index 0xFFFFFFFF and the probability NaN. workspace: iek_sample_workspace bytes (may be 0), 16-byte aligned, its
+ * contents of no matter. IEK_ERR_SAMPLING for n == 0, IEK_ERR_OP for null or misaligned pointers, row_stride < n, n above
+ * 2^30 or rows above 2^21; rows == 0 does nothing. */
+iek_status iek_sample_workspace(size_t rows, size_t n, size_t* bytes);
+iek_status iek_dev_sample(const float* logits, size_t rows, size_t n, size_t row_stride, const float* temperature,
+                          const int32_t* top_k, const float* top_p, const float* min_p, const float* r,
+                          uint32_t* out_index, float* out_prob, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- device memory helpers for FFI callers without a HIP binding ---------------------------- */
 iek_status iek_device_alloc(size_t bytes, void** out);

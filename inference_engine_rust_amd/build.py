@@ -49,6 +49,9 @@ SOURCES = [
     "kernels/sampling.hip",
     "kernels/kv8.hip",
     "kernels/kv8_attention.hip",
+    "kernels/paged.hip",
+    "kernels/paged_attention.hip",
+    "kernels/sampling_filters.hip",
     "model.cpp",
     "session.cpp",
     "api.cpp",

@@ -7,6 +7,8 @@
 
 #include "../../include/iek.h"
 #include "kernels/kv8.h"
+#include "kernels/paged.h"
+#include "kernels/sampling.h"
 #include "session.h"
 
 namespace iek {
@@ -314,6 +316,11 @@ iek_status iek_greedy_next_token(iek_session* s, uint32_t* out) { IEK_API_TRY(*o
 
 iek_status iek_session_sample_temperature(iek_session* s, float temperature, float r, uint32_t* out) {
   IEK_API_TRY(*out = s->s->sample_temperature(temperature, r))
+}
+
+iek_status iek_session_sample(iek_session* s, float temperature, int32_t top_k, float top_p, float min_p, float r,
+                              uint32_t* out) {
+  IEK_API_TRY(*out = s->s->sample(SampleParams{temperature, top_p, min_p, r, top_k}))
 }
 
 iek_status iek_session_generate_greedy(iek_session* s, size_t n, uint32_t* out) {
@@ -653,19 +660,21 @@ class OnDeviceOf {
   int was_ = -1;
 };
 
-static void aligned(const void* p, size_t to, const char* what) {
-  if (!p) fail(ST_OP, std::string("kv8: null ") + what);
+// (op: the name that a message begins with)
+static void aligned(const void* p, size_t to, const char* what, const char* op = "kv8") {
+  if (!p) fail(ST_OP, std::string(op) + ": null " + what);
   if (reinterpret_cast<uintptr_t>(p) % to)
-    fail(ST_OP, std::string("kv8: ") + what + " is not " + std::to_string(to) + "-byte aligned");
+    fail(ST_OP, std::string(op) + ": " + what + " is not " + std::to_string(to) + "-byte aligned");
 }
-static void optional_aligned(const void* p, size_t to, const char* what) {
-  if (p) aligned(p, to, what);
+static void optional_aligned(const void* p, size_t to, const char* what, const char* op = "kv8") {
+  if (p) aligned(p, to, what, op);
 }
 // a and b are one array, or do not overlap; returns whether they are one
-static bool same_or_apart(const void* a, size_t a_bytes, const void* b, size_t b_bytes, const char* what) {
+static bool same_or_apart(const void* a, size_t a_bytes, const void* b, size_t b_bytes, const char* what,
+                          const char* op = "kv8") {
   if (!a || !b) return false;
   const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-  if (x != y && x < y + b_bytes && y < x + a_bytes) fail(ST_OP, std::string("kv8: ") + what + " overlap");
+  if (x != y && x < y + b_bytes && y < x + a_bytes) fail(ST_OP, std::string(op) + ": " + what + " overlap");
   return x == y;
 }
 
@@ -698,21 +707,24 @@ static Kv8 kv8_view(const iek_kv8* c, bool buffers = true) {
   o.e4m3 = c->dtype == IEK_E4M3;
   return o;
 }
-static void kv8_rows(size_t stride, size_t width, const char* what) {
+static void row_stride_of(size_t stride, size_t width, const char* what, const char* op) {
   if (stride % 4 || stride < width)
-    fail(ST_OP, std::string("kv8: ") + what + " must be a multiple of 4 and at least a row");
-  if (stride > (1u << 30)) fail(ST_OP, "kv8: dims too large");
+    fail(ST_OP, std::string(op) + ": " + what + " must be a multiple of 4 and at least a row");
+  if (stride > (1u << 30)) fail(ST_OP, std::string(op) + ": dims too large");
 }
-static void kv8_length(const Kv8& c, size_t max_len) {
-  if (max_len > (size_t)c.cap)
+static void length_within(size_t max_len, int cap) {
+  if (max_len > (size_t)cap)
     fail(ST_KVCACHE, "KV cache position " + std::to_string(max_len - 1) + " is out of bounds (max_seq_len is " +
-                         std::to_string(c.cap) + ")");
+                         std::to_string(cap) + ")");
 }
-static void kv8_heads(const Kv8& c, size_t n_heads, size_t n_q) {
-  if (n_heads == 0 || n_heads % c.n_kv != 0 || n_heads / c.n_kv > 8)
-    fail(ST_OP, "kv8: GQA group must divide the heads and be at most 8");
-  if (n_q > 64) fail(ST_OP, "kv8: at most 64 query tokens");
+static void query_heads(int n_kv, size_t n_heads, size_t n_q, const char* op) {
+  if (n_heads == 0 || n_heads % n_kv != 0 || n_heads / n_kv > 8)
+    fail(ST_OP, std::string(op) + ": GQA group must divide the heads and be at most 8");
+  if (n_q > 64) fail(ST_OP, std::string(op) + ": at most 64 query tokens");
 }
+static void kv8_rows(size_t stride, size_t width, const char* what) { row_stride_of(stride, width, what, "kv8"); }
+static void kv8_length(const Kv8& c, size_t max_len) { length_within(max_len, c.cap); }
+static void kv8_heads(const Kv8& c, size_t n_heads, size_t n_q) { query_heads(c.n_kv, n_heads, n_q, "kv8"); }
 
 iek_status iek_dev_kv8_append(const iek_kv8* cache, const float* k, const float* v, size_t n, size_t row_stride,
                               const int32_t* start, const int32_t* count, int32_t* len_out, float* weights,
@@ -841,6 +853,184 @@ iek_status iek_dev_kv8_evict(const iek_kv8* src, const iek_kv8* dst, const float
     OnDeviceOf on(as_stream(stream));
     const Kv8Evict a{weights, weights_out, len, len_out, (int)max_len, (int)keep, (int)first, (int)last, index_out};
     launch_kv8_evict(s, d, a, workspace, as_stream(stream));
+    after_launch();
+  })
+}
+
+// ---- paged KV cache ----
+// Checks of the cache's shape (and, with `buffers`, of its pointers).
+static Paged paged_view(const iek_paged_kv* c, bool buffers = true) {
+  constexpr const char* op = "paged";
+  if (!c) fail(ST_OP, "paged: null cache");
+  if (c->dtype != IEK_F32 && c->dtype != IEK_F16) fail(ST_OP, "paged: the cache dtype must be F32 or F16");
+  if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256 && c->head_dim != 512)
+    fail(ST_OP, "paged: head_dim must be 64, 128, 256 or 512");
+  if (c->page_size < 16 || c->page_size > 1024 || (c->page_size & (c->page_size - 1)))
+    fail(ST_OP, "paged: page_size must be a power of two from 16 to 1024");
+  if (c->n_kv_heads == 0 || c->n_pages == 0 || c->max_pages == 0) fail(ST_OP, "paged: no KV heads or no pages");
+  if (c->n_kv_heads > 4096 || c->batch > 65535 || c->n_pages > (size_t)INT32_MAX || c->max_pages > (1u << 26) / c->page_size)
+    fail(ST_OP, "paged: dims too large");
+  if (buffers) {
+    aligned(c->k, 16, "k", op);
+    aligned(c->v, 16, "v", op);
+    if (c->batch) aligned(c->table, 4, "table", op);
+  }
+  Paged o;
+  o.k = c->k;
+  o.v = c->v;
+  o.table = c->table;
+  o.n_pages = (int)c->n_pages;
+  o.n_kv = (int)c->n_kv_heads;
+  o.shift = __builtin_ctzll(c->page_size);
+  o.hd = (int)c->head_dim;
+  o.batch = (int)c->batch;
+  o.max_pages = (int)c->max_pages;
+  o.f16 = c->dtype == IEK_F16;
+  return o;
+}
+
+iek_status iek_rope_table(uint32_t head_dim, uint32_t rotary_dim, float base, size_t n, const float* ff, size_t ff_len,
+                          float* out) {
+  IEK_API_TRY({
+    if (n > (1u << 26)) fail(ST_OP, "RoPE table: too many positions");
+    const size_t row = rope_table(head_dim, rotary_dim, base, 0, ff, ff_len).size();  // (the checks)
+    if (n == 0 || row == 0) return IEK_OK;
+    if (!out) fail(ST_OP, "null argument");
+    for (size_t p = 0; p < n; ++p) {
+      const std::vector<float> cs = rope_table(head_dim, rotary_dim, base, (uint32_t)p, ff, ff_len);
+      std::memcpy(out + p * row, cs.data(), row * 4);
+    }
+  })
+}
+
+iek_status iek_dev_paged_append(const iek_paged_kv* cache, const float* q, const float* k, const float* v, size_t n_heads,
+                                size_t n, size_t row_stride, const float* rope, size_t rope_rows, size_t rotary_dim,
+                                const int32_t* start, const int32_t* count, int32_t* len_out, float* q_out,
+                                size_t q_out_stride, void* stream) {
+  IEK_API_TRY({
+    constexpr const char* op = "paged";
+    const Paged c = paged_view(cache);
+    row_stride_of(row_stride, (size_t)c.n_kv * c.hd, "row_stride", op);
+    if (q) {
+      if (n_heads == 0 || n_heads > 65536) fail(ST_OP, "paged: query heads must be 1 to 65536");
+      row_stride_of(row_stride, n_heads * c.hd, "row_stride", op);
+      row_stride_of(q_out_stride, n_heads * c.hd, "q_out_stride", op);
+    }
+    if (rotary_dim > (size_t)c.hd || rotary_dim % 2) fail(ST_OP, "paged: rotary_dim must be even and at most head_dim");
+    if (rotary_dim && !rope) fail(ST_OP, "paged: null rope");
+    if (q && !rotary_dim) fail(ST_OP, "paged: q without a rotation");
+    if (rotary_dim && rope_rows < (size_t)c.cap()) fail(ST_OP, "paged: fewer rope rows than entries in a sequence");
+    if (n > (size_t)c.cap()) fail(ST_KVCACHE, "KVCache is Full: max len is " + std::to_string(c.cap()) + ".");
+    if (n > (1u << 23)) fail(ST_OP, "paged: dims too large");
+    if (n == 0 || c.batch == 0) return IEK_OK;
+    aligned(k, 16, "k rows", op);
+    aligned(v, 16, "v rows", op);
+    optional_aligned(rope, 8, "rope", op);
+    optional_aligned(start, 4, "start", op);
+    optional_aligned(count, 4, "count", op);
+    optional_aligned(len_out, 4, "len_out", op);
+    if (q) {
+      aligned(q, 16, "q rows", op);
+      aligned(q_out, 16, "q_out", op);
+      const size_t rows = (size_t)c.batch * n - 1;
+      const size_t width = n_heads * c.hd;
+      if (same_or_apart(q, (rows * row_stride + width) * 4, q_out, (rows * q_out_stride + width) * 4, "q and q_out", op) &&
+          row_stride != q_out_stride)
+        fail(ST_OP, "paged: q and q_out overlap");
+    }
+    const size_t lens = (size_t)c.batch * 4;
+    same_or_apart(start, lens, len_out, lens, "start and len_out", op);
+    if (same_or_apart(count, lens, len_out, lens, "count and len_out", op)) fail(ST_OP, "paged: count and len_out overlap");
+    OnDeviceOf on(as_stream(stream));
+    const PagedAppend a{q, k, v, q ? (int)n_heads : 0, (int)n, row_stride, rope, (int)(rotary_dim / 2), start, count,
+                        len_out, q_out, q_out_stride};
+    launch_paged_append(c, a, as_stream(stream));
+    after_launch();
+  })
+}
+
+static void paged_shared(size_t max_shared, size_t max_len) {
+  if (max_shared > max_len) fail(ST_OP, "paged: more shared entries than entries");
+}
+
+iek_status iek_paged_attention_workspace(const iek_paged_kv* cache, size_t n_heads, size_t n_q, size_t max_len,
+                                         size_t max_shared, size_t* bytes) {
+  IEK_API_TRY({
+    const Paged c = paged_view(cache, false);
+    query_heads(c.n_kv, n_heads, n_q, "paged");
+    length_within(max_len, c.cap());
+    paged_shared(max_shared, max_len);
+    if (!bytes) fail(ST_OP, "null argument");
+    *bytes = paged_attention_workspace(c, (int)n_heads, (int)n_q, (int)max_len, (int)max_shared);
+  })
+}
+
+iek_status iek_dev_paged_attention(const iek_paged_kv* cache, const float* q, size_t n_heads, size_t n_q, size_t q_stride,
+                                   const int32_t* len, size_t max_len, const int32_t* shared_pages, const int32_t* shared,
+                                   size_t max_shared, size_t sliding_window, float scale, float* out, void* workspace,
+                                   size_t workspace_bytes, void* stream) {
+  IEK_API_TRY({
+    constexpr const char* op = "paged";
+    const Paged c = paged_view(cache);
+    query_heads(c.n_kv, n_heads, n_q, op);
+    row_stride_of(q_stride, n_heads * c.hd, "q_stride", op);
+    length_within(max_len, c.cap());
+    paged_shared(max_shared, max_len);
+    if (n_q == 0 || c.batch == 0) return IEK_OK;
+    aligned(q, 16, "q", op);
+    aligned(len, 4, "len", op);
+    aligned(out, 16, "out", op);
+    if (max_shared) {
+      aligned(shared_pages, 4, "shared_pages", op);
+      aligned(shared, 4, "shared", op);
+    }
+    if (workspace_bytes < paged_attention_workspace(c, (int)n_heads, (int)n_q, (int)max_len, (int)max_shared))
+      fail(ST_OP, "paged: the workspace is too small");
+    if (workspace_bytes) aligned(workspace, 16, "workspace", op);
+    OnDeviceOf on(as_stream(stream));
+    const PagedAttn a{q, q_stride, (int)n_heads, (int)n_q, len, (int)max_len, shared_pages, shared, (int)max_shared,
+                      sliding_window >= max_len ? 0 : (int)sliding_window, scale, out};
+    launch_paged_attention(c, a, workspace, as_stream(stream));
+    after_launch();
+  })
+}
+
+// ---- sampling of a batch ----
+static void sample_shape(size_t rows, size_t n) {
+  if (n == 0) fail(ST_SAMPLING, "logits slice is empty");
+  if (n > (1u << 30) || rows > (1u << 21)) fail(ST_OP, "sample: dims too large");
+}
+
+iek_status iek_sample_workspace(size_t rows, size_t n, size_t* bytes) {
+  IEK_API_TRY({
+    sample_shape(rows, n);
+    if (!bytes) fail(ST_OP, "null argument");
+    *bytes = sample_workspace(rows, n);
+  })
+}
+
+iek_status iek_dev_sample(const float* logits, size_t rows, size_t n, size_t row_stride, const float* temperature,
+                          const int32_t* top_k, const float* top_p, const float* min_p, const float* r,
+                          uint32_t* out_index, float* out_prob, void* workspace, size_t workspace_bytes, void* stream) {
+  IEK_API_TRY({
+    constexpr const char* op = "sample";
+    sample_shape(rows, n);
+    if (row_stride < n) fail(ST_OP, "sample: row_stride must be at least a row");
+    if (row_stride > (1u << 30)) fail(ST_OP, "sample: dims too large");
+    if (rows == 0) return IEK_OK;
+    aligned(logits, 4, "logits", op);
+    aligned(temperature, 4, "temperature", op);
+    optional_aligned(top_k, 4, "top_k", op);
+    optional_aligned(top_p, 4, "top_p", op);
+    optional_aligned(min_p, 4, "min_p", op);
+    aligned(r, 4, "r", op);
+    aligned(out_index, 4, "out_index", op);
+    optional_aligned(out_prob, 4, "out_prob", op);
+    if (workspace_bytes < sample_workspace(rows, n)) fail(ST_OP, "sample: the workspace is too small");
+    if (sample_workspace(rows, n)) aligned(workspace, 16, "workspace", op);
+    OnDeviceOf on(as_stream(stream));
+    const SampleArgs a{logits, (int)n, row_stride, temperature, top_k, top_p, min_p, r, out_index, out_prob, {}};
+    launch_sample(a, (int)rows, workspace, as_stream(stream));
     after_launch();
   })
 }
@@ -1030,6 +1220,27 @@ iek_status iek_sample_temperature(const float* logits, size_t n, float temperatu
     HostCall hc({n * 4, 64});
     const float* dl = hc.up<float>(0, logits, n * 4);
     *out_index = sample_dev(dl, n, temperature, r, hc.ptr<uint32_t>(1), hc.st);
+  })
+}
+
+iek_status iek_sample(const float* logits, size_t n, float temperature, int32_t top_k, float top_p, float min_p, float r,
+                      uint32_t* out_index, float* out_prob) {
+  IEK_API_TRY({
+    sample_shape(1, n);
+    const SampleParams one{temperature, top_p, min_p, r, top_k};
+    check_sample_params(one);
+    const size_t ws = sample_workspace(1, n);
+    HostCall hc({n * 4, 8, ws});
+    const float* dl = hc.up<float>(0, logits, n * 4);
+    uint32_t* word = hc.ptr<uint32_t>(1);
+    launch_sample({dl, (int)n, n, nullptr, nullptr, nullptr, nullptr, nullptr, word, reinterpret_cast<float*>(word + 1), one},
+                  1, hc.ptr<char>(2), hc.st);
+    uint32_t got[2];
+    hc.down(got, word, 8);
+    hc.finish();
+    if (got[0] == NO_TOKEN) fail(ST_SAMPLING, "invalid logits for sampling (empty or non-finite)");
+    *out_index = got[0];
+    if (out_prob) std::memcpy(out_prob, &got[1], 4);
   })
 }
 

@@ -1,0 +1,900 @@
+// Attention of one or several new tokens per sequence over the paged KV cache (paged.h), the entries that the
+// batch shares read once for all.
+//
+// Column (b * n_q + t) * G + g of a KV head is query token t of sequence b, query head g of its group of G. It
+// sees the entries [lo, hi): hi = len[b] - (n_q - 1 - t), lo = hi - window with a window, else 0. The entries
+// [0, shared) are the same ones for every sequence and are found by one list of pages; so there are two kinds of
+// job: all columns over a chunk of the shared entries, and a sequence's columns over a chunk of its own. With
+// scores s in base 2, out = (sum 2^(s - m) v) / (sum 2^(s - m)); a job leaves (m, sum, o), a second launch joins.
+//
+// Both products run on the matrix cores with 16 columns a product:
+//   S^T[slot][column] = K q: K's rows as they lie, a lane 16 bytes of one;
+//   O^T[dim][column] += V^T P: P comes out of the first product in the layout that the second one takes.
+// f32 pages: mfma_f32_16x16x4_f32, a tile of 16 slots, operands straight from the loads (V's four dims of a lane
+// go to four products). fp16 pages: mfma_f32_16x16x32_f16, a tile of 32 slots; K and V are exact, q and P are fp16
+// (hi, lo) pairs of 22 bits, two products each; V's rows are transposed in registers, 2 x 2 values at a time.
+// q is scaled by a power of two into fp16's range, P to at most 2^15.
+#include <type_traits>
+
+#include "common.cuh"
+#include "paged.h"
+
+namespace iek {
+
+namespace {
+
+typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
+typedef float f4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
+
+constexpr int WAVES = 4;
+constexpr int MAX_SPLIT = 256;
+constexpr int SHARED_BATCH = 64;
+
+// The running maximum is only a reference: it moves when a tile's is more than 2^LAG above it. For fp16 pages P is held
+// at 2^UP times its share, at most 2^15, so that what fp16 cuts off at its lower end, 2^-25, is 2^-38 of the largest.
+template <bool F16>
+constexpr float LAG = F16 ? 2.f : 8.f;
+template <bool F16>
+constexpr float UP = F16 ? 8192.f : 1.f;
+
+// A wave takes DIMS of a row; of wider rows two or four waves take 128 each of one tile and exchange their parts
+// of the scores through LDS.
+constexpr int dims_of(int hd) { return hd < 128 ? hd : 128; }
+constexpr int sets_of(int hd) { return WAVES * dims_of(hd) / hd; }  // sets of waves that have a row between them
+template <bool F16>
+constexpr int tile_of() { return F16 ? 32 : 16; }
+
+struct Plan {
+  int group, cols;           // query heads of a KV head, columns of a sequence
+  int all;                   // columns of the batch
+  bool own_wide, pre_wide;   // the sets of waves split the columns, not the tiles
+  int own_blocks, pre_blocks;  // workgroups that the columns of a job are spread over
+  int share;                 // own chunks of a KV head to aim at; 0: sequences are cut by `tiles`
+  int tiles, nsplit;         // share 0: tiles a chunk, chunks a sequence at most; else the smallest chunk
+  int chunks;                // own chunks of a KV head at most
+  int pre_chunks;            // chunks of the shared entries at most (0: nothing is shared)
+  int pre_tiles;             // the smallest of them
+  bool direct;               // nothing is shared and every sequence is one chunk
+  float *ml, *o;             // own: [chunks][n_kv][cols] pairs (m, sum), [chunks][n_kv][cols][hd]
+  float *pml, *po;           // shared: [pre_chunks][n_kv][all] pairs, [pre_chunks][n_kv][all][hd]
+};
+
+// Constant while the kernel runs: read through the scalar cache.
+IEK_DEV int scalar(const int* p, size_t i) {
+  return ((const __attribute__((address_space(4))) int*)p)[i];
+}
+IEK_DEV int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+IEK_DEV int col_hi(const PagedAttn& a, int n, int t) { return n - (a.n_q - 1 - t); }
+IEK_DEV int col_lo(const PagedAttn& a, int hi) { return a.window > 0 ? max(0, hi - a.window) : 0; }
+IEK_DEV int bounded(int n, int most) { return max(0, min(n, most)); }
+IEK_DEV int shared_entries(const PagedAttn& a) { return a.max_shared > 0 ? bounded(uniform(scalar(a.shared, 0)), a.max_shared) : 0; }
+// The tiles [t0, t1) of a sequence's own entries that any of its columns sees.
+template <int TILE>
+IEK_DEV void own_range(const PagedAttn& a, int n, int shared, int& t0, int& t1) {
+  t0 = max(shared, col_lo(a, max(0, col_hi(a, n, 0)))) / TILE;
+  t1 = n > shared ? max(t0, (n + TILE - 1) / TILE) : t0;
+}
+// (tiles of a sequence: below 2^23, so that the product with the reciprocal is off by less than one)
+IEK_DEV int ceil_div(int a, int b) {
+  const int up = a + b - 1, q = (int)((float)up * __builtin_amdgcn_rcpf((float)b)), r = up - q * b;
+  return q + (r >= b ? 1 : 0) - (r < 0 ? 1 : 0);
+}
+IEK_DEV int scan(int v) {
+  auto up = [](auto ctrl, auto rows, int x) {
+    return __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, decltype(rows)::value, 0xF, false);
+  };
+  using std::integral_constant;
+  v += up(integral_constant<int, 0x111>{}, integral_constant<int, 0xF>{}, v);  // row_shr 1, 2, 4, 8
+  v += up(integral_constant<int, 0x112>{}, integral_constant<int, 0xF>{}, v);
+  v += up(integral_constant<int, 0x114>{}, integral_constant<int, 0xF>{}, v);
+  v += up(integral_constant<int, 0x118>{}, integral_constant<int, 0xF>{}, v);
+  v += up(integral_constant<int, DPP_BCAST15>{}, integral_constant<int, 0xA>{}, v);
+  return v + up(integral_constant<int, DPP_BCAST31>{}, integral_constant<int, 0xC>{}, v);
+}
+
+// Own chunk x of a KV head (FIND), or the chunks of sequence b: its length, tiles a chunk, number of chunks
+// (0 with FIND: there is no chunk x) and first chunk. Up to SHARED_BATCH sequences the chunk's size is found from
+// the lengths themselves: their total by the chunks that fill the chip, each sequence evenly into as many as that
+// takes. Larger batches are cut by max_len.
+struct Cut {
+  int b, n, tiles, count, first;
+};
+template <bool FIND, int TILE, int STEP>
+IEK_DEV Cut cut(const Paged& c, const PagedAttn& a, const Plan& p, int shared, int x, int b) {
+  Cut r{b, 0, p.tiles, 0, 0};
+  int t0, t1;
+  const int least = p.direct ? 1 : 0;  // (a sequence without entries: its zeros are written)
+  if (p.share == 0 || c.batch == 1) {
+    if (FIND) r.b = c.batch == 1 ? 0 : min(x / p.nsplit, c.batch - 1);
+    r.n = uniform(bounded(scalar(a.len, r.b), a.max_len));
+    own_range<TILE>(a, r.n, shared, t0, t1);
+    if (p.share != 0) r.tiles = max(p.tiles, ceil_div(ceil_div(t1 - t0, min(p.share, MAX_SPLIT)), STEP) * STEP);
+    r.tiles = uniform(r.tiles);
+    r.count = max(least, uniform(ceil_div(t1 - t0, r.tiles)));
+    r.first = r.b * p.nsplit;
+    if (FIND && x - r.first >= r.count) r.count = 0;
+    return r;
+  }
+  const int lane = threadIdx.x & 63;
+  const int n = lane < c.batch ? bounded(a.len[lane], a.max_len) : 0;
+  own_range<TILE>(a, n, shared, t0, t1);
+  const int each = lane < c.batch ? t1 - t0 : 0;
+  const int total = __builtin_amdgcn_readlane(scan(each), 63);
+  const int most = (int)wave_max((float)each);
+  const int aim = max(p.share - c.batch / 2, (p.share + 1) / 2);
+  const int size = max(p.tiles, ceil_div(max((int)(((unsigned)total + aim - 1) / (unsigned)aim), ceil_div(most, MAX_SPLIT)), STEP) * STEP);
+  const int even = max(p.tiles, ceil_div(ceil_div(each, max(1, ceil_div(each, size))), STEP) * STEP);
+  const int mine = lane < c.batch ? max(least, ceil_div(each, even)) : 0, upto = scan(mine);
+  if (FIND) {
+    const unsigned long long here = __ballot(upto > x && upto - mine <= x);
+    if (here == 0) return r;
+    r.b = __ffsll(here) - 1;
+  }
+  r.n = __builtin_amdgcn_readlane(n, r.b);
+  r.tiles = __builtin_amdgcn_readlane(even, r.b);
+  r.count = __builtin_amdgcn_readlane(mine, r.b);
+  r.first = __builtin_amdgcn_readlane(upto, r.b) - r.count;
+  return r;
+}
+
+// The shared entries' tiles [t0, t1) that any column sees, cut into `count` chunks of `tiles`.
+struct PreCut {
+  int t0, t1, tiles, count;
+};
+template <int TILE>
+IEK_DEV PreCut pre_cut(const Paged& c, const PagedAttn& a, const Plan& p, int shared) {
+  PreCut r{0, (shared + TILE - 1) / TILE, 1, 0};
+  if (a.window > 0) {  // from the shortest sequence's window on
+    int least = INT32_MAX;
+    for (int b = threadIdx.x & 63; b < c.batch; b += 64) {
+      const int n = bounded(a.len[b], a.max_len);
+      if (n > 0) least = min(least, col_lo(a, max(0, col_hi(a, n, 0))));
+    }
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) least = min(least, __shfl_xor(least, s));
+    r.t0 = min(uniform(least) / TILE, r.t1);
+  }
+  r.tiles = max(p.pre_tiles, uniform(ceil_div(r.t1 - r.t0, max(1, p.pre_chunks))));
+  r.count = uniform(ceil_div(r.t1 - r.t0, r.tiles));
+  return r;
+}
+
+// v over the wave's four groups of 16 lanes
+IEK_DEV float groups_max(float v) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+IEK_DEV float groups_sum(float v) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+IEK_DEV f4_t mfma(u4_t a, u4_t b, f4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, a), __builtin_bit_cast(h8_t, b), c, 0, 0, 0);
+}
+IEK_DEV f4_t mfma(float a, float b, f4_t c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+
+// Where 16 slots lie: the pages of a job, and the numbers of a tile's.
+struct Pages {
+  const int* list;
+  int end;  // entries
+};
+template <bool F16>
+struct Ids {
+  int id[F16 ? 2 : 1];
+};
+template <bool F16>
+IEK_DEV Ids<F16> ids_of(const Paged& c, const Pages& g, int tile) {
+  Ids<F16> r;
+#pragma unroll
+  for (int x = 0; x < (F16 ? 2 : 1); ++x) {
+    const int j = tile * tile_of<F16>() + 16 * x;
+    r.id[x] = j < g.end ? scalar(g.list, j >> c.shift) : -1;
+    if ((unsigned)r.id[x] >= (unsigned)c.n_pages) r.id[x] = -1;
+  }
+  return r;
+}
+
+// Buffer accesses end at the last live row of the 16, and at none where there is no page: the rows behind it read
+// as zeros, whatever they hold (a NaN would reach O through a weight of 0).
+template <int HD, bool F16>
+IEK_DEV __amdgpu_buffer_rsrc_t rows_rsrc(const Paged& c, const void* pool, int h, int id, int j, int end) {
+  const size_t row = (((size_t)max(id, 0) * c.n_kv + h) << c.shift) + (j & ((1 << c.shift) - 1));
+  const int live = id < 0 ? 0 : max(0, min(16, end - j));
+  const char* base = static_cast<const char*>(pool) + row * (HD * (F16 ? 2 : 4));
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), (short)0, live * HD * (F16 ? 2 : 4), 0x00020000);
+}
+
+// A wave's part of a tile: lane (r = lane & 15, kg = lane >> 4). sum: o[x]'s V^T, of f(v) in v's
+// place, times weights (for the rare tiles with a V that is not finite).
+template <int DIMS, bool F16>
+struct Tile;
+template <int DIMS>
+struct Tile<DIMS, false> {
+  f4_t k[DIMS / 16];     // K[r][16 i + 4 kg + e]
+  f4_t v[4][DIMS / 64];  // V[4 kg + i][64 u + 4 r + e]
+  static IEK_DEV bool bad(float x) { return (__float_as_uint(x) & 0x7F800000u) == 0x7F800000u; }
+  IEK_DEV bool not_finite() const {
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < 4 * (DIMS / 64) * 4; ++i) any |= bad(v[i & 3][i >> 4][i >> 2 & 3]);
+    return any;
+  }
+  IEK_DEV void drop() {
+#pragma unroll
+    for (int i = 0; i < 4 * (DIMS / 64) * 4; ++i)
+      if (bad(v[i & 3][i >> 4][i >> 2 & 3])) v[i & 3][i >> 4][i >> 2 & 3] = 0.f;
+  }
+  template <class F>
+  IEK_DEV f4_t sum(int x, const float (&w)[4], F f) const {
+    f4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float y = v[i][x >> 2][x & 3];
+      asm volatile("" : "+v"(y));  // (nothing of this is to be kept for another column, in registers of the common path)
+      o = mfma(f(y), w[i], o);
+    }
+    return o;
+  }
+};
+template <int DIMS>
+struct Tile<DIMS, true> {
+  static constexpr int VW = DIMS / 32;
+  u4_t k[2][VW];         // K[16 s + r][32 i + 8 kg + (0 .. 7)]
+  uint32_t v[8][VW];     // V[16 (j >> 2) + 4 kg + (j & 3)][DIMS / 16 * r + ...]
+  static IEK_DEV bool bad(uint32_t x) { return (x & 0x7C00u) == 0x7C00u; }
+  IEK_DEV bool not_finite() const {
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < 8 * VW; ++i) any |= bad(v[i & 7][i >> 3]) || bad(v[i & 7][i >> 3] >> 16);
+    return any;
+  }
+  IEK_DEV void drop() {
+#pragma unroll
+    for (int i = 0; i < 8 * VW; ++i) {
+      uint32_t& x = v[i & 7][i >> 3];
+      x = bad(x) ? x & 0xFFFF0000u : x;
+      x = bad(x >> 16) ? x & 0x0000FFFFu : x;
+    }
+  }
+  // V^T's operand for the dims 2 w + e
+  IEK_DEV u4_t operand(int w, int e) const {
+    u4_t r;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r[j] = __builtin_amdgcn_perm(v[2 * j + 1][w], v[2 * j][w], e ? 0x07060302u : 0x05040100u);
+    return r;
+  }
+  template <class F>
+  IEK_DEV f4_t sum(int x, const float (&w)[8], F f) const {
+    u4_t y = operand(x >> 1, x & 1), z;
+    asm volatile("" : "+v"(y));  // (nothing of this is to be kept for another column, in registers of the common path)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t both = y[j];  // (bit_cast of an element of a vector takes the vector's first)
+      const h2_t p = __builtin_bit_cast(h2_t, both);
+      y[j] = __builtin_bit_cast(uint32_t, h2_t{(_Float16)f((float)p[0]), (_Float16)f((float)p[1])});
+      z[j] = __builtin_bit_cast(uint32_t, h2_t{(_Float16)w[2 * j], (_Float16)w[2 * j + 1]});
+    }
+    return mfma(y, z, f4_t{0.f, 0.f, 0.f, 0.f});
+  }
+};
+
+template <int HD, int DIMS, bool F16>
+IEK_DEV void load_k(Tile<DIMS, F16>& T, const Paged& c, int h, const Ids<F16>& id, int tile, int end, int dim0, int lane) {
+  if constexpr (F16) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const auto rs = rows_rsrc<HD, true>(c, c.k, h, id.id[s], 32 * tile + 16 * s, end);
+#pragma unroll
+      for (int i = 0; i < DIMS / 32; ++i)
+        T.k[s][i] = __builtin_amdgcn_raw_buffer_load_b128(rs, 2 * ((lane & 15) * HD + 8 * (lane >> 4)), 2 * (dim0 + 32 * i), 0);
+    }
+  } else {
+    const auto rs = rows_rsrc<HD, false>(c, c.k, h, id.id[0], 16 * tile, end);
+#pragma unroll
+    for (int i = 0; i < DIMS / 16; ++i)
+      T.k[i] = __builtin_bit_cast(f4_t, __builtin_amdgcn_raw_buffer_load_b128(rs, 4 * ((lane & 15) * HD + 4 * (lane >> 4)),
+                                                                              4 * (dim0 + 16 * i), 0));
+  }
+}
+
+template <int HD, int DIMS, bool F16>
+IEK_DEV void load_v(Tile<DIMS, F16>& T, const Paged& c, int h, const Ids<F16>& id, int tile, int end, int dim0, int lane) {
+  if constexpr (F16) {
+    const int off = 2 * (4 * (lane >> 4) * HD + DIMS / 16 * (lane & 15));
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const auto rs = rows_rsrc<HD, true>(c, c.v, h, id.id[s], 32 * tile + 16 * s, end);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (DIMS == 64) {
+          const auto x = __builtin_amdgcn_raw_buffer_load_b64(rs, off, 2 * (dim0 + j * HD), 0);
+          T.v[4 * s + j][0] = x[0];
+          T.v[4 * s + j][1] = x[1];
+        } else {
+          const auto x = __builtin_amdgcn_raw_buffer_load_b128(rs, off, 2 * (dim0 + j * HD), 0);
+#pragma unroll
+          for (int w = 0; w < 4; ++w) T.v[4 * s + j][w] = x[w];
+        }
+      }
+    }
+  } else {
+    const int off = 4 * (4 * (lane >> 4) * HD + 4 * (lane & 15));
+    const auto rs = rows_rsrc<HD, false>(c, c.v, h, id.id[0], 16 * tile, end);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int u = 0; u < DIMS / 64; ++u)
+        T.v[i][u] = __builtin_bit_cast(f4_t, __builtin_amdgcn_raw_buffer_load_b128(rs, off, 4 * (dim0 + i * HD + 64 * u), 0));
+  }
+}
+
+// The dim (of the wave's) that element r of o[x] of lane group kg is.
+template <int DIMS, bool F16>
+IEK_DEV int dim_at(int x, int kg, int r) {
+  return F16 ? DIMS / 16 * (4 * kg + r) + x : 64 * (x >> 2) + 4 * (4 * kg + r) + (x & 3);
+}
+
+template <int DIMS, bool F16, int CG>
+struct Query;
+template <int DIMS, int CG>
+struct Query<DIMS, false, CG> {
+  f4_t q[CG][DIMS / 16];
+};
+template <int DIMS, int CG>
+struct Query<DIMS, true, CG> {
+  u4_t hi[CG][DIMS / 32], lo[CG][DIMS / 32];
+};
+
+// What a job's columns and entries are.
+struct Job {
+  int h;
+  int col0, cols;  // the batch's columns [col0, col0 + cols)
+  int block;       // of the workgroups that these are spread over
+  Pages pages;
+  int begin;       // entries [begin, pages.end)
+  int t0, t1;      // this chunk's tiles
+  float *ml, *o;   // the partial results of column col0, or, if null, the output is written
+};
+
+template <int HD, bool F16>
+struct Shared {
+  static constexpr int SETS = sets_of(HD), DW = WAVES / SETS;
+  f4_t parts[DW > 1 ? 2 : 1][DW > 1 ? WAVES : 1][2][F16 ? 2 : 1][64];
+  float m[SETS][16], l[SETS][16];
+  float o[SETS][16][HD];
+};
+
+template <int HD, bool F16, bool WIDE, int CG>
+IEK_DEV void run_job(const Paged& c, const PagedAttn& a, const Plan& p, const Job& J, Shared<HD, F16>& L) {
+  constexpr int DIMS = dims_of(HD), SETS = sets_of(HD), DW = WAVES / SETS, TILE = tile_of<F16>();
+  constexpr int STEP = WIDE ? 1 : SETS, NH = F16 ? 2 : 1, NX = 4 * NH, ND = DIMS / 16;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int kg = lane >> 4, cl = lane & 15;
+  const int set = wave / DW, dim0 = (wave % DW) * DIMS;
+  const int col_base = WIDE ? (J.block * SETS + set) * CG * 16 : J.block * CG * 16;
+  const float ks = a.scale * 1.44269504088896340736f;
+  const int G = p.group;
+  int tile = J.t0 + (WIDE ? 0 : set);
+  Ids<F16> id = ids_of<F16>(c, J.pages, tile < J.t1 ? tile : J.t0), next = id;
+  if (tile + STEP < J.t1) next = ids_of<F16>(c, J.pages, tile + STEP);
+  Tile<DIMS, F16> T;
+  // this lane's columns
+  int hi[CG], lo[CG];
+  float qs[CG];
+  Query<DIMS, F16, CG> Q;
+  const float* rows[CG];
+#pragma unroll
+  for (int u = 0; u < CG; ++u) {
+    const int col = J.col0 + min(col_base + 16 * u + cl, J.cols - 1);
+    const int b = col / p.cols, t = (col - b * p.cols) / G, g = col - b * p.cols - t * G;
+    hi[u] = col_hi(a, bounded(a.len[b], a.max_len), t);
+    lo[u] = max(col_lo(a, hi[u]), J.begin);
+    hi[u] = min(hi[u], J.pages.end);
+    rows[u] = a.q + ((size_t)b * a.n_q + t) * a.q_stride + (size_t)(J.h * G + g) * HD + dim0;
+  }
+  f4_t raw[F16 ? CG : 1][F16 ? DIMS / 16 : 1];
+#pragma unroll
+  for (int u = 0; u < CG; ++u) {
+    if constexpr (F16) {
+#pragma unroll
+      for (int i = 0; i < DIMS / 32; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) raw[u][2 * i + e] = *reinterpret_cast<const f4_t*>(rows[u] + 32 * i + 8 * kg + 4 * e);
+    } else {
+#pragma unroll
+      for (int i = 0; i < DIMS / 16; ++i) Q.q[u][i] = *reinterpret_cast<const f4_t*>(rows[u] + 16 * i + 4 * kg);
+    }
+  }
+  if (tile < J.t1) {
+    load_k<HD>(T, c, J.h, id, tile, J.pages.end, dim0, lane);
+    load_v<HD>(T, c, J.h, id, tile, J.pages.end, dim0, lane);
+  }
+  int lo_max = 0, hi_min = INT32_MAX;
+#pragma unroll
+  for (int u = 0; u < CG; ++u) {
+    qs[u] = ks;
+    if constexpr (F16) {
+      float top = 0.f;
+#pragma unroll
+      for (int i = 0; i < DIMS / 16; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(raw[u][i][e]));
+      top = groups_max(top);
+      // into [2^13, 2^14) by a power of two (an infinity or NaN, or a row of zeros, stays what it is)
+      int ex = (int)(__float_as_uint(top) >> 23) - 127;
+      ex = ex == 128 ? 0 : min(13 - ex, 126);
+      const float up = __builtin_amdgcn_ldexpf(1.f, ex);
+      qs[u] = __builtin_amdgcn_ldexpf(ks, -ex);
+#pragma unroll
+      for (int i = 0; i < DIMS / 32; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const f4_t v = raw[u][2 * i + (e >> 1)];
+          const float y0 = v[2 * (e & 1)] * up, y1 = v[2 * (e & 1) + 1] * up;
+          const h2_t w = {(_Float16)y0, (_Float16)y1};
+          const h2_t z = {(_Float16)(y0 - (float)w[0]), (_Float16)(y1 - (float)w[1])};
+          Q.hi[u][i][e] = __builtin_bit_cast(uint32_t, w);
+          Q.lo[u][i][e] = __builtin_bit_cast(uint32_t, z);
+        }
+    }
+    lo_max = max(lo_max, lo[u]);
+    hi_min = min(hi_min, hi[u]);
+  }
+#pragma unroll
+  for (int s = 1; s < 16; s <<= 1) {
+    lo_max = max(lo_max, __shfl_xor(lo_max, s));
+    hi_min = min(hi_min, __shfl_xor(hi_min, s));
+  }
+  lo_max = uniform(lo_max);
+  hi_min = uniform(hi_min);
+  float m[CG], l[CG];
+  f4_t o[CG][ND];
+#pragma unroll
+  for (int u = 0; u < CG; ++u) {
+    m[u] = -INFINITY;
+    l[u] = 0.f;
+#pragma unroll
+    for (int i = 0; i < ND; ++i) o[u][i] = f4_t{0.f, 0.f, 0.f, 0.f};
+  }
+  const int span = J.t1 - J.t0;
+  const int t_end = DW > 1 ? J.t0 + (span + STEP - 1) / STEP * STEP : J.t1;  // (all waves go through the barriers)
+  for (int turn = 0; tile < t_end; tile += STEP, turn ^= 1) {
+    const bool have = DW == 1 || tile < J.t1, more = tile + STEP < J.t1;
+    float s[CG][NX];
+    Ids<F16> after = next;
+    if (have) {
+      if (tile + 2 * STEP < J.t1) after = ids_of<F16>(c, J.pages, tile + 2 * STEP);
+      f4_t d[CG][NH];
+#pragma unroll
+      for (int u = 0; u < CG; ++u)
+#pragma unroll
+        for (int x = 0; x < NH; ++x) d[u][x] = f4_t{0.f, 0.f, 0.f, 0.f};
+      if constexpr (F16) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int i = 0; i < DIMS / 32; ++i)
+#pragma unroll
+            for (int u = 0; u < CG; ++u) {
+              d[u][x] = mfma(T.k[x][i], Q.hi[u][i], d[u][x]);
+              d[u][x] = mfma(T.k[x][i], Q.lo[u][i], d[u][x]);
+            }
+      } else {
+#pragma unroll
+        for (int i = 0; i < DIMS / 16; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int u = 0; u < CG; ++u) d[u][0] = mfma(T.k[i][e], Q.q[u][i][e], d[u][0]);
+      }
+      if (more) load_k<HD>(T, c, J.h, next, tile + STEP, J.pages.end, dim0, lane);
+#pragma unroll
+      for (int u = 0; u < CG; ++u)
+#pragma unroll
+        for (int x = 0; x < NH; ++x) {
+          d[u][x] *= qs[u];
+          if constexpr (DW > 1) L.parts[turn][wave][u][x][lane] = d[u][x];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[u][4 * x + i] = d[u][x][i];
+        }
+    }
+    if constexpr (DW > 1) {
+      __syncthreads();
+      if (have) {
+#pragma unroll
+        for (int u = 0; u < CG; ++u)
+#pragma unroll
+          for (int x = 0; x < NH; ++x) {
+            f4_t y = L.parts[turn][set * DW][u][x][lane];
+#pragma unroll
+            for (int w = 1; w < DW; ++w) y += L.parts[turn][set * DW + w][u][x][lane];  // (the same order in every wave)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[u][4 * x + i] = y[i];
+          }
+      }
+    }
+    if (!have) continue;
+    const bool inner = tile * TILE >= lo_max && (tile + 1) * TILE <= hi_min && id.id[0] >= 0 && id.id[NH - 1] >= 0;
+#pragma unroll
+    for (int u = 0; u < CG; ++u) {
+      if (!inner) {
+#pragma unroll
+        for (int i = 0; i < NX; ++i) {
+          const int j = tile * TILE + 16 * (i >> 2) + 4 * kg + (i & 3);
+          if (j < lo[u] || j >= hi[u] || id.id[i >> 2] < 0) s[u][i] = -INFINITY;
+        }
+      }
+      float top = s[u][0];
+#pragma unroll
+      for (int i = 1; i < NX; ++i) top = fmaxf(top, s[u][i]);
+      top = groups_max(top);
+      if (__any(top > m[u] + LAG<F16> || (m[u] == -INFINITY && top > m[u]))) {
+        const bool up = top > m[u] + LAG<F16> || m[u] == -INFINITY;
+        const float corr = up && m[u] != -INFINITY ? __builtin_amdgcn_exp2f(m[u] - top) : 1.f;  // (all is 0 before)
+        if (up) m[u] = top;
+        l[u] *= corr;
+#pragma unroll
+        for (int i = 0; i < ND; ++i) o[u][i] *= corr;
+      }
+      const float ref = m[u] == -INFINITY ? 0.f : m[u];
+#pragma unroll
+      for (int i = 0; i < NX; ++i) {
+        s[u][i] = __builtin_amdgcn_exp2f(s[u][i] - ref);
+        l[u] += s[u][i];
+      }
+    }
+    if (!inner && __any(T.not_finite())) {
+      // V that is not finite, in entries that some columns may not see: taken out of the product (where a weight of 0
+      // would make NaN of it), and given as infinities of the same sign (both for NaN) to the columns that do see it
+#pragma unroll
+      for (int u = 0; u < CG; ++u) {
+        float sees[NX];
+#pragma unroll
+        for (int i = 0; i < NX; ++i) {
+          const int j = tile * TILE + 16 * (i >> 2) + 4 * kg + (i & 3);
+          sees[i] = j < lo[u] || j >= hi[u] || id.id[i >> 2] < 0 ? 0.f : 1.f;
+        }
+#pragma unroll
+        for (int x = 0; x < ND; ++x) {
+          const f4_t up = T.sum(x, sees, [](float v) { return v == INFINITY || v != v ? 1.f : 0.f; });
+          const f4_t down = T.sum(x, sees, [](float v) { return v == -INFINITY || v != v ? 1.f : 0.f; });
+#pragma unroll
+          for (int r = 0; r < 4; ++r) o[u][x][r] += (up[r] > 0.f ? INFINITY : 0.f) + (down[r] > 0.f ? -INFINITY : 0.f);
+        }
+      }
+      T.drop();
+    }
+    if constexpr (F16) {
+      u4_t ph[CG], pl[CG];
+#pragma unroll
+      for (int u = 0; u < CG; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float y0 = s[u][2 * i] * UP<F16>, y1 = s[u][2 * i + 1] * UP<F16>;
+          const h2_t w = {(_Float16)y0, (_Float16)y1};
+          const h2_t z = {(_Float16)(y0 - (float)w[0]), (_Float16)(y1 - (float)w[1])};
+          ph[u][i] = __builtin_bit_cast(uint32_t, w);
+          pl[u][i] = __builtin_bit_cast(uint32_t, z);
+        }
+#pragma unroll
+      for (int w = 0; w < DIMS / 32; ++w)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const u4_t v = T.operand(w, e);
+#pragma unroll
+          for (int u = 0; u < CG; ++u) {
+            o[u][2 * w + e] = mfma(v, ph[u], o[u][2 * w + e]);
+            o[u][2 * w + e] = mfma(v, pl[u], o[u][2 * w + e]);
+          }
+        }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int x = 0; x < ND; ++x)
+#pragma unroll
+          for (int u = 0; u < CG; ++u) o[u][x] = mfma(T.v[i][x >> 2][x & 3], s[u][i], o[u][x]);
+    }
+    if (more) load_v<HD>(T, c, J.h, next, tile + STEP, J.pages.end, dim0, lane);
+    id = next;
+    next = after;
+  }
+
+  auto put = [&](int cc, int dim, f4_t y, float sum) {  // four dims of a column
+    if (J.o) {
+      *reinterpret_cast<f4_t*>(J.o + (size_t)cc * HD + dim) = y;
+    } else {
+      const int col = J.col0 + cc, b = col / p.cols, t = (col - b * p.cols) / G, g = col - b * p.cols - t * G;
+      float* out = a.out + (((size_t)b * a.n_q + t) * a.n_heads + J.h * G + g) * HD + dim;
+      *reinterpret_cast<f4_t*>(out) = sum == 0.f ? f4_t{0.f, 0.f, 0.f, 0.f} : y / sum;
+    }
+  };
+  constexpr float DOWN = 1.f / UP<F16>;
+  if constexpr (WIDE) {
+#pragma unroll
+    for (int u = 0; u < CG; ++u) {
+      l[u] = groups_sum(l[u]);
+      const int cc = col_base + 16 * u + cl;
+      if (cc >= J.cols) continue;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int i = 0; i < ND; i += 4)
+          put(cc, dim0 + dim_at<DIMS, F16>(i, kg, r), f4_t{o[u][i][r], o[u][i + 1][r], o[u][i + 2][r], o[u][i + 3][r]} * DOWN, l[u]);
+      if (J.ml && dim0 == 0 && kg == 0) {
+        J.ml[2 * cc] = isnan(l[u]) ? l[u] : m[u];  // (a NaN: the maxima pass it over)
+        J.ml[2 * cc + 1] = l[u];
+      }
+    }
+  } else {
+    // the sets' parts: to a common maximum, then summed through LDS
+#pragma unroll
+    for (int u = 0; u < CG; ++u) {
+      if (u > 0) __syncthreads();
+      l[u] = groups_sum(l[u]);
+      if (kg == 0 && dim0 == 0) {
+        L.m[set][cl] = m[u];
+        L.l[set][cl] = l[u];
+      }
+      __syncthreads();
+      float top = L.m[0][cl];
+#pragma unroll
+      for (int w = 1; w < SETS; ++w) top = fmaxf(top, L.m[w][cl]);
+      const float mine = m[u] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[u] - top) * DOWN;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int i = 0; i < ND; i += 4)
+          *reinterpret_cast<f4_t*>(&L.o[set][cl][dim0 + dim_at<DIMS, F16>(i, kg, r)]) =
+              f4_t{o[u][i][r], o[u][i + 1][r], o[u][i + 2][r], o[u][i + 3][r]} * mine;
+      __syncthreads();
+      for (int i = threadIdx.x; i < 16 * HD / 4; i += 64 * WAVES) {
+        const int col = i / (HD / 4), dim = 4 * (i % (HD / 4)), cc = col_base + 16 * u + col;
+        if (cc >= J.cols) continue;
+        f4_t y = *reinterpret_cast<const f4_t*>(&L.o[0][col][dim]);
+#pragma unroll
+        for (int w = 1; w < SETS; ++w) y += *reinterpret_cast<const f4_t*>(&L.o[w][col][dim]);
+        float mm = L.m[0][col], ll = 0.f;
+#pragma unroll
+        for (int w = 1; w < SETS; ++w) mm = fmaxf(mm, L.m[w][col]);
+#pragma unroll
+        for (int w = 0; w < SETS; ++w)
+          ll += L.l[w][col] * (L.m[w][col] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(L.m[w][col] - mm));
+        put(cc, dim, y, ll);
+        if (J.ml && dim == 0) {
+          J.ml[2 * cc] = isnan(ll) ? ll : mm;
+          J.ml[2 * cc + 1] = ll;
+        }
+      }
+    }
+  }
+}
+
+constexpr int WIDE_CG = 2;
+
+// Workgroups: first the shared entries' ([chunk][column block][head]), then the own ones'. The chunks that do not
+// exist are the last of their kind.
+template <int HD, bool F16, bool PRE_WIDE, bool OWN_WIDE>
+__global__ __launch_bounds__(64 * WAVES, 2) void part_kernel(Paged c, PagedAttn a, Plan p, int pre_groups) {
+  constexpr int TILE = tile_of<F16>(), SETS = sets_of(HD);
+  __shared__ __align__(16) Shared<HD, F16> L;
+  const int shared = shared_entries(a);
+  Job J;
+  int id = blockIdx.x;
+  if (id < pre_groups) {
+    J.h = id % c.n_kv;
+    id /= c.n_kv;
+    J.block = id % p.pre_blocks;
+    const int x = id / p.pre_blocks;
+    const PreCut pc = pre_cut<TILE>(c, a, p, shared);
+    if (x >= pc.count) return;
+    J.col0 = 0;
+    J.cols = p.all;
+    J.pages = Pages{a.shared_pages, shared};
+    J.begin = 0;
+    J.t0 = pc.t0 + x * pc.tiles;
+    J.t1 = min(pc.t1, J.t0 + pc.tiles);
+    const size_t row = ((size_t)x * c.n_kv + J.h) * p.all;
+    J.ml = p.pml + 2 * row;
+    J.o = p.po + row * HD;
+    run_job<HD, F16, PRE_WIDE, PRE_WIDE ? WIDE_CG : 1>(c, a, p, J, L);
+    return;
+  }
+  id -= pre_groups;
+  J.h = id % c.n_kv;
+  id /= c.n_kv;
+  J.block = id % p.own_blocks;
+  const int x = id / p.own_blocks;
+  const Cut ct = cut<true, TILE, OWN_WIDE ? 1 : SETS>(c, a, p, shared, x, 0);
+  if (ct.count == 0) return;  // uniform
+  J.col0 = ct.b * p.cols;
+  J.cols = p.cols;
+  J.pages = Pages{c.table + (size_t)ct.b * c.max_pages, ct.n};
+  J.begin = shared;
+  int t0, t1;
+  own_range<TILE>(a, ct.n, shared, t0, t1);
+  J.t0 = t0 + (x - ct.first) * ct.tiles;
+  J.t1 = min(t1, J.t0 + ct.tiles);
+  const size_t row = ((size_t)x * c.n_kv + J.h) * p.cols;
+  J.ml = p.direct ? nullptr : p.ml + 2 * row;
+  J.o = p.direct ? nullptr : p.o + row * HD;
+  run_job<HD, F16, OWN_WIDE, OWN_WIDE ? WIDE_CG : 1>(c, a, p, J, L);
+}
+
+// The join: 64 dims of a column of a KV head a workgroup, sixteen partial results at a time.
+template <int HD, bool F16>
+__global__ __launch_bounds__(256) void join_kernel(Paged c, PagedAttn a, Plan p) {
+  constexpr int TILE = tile_of<F16>(), SETS = sets_of(HD), SD = 64, TPR = SD / 4, GRP = 256 / TPR;
+  __shared__ float w[2 * MAX_SPLIT];
+  __shared__ float red[2][4];
+  __shared__ __align__(16) f4_t acc[GRP][TPR];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int slice = blockIdx.x % (HD / SD), hc = blockIdx.x / (HD / SD), h = hc / p.all, col = hc - h * p.all;
+  const int b = col / p.cols, cc = col - b * p.cols;
+  const int shared = shared_entries(a);
+  const int pre = p.pre_chunks > 0 ? pre_cut<TILE>(c, a, p, shared).count : 0;
+  const Cut ct = p.own_wide ? cut<false, TILE, 1>(c, a, p, shared, 0, b) : cut<false, TILE, SETS>(c, a, p, shared, 0, b);
+  const int live = pre + ct.count;
+  const size_t pstep = (size_t)c.n_kv * p.all, ostep = (size_t)c.n_kv * p.cols;
+  const size_t prow = (size_t)h * p.all + col, orow = (size_t)ct.first * ostep + (size_t)h * p.cols + cc;
+  float m[2], l[2], top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int k = t + 256 * i;
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+    if (k < live) {
+      const float* ml = k < pre ? p.pml + 2 * (prow + k * pstep) : p.ml + 2 * (orow + (k - pre) * ostep);
+      m[i] = ml[0];
+      l[i] = ml[1];
+    }
+    top = fmaxf(top, m[i]);
+  }
+  top = wave_max(top);
+  if (lane == 0) red[0][wave] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float f = m[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[i] - top);
+    if (t + 256 * i < live) w[t + 256 * i] = f;
+    sum += l[i] * f;
+  }
+  sum = wave_sum(sum);
+  if (lane == 0) red[1][wave] = sum;
+  __syncthreads();
+  sum = red[1][0] + red[1][1] + red[1][2] + red[1][3];
+  const int g = t / TPR, d = slice * SD + 4 * (t % TPR);
+  f4_t y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int i = g; i < live; i += GRP) {
+    const float* o = i < pre ? p.po + (prow + i * pstep) * HD : p.o + (orow + (i - pre) * ostep) * HD;
+    y += *reinterpret_cast<const f4_t*>(o + d) * w[i];
+  }
+  acc[g][t % TPR] = y;
+  __syncthreads();
+  if (t < TPR) {
+#pragma unroll
+    for (int i = 1; i < GRP; ++i) y += acc[i][t];
+    const int tq = cc / p.group;
+    float* out = a.out + (((size_t)b * a.n_q + tq) * a.n_heads + h * p.group + cc - tq * p.group) * HD + d;
+    *reinterpret_cast<f4_t*>(out) = sum == 0.f ? f4_t{0.f, 0.f, 0.f, 0.f} : y / sum;
+  }
+}
+
+size_t up256(size_t x) { return (x + 255) / 256 * 256; }
+int blocks_of(int hd, long long cols, bool wide) {
+  const int per = wide ? sets_of(hd) * WIDE_CG * 16 : 16;
+  return (int)((cols + per - 1) / per);
+}
+
+// The plan for own parts of at most `own` entries (which may begin inside a tile: `edge`) and `shared` shared ones;
+// more of them never need less.
+Plan make_plan(const Paged& c, int n_heads, int n_q, int own, int shared, bool edge) {
+  Plan p{};
+  const int tile = c.f16 ? 32 : 16, sets = sets_of(c.hd);
+  p.group = n_heads / c.n_kv;
+  p.cols = p.group * n_q;
+  p.all = p.cols * c.batch;
+  p.own_wide = p.cols > 16;
+  p.pre_wide = p.all > 16;
+  p.own_blocks = blocks_of(c.hd, p.cols, p.own_wide);
+  p.pre_blocks = blocks_of(c.hd, p.all, p.pre_wide);
+  constexpr int target = 512;  // workgroups that fill the chip once, two a CU
+  const int tiles = (own + tile - 1) / tile + (edge ? 1 : 0);
+  const int step = p.own_wide ? 1 : sets;
+  p.tiles = p.own_wide ? 4 : 2 * step;
+  p.direct = shared == 0 && tiles <= p.tiles;
+  if (c.batch <= SHARED_BATCH) {
+    p.share = std::max(1, target / (c.n_kv * p.own_blocks));
+    p.nsplit = 0;
+    // (sum of ceil(tiles / size) <= total / size + batch, size >= total / share)
+    p.chunks = (int)std::min<long long>(p.share + c.batch, (long long)c.batch * std::max(1, (tiles + p.tiles - 1) / p.tiles));
+  } else {
+    const long long units = (long long)c.batch * c.n_kv * p.own_blocks;
+    const int want = (int)std::max<long long>(1, std::min<long long>(MAX_SPLIT, 2 * target / units));
+    p.nsplit = std::max(1, std::min(want, (tiles + p.tiles - 1) / p.tiles));
+    p.tiles = std::max(p.tiles, ((tiles + p.nsplit - 1) / p.nsplit + step - 1) / step * step);
+    p.chunks = c.batch * p.nsplit;
+    p.direct = shared == 0 && p.nsplit == 1;
+  }
+  if (shared > 0) {
+    const int pt = (shared + tile - 1) / tile;
+    p.pre_tiles = p.pre_wide ? 4 : 2 * sets;
+    p.pre_chunks = std::max(1, std::min({MAX_SPLIT, (pt + p.pre_tiles - 1) / p.pre_tiles, target / (c.n_kv * p.pre_blocks)}));
+  }
+  return p;
+}
+
+struct Sizes {
+  size_t ml, o, pml, po;
+  size_t all() const { return ml + o + pml + po; }
+};
+Sizes sizes(const Paged& c, const Plan& p) {
+  const size_t own = p.direct ? 0 : (size_t)p.chunks * c.n_kv * p.cols, pre = (size_t)p.pre_chunks * c.n_kv * p.all;
+  return {up256(own * 8), up256(own * c.hd * 4), up256(pre * 8), up256(pre * c.hd * 4)};
+}
+
+// Workgroups of the shared entries, of the own ones and of the join.
+struct Grid {
+  int pre, own, join;
+};
+Grid grid_of(const Paged& c, const Plan& p) {
+  const long long pre = (long long)p.pre_chunks * p.pre_blocks * c.n_kv, own = (long long)p.chunks * p.own_blocks * c.n_kv;
+  const long long join = p.direct ? 0 : (long long)c.n_kv * p.all * (c.hd / 64);
+  if (pre + own >= 1 << 24 || join >= 1 << 24) fail(ST_OP, "paged: dims too large");  // (2^32 threads)
+  return {(int)pre, (int)own, (int)join};
+}
+
+template <int HD, bool F16>
+void launch_hd(const Paged& c, const PagedAttn& a, const Plan& p, hipStream_t st) {
+  const Grid g = grid_of(c, p);
+  // (own_wide: pre_wide, too)
+  auto fn = p.own_wide   ? part_kernel<HD, F16, true, true>
+            : p.pre_wide ? part_kernel<HD, F16, true, false>
+                         : part_kernel<HD, F16, false, false>;
+  hipLaunchKernelGGL(fn, dim3((unsigned)(g.pre + g.own)), dim3(64 * WAVES), 0, st, c, a, p, g.pre);
+  if (g.join) hipLaunchKernelGGL((join_kernel<HD, F16>), dim3((unsigned)g.join), dim3(256), 0, st, c, a, p);
+}
+
+}  // namespace
+
+size_t paged_attention_workspace(const Paged& c, int n_heads, int n_q, int max_len, int max_shared) {
+  if (c.batch == 0 || n_q == 0) return 0;
+  const Plan p = make_plan(c, n_heads, n_q, max_len, max_shared, true);
+  grid_of(c, p);  // (refuses)
+  return sizes(c, p).all();
+}
+
+void launch_paged_attention(const Paged& c, const PagedAttn& a, void* ws, hipStream_t st) {
+  // the entries that a sequence's columns see at most, wherever they begin in their tile
+  const long long span = a.window > 0 ? std::min<long long>(a.max_len, (long long)a.window + a.n_q - 1) : a.max_len;
+  Plan p = make_plan(c, a.n_heads, a.n_q, (int)span, a.max_shared, span < a.max_len);
+  const Sizes z = sizes(c, p);
+  char* base = static_cast<char*>(ws);
+  p.ml = reinterpret_cast<float*>(base);
+  p.o = reinterpret_cast<float*>(base + z.ml);
+  p.pml = reinterpret_cast<float*>(base + z.ml + z.o);
+  p.po = reinterpret_cast<float*>(base + z.ml + z.o + z.pml);
+  auto go = [&](auto f) {
+    constexpr bool F16 = decltype(f)::value;
+    switch (c.hd) {
+      case 64: launch_hd<64, F16>(c, a, p, st); break;
+      case 128: launch_hd<128, F16>(c, a, p, st); break;
+      case 256: launch_hd<256, F16>(c, a, p, st); break;
+      default: launch_hd<512, F16>(c, a, p, st); break;
+    }
+  };
+  if (c.f16) go(std::true_type{});
+  else go(std::false_type{});
+}
+
+}  // namespace iek

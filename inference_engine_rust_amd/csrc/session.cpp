@@ -157,7 +157,7 @@ Session::~Session() {
   for (void* p : {(void*)x_, (void*)xn_, (void*)q_, (void*)k_, (void*)v_, (void*)att_, (void*)g_, (void*)u_,
                   (void*)act_, (void*)tmp_, (void*)xdec_, (void*)xndec_, (void*)qd_, (void*)kd_, (void*)vd_,
                   (void*)attd_, (void*)actd_, (void*)logits_, (void*)part_, (void*)tmpd_, (void*)d_pos_,
-                  (void*)d_step_, (void*)d_flags_, (void*)d_tok_, (void*)d_ids_, (void*)d_gen_, (void*)d_key_,
+                  (void*)d_step_, (void*)d_flags_, (void*)d_tok_, (void*)sample_ws_, (void*)d_ids_, (void*)d_gen_, (void*)d_key_,
                   (void*)d_flag_, (void*)d_cnt_, (void*)xs_, (void*)xsum_, kv_blob_, (void*)ple_tok_,
                   (void*)ple_proj_, (void*)ple_pack_, (void*)ple_tokd_, (void*)ple_projd_, (void*)ple_packd_,
                   (void*)xdec2_, (void*)xdec_save_, chain_blob_, (void*)d_chain_cnt_, (void*)d_chain_err_,
@@ -1545,6 +1545,21 @@ uint32_t Session::sample_temperature(float temperature, float r) {
   uint32_t tok = 0;
   IEK_HIP(hipMemcpyAsync(&tok, d_tok_, 4, hipMemcpyDeviceToHost, st_));
   sync();
+  return tok;
+}
+
+uint32_t Session::sample(const SampleParams& p) {
+  check_state();
+  if (m_->cfg.vocab == 0) fail(ST_SAMPLING, "logits slice is empty");
+  check_sample_params(p);
+  const size_t vocab = (size_t)m_->cfg.vocab;
+  if (!sample_ws_) sample_ws_ = dev_alloc<char>(sample_workspace(1, vocab) + 16);
+  logits_body(false);
+  launch_sample({logits_, (int)vocab, vocab, nullptr, nullptr, nullptr, nullptr, nullptr, d_tok_, nullptr, p}, 1, sample_ws_, st_);
+  uint32_t tok = 0;
+  IEK_HIP(hipMemcpyAsync(&tok, d_tok_, 4, hipMemcpyDeviceToHost, st_));
+  sync();
+  if (tok == NO_TOKEN) fail(ST_SAMPLING, "invalid logits for sampling (empty or non-finite)");
   return tok;
 }
 

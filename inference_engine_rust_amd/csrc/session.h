@@ -3,6 +3,7 @@
 #pragma once
 #include <vector>
 
+#include "kernels/sampling.h"
 #include "model.h"
 #include "kernels/chain.h"
 #include "kernels/mv_args.h"
@@ -29,6 +30,7 @@ class Session {
   void logits_last_token(float* out, int n);       // session.rs:71-74 (final_logits_last_token)
   uint32_t greedy_next_token();                    // generation.rs:10-16
   uint32_t sample_temperature(float temperature, float r);  // sampling.rs:54-79 on the device
+  uint32_t sample(const SampleParams& p);                   // with top-k, top-p and min-p
   // n x (greedy_next_token; decode_token), the loop of main.rs:100-116 / bench_metrics.rs:178-182,
   // replayed as one captured decode-step graph. Returns the n chosen ids.
   void generate_greedy(int n, uint32_t* out_ids, bool use_graph = true);
@@ -126,6 +128,7 @@ class Session {
   int* d_step_ = nullptr;
   int* d_flags_ = nullptr;
   uint32_t* d_tok_ = nullptr;
+  char* sample_ws_ = nullptr;  // of `sample`, from its first call on
   uint32_t* d_ids_ = nullptr;  // prompt ids / generated ids
   uint32_t* d_gen_ = nullptr;
   unsigned long long* d_key_ = nullptr;

@@ -55,6 +55,16 @@ class KV8Cache(ctypes.Structure):
     BLOCK = 32
 
 
+class PagedKV(ctypes.Structure):
+    """iek_paged_kv: a paged KV cache (dtype F32 or F16) over the caller's device buffers (addresses): pools k, v
+    [n_pages][n_kv_heads][page_size][head_dim] and int32 page numbers table [batch][max_pages]. The buffers must outlive
+    it."""
+    _fields_ = [("dtype", ctypes.c_int32), ("n_pages", ctypes.c_uint64), ("n_kv_heads", ctypes.c_uint64),
+                ("page_size", ctypes.c_uint64), ("head_dim", ctypes.c_uint64), ("k", ctypes.c_void_p),
+                ("v", ctypes.c_void_p), ("batch", ctypes.c_uint64), ("max_pages", ctypes.c_uint64),
+                ("table", ctypes.c_void_p)]
+
+
 class TokenizerPrompt(ctypes.Structure):
     """TokenizerPromptConfig (src/model_config.rs:8-60)."""
     _fields_ = [("add_bos_token", ctypes.c_int32), ("add_eos_token", ctypes.c_int32),
@@ -73,6 +83,8 @@ class ModelConfig(ctypes.Structure):
 _P = ctypes.c_void_p
 _SZ = ctypes.c_size_t
 _PKV8 = ctypes.POINTER(KV8Cache)
+_PPAGED = ctypes.POINTER(PagedKV)
+_F = ctypes.c_float
 EXPORTS = {
     "iek_last_error": ([], ctypes.c_char_p),
     "iek_model_load": ([ctypes.c_char_p, ctypes.c_int, ctypes.POINTER(_P)], ctypes.c_int),
@@ -95,6 +107,7 @@ EXPORTS = {
     "iek_greedy_next_token": ([_P, ctypes.POINTER(ctypes.c_uint32)], ctypes.c_int),
     "iek_session_sample_temperature": ([_P, ctypes.c_float, ctypes.c_float, ctypes.POINTER(ctypes.c_uint32)],
                                        ctypes.c_int),
+    "iek_session_sample": ([_P, _F, ctypes.c_int32, _F, _F, _F, ctypes.POINTER(ctypes.c_uint32)], ctypes.c_int),
     "iek_session_generate_greedy": ([_P, _SZ, _P], ctypes.c_int),
     "iek_session_kv_len": ([_P, ctypes.POINTER(ctypes.c_uint64)], ctypes.c_int),
     "iek_session_decode_path": ([_P, ctypes.POINTER(ctypes.c_int)], ctypes.c_int),
@@ -122,6 +135,8 @@ EXPORTS = {
     "iek_argmax": ([_P, _SZ, ctypes.POINTER(ctypes.c_uint32)], ctypes.c_int),
     "iek_sample_temperature": ([_P, _SZ, ctypes.c_float, ctypes.c_float, ctypes.POINTER(ctypes.c_uint32)],
                                ctypes.c_int),
+    "iek_sample": ([_P, _SZ, _F, ctypes.c_int32, _F, _F, _F, ctypes.POINTER(ctypes.c_uint32), ctypes.POINTER(_F)],
+                   ctypes.c_int),
     "iek_attention_decode": ([_P, _P, _P, _SZ, _SZ, _SZ, _SZ, _SZ, ctypes.c_float, _P], ctypes.c_int),
     "iek_dev_dequantize": ([ctypes.c_int, _P, _SZ, _P, _P], ctypes.c_int),
     "iek_dev_matmul": ([_P, _SZ, _SZ, ctypes.c_int, _P, _SZ, _SZ, _P, _P], ctypes.c_int),
@@ -147,6 +162,13 @@ EXPORTS = {
                               ctypes.c_int),
     "iek_kv8_evict_workspace": ([_PKV8, _SZ, _SZ, ctypes.POINTER(_SZ)], ctypes.c_int),
     "iek_dev_kv8_evict": ([_PKV8, _PKV8, _P, _P, _P, _P, _SZ, _SZ, _SZ, _SZ, _P, _P, _SZ, _P], ctypes.c_int),
+    "iek_rope_table": ([ctypes.c_uint32, ctypes.c_uint32, _F, _SZ, _P, _SZ, _P], ctypes.c_int),
+    "iek_dev_paged_append": ([_PPAGED, _P, _P, _P, _SZ, _SZ, _SZ, _P, _SZ, _SZ, _P, _P, _P, _P, _SZ, _P], ctypes.c_int),
+    "iek_paged_attention_workspace": ([_PPAGED, _SZ, _SZ, _SZ, _SZ, ctypes.POINTER(_SZ)], ctypes.c_int),
+    "iek_dev_paged_attention": ([_PPAGED, _P, _SZ, _SZ, _SZ, _P, _SZ, _P, _P, _SZ, _SZ, _F, _P, _P, _SZ, _P],
+                                ctypes.c_int),
+    "iek_sample_workspace": ([_SZ, _SZ, ctypes.POINTER(_SZ)], ctypes.c_int),
+    "iek_dev_sample": ([_P, _SZ, _SZ, _SZ, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P], ctypes.c_int),
     "iek_device_alloc": ([_SZ, ctypes.POINTER(_P)], ctypes.c_int),
     "iek_device_free": ([_P], ctypes.c_int),
     "iek_memcpy_h2d": ([_P, _P, _SZ], ctypes.c_int),
@@ -356,6 +378,15 @@ def sample_temperature_next_token(session: InferenceSession, temperature: float,
     return v.value
 
 
+def sample_next_token(session: InferenceSession, temperature: float, r: float, top_k: int = 0, top_p: float = 1.0,
+                      min_p: float = 0.0) -> int:
+    """A token of the session's last-token logits by temperature, top-k, top-p and min-p (include/iek.h, iek_sample) on
+    the device; r is a uniform draw in [0, 1)."""
+    v = ctypes.c_uint32()
+    _check(lib().iek_session_sample(session._h, temperature, top_k, top_p, min_p, r, ctypes.byref(v)))
+    return v.value
+
+
 def greedy_next_token(session: InferenceSession) -> int:
     """generation::greedy_next_token (src/engine/generation.rs:10-16), argmax on the device."""
     v = ctypes.c_uint32()
@@ -448,6 +479,24 @@ def host_sample_temperature(logits, temperature: float, r: float) -> int:
     v = ctypes.c_uint32()
     _check(lib().iek_sample_temperature(_np_ptr(x), x.size, temperature, r, ctypes.byref(v)))
     return v.value
+
+
+def host_sample(logits, temperature: float, r: float, top_k: int = 0, top_p: float = 1.0,
+                min_p: float = 0.0) -> tuple[int, float]:
+    """iek_sample: the token of one row of logits and its probability."""
+    x = _f32(logits)
+    v, p = ctypes.c_uint32(), ctypes.c_float()
+    _check(lib().iek_sample(_np_ptr(x), x.size, temperature, top_k, top_p, min_p, r, ctypes.byref(v), ctypes.byref(p)))
+    return v.value, p.value
+
+
+def rope_table(head_dim: int, rotary_dim: int, base: float, n: int, freq_factors=None) -> np.ndarray:
+    """(cos, sin) of the positions 0 .. n - 1, [n][rotary_dim / 2][2], as a session holds them (host memory)."""
+    out = np.empty((n, rotary_dim // 2, 2), np.float32)
+    ff = None if freq_factors is None else _f32(freq_factors)
+    _check(lib().iek_rope_table(head_dim, rotary_dim, base, n, None if ff is None else _np_ptr(ff),
+                                0 if ff is None else ff.size, _np_ptr(out)))
+    return out
 
 
 def host_argmax(logits) -> int:
@@ -590,6 +639,53 @@ def kv8_evict(src: KV8Cache, dst: KV8Cache, weights_ptr: int, weights_out_ptr: i
     """Sequences of more than `keep` entries cut down to the first, the last and the ones of the largest weight."""
     _check(lib().iek_dev_kv8_evict(src, dst, weights_ptr, weights_out_ptr, len_ptr, len_out_ptr, max_len, keep, first,
                                    last, index_out_ptr or None, workspace_ptr or None, workspace_bytes, stream or None))
+
+
+# ---- paged KV cache (include/iek.h): device pointers, asynchronous; a pointer of 0 is NULL ----
+
+def paged_append(cache: PagedKV, q_ptr: int, k_ptr: int, v_ptr: int, n_heads: int, n: int, row_stride: int, rope_ptr: int,
+                 rope_rows: int, rotary_dim: int, start_ptr: int = 0, count_ptr: int = 0, len_out_ptr: int = 0,
+                 q_out_ptr: int = 0, q_out_stride: int = 0, stream: int = 0) -> None:
+    """f32 rows [batch][n] (row_stride floats apart) rotated to the positions start[b] + i, i < count[b]: keys and values
+    into their pages, queries to q_out."""
+    _check(lib().iek_dev_paged_append(cache, q_ptr or None, k_ptr, v_ptr, n_heads, n, row_stride, rope_ptr or None, rope_rows,
+                                      rotary_dim, start_ptr or None, count_ptr or None, len_out_ptr or None,
+                                      q_out_ptr or None, q_out_stride, stream or None))
+
+
+def paged_attention_workspace(cache: PagedKV, n_heads: int, n_q: int, max_len: int, max_shared: int = 0) -> int:
+    """Bytes of the workspace of paged_attention."""
+    v = ctypes.c_size_t()
+    _check(lib().iek_paged_attention_workspace(cache, n_heads, n_q, max_len, max_shared, ctypes.byref(v)))
+    return v.value
+
+
+def paged_attention(cache: PagedKV, q_ptr: int, n_heads: int, n_q: int, q_stride: int, len_ptr: int, max_len: int,
+                    shared_pages_ptr: int, shared_ptr: int, max_shared: int, sliding_window: int, scale: float, out_ptr: int,
+                    workspace_ptr: int, workspace_bytes: int, stream: int = 0) -> None:
+    """Attention of the last n_q tokens of every sequence; the first *shared entries, which all of them begin with, are
+    read once."""
+    _check(lib().iek_dev_paged_attention(cache, q_ptr, n_heads, n_q, q_stride, len_ptr, max_len, shared_pages_ptr or None,
+                                         shared_ptr or None, max_shared, sliding_window, scale, out_ptr,
+                                         workspace_ptr or None, workspace_bytes, stream or None))
+
+
+# ---- sampling of a batch ----
+
+def sample_workspace(rows: int, n: int) -> int:
+    """Bytes of the workspace of sample."""
+    v = ctypes.c_size_t()
+    _check(lib().iek_sample_workspace(rows, n, ctypes.byref(v)))
+    return v.value
+
+
+def sample(logits_ptr: int, rows: int, n: int, row_stride: int, temperature_ptr: int, top_k_ptr: int, top_p_ptr: int,
+           min_p_ptr: int, r_ptr: int, out_index_ptr: int, out_prob_ptr: int, workspace_ptr: int, workspace_bytes: int,
+           stream: int = 0) -> None:
+    """The next token of every row of logits, by that row's temperature, top_k, top_p, min_p and uniform draw r."""
+    _check(lib().iek_dev_sample(logits_ptr, rows, n, row_stride, temperature_ptr, top_k_ptr or None, top_p_ptr or None,
+                                min_p_ptr or None, r_ptr, out_index_ptr, out_prob_ptr or None, workspace_ptr or None,
+                                workspace_bytes, stream or None))
 
 
 def synchronize() -> None:
