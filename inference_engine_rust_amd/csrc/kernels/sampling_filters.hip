@@ -6,11 +6,19 @@
 //   min-p: the ones with w_i >= min_p (M's token has 1).
 // The pick is the first token in index order up to which the kept weights sum to more than r times their total.
 //
-// Weights are summed as integers, w 2^S rounded, with S as large as n of them allow in 64 bits: sums do not depend on
-// their order, so atomics on histograms and any split give the same token every time, and a weight is off by 2^-S-1
-// of the largest (2^-48 at 32000 tokens), where f32 sums would move the borders of tokens by 1e-7 of the total.
-// A prefix is found by a radix selection on the logits' bits as ordered integers, 11, 11 and 10 bits at a time, of
-// counts (top-k) or of weights (top-p).
+// Weights are summed as integers, w 2^S rounded, with S as large as n of them allow in 64 bits and at most 50: sums do
+// not depend on their order, so atomics on histograms and any split give the same token every time, and a weight is
+// off by about 2^-S of the largest (2^-49 at 32000 tokens), where f32 sums would move the borders of tokens by 1e-7
+// of the total.
+//
+// A row of up to 32768 logits stays in the LDS of one workgroup. A border (top-k, top-p) is found by one histogram over
+// the distance to the maximum, of counts or of weights, in 2048 bins; the few tokens of the bin that the border is in
+// are ranked against each other. For a top-k of up to 1024 the threads' own maxima come first: the k-th largest of them
+// is no larger than the k-th logit, so what lies below it (all but about k tokens) is out, and the rest goes on as a
+// list; so do the tokens that top-p or min-p leave. A list of up to 512 is ranked as a whole. Rows that the bins do not
+// suit (thousands of equal logits at a border, a larger top-k, a draw of exactly 0) take any_row: a radix selection on
+// the logits' bits as ordered integers, 11, 11 and 10 bits at a time, from memory.
+// Bound by the latency of one workgroup's phases, and by the exponentials where every token needs one.
 #include "common.cuh"
 #include "sampling.h"
 
@@ -29,48 +37,157 @@ IEK_DEV uint32_t key_of(float x) {
 }
 IEK_DEV float value_of(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k); }
 
-// Weights of a row: w 2^S as an integer.
+// Weights of a row: w 2^S as an integer. 2^(y / 64), y = i + f, is a table's entry of 64 (in LDS) times a polynomial in
+// f of degree 5, which leaves out (f ln 2 / 64)^6 / 720 < 2^-54; the additions of 1.5 2^52 round to integers.
 struct Weigh {
-  double top, inv, one;  // one = 2^S
-  IEK_DEV double real(float x) const { return exp(((double)x - top) * inv); }
-  IEK_DEV u64 operator()(float x) const { return (u64)(real(x) * one + 0.5); }
-};
-
-IEK_DEV u64 wave_sum64(u64 v) {
-#pragma unroll
-  for (int s = 1; s < 64; s <<= 1) v += __shfl_xor(v, s);
-  return v;
-}
-// Inclusive prefix sum over the lanes.
-IEK_DEV u64 wave_scan64(u64 v) {
-#pragma unroll
-  for (int s = 1; s < 64; s <<= 1) {
-    const u64 up = __shfl_up(v, s);
-    if ((int)(threadIdx.x & 63) >= s) v += up;
+  double top, rate;  // 64 log2 e / T
+  double one;        // 2^S
+  const double* table;
+  IEK_DEV double real(float x) const {  // (2^-64 stands for everything below it)
+    const double y = fmax(((double)x - top) * rate, -4096.0), n = y + 0x1.8p52, f = y - (n - 0x1.8p52);
+    constexpr double L = 0.693147180559945309417232 / 64;
+    double e = L * L * L * L * L / 120;
+    e = fma(e, f, L * L * L * L / 24);
+    e = fma(e, f, L * L * L / 6);
+    e = fma(e, f, L * L / 2);
+    e = fma(e, f, L);
+    e = fma(e, f, 1.0);
+    const int i = (int)__double_as_longlong(n);
+    e *= table[i & 63];
+    return __longlong_as_double(__double_as_longlong(e) + ((long long)(i >> 6) << 52));
   }
-  return v;
+  IEK_DEV u64 whole(double w) const {  // w 2^S <= 2^50, to nearest
+    return (u64)__double_as_longlong(fma(w, one, 0x1p52)) & 0xFFFFFFFFFFFFFull;
+  }
+  IEK_DEV u64 operator()(float x) const { return whole(real(x)); }
+};
+IEK_DEV int scale_bits(int n) { return min(50, 32 + __clz(n)); }
+
+template <int CTRL, int ROWS = 0xF>
+IEK_DEV u64 dpp64(u64 v) {
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xF, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xF, false);
+  return (u64)hi << 32 | lo;
+}
+// Inclusive prefix sums over a row of 16 lanes, and over the wave.
+IEK_DEV u64 row_scan64(u64 v) {
+  v += dpp64<0x111>(v);  // row_shr 1, 2, 4, 8
+  v += dpp64<0x112>(v);
+  v += dpp64<0x114>(v);
+  return v + dpp64<0x118>(v);
+}
+IEK_DEV u64 wave_scan64(u64 v) {
+  v = row_scan64(v);
+  v += dpp64<DPP_BCAST15, 0xA>(v);
+  return v + dpp64<DPP_BCAST31, 0xC>(v);
+}
+IEK_DEV u64 lane64(u64 v, int lane) {
+  const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)v, lane), hi = __builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), lane);
+  return (u64)hi << 32 | lo;
 }
 
+constexpr int SLICE = 32768, LIST = 2048, NEAR = 512;  // tokens of a workgroup, of a list, and of a bin that are ranked
+
+// What the phases share beside the tokens.
 struct Smem {
-  u64 hist[BINS];
-  u64 part[NW];
+  double table[64];
+  u64 part[2][NW];
   u64 word;
-  int word2;
+  int word2, count, ties;
+  float border;
+};
+// Room for a histogram and for the tokens of its border: their keys << 32 | ~index (larger ones come first in
+// descending order) and weights.
+struct Bins {
+  u64 hist[BINS];
+  u64 near[NEAR], near_w[NEAR];
 };
 
-// The bin, from the top, in which the running sum of the histogram passes `need`, and the sum above it: the first
-// with above + hist > need (strictly) if STRICT, else >= need. (Some bin does.)
+// What a row keeps: the keys above `key` and the first `ties` of those that are it.
+struct Kept {
+  uint32_t key;
+  int ties;
+};
+
+// A row's parameters, its maximum, and whether there is a token to choose.
+struct Head {
+  float t, p, m, r;
+  int k;
+  float top;
+  bool good;
+};
+IEK_DEV SampleParams params_of(const SampleArgs& a, int b) {
+  if (!a.temperature) return a.one;
+  return {a.temperature[b], a.top_p ? a.top_p[b] : 1.f, a.min_p ? a.min_p[b] : 0.f, a.r[b], a.top_k ? a.top_k[b] : 0};
+}
+IEK_DEV Head head_of(const SampleParams& o, int n, float top) {  // (top: +inf if there is a NaN)
+  Head h{o.temperature, o.top_p, o.min_p, o.r, o.top_k >= n ? 0 : o.top_k, top, false};
+  // (a NaN parameter fails its comparison)
+  h.good = fabsf(h.top) < INFINITY && h.t >= 0.f && h.t < INFINITY && h.r >= 0.f && h.r < 1.f && h.p == h.p && h.m == h.m;
+  return h;
+}
+IEK_DEV void store(const SampleArgs& a, int b, uint32_t index, float prob) {
+  a.index[b] = index;
+  if (a.prob) a.prob[b] = prob;
+}
+IEK_DEV Weigh weigh_of(const Head& h, int n, const double* table) {
+  return Weigh{(double)h.top, 64 * 1.44269504088896340735992 / (double)h.t, (double)(1ull << scale_bits(n)), table};
+}
+// (the table is there after the next barrier)
+IEK_DEV void fill_table(double* table) {
+  if (threadIdx.x < 64) table[threadIdx.x] = exp2((double)threadIdx.x / 64);
+}
+// The probability of a token that was chosen.
+IEK_DEV float share(const Head& h, const Weigh& w, float x, u64 total) {
+  return (float)(exp(((double)x - w.top) / (double)h.t) / ((double)total / w.one));
+}
+
+// Sums over the workgroup, one barrier each: two of them in a row use different parts of m.part.
+struct Group {
+  Smem& m;
+  int turn;
+  IEK_DEV explicit Group(Smem& s) : m(s), turn(0) {}
+  // The sum of v over the threads before this one; total: over all.
+  IEK_DEV u64 before(u64 v, u64& total) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const u64 incl = wave_scan64(v);
+    if (lane == 63) m.part[turn][wave] = incl;
+    __syncthreads();
+    const u64 each = m.part[turn][lane & (NW - 1)], upto = row_scan64(each);
+    turn ^= 1;
+    total = lane64(upto, NW - 1);
+    return lane64(upto - each, wave) + incl - v;
+  }
+  IEK_DEV u64 sum(u64 v) {
+    u64 total;
+    before(v, total);
+    return total;
+  }
+  // The largest v, in every thread.
+  IEK_DEV float most(float v) {
+    v = wave_max(v);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    float* part = reinterpret_cast<float*>(m.part[turn]);
+    if (lane == 0) part[wave] = v;
+    __syncthreads();
+    v = row16_max(part[lane & (NW - 1)]);
+    turn ^= 1;
+    return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v)));
+  }
+};
+static_assert(NW == 16, "a row of lanes has the waves' parts");
+
+// ---- any row, from memory ---------------------------------------------------------------------------
+
+// The bin, from the top, in which the running sum of the histogram passes, and the sum above it. (Some bin does.)
 template <class Passes>
-IEK_DEV int pick_bin(Smem& m, Passes passes, u64& above) {
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+IEK_DEV int pick_bin(Group& q, const u64* hist, Passes passes, u64& above) {
+  Smem& m = q.m;
+  const int t = threadIdx.x;
   // thread t: bins BINS - 1 - 2 t and the next below
-  const u64 a = m.hist[BINS - 1 - 2 * t], b = m.hist[BINS - 2 - 2 * t];
-  const u64 incl = wave_scan64(a + b);
-  if (lane == 63) m.part[wave] = incl;
-  __syncthreads();
-  u64 base = 0;
-  for (int w = 0; w < wave; ++w) base += m.part[w];
-  const u64 before = base + incl - a - b;
+  const u64 a = hist[BINS - 1 - 2 * t], b = hist[BINS - 2 - 2 * t];
+  u64 total;
+  const u64 before = q.before(a + b, total);
   // (sums only grow: the one thread where it first passes)
   if (!passes(before) && passes(before + a + b)) {
     const bool first = passes(before + a);
@@ -84,13 +201,7 @@ IEK_DEV int pick_bin(Smem& m, Passes passes, u64& above) {
   return bin;
 }
 
-// What a row keeps: the keys above `key` and the first `ties` of those that are it.
-struct Kept {
-  uint32_t key;
-  int ties;
-};
-
-// A wave's run of the row: Q groups of 256 logits, four a lane.
+// A wave's run of the row: groups of 256 logits, four a lane.
 struct Row {
   const float* x;
   int n, groups, first;  // of a wave: groups of 256, from index `first`
@@ -107,25 +218,25 @@ struct Row {
 };
 
 template <bool WEIGHTS, class Passes>
-IEK_DEV Kept select(const Row& row, Smem& m, const Kept& now, const Weigh& weigh, Passes passes, u64& above) {
+IEK_DEV Kept select(const Row& row, Group& q, u64* hist, const Kept& now, const Weigh& weigh, Passes passes, u64& above) {
   uint32_t prefix = 0;
   u64 sum = 0;
   const uint32_t shifts[3] = {21, 10, 0};
   for (int d = 0; d < 3; ++d) {
     const uint32_t shift = shifts[d], bits = d == 2 ? 10 : 11;
-    for (int i = threadIdx.x; i < BINS; i += ST) m.hist[i] = 0;
+    for (int i = threadIdx.x; i < BINS; i += ST) hist[i] = 0;
     __syncthreads();
     row.each([&](float x, int) {
       const uint32_t k = key_of(x);
       if (k <= now.key || (d > 0 && (k >> (shift + bits)) != prefix)) return;
-      atomicAdd(&m.hist[(k >> shift) & ((1u << bits) - 1)], WEIGHTS ? weigh(x) : 1ull);
+      atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1)], WEIGHTS ? weigh(x) : 1ull);
     });
     // of the last key kept so far only its first ones
     if (threadIdx.x == 0 && (d == 0 || (now.key >> (shift + bits)) == prefix) && now.ties > 0)
-      atomicAdd(&m.hist[(now.key >> shift) & ((1u << bits) - 1)], (u64)now.ties * (WEIGHTS ? weigh(value_of(now.key)) : 1ull));
+      atomicAdd(&hist[(now.key >> shift) & ((1u << bits) - 1)], (u64)now.ties * (WEIGHTS ? weigh(value_of(now.key)) : 1ull));
     __syncthreads();
     u64 up;
-    const int bin = pick_bin(m, [&](u64 s) { return passes(sum + s); }, up);
+    const int bin = pick_bin(q, hist, [&](u64 s) { return passes(sum + s); }, up);
     sum += up;
     prefix = prefix << bits | (uint32_t)bin;
   }
@@ -133,87 +244,53 @@ IEK_DEV Kept select(const Row& row, Smem& m, const Kept& now, const Weigh& weigh
   return Kept{prefix, 0};
 }
 
-__global__ __launch_bounds__(ST) void sample_kernel(SampleArgs a) {
-  __shared__ Smem m;
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, b = blockIdx.x;
+// How many tokens of one weight the sum `above` them leaves room for below the limit of top-p (the first always).
+IEK_DEV int ties_below(double limit, u64 above, u64 weight) {
+  const double fit = ceil((limit - (double)above) / (double)weight);
+  return fit < 1 ? 1 : fit > 1e9 ? 1000000000 : (int)fit;
+}
+
+// A draw of 0 takes the first token of any weight, however small: `any` counts them.
+__device__ __noinline__ void any_row(const SampleArgs& a, int b, const Head& h, Smem& m, u64* hist) {
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  Group q(m);
+  __syncthreads();
   Row row{a.logits + (size_t)b * a.stride, a.n, 0, 0};
   row.groups = ((a.n + 255) / 256 + NW - 1) / NW;
   row.first = wave * row.groups * 256;
-  SampleParams o = a.one;
-  if (a.temperature) o = {a.temperature[b], a.top_p ? a.top_p[b] : 1.f, a.min_p ? a.min_p[b] : 0.f, a.r[b], a.top_k ? a.top_k[b] : 0};
-  const float temp = o.temperature, r = o.r, p = o.top_p;
-  const int k = o.top_k;
-  // the largest logit and its lowest index; a NaN counts as the largest
-  u64 best = 0;
-  row.each([&](float x, int i) {
-    const u64 v = (u64)(x != x ? 0xFFFFFFFFu : key_of(x)) << 32 | (uint32_t)~i;
-    best = best > v ? best : v;
-  });
-#pragma unroll
-  for (int s = 1; s < 64; s <<= 1) {
-    const u64 o = __shfl_xor(best, s);
-    best = best > o ? best : o;
-  }
-  if (lane == 0) m.part[wave] = best;
-  __syncthreads();
-  for (int w = 0; w < NW; ++w) best = best > m.part[w] ? best : m.part[w];
-  __syncthreads();
-  const uint32_t top_key = (uint32_t)(best >> 32);
-  const float top = value_of(top_key);
-  // (a NaN parameter fails its comparison)
-  const bool good = top_key != 0xFFFFFFFFu && fabsf(top) < INFINITY && temp >= 0.f && temp < INFINITY && r >= 0.f && r < 1.f &&
-                    p == p && o.min_p == o.min_p;
-  if (!good || temp == 0.f) {
-    if (t == 0) {
-      a.index[b] = good ? ~(uint32_t)best : NO_TOKEN;
-      if (a.prob) a.prob[b] = good ? 1.f : NAN;
-    }
-    return;
-  }
-  const Weigh weigh{(double)top, 1.0 / (double)temp, (double)(1ull << (32 + __clz(a.n)))};
+  const Weigh weigh = weigh_of(h, a.n, m.table);
   Kept kept{0, 0};
-  if (k > 0 && k < a.n) {
+  u64 unused;
+  if (h.k > 0) {
     u64 above;
-    kept = select<false>(row, m, kept, weigh, [&](u64 s) { return s >= (u64)k; }, above);
-    kept.ties = k - (int)above;
+    kept = select<false>(row, q, hist, kept, weigh, [&](u64 s) { return s >= (u64)h.k; }, above);
+    kept.ties = h.k - (int)above;
   }
-  if (p < 1.f) {
+  if (h.p < 1.f) {
     u64 total = 0;
     row.each([&](float x, int) {
       if (key_of(x) > kept.key) total += weigh(x);
     });
-    total = wave_sum64(total);
-    if (lane == 0) m.part[wave] = total;
-    __syncthreads();
-    total = (u64)kept.ties * weigh(value_of(kept.key));
-    for (int w = 0; w < NW; ++w) total += m.part[w];
-    __syncthreads();
-    const double limit = (double)p * (double)total;
+    total = q.sum(total);
+    total += (u64)kept.ties * weigh(value_of(kept.key));
+    const double limit = (double)h.p * (double)total;
     u64 above;
     // (of p <= 0 the first token stays)
-    const Kept next = select<true>(row, m, kept, weigh, [&](u64 s) { return s > 0 && !((double)s < limit); }, above);
-    const double w = (double)weigh(value_of(next.key));
-    const double fit = ceil((limit - (double)above) / w);
-    const int ties = fit < 1 ? 1 : fit > (double)a.n ? a.n : (int)fit;
+    const Kept next = select<true>(row, q, hist, kept, weigh, [&](u64 s) { return s > 0 && !((double)s < limit); }, above);
+    const int ties = ties_below(limit, above, weigh(value_of(next.key)));
     kept.ties = next.key == kept.key ? min(kept.ties, ties) : ties;
     kept.key = next.key;
   }
   // in index order: each wave's ties, then its sum of kept weights
   int equal = 0;
   row.each([&](float x, int) { equal += kept.ties > 0 && key_of(x) == kept.key; });
-  equal = (int)wave_sum64(equal);
-  if (lane == 0) m.part[wave] = equal;
-  __syncthreads();
-  int seen = 0;  // ties before the wave's run
-  for (int w = 0; w < wave; ++w) seen += (int)m.part[w];
-  __syncthreads();
-  const double floor_w = fminf(o.min_p, 1.f);
-  // of a draw of 0, which takes the first token of any weight, all of them have one here
+  const int seen = __shfl((int)q.before(equal, unused), 0);  // ties before the wave's run
+  const double least = fminf(h.m, 1.f);
   auto weight = [&](float x, bool tie_kept, bool any) -> u64 {
     const uint32_t key = key_of(x);
     if (!(key > kept.key || (tie_kept && key == kept.key))) return 0;
     const double w = weigh.real(x);
-    return !(w >= floor_w) ? 0 : any ? w > 0 : (u64)(w * weigh.one + 0.5);
+    return !(w >= least) ? 0 : any ? exp(((double)x - weigh.top) / (double)h.t) > 0 : weigh.whole(w);
   };
   // one pass over the run, group by group: f(weights of the lane's four, their index)
   auto walk = [&](bool any, auto f) {
@@ -240,44 +317,28 @@ __global__ __launch_bounds__(ST) void sample_kernel(SampleArgs a) {
       if (f(w, i0)) break;
     }
   };
-  u64 mine = 0;
-  walk(false, [&](const u64(&w)[4], int) {
-    mine += w[0] + w[1] + w[2] + w[3];
-    return false;
-  });
-  mine = wave_sum64(mine);
-  if (lane == 0) m.part[wave] = mine;
-  __syncthreads();
-  u64 total = 0, base = 0;
-  for (int w = 0; w < NW; ++w) {
-    if (w == wave) base = total;
-    total += m.part[w];
-  }
-  const u64 all_of_it = total;
-  if (r == 0.f) {
-    mine = 0;
-    walk(true, [&](const u64(&w)[4], int) {
-      mine += w[0] + w[1] + w[2] + w[3];
+  auto sums = [&](bool any, u64& mine, u64& base, u64& total) {
+    u64 s = 0;
+    walk(any, [&](const u64(&w)[4], int) {
+      s += w[0] + w[1] + w[2] + w[3];
       return false;
     });
-    mine = wave_sum64(mine);
-    __syncthreads();
-    if (lane == 0) m.part[wave] = mine;
-    __syncthreads();
-    total = base = 0;
-    for (int w = 0; w < NW; ++w) {
-      if (w == wave) base = total;
-      total += m.part[w];
-    }
-  }
-  const double limit = (double)r * (double)total;
+    const u64 upto = wave_scan64(s);
+    mine = lane64(upto, 63);
+    base = lane64(q.before(s, total), 0);
+  };
+  u64 mine, base, total, whole;
+  sums(false, mine, base, total);
+  whole = total;
+  if (h.r == 0.f) sums(true, mine, base, total);
+  const double limit = (double)h.r * (double)total;
   if ((double)base > limit || !((double)(base + mine) > limit)) return;  // another wave's
   u64 sum = base;
-  walk(r == 0.f, [&](const u64(&w)[4], int i0) {
+  walk(h.r == 0.f, [&](const u64(&w)[4], int i0) {
     const u64 all = w[0] + w[1] + w[2] + w[3], upto = sum + wave_scan64(all);
     const u64 here = __ballot((double)upto > limit);
     if (here == 0) {
-      sum = __shfl(upto, 63);
+      sum = lane64(upto, 63);
       return false;
     }
     if (lane == __ffsll(here) - 1) {
@@ -286,11 +347,469 @@ __global__ __launch_bounds__(ST) void sample_kernel(SampleArgs a) {
 #pragma unroll
       for (int j = 0; j < 3; ++j)
         if (c == j && !((double)(s += w[j]) > limit)) c = j + 1;
-      a.index[b] = (uint32_t)(i0 + c);
-      if (a.prob) a.prob[b] = (float)(weigh.real(row.x[i0 + c]) / ((double)all_of_it / weigh.one));
+      store(a, b, (uint32_t)(i0 + c), share(h, weigh, row.x[i0 + c], whole));
     }
     return true;
   });
+}
+
+// ---- rows and lists in LDS ----------------------------------------------------------------------------
+
+// Tokens in index order, each thread with a run of 4 * quads of them in a row; -inf behind the last one, up to the last
+// thread's. Quad s is stored at s ^ (s >> 3 & 7): the quads that neighbouring threads read at a time, `quads` apart, are
+// then in different banks. index: the tokens' indexes, or null: first, first + 1, ...
+IEK_DEV int stored(int quad) { return quad ^ (quad >> 3 & 7); }
+IEK_DEV int quads_of(int n) { return (n + 4 * ST - 1) / (4 * ST); }
+struct Tokens {
+  const float4* x;
+  const uint32_t* index;
+  int quads, first;
+  IEK_DEV float value(int i) const { return reinterpret_cast<const float*>(x + stored(i >> 2))[i & 3]; }
+  IEK_DEV uint32_t at(int i) const { return index ? index[i] : (uint32_t)(first + i); }
+  template <int U = 2, class F>
+  IEK_DEV void each(F f) const {  // f(value, place)
+#pragma unroll U
+    for (int j = 0; j < quads; ++j) {
+      const int s = (int)threadIdx.x * quads + j;
+      const float4 v = x[stored(s)];
+      f(v.x, 4 * s);
+      f(v.y, 4 * s + 1);
+      f(v.z, 4 * s + 2);
+      f(v.w, 4 * s + 3);
+    }
+  }
+};
+
+// n <= SLICE logits from p on into LDS; returns the largest of those that the thread loaded, +inf for a NaN. (A
+// row's address is a multiple of 4 bytes.)
+IEK_DEV float load_tokens(float4* to, const float* p, int n) {
+  typedef float f4u_t __attribute__((ext_vector_type(4), aligned(4)));
+  constexpr int U = SLICE / (4 * ST);
+  const int t = threadIdx.x, quads = quads_of(n);
+  f4u_t v[U];
+  // all loads first, the last quads from where four are left (a row of fewer than four has no vector to load)
+#pragma unroll
+  for (int q = 0; q < U; ++q) {
+    if (q >= quads) break;  // uniform
+    if (n >= 4) {
+      v[q] = *reinterpret_cast<const f4u_t*>(p + min(4 * (q * ST + t), n - 4));
+    } else {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) v[q][c] = p[min(c, n - 1)];
+    }
+  }
+  float most = -INFINITY;
+  bool nan = false;
+#pragma unroll
+  for (int q = 0; q < U; ++q) {
+    if (q >= quads) break;
+    const int i = 4 * (q * ST + t);
+    float x[4] = {v[q][0], v[q][1], v[q][2], v[q][3]};
+    if (4 * ST * (q + 1) > n) {  // uniform: the last ones
+      const int s = n >= 4 ? max(0, i - (n - 4)) : 0;  // (the loaded ones begin s before i)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        float y = v[q][c];
+#pragma unroll
+        for (int d = 1; d < 4; ++d)
+          if (s == d) y = v[q][(c + d) & 3];
+        x[c] = i + c < n ? y : -INFINITY;
+      }
+    }
+    to[stored(q * ST + t)] = make_float4(x[0], x[1], x[2], x[3]);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      nan |= x[c] != x[c];
+      most = fmaxf(most, x[c]);
+    }
+  }
+  return nan ? INFINITY : most;
+}
+
+IEK_DEV float steps(float x, float top, float scale) { return fminf((top - x) * scale, (float)(BINS - 1)); }
+IEK_DEV int bin_of(float x, float top, float scale) { return (int)steps(x, top, scale); }
+
+IEK_DEV void clear_bins(Smem& m, u64* hist) {
+#pragma unroll
+  for (int i = 0; i < BINS / ST; ++i) hist[threadIdx.x + ST * i] = 0;
+  if (threadIdx.x == 0) {
+    m.count = 0;
+    m.word2 = -1;
+  }
+  __syncthreads();
+}
+// The bin in which the tokens stop being kept: keeps(sum before it, the total), but not all of it; -1 if all are kept.
+// above: the sum before it.
+template <class Keeps>
+IEK_DEV int cross(Group& q, const u64* hist, Keeps keeps, u64& above, u64& total) {
+  const int t = threadIdx.x;
+  Smem& m = q.m;
+  const u64 a = hist[2 * t], b = hist[2 * t + 1];
+  const u64 before = q.before(a + b, total);
+  if (keeps(before, total) && !keeps(before + a + b, total)) {
+    const bool first = !keeps(before + a, total);
+    m.word = first ? before : before + a;
+    m.word2 = 2 * t + (first ? 0 : 1);
+  }
+  __syncthreads();
+  above = m.word;
+  return m.word2;
+}
+
+// What is kept: the tokens above `over`, and the first `ties` of those that are it.
+struct Cut {
+  float over;
+  int ties;
+};
+
+// The border among n <= NEAR tokens of a bin: keeps(the sum before a token). m.border, m.ties: the last value that stays
+// and how many of it; m.word: the sum up to it; m.word2: whether it is the last of them.
+template <class Keeps>
+IEK_DEV void rank_near(Smem& m, const Bins& s, int n, u64 above, Keeps keeps) {
+  const int t = threadIdx.x;
+  if (t < n) {
+    const u64 me = s.near[t], own = s.near_w[t];
+    u64 sum = above;
+    int equal = 1;
+    bool last = true;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) {
+      const u64 o = s.near[j], w = s.near_w[j];
+      const bool before = o > me;
+      sum += before ? w : 0;
+      equal += before && (uint32_t)(o >> 32) == (uint32_t)(me >> 32);
+      last &= o >= me;
+    }
+    if (keeps(sum) && (last || !keeps(sum + own))) {
+      m.border = value_of((uint32_t)(me >> 32));
+      m.ties = equal;
+      m.word = sum + own;
+      m.word2 = last;
+    }
+  }
+  __syncthreads();
+}
+
+// Adds up weights (or counts) of the tokens above `over` in bins of 1 / scale from the top.
+IEK_DEV void fill_bins(const Tokens& T, u64* hist, const Weigh& weigh, bool counts, float top, float scale, float over) {
+  T.each([&](float x, int) {
+    const u64 w = counts ? 1 : weigh(x);
+    if (x > over && w) atomicAdd(&hist[bin_of(x, top, scale)], w);
+  });
+}
+// Puts the tokens above `over` of a bin into s.near, in any order; m.count of them (more than NEAR: not all are there).
+IEK_DEV void gather_near(const Tokens& T, Smem& m, Bins& s, const Weigh& weigh, bool counts, float top, float scale, float over, int bin) {
+  T.each([&](float x, int i) {
+    if (!(x > over && bin_of(x, top, scale) == bin)) return;
+    const int at = atomicAdd(&m.count, 1);
+    if (at < NEAR) {
+      s.near[at] = (u64)key_of(x) << 32 | (uint32_t)~T.at(i);
+      s.near_w[at] = counts ? 1 : weigh(x);
+    }
+  });
+  __syncthreads();
+}
+
+// Cuts the tokens kept to those that keeps(the sum before them, the total). False: the bin of the border has too many
+// tokens. counts: sums are of tokens, not of weights. (Of now.over only now.ties stay.)
+template <class Keeps>
+IEK_DEV bool cut_at(const Tokens& T, Group& q, Bins& s, const Weigh& weigh, bool counts, float top, float scale, Cut& now, Keeps keeps) {
+  Smem& m = q.m;
+  clear_bins(m, s.hist);
+  fill_bins(T, s.hist, weigh, counts, top, scale, now.over);
+  const int tie_bin = now.ties > 0 ? bin_of(now.over, top, scale) : -1;
+  const u64 tie_w = now.ties > 0 ? (counts ? 1 : weigh(now.over)) : 0;
+  if (threadIdx.x == 0 && now.ties > 0) atomicAdd(&s.hist[tie_bin], tie_w * (u64)now.ties);
+  __syncthreads();
+  u64 above, total;
+  const int bin = cross(q, s.hist, keeps, above, total);
+  if (bin < 0) return true;  // all of them
+  gather_near(T, m, s, weigh, counts, top, scale, now.over, bin);
+  const int n = m.count;
+  if (n > NEAR) return false;
+  if (threadIdx.x == 0) {
+    m.word2 = n == 0;
+    m.word = above;
+  }
+  __syncthreads();
+  rank_near(m, s, n, above, [&](u64 v) { return keeps(v, total); });
+  // all of the bin's, and some of the value that was the last one before
+  const u64 sum = m.word;
+  if (m.word2 && bin == tie_bin && keeps(sum, total)) {
+    // (the sums before them are sum + j tie_w)
+    int lo = 0, hi = now.ties;  // keeps(lo); not keeps(hi), or hi is all of them
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      (keeps(sum + tie_w * (u64)mid, total) ? lo : hi) = mid;
+    }
+    now.ties = lo + 1;
+  } else {
+    now = Cut{m.border, m.ties};
+  }
+  __syncthreads();
+  return true;
+}
+
+// How a row's tokens are weighed at the end: those kept, if not below min-p.
+struct Final {
+  Weigh weigh;
+  double least;
+  Cut cut;
+  u64 tie_w;
+  IEK_DEV Final(const Weigh& w, const Head& h, const Cut& c) : weigh(w), least(fminf(h.m, 1.f)), cut(c), tie_w(0) {
+    if (c.ties > 0) tie_w = weight(c.over);
+  }
+  IEK_DEV u64 weight(float x) const {
+    const double w = weigh.real(x);
+    return w >= least ? weigh.whole(w) : 0;
+  }
+};
+
+// The thread's sum of kept weights. ties: how many of the value `over` come before its run.
+IEK_DEV u64 run_sum(const Tokens& T, Group& q, const Final& f, int& ties) {
+  u64 sum = 0;
+  int equal = 0;
+#pragma unroll 2
+  for (int j = 0; j < T.quads; ++j) {
+    const float4 v = T.x[stored((int)threadIdx.x * T.quads + j)];
+    const float x[4] = {v.x, v.y, v.z, v.w};
+    const float most = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+    if (f.cut.ties > 0) equal += (x[0] == f.cut.over) + (x[1] == f.cut.over) + (x[2] == f.cut.over) + (x[3] == f.cut.over);
+    if (!__any(most > f.cut.over)) continue;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const u64 w = f.weight(x[c]);
+      sum += x[c] > f.cut.over ? w : 0;
+    }
+  }
+  ties = 0;
+  if (f.cut.ties > 0) {
+    u64 unused;
+    ties = (int)q.before(equal, unused);
+    sum += f.tie_w * (u64)max(0, min(f.cut.ties - ties, equal));
+  }
+  return sum;
+}
+// Stores the token of T at which the running sum first exceeds the limit: `base` before the thread's run, `sum` in it.
+IEK_DEV void pick_in_run(const Tokens& T, const Final& f, u64 base, u64 sum, int ties, double limit, const SampleArgs& a, int b, const Head& h,
+                         u64 total) {
+  const unsigned long long here = __ballot(!((double)base > limit) && (double)(base + sum) > limit);
+  if (here == 0) return;  // another wave's
+  // the wave goes through that thread's run, a token a lane
+  const int owner = __ffsll(here) - 1, lane = threadIdx.x & 63, per = 4 * T.quads;
+  const int i = (((int)threadIdx.x & ~63) + owner) * per + min(lane, per - 1);
+  const float x = T.value(i);
+  const bool live = lane < per, tie = live && f.cut.ties > 0 && x == f.cut.over;
+  const int rank = __builtin_amdgcn_readlane(ties, owner) + __popcll(__ballot(tie) & ((1ull << lane) - 1));
+  const u64 w = live && x > f.cut.over ? f.weight(x) : tie && rank < f.cut.ties ? f.tie_w : 0;
+  const u64 upto = lane64(base, owner) + wave_scan64(w);
+  const unsigned long long past = __ballot(live && (double)upto > limit);
+  if (past != 0 && lane == __ffsll(past) - 1) store(a, b, T.at(i), share(h, f.weigh, x, total));
+}
+
+// The token of a row, of tokens T cut to `cut`.
+IEK_DEV void pick(const Tokens& T, Group& q, const SampleArgs& a, int b, const Head& h, const Weigh& weigh, const Cut& cut) {
+  const Final f(weigh, h, cut);
+  int ties;
+  const u64 sum = run_sum(T, q, f, ties);
+  u64 total;
+  const u64 base = q.before(sum, total);
+  pick_in_run(T, f, base, sum, ties, (double)h.r * (double)total, a, b, h, total);
+}
+
+// A list of tokens in LDS, in index order, and its room.
+struct List {
+  float4* x;
+  uint32_t* index;
+  IEK_DEV void put(int at, float v, uint32_t i) const {
+    reinterpret_cast<float*>(x + stored(at >> 2))[at & 3] = v;
+    index[at] = i;
+  }
+  // the list of n as tokens
+  IEK_DEV Tokens tokens(int n) const {
+    for (int i = n + (int)threadIdx.x; i < LIST; i += ST) put(i, -INFINITY, 0);
+    for (int i = LIST / 4 + (int)threadIdx.x; i < ST; i += ST) x[stored(i)] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    __syncthreads();
+    return Tokens{x, index, 1, 0};
+  }
+};
+constexpr int LIST_BYTES = 16 * ST + 4 * LIST;
+
+// The tokens that in(value) holds for, in index order, to put(place, value, index), if there are at most `room`; returns
+// how many there are.
+template <class In, class Put>
+IEK_DEV int compact(const Tokens& T, Group& q, int room, In in, Put put) {
+  int mine = 0;
+  T.each([&](float v, int) { mine += in(v); });
+  u64 total;
+  int at = (int)q.before(mine, total);
+  if ((int)total <= room && mine > 0)
+    T.each([&](float v, int i) {
+      if (in(v)) put(at++, v, T.at(i));
+    });
+  return (int)total;
+}
+
+// A bound on the distance of the first k tokens, as steps below `far` of 1 / scale from the top. most: the largest of a
+// thread's share of the tokens.
+IEK_DEV float bound_of_k(Group& q, u64* hist, float most, int k, float top, float& scale) {
+  // bins from the largest to the least of the threads' largest
+  const float span = q.most(most > -INFINITY ? top - most : 0.f);
+  scale = fminf((float)(BINS - 1) / span, 1e30f);  // (a span of 0: 1e30)
+  clear_bins(q.m, hist);
+  if (most > -INFINITY) atomicAdd(&hist[bin_of(most, top, scale)], 1ull);
+  __syncthreads();
+  u64 above, all;
+  const int bin = cross(q, hist, [&](u64 v, u64) { return v < (u64)k; }, above, all);
+  return bin < 0 ? INFINITY : (float)(bin + 1);  // (no bin: fewer than k threads have any)
+}
+
+// The token of a row whose n <= NEAR tokens that may be kept are the list: all of them ranked against each other.
+IEK_DEV void pick_of_few(const Tokens& T, int n, Group& q, Bins& s, const SampleArgs& a, int b, const Head& h, const Weigh& weigh) {
+  const int t = threadIdx.x;
+  const bool live = t < n;
+  const float x = live ? T.value(t) : -INFINITY;
+  const double real = weigh.real(x);
+  const u64 w = live ? weigh.whole(real) : 0;
+  if (live) {
+    s.near[t] = (u64)key_of(x) << 32 | (uint32_t)~T.at(t);
+    s.near_w[t] = w;
+  }
+  __syncthreads();
+  // `each` threads a token (a power of two up to a wave), the sums and counts before it joined over their lanes
+  const int size = n <= 16 ? 16 : 1 << (32 - __clz(n - 1)), each = ST / size, me = t / each;
+  u64 sum = 0;
+  int count = 0;
+  if (me < n) {
+    const u64 mine = s.near[me];
+#pragma unroll 4
+    for (int j = t & (each - 1); j < n; j += each) {
+      const bool before = s.near[j] > mine;
+      sum += before ? s.near_w[j] : 0;
+      count += before;
+    }
+  }
+  for (int d = 1; d < each; d <<= 1) {
+    sum += __shfl_xor(sum, d);
+    count += __shfl_xor(count, d);
+  }
+  if ((t & (each - 1)) == 0 && me < n) {
+    s.hist[me] = sum;
+    s.hist[NEAR + me] = (u64)count;
+  }
+  __syncthreads();
+  const u64 above = live ? s.hist[t] : 0;
+  const bool first = live && (h.k <= 0 || (int)s.hist[NEAR + t] < h.k);
+  bool kept = first && (t >= n || real >= fminf(h.m, 1.f));
+  if (h.p < 1.f) {
+    const u64 all = q.sum(first ? w : 0);
+    kept &= above == 0 || (double)above < (double)h.p * (double)all;
+  }
+  u64 total;
+  const u64 base = q.before(kept ? w : 0, total);
+  const double limit = (double)h.r * (double)total;
+  if (kept && !((double)base > limit) && (double)(base + w) > limit) store(a, b, T.at(t), share(h, weigh, x, total));
+}
+
+// What top-k and top-p keep of T. False: it is left to any_row.
+IEK_DEV bool filter(const Tokens& T, Group& q, Bins& s, const Head& h, const Weigh& weigh, float k_scale, float p_scale, Cut& cut) {
+  if (h.k > 0 && !cut_at(T, q, s, weigh, true, h.top, k_scale, cut, [&](u64 v, u64) { return v < (u64)h.k; })) return false;
+  return !(h.p < 1.f) ||
+         cut_at(T, q, s, weigh, false, h.top, p_scale, cut, [&](u64 v, u64 all) { return v == 0 || (double)v < (double)h.p * (double)all; });
+}
+
+IEK_DEV float weight_scale(const Head& h) { return fminf(64.f * 1.44269504f / h.t, 1e30f); }
+
+// The lowest index of the largest logit, by one thread of the workgroup.
+IEK_DEV void store_top(const Tokens& T, Group& q, const SampleArgs& a, int b, float top) {
+  int at = INT32_MAX;
+  T.each([&](float x, int i) { at = x == top ? min(at, i) : at; });
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) at = min(at, __shfl_xor(at, d));
+  u64 total;
+  const u64 before = q.before((threadIdx.x & 63) == 0 && at != INT32_MAX, total);
+  if ((threadIdx.x & 63) == 0 && at != INT32_MAX && before == 0) store(a, b, T.at(at), 1.f);
+}
+
+// Rows of up to SLICE logits.
+__global__ __launch_bounds__(ST) void row_kernel(SampleArgs a) {
+  __shared__ Smem m;
+  __shared__ float4 data[SLICE / 4];
+  __shared__ __align__(16) char more[sizeof(Bins) > LIST_BYTES ? sizeof(Bins) : LIST_BYTES];
+  const int b = blockIdx.x;
+  const SampleParams o = params_of(a, b);
+  Group q(m);
+  const float most = load_tokens(data, a.logits + (size_t)b * a.stride, a.n);
+  fill_table(m.table);
+  const Head h = head_of(o, a.n, q.most(most));
+  Tokens T{data, nullptr, quads_of(a.n), 0};
+  if (!h.good) {
+    if (threadIdx.x == 0) store(a, b, NO_TOKEN, NAN);
+    return;
+  }
+  if (h.t == 0.f) return store_top(T, q, a, b, h.top);
+  const Weigh weigh = weigh_of(h, a.n, m.table);
+  Bins& bins = *reinterpret_cast<Bins*>(more);
+  // the list takes the histogram's place after it, and the bins then the tokens'
+  const List list{reinterpret_cast<float4*>(more), reinterpret_cast<uint32_t*>(more + 16 * ST)};
+  Bins& room = *reinterpret_cast<Bins*>(data);
+  auto put = [&](int at, float v, uint32_t i) { list.put(at, v, i); };
+  Cut cut{-INFINITY, 0};
+  if (h.r == 0.f) return any_row(a, b, h, m, bins.hist);
+  float scale = 0.f;
+  int n = LIST + 1;
+  if (h.k > 0 && (h.k <= ST || a.n <= LIST)) {
+    const float far = bound_of_k(q, bins.hist, most, min(h.k, ST), h.top, scale);
+    n = compact(T, q, LIST, [&](float v) { return v > -INFINITY && fminf((h.top - v) * scale, 1e30f) < far; }, put);
+    if (far < INFINITY) scale = fminf(scale * ((float)BINS / far), 1e30f);
+  } else if (h.k <= 0 && !(h.p < 1.f) && h.m > 0.f) {
+    // (a distance that is too large by the roundings at least: min-p itself is looked at later)
+    const float far = -logf(fminf(h.m, 1.f)) * h.t * 1.0001f + 1e-6f * fabsf(h.top) + 1e-30f;
+    n = compact(T, q, LIST, [&](float v) { return h.top - v <= far; }, put);
+  }
+  if (n <= LIST) {
+    const Tokens L = list.tokens(n);
+    if (n <= NEAR) return pick_of_few(L, n, q, room, a, b, h, weigh);
+    if (!filter(L, q, room, h, weigh, scale, scale, cut)) return any_row(a, b, h, m, room.hist);
+    return pick(L, q, a, b, h, weigh, cut);
+  }
+  if (h.k > 0) {
+    float span = 0.f;
+    T.each([&](float x, int) { span = x > -INFINITY ? fmaxf(span, h.top - x) : span; });
+    scale = fminf((float)(BINS - 1) / q.most(span), 1e30f);
+  }
+  if (!filter(T, q, bins, h, weigh, scale, weight_scale(h), cut)) return any_row(a, b, h, m, bins.hist);
+  if (cut.ties > 0) {
+    n = compact(T, q, LIST, [&](float v) { return v >= cut.over; }, put);
+    if (n <= LIST) return pick(list.tokens(n), q, a, b, h, weigh, cut);
+  }
+  pick(T, q, a, b, h, weigh, cut);
+}
+
+__global__ __launch_bounds__(ST) void any_kernel(SampleArgs a) {
+  __shared__ Smem m;
+  __shared__ float4 data[SLICE / 4];
+  __shared__ u64 hist[BINS];
+  const int b = blockIdx.x;
+  const SampleParams o = params_of(a, b);
+  Group q(m);
+  fill_table(m.table);
+  float most = -INFINITY;
+  for (int s0 = 0; s0 < a.n; s0 += SLICE) most = fmaxf(most, load_tokens(data, a.logits + (size_t)b * a.stride + s0, min(SLICE, a.n - s0)));
+  const Head h = head_of(o, a.n, q.most(most));
+  if (!h.good) {
+    if (threadIdx.x == 0) store(a, b, NO_TOKEN, NAN);
+    return;
+  }
+  if (h.t == 0.f) {
+    for (int s0 = 0; s0 < a.n; s0 += SLICE) {
+      const int n = min(SLICE, a.n - s0);
+      __syncthreads();
+      const float here = load_tokens(data, a.logits + (size_t)b * a.stride + s0, n);
+      if (q.most(here) == h.top) return store_top(Tokens{data, nullptr, quads_of(n), s0}, q, a, b, h.top);
+    }
+  }
+  any_row(a, b, h, m, hist);
 }
 
 }  // namespace
@@ -305,7 +824,7 @@ void check_sample_params(const SampleParams& p) {
 size_t sample_workspace(size_t rows, size_t n) { return 0; }
 
 void launch_sample(const SampleArgs& a, int rows, void* ws, hipStream_t st) {
-  hipLaunchKernelGGL(sample_kernel, dim3((unsigned)rows), dim3(ST), 0, st, a);
+  hipLaunchKernelGGL((a.n <= SLICE ? row_kernel : any_kernel), dim3((unsigned)rows), dim3(ST), 0, st, a);
 }
 
 }  // namespace iek
