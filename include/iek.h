@@ -461,7 +461,7 @@ iek_status iek_dev_paged_attention(const iek_paged_kv* cache, const float* q, si
  * one whose temperature is negative or not finite, whose r is outside [0, 1) or which has a NaN among its filters gets
  * the index 0xFFFFFFFF and the probability NaN. workspace: iek_sample_workspace bytes (may be 0), 16-byte aligned, its
  * contents of no matter. IEK_ERR_SAMPLING for n == 0, IEK_ERR_OP for null or misaligned pointers, row_stride < n, n above
- * 2^30 or rows above 2^21; rows == 0 does nothing. */
+ * 2^25 or rows above 2^21; rows == 0 does nothing. */
 iek_status iek_sample_workspace(size_t rows, size_t n, size_t* bytes);
 iek_status iek_dev_sample(const float* logits, size_t rows, size_t n, size_t row_stride, const float* temperature,
                           const int32_t* top_k, const float* top_p, const float* min_p, const float* r,

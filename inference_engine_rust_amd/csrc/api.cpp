@@ -998,7 +998,7 @@ iek_status iek_dev_paged_attention(const iek_paged_kv* cache, const float* q, si
 // ---- sampling of a batch ----
 static void sample_shape(size_t rows, size_t n) {
   if (n == 0) fail(ST_SAMPLING, "logits slice is empty");
-  if (n > (1u << 30) || rows > (1u << 21)) fail(ST_OP, "sample: dims too large");
+  if (n > (1u << 25) || rows > (1u << 21)) fail(ST_OP, "sample: dims too large");
 }
 
 iek_status iek_sample_workspace(size_t rows, size_t n, size_t* bytes) {

@@ -38,7 +38,7 @@ IEK_DEV uint32_t key_of(float x) {
 IEK_DEV float value_of(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k); }
 
 // Weights of a row: w 2^S as an integer. 2^(y / 64), y = i + f, is a table's entry of 64 (in LDS) times a polynomial in
-// f of degree 5, which leaves out (f ln 2 / 64)^6 / 720 < 2^-54; the additions of 1.5 2^52 round to integers.
+// f of degree 4, which leaves out (f ln 2 / 64)^5 / 120 < 2^-44; the additions of 1.5 2^52 round to integers.
 struct Weigh {
   double top, rate;  // 64 log2 e / T
   double one;        // 2^S
@@ -46,8 +46,7 @@ struct Weigh {
   IEK_DEV double real(float x) const {  // (2^-64 stands for everything below it)
     const double y = fmax(((double)x - top) * rate, -4096.0), n = y + 0x1.8p52, f = y - (n - 0x1.8p52);
     constexpr double L = 0.693147180559945309417232 / 64;
-    double e = L * L * L * L * L / 120;
-    e = fma(e, f, L * L * L * L / 24);
+    double e = L * L * L * L / 24;
     e = fma(e, f, L * L * L / 6);
     e = fma(e, f, L * L / 2);
     e = fma(e, f, L);
@@ -116,9 +115,16 @@ struct Head {
   float top;
   bool good;
 };
+// (all loads at once, of an array that is there in place of those that are not)
 IEK_DEV SampleParams params_of(const SampleArgs& a, int b) {
   if (!a.temperature) return a.one;
-  return {a.temperature[b], a.top_p ? a.top_p[b] : 1.f, a.min_p ? a.min_p[b] : 0.f, a.r[b], a.top_k ? a.top_k[b] : 0};
+  const float *p = a.top_p ? a.top_p : a.r, *m = a.min_p ? a.min_p : a.r;
+  const int* k = a.top_k ? a.top_k : reinterpret_cast<const int*>(a.r);
+  SampleParams o{a.temperature[b], p[b], m[b], a.r[b], k[b]};
+  if (!a.top_p) o.top_p = 1.f;
+  if (!a.min_p) o.min_p = 0.f;
+  if (!a.top_k) o.top_k = 0;
+  return o;
 }
 IEK_DEV Head head_of(const SampleParams& o, int n, float top) {  // (top: +inf if there is a NaN)
   Head h{o.temperature, o.top_p, o.min_p, o.r, o.top_k >= n ? 0 : o.top_k, top, false};
@@ -251,7 +257,7 @@ IEK_DEV int ties_below(double limit, u64 above, u64 weight) {
 }
 
 // A draw of 0 takes the first token of any weight, however small: `any` counts them.
-__device__ __noinline__ void any_row(const SampleArgs& a, int b, const Head& h, Smem& m, u64* hist) {
+IEK_DEV void any_row(const SampleArgs& a, int b, const Head& h, Smem& m, u64* hist) {
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   Group q(m);
   __syncthreads();
@@ -380,6 +386,26 @@ struct Tokens {
   }
 };
 
+// A thread's tokens that in(value) holds for, as bits.
+template <class In>
+IEK_DEV uint32_t bits_of(const Tokens& T, In in) {
+  uint32_t bits = 0;
+#pragma unroll 4
+  for (int j = 0; j < T.quads; ++j) {
+    const float4 v = T.x[stored((int)threadIdx.x * T.quads + j)];
+    bits |= ((in(v.x) ? 1u : 0u) | (in(v.y) ? 2u : 0u) | (in(v.z) ? 4u : 0u) | (in(v.w) ? 8u : 0u)) << 4 * j;
+  }
+  return bits;
+}
+// f(value, place) of these
+template <class F>
+IEK_DEV void each_of(const Tokens& T, uint32_t bits, F f) {
+  for (; bits; bits &= bits - 1) {
+    const int i = (int)threadIdx.x * 4 * T.quads + __ffs(bits) - 1;
+    f(T.value(i), i);
+  }
+}
+
 // n <= SLICE logits from p on into LDS; returns the largest of those that the thread loaded, +inf for a NaN. (A
 // row's address is a multiple of 4 bytes.)
 IEK_DEV float load_tokens(float4* to, const float* p, int n) {
@@ -462,45 +488,69 @@ struct Cut {
   int ties;
 };
 
+// Ranks n <= NEAR tokens of s.near against each other, with several threads a token (a power of two up to a wave, their
+// parts joined over the lanes): to(token, the sum of those before it, how many those are and how many of them equal it, whether
+// it is the last), in the first thread of each.
+template <class To>
+IEK_DEV void rank(const Bins& s, int n, To to) {
+  const int t = threadIdx.x, size = n <= 16 ? 16 : 1 << (32 - __clz(n - 1)), each = ST / size, me = t / each;
+  u64 sum = 0;
+  int count = 0, equal = 0;
+  if (me < n) {
+    const u64 mine = s.near[me];
+#pragma unroll 4
+    for (int j = t & (each - 1); j < n; j += each) {
+      const u64 o = s.near[j], w = s.near_w[j];
+      const bool before = o > mine;
+      sum += before ? w : 0;
+      count += before;
+      equal += before && (uint32_t)(o >> 32) == (uint32_t)(mine >> 32);
+    }
+  }
+  for (int d = 1; d < each; d <<= 1) {
+    sum += __shfl_xor(sum, d);
+    count += __shfl_xor(count, d);
+    equal += __shfl_xor(equal, d);
+  }
+  if ((t & (each - 1)) == 0 && me < n) to(me, sum, count, equal);
+}
+
 // The border among n <= NEAR tokens of a bin: keeps(the sum before a token). m.border, m.ties: the last value that stays
 // and how many of it; m.word: the sum up to it; m.word2: whether it is the last of them.
 template <class Keeps>
 IEK_DEV void rank_near(Smem& m, const Bins& s, int n, u64 above, Keeps keeps) {
-  const int t = threadIdx.x;
-  if (t < n) {
-    const u64 me = s.near[t], own = s.near_w[t];
-    u64 sum = above;
-    int equal = 1;
-    bool last = true;
-#pragma unroll 4
-    for (int j = 0; j < n; ++j) {
-      const u64 o = s.near[j], w = s.near_w[j];
-      const bool before = o > me;
-      sum += before ? w : 0;
-      equal += before && (uint32_t)(o >> 32) == (uint32_t)(me >> 32);
-      last &= o >= me;
-    }
+  rank(s, n, [&](int i, u64 sum, int count, int equal) {
+    const u64 own = s.near_w[i];
+    sum += above;
+    const bool last = count == n - 1;
     if (keeps(sum) && (last || !keeps(sum + own))) {
-      m.border = value_of((uint32_t)(me >> 32));
-      m.ties = equal;
+      m.border = value_of((uint32_t)(s.near[i] >> 32));
+      m.ties = equal + 1;
       m.word = sum + own;
       m.word2 = last;
     }
-  }
+  });
   __syncthreads();
 }
 
 // Adds up weights (or counts) of the tokens above `over` in bins of 1 / scale from the top.
 IEK_DEV void fill_bins(const Tokens& T, u64* hist, const Weigh& weigh, bool counts, float top, float scale, float over) {
+  // (the last bin, which may have most of the tokens, from a sum of each wave)
+  u64 far = 0;
   T.each([&](float x, int) {
-    const u64 w = counts ? 1 : weigh(x);
-    if (x > over && w) atomicAdd(&hist[bin_of(x, top, scale)], w);
+    const u64 all = counts ? 1 : weigh(x), w = x > over ? all : 0;
+    const int bin = bin_of(x, top, scale);
+    const bool last = bin == BINS - 1;
+    far += last ? w : 0;
+    if (!last) atomicAdd(&hist[bin], w);
   });
+  far = wave_scan64(far);
+  if ((threadIdx.x & 63) == 63 && far) atomicAdd(&hist[BINS - 1], far);
 }
 // Puts the tokens above `over` of a bin into s.near, in any order; m.count of them (more than NEAR: not all are there).
 IEK_DEV void gather_near(const Tokens& T, Smem& m, Bins& s, const Weigh& weigh, bool counts, float top, float scale, float over, int bin) {
-  T.each([&](float x, int i) {
-    if (!(x > over && bin_of(x, top, scale) == bin)) return;
+  const uint32_t bits = bits_of(T, [&](float x) { return x > over && bin_of(x, top, scale) == bin; });
+  each_of(T, bits, [&](float x, int i) {
     const int at = atomicAdd(&m.count, 1);
     if (at < NEAR) {
       s.near[at] = (u64)key_of(x) << 32 | (uint32_t)~T.at(i);
@@ -569,7 +619,6 @@ struct Final {
 IEK_DEV u64 run_sum(const Tokens& T, Group& q, const Final& f, int& ties) {
   u64 sum = 0;
   int equal = 0;
-#pragma unroll 2
   for (int j = 0; j < T.quads; ++j) {
     const float4 v = T.x[stored((int)threadIdx.x * T.quads + j)];
     const float x[4] = {v.x, v.y, v.z, v.w};
@@ -639,14 +688,10 @@ constexpr int LIST_BYTES = 16 * ST + 4 * LIST;
 // how many there are.
 template <class In, class Put>
 IEK_DEV int compact(const Tokens& T, Group& q, int room, In in, Put put) {
-  int mine = 0;
-  T.each([&](float v, int) { mine += in(v); });
+  const uint32_t bits = bits_of(T, in);
   u64 total;
-  int at = (int)q.before(mine, total);
-  if ((int)total <= room && mine > 0)
-    T.each([&](float v, int i) {
-      if (in(v)) put(at++, v, T.at(i));
-    });
+  int at = (int)q.before(__popc(bits), total);
+  if ((int)total <= room) each_of(T, bits, [&](float v, int i) { put(at++, v, T.at(i)); });
   return (int)total;
 }
 
@@ -676,27 +721,10 @@ IEK_DEV void pick_of_few(const Tokens& T, int n, Group& q, Bins& s, const Sample
     s.near_w[t] = w;
   }
   __syncthreads();
-  // `each` threads a token (a power of two up to a wave), the sums and counts before it joined over their lanes
-  const int size = n <= 16 ? 16 : 1 << (32 - __clz(n - 1)), each = ST / size, me = t / each;
-  u64 sum = 0;
-  int count = 0;
-  if (me < n) {
-    const u64 mine = s.near[me];
-#pragma unroll 4
-    for (int j = t & (each - 1); j < n; j += each) {
-      const bool before = s.near[j] > mine;
-      sum += before ? s.near_w[j] : 0;
-      count += before;
-    }
-  }
-  for (int d = 1; d < each; d <<= 1) {
-    sum += __shfl_xor(sum, d);
-    count += __shfl_xor(count, d);
-  }
-  if ((t & (each - 1)) == 0 && me < n) {
-    s.hist[me] = sum;
-    s.hist[NEAR + me] = (u64)count;
-  }
+  rank(s, n, [&](int i, u64 sum, int count, int) {
+    s.hist[i] = sum;
+    s.hist[NEAR + i] = (u64)count;
+  });
   __syncthreads();
   const u64 above = live ? s.hist[t] : 0;
   const bool first = live && (h.k <= 0 || (int)s.hist[NEAR + t] < h.k);
@@ -718,6 +746,7 @@ IEK_DEV bool filter(const Tokens& T, Group& q, Bins& s, const Head& h, const Wei
          cut_at(T, q, s, weigh, false, h.top, p_scale, cut, [&](u64 v, u64 all) { return v == 0 || (double)v < (double)h.p * (double)all; });
 }
 
+IEK_DEV float list_scale(float span) { return fminf((float)(BINS - 1) / span, 1e30f); }  // (a span of 0: 1e30)
 IEK_DEV float weight_scale(const Head& h) { return fminf(64.f * 1.44269504f / h.t, 1e30f); }
 
 // The lowest index of the largest logit, by one thread of the workgroup.
@@ -731,6 +760,53 @@ IEK_DEV void store_top(const Tokens& T, Group& q, const SampleArgs& a, int b, fl
   if ((threadIdx.x & 63) == 0 && at != INT32_MAX && before == 0) store(a, b, T.at(at), 1.f);
 }
 
+// The token of a row of up to SLICE logits, which are in `data`. False: it is left to any_row. The list takes the
+// histogram's place after it, and the bins then the tokens'.
+IEK_DEV bool one_row(const SampleArgs& a, int b, const Head& h, Group& q, float4* data, char* more, float most) {
+  const Tokens T{data, nullptr, quads_of(a.n), 0};
+  const Weigh weigh = weigh_of(h, a.n, q.m.table);
+  Bins& bins = *reinterpret_cast<Bins*>(more);
+  const List list{reinterpret_cast<float4*>(more), reinterpret_cast<uint32_t*>(more + 16 * ST)};
+  Bins& room = *reinterpret_cast<Bins*>(data);
+  auto put = [&](int at, float v, uint32_t i) { list.put(at, v, i); };
+  Cut cut{-INFINITY, 0};
+  float scale = 0.f, far = -1.f;
+  if (h.k > 0 && (h.k <= ST || a.n <= LIST)) {
+    far = bound_of_k(q, bins.hist, most, min(h.k, ST), h.top, scale);
+  } else if (h.k <= 0 && !(h.p < 1.f) && h.m > 0.f) {
+    // (a distance that is too large by the roundings at least: min-p itself is looked at later)
+    scale = 1.f;
+    far = -logf(fminf(h.m, 1.f)) * h.t * 1.0001f + 1e-6f * fabsf(h.top) + 1e-30f;
+  }
+  if (far >= 0.f) {
+    const int n = compact(T, q, LIST, [&](float v) { return v > -INFINITY && fminf((h.top - v) * scale, 1e30f) < far; }, put);
+    if (n <= LIST) {
+      const Tokens L = list.tokens(n);
+      if (n <= NEAR) {
+        pick_of_few(L, n, q, room, a, b, h, weigh);
+        return true;
+      }
+      if (far < INFINITY) scale = fminf(scale * ((float)BINS / far), 1e30f);
+      if (!filter(L, q, room, h, weigh, scale, scale, cut)) return false;
+      pick(L, q, a, b, h, weigh, cut);
+      return true;
+    }
+  }
+  if (h.k > 0) {
+    float span = 0.f;
+    T.each([&](float x, int) { span = x > -INFINITY ? fmaxf(span, h.top - x) : span; });
+    scale = fminf((float)(BINS - 1) / q.most(span), 1e30f);
+  }
+  if (!filter(T, q, bins, h, weigh, scale, weight_scale(h), cut)) return false;
+  Tokens left = T;
+  if (cut.ties > 0) {
+    const int n = compact(T, q, LIST, [&](float v) { return v >= cut.over; }, put);
+    if (n <= LIST) left = list.tokens(n);
+  }
+  pick(left, q, a, b, h, weigh, cut);
+  return true;
+}
+
 // Rows of up to SLICE logits.
 __global__ __launch_bounds__(ST) void row_kernel(SampleArgs a) {
   __shared__ Smem m;
@@ -742,74 +818,287 @@ __global__ __launch_bounds__(ST) void row_kernel(SampleArgs a) {
   const float most = load_tokens(data, a.logits + (size_t)b * a.stride, a.n);
   fill_table(m.table);
   const Head h = head_of(o, a.n, q.most(most));
-  Tokens T{data, nullptr, quads_of(a.n), 0};
   if (!h.good) {
     if (threadIdx.x == 0) store(a, b, NO_TOKEN, NAN);
-    return;
+  } else if (h.t == 0.f) {
+    store_top(Tokens{data, nullptr, quads_of(a.n), 0}, q, a, b, h.top);
+  } else if (h.r == 0.f || !one_row(a, b, h, q, data, more, most)) {
+    any_row(a, b, h, m, reinterpret_cast<Bins*>(more)->hist);
   }
-  if (h.t == 0.f) return store_top(T, q, a, b, h.top);
-  const Weigh weigh = weigh_of(h, a.n, m.table);
-  Bins& bins = *reinterpret_cast<Bins*>(more);
-  // the list takes the histogram's place after it, and the bins then the tokens'
-  const List list{reinterpret_cast<float4*>(more), reinterpret_cast<uint32_t*>(more + 16 * ST)};
-  Bins& room = *reinterpret_cast<Bins*>(data);
-  auto put = [&](int at, float v, uint32_t i) { list.put(at, v, i); };
-  Cut cut{-INFINITY, 0};
-  if (h.r == 0.f) return any_row(a, b, h, m, bins.hist);
-  float scale = 0.f;
-  int n = LIST + 1;
-  if (h.k > 0 && (h.k <= ST || a.n <= LIST)) {
-    const float far = bound_of_k(q, bins.hist, most, min(h.k, ST), h.top, scale);
-    n = compact(T, q, LIST, [&](float v) { return v > -INFINITY && fminf((h.top - v) * scale, 1e30f) < far; }, put);
-    if (far < INFINITY) scale = fminf(scale * ((float)BINS / far), 1e30f);
-  } else if (h.k <= 0 && !(h.p < 1.f) && h.m > 0.f) {
-    // (a distance that is too large by the roundings at least: min-p itself is looked at later)
-    const float far = -logf(fminf(h.m, 1.f)) * h.t * 1.0001f + 1e-6f * fabsf(h.top) + 1e-30f;
-    n = compact(T, q, LIST, [&](float v) { return h.top - v <= far; }, put);
-  }
-  if (n <= LIST) {
-    const Tokens L = list.tokens(n);
-    if (n <= NEAR) return pick_of_few(L, n, q, room, a, b, h, weigh);
-    if (!filter(L, q, room, h, weigh, scale, scale, cut)) return any_row(a, b, h, m, room.hist);
-    return pick(L, q, a, b, h, weigh, cut);
-  }
-  if (h.k > 0) {
-    float span = 0.f;
-    T.each([&](float x, int) { span = x > -INFINITY ? fmaxf(span, h.top - x) : span; });
-    scale = fminf((float)(BINS - 1) / q.most(span), 1e30f);
-  }
-  if (!filter(T, q, bins, h, weigh, scale, weight_scale(h), cut)) return any_row(a, b, h, m, bins.hist);
-  if (cut.ties > 0) {
-    n = compact(T, q, LIST, [&](float v) { return v >= cut.over; }, put);
-    if (n <= LIST) return pick(list.tokens(n), q, a, b, h, weigh, cut);
-  }
-  pick(T, q, a, b, h, weigh, cut);
 }
 
-__global__ __launch_bounds__(ST) void any_kernel(SampleArgs a) {
+// ---- rows of several slices -----------------------------------------------------------------------------
+
+// Candidates of a slice, slices of a row at most (one a thread of the last launch).
+constexpr int SEGMENT = 256, MOST_SLICES = ST;
+
+// A row in slices of `length` logits, and its part of the workspace.
+struct Slices {
+  int length, count;
+  size_t bytes;  // of a row
+  char* base;
+};
+struct RowSpace {
+  u64 *hist, *near, *near_w, *sum;   // [BINS], [NEAR], [NEAR], [slices]
+  float *most, *least;               // [slices]: the largest logit, and the least of the threads' largest
+  int* found;                        // [slices]: candidates; [slices]: tokens of the border's bin
+  float* x;                          // [slices][SEGMENT] candidates
+  uint32_t* index;
+};
+__host__ IEK_DEV RowSpace space_of(const Slices& z, int b) {
+  char* p = z.base + (size_t)b * z.bytes;
+  const size_t n = (size_t)z.count;
+  RowSpace r;
+  r.hist = reinterpret_cast<u64*>(p);
+  r.near = r.hist + BINS;
+  r.near_w = r.near + NEAR;
+  r.sum = r.near_w + NEAR;
+  r.most = reinterpret_cast<float*>(r.sum + n);
+  r.least = r.most + n;
+  r.found = reinterpret_cast<int*>(r.least + n);
+  r.x = reinterpret_cast<float*>(r.found + n + 1);
+  r.index = reinterpret_cast<uint32_t*>(r.x + n * SEGMENT);
+  return r;
+}
+// Which rows go which way (the others are left to the last launch, to any_row).
+IEK_DEV bool by_list(const Head& h) { return h.k > 0 && h.k <= ST; }
+IEK_DEV bool by_slices(const Head& h) { return h.good && h.t > 0.f && h.r > 0.f && h.k <= ST; }
+
+// The row's head from its slices' maxima, and the span of the threads' maxima.
+IEK_DEV Head head_of_slices(const SampleArgs& a, const Slices& z, int b, const RowSpace& r, Group& q, float& span) {
+  const SampleParams o = params_of(a, b);
+  const int t = threadIdx.x;
+  const float top = q.most(t < z.count ? r.most[t] : -INFINITY);
+  span = q.most(t < z.count ? top - r.least[t] : 0.f);
+  return head_of(o, a.n, top);
+}
+IEK_DEV float load_slice(float4* to, const SampleArgs& a, const Slices& z, int b, int s, Tokens& T) {
+  const int first = s * z.length, n = min(z.length, a.n - first);
+  T = Tokens{to, nullptr, quads_of(n), first};
+  return load_tokens(to, a.logits + (size_t)b * a.stride + first, n);
+}
+
+// First launch: the slices' maxima; the row's histogram and counter are cleared.
+__global__ __launch_bounds__(ST) void slice_most_kernel(SampleArgs a, Slices z) {
+  __shared__ Smem m;
+  __shared__ float4 data[SLICE / 4];
+  const int b = blockIdx.y, s = blockIdx.x, t = threadIdx.x;
+  const RowSpace r = space_of(z, b);
+  for (int i = s * ST + t; i < BINS; i += z.count * ST) r.hist[i] = 0;
+  if (s == 0 && t == 0) r.found[z.count] = 0;
+  Group q(m);
+  Tokens T;
+  const float most = load_slice(data, a, z, b, s, T), top = q.most(most);
+  const float span = q.most(most > -INFINITY ? top - most : 0.f);
+  if (t == 0) {
+    r.most[s] = top;
+    r.least[s] = top > -INFINITY ? top - span : INFINITY;  // (a slice of nothing has no say)
+  }
+}
+
+// Second: the row's histogram, of the threads' maxima (top-k) or of weights (top-p); or the slice's sum of weights.
+__global__ __launch_bounds__(ST) void slice_bins_kernel(SampleArgs a, Slices z) {
   __shared__ Smem m;
   __shared__ float4 data[SLICE / 4];
   __shared__ u64 hist[BINS];
-  const int b = blockIdx.x;
-  const SampleParams o = params_of(a, b);
+  const int b = blockIdx.y, s = blockIdx.x, t = threadIdx.x;
+  const RowSpace r = space_of(z, b);
   Group q(m);
+  Tokens T;
+  const float most = load_slice(data, a, z, b, s, T);
   fill_table(m.table);
-  float most = -INFINITY;
-  for (int s0 = 0; s0 < a.n; s0 += SLICE) most = fmaxf(most, load_tokens(data, a.logits + (size_t)b * a.stride + s0, min(SLICE, a.n - s0)));
-  const Head h = head_of(o, a.n, q.most(most));
-  if (!h.good) {
-    if (threadIdx.x == 0) store(a, b, NO_TOKEN, NAN);
+  float span;
+  const Head h = head_of_slices(a, z, b, r, q, span);
+  if (!by_slices(h)) return;
+  const Weigh weigh = weigh_of(h, a.n, m.table);
+  if (!by_list(h) && !(h.p < 1.f)) {
+    int ties;
+    const u64 sum = q.sum(run_sum(T, q, Final(weigh, h, Cut{-INFINITY, 0}), ties));
+    if (t == 0) r.sum[s] = sum;
     return;
   }
-  if (h.t == 0.f) {
-    for (int s0 = 0; s0 < a.n; s0 += SLICE) {
-      const int n = min(SLICE, a.n - s0);
-      __syncthreads();
-      const float here = load_tokens(data, a.logits + (size_t)b * a.stride + s0, n);
-      if (q.most(here) == h.top) return store_top(Tokens{data, nullptr, quads_of(n), s0}, q, a, b, h.top);
-    }
+  clear_bins(m, hist);
+  if (by_list(h)) {
+    if (most > -INFINITY) atomicAdd(&hist[bin_of(most, h.top, list_scale(span))], 1ull);
+  } else {
+    fill_bins(T, hist, weigh, false, h.top, weight_scale(h), -INFINITY);
   }
-  any_row(a, b, h, m, hist);
+  __syncthreads();
+  for (int i = t; i < BINS; i += ST)
+    if (hist[i]) atomicAdd(&r.hist[i], hist[i]);
+}
+
+// The bin of the row's histogram that the border is in; into m.hist's copy.
+IEK_DEV int cross_row(const Head& h, const RowSpace& r, Group& q, u64* hist, u64& above, u64& total) {
+  clear_bins(q.m, hist);
+  for (int i = threadIdx.x; i < BINS; i += ST) hist[i] = r.hist[i];
+  __syncthreads();
+  const bool list = by_list(h);
+  return cross(q, hist, [&](u64 v, u64 all) { return list ? v < (u64)h.k : v == 0 || (double)v < (double)h.p * (double)all; }, above, total);
+}
+
+// Third: the slice's candidates for top-k; or its sum of the weights above top-p's bin, and its tokens in that.
+__global__ __launch_bounds__(ST) void slice_cut_kernel(SampleArgs a, Slices z) {
+  __shared__ Smem m;
+  __shared__ float4 data[SLICE / 4];
+  __shared__ Bins bins;
+  const int b = blockIdx.y, s = blockIdx.x, t = threadIdx.x;
+  const RowSpace r = space_of(z, b);
+  Group q(m);
+  Tokens T;
+  load_slice(data, a, z, b, s, T);
+  fill_table(m.table);
+  float span;
+  const Head h = head_of_slices(a, z, b, r, q, span);
+  if (!by_slices(h) || (!by_list(h) && !(h.p < 1.f))) return;
+  u64 above, total;
+  const int bin = cross_row(h, r, q, bins.hist, above, total);
+  if (by_list(h)) {
+    const float scale = list_scale(span), far = bin < 0 ? INFINITY : (float)(bin + 1);
+    float* x = r.x + (size_t)s * SEGMENT;
+    uint32_t* index = r.index + (size_t)s * SEGMENT;
+    const int n = compact(T, q, SEGMENT, [&](float v) { return v > -INFINITY && fminf((h.top - v) * scale, 1e30f) < far; },
+                          [&](int at, float v, uint32_t i) {
+                            x[at] = v;
+                            index[at] = i;
+                          });
+    if (t == 0) r.found[s] = n;
+    return;
+  }
+  // (top-p below 1: some bin is the border's)
+  const Weigh weigh = weigh_of(h, a.n, m.table);
+  const Final f(weigh, h, Cut{-INFINITY, 0});
+  const float scale = weight_scale(h);
+  u64 sum = 0;
+  const uint32_t over = bits_of(T, [&](float x) { return x > -INFINITY && bin_of(x, h.top, scale) < bin; });
+  each_of(T, over, [&](float x, int) { sum += f.weight(x); });
+  sum = q.sum(sum);
+  if (t == 0) r.sum[s] = sum;
+  const uint32_t at_border = bits_of(T, [&](float x) { return x > -INFINITY && bin_of(x, h.top, scale) == bin; });
+  each_of(T, at_border, [&](float x, int i) {
+    const int at = atomicAdd(&r.found[z.count], 1);
+    if (at < NEAR) {
+      r.near[at] = (u64)key_of(x) << 32 | (uint32_t)~T.at(i);
+      r.near_w[at] = weigh(x);
+    }
+  });
+}
+
+// The token of a row of slices. False: it is left to any_row.
+IEK_DEV bool join_slices(const SampleArgs& a, const Slices& z, int b, const Head& h, const RowSpace& r, float span, Group& q, float4* data, char* more) {
+  const int t = threadIdx.x;
+  Smem& m = q.m;
+  Bins& bins = *reinterpret_cast<Bins*>(more);
+  const Weigh weigh = weigh_of(h, a.n, m.table);
+  if (by_list(h)) {
+    const List list{reinterpret_cast<float4*>(more), reinterpret_cast<uint32_t*>(more + 16 * ST)};
+    Bins& room = *reinterpret_cast<Bins*>(data);
+    const int mine = t < z.count ? r.found[t] : 0;
+    u64 total, most;
+    const int at = (int)q.before(mine, total);
+    q.before(mine > SEGMENT, most);
+    if (most > 0 || total > LIST) return false;
+    // each segment by its thread's wave: (place, count) from the lane that has them
+    for (int i = 0; i < 64; ++i) {
+      const int n = __builtin_amdgcn_readlane(mine, i), to = __builtin_amdgcn_readlane(at, i);
+      const size_t from = (size_t)((t & ~63) + i) * SEGMENT;
+      for (int j = t & 63; j < n; j += 64) list.put(to + j, r.x[from + j], r.index[from + j]);
+    }
+    const int n = (int)total;
+    const Tokens L = list.tokens(n);
+    if (n <= NEAR) {
+      pick_of_few(L, n, q, room, a, b, h, weigh);
+      return true;
+    }
+    Cut cut{-INFINITY, 0};
+    float low = 0.f;
+    L.each([&](float x, int) { low = x > -INFINITY ? fmaxf(low, h.top - x) : low; });
+    const float scale = list_scale(q.most(low));
+    if (!filter(L, q, room, h, weigh, scale, scale, cut)) return false;
+    pick(L, q, a, b, h, weigh, cut);
+    return true;
+  }
+  Cut cut{-INFINITY, 0};
+  u64 mine = t < z.count ? r.sum[t] : 0;
+  const float least = fminf(h.m, 1.f);
+  if (h.p < 1.f) {
+    u64 above, total;
+    cross_row(h, r, q, bins.hist, above, total);
+    const int n = r.found[z.count];
+    if (n > NEAR) return false;
+    if (t < n) {
+      bins.near[t] = r.near[t];
+      bins.near_w[t] = r.near_w[t];
+    }
+    u64* add = bins.hist;  // (of each slice, the kept ones of these)
+    __syncthreads();
+    add[t] = 0;
+    __syncthreads();
+    rank_near(m, bins, n, above, [&](u64 v) { return v == 0 || (double)v < (double)h.p * (double)total; });
+    cut = Cut{m.border, m.ties};
+    rank(bins, n, [&](int i, u64, int, int equal) {
+      const float x = value_of((uint32_t)(bins.near[i] >> 32));
+      if ((x > cut.over || (x == cut.over && equal < cut.ties)) && weigh.real(x) >= least)
+        atomicAdd(&add[~(uint32_t)bins.near[i] / (uint32_t)z.length], bins.near_w[i]);
+    });
+    __syncthreads();
+    mine += add[t];
+  }
+  // the slice that has the token
+  u64 total;
+  const u64 base = q.before(mine, total);
+  const double limit = (double)h.r * (double)total;
+  if (!((double)base > limit) && (double)(base + mine) > limit) {
+    m.word = base;
+    m.word2 = t;
+  }
+  __syncthreads();
+  const u64 from = m.word;
+  const int s = m.word2;
+  if (cut.ties > 0) {  // the kept ties before it
+    const uint32_t index = t < r.found[z.count] ? ~(uint32_t)bins.near[t] : 0xFFFFFFFFu;
+    const bool tie = t < r.found[z.count] && value_of((uint32_t)(bins.near[t] >> 32)) == cut.over && index < (uint32_t)(s * z.length);
+    cut.ties = max(0, cut.ties - (int)q.sum(tie));
+  }
+  Tokens T;
+  load_slice(data, a, z, b, s, T);
+  __syncthreads();
+  const Final f(weigh, h, cut);
+  int ties;
+  const u64 sum = run_sum(T, q, f, ties);
+  u64 unused;
+  const u64 before = from + q.before(sum, unused);
+  pick_in_run(T, f, before, sum, ties, limit, a, b, h, total);
+  return true;
+}
+
+// Fourth: a workgroup a row.
+__global__ __launch_bounds__(ST) void slice_join_kernel(SampleArgs a, Slices z) {
+  __shared__ Smem m;
+  __shared__ float4 data[SLICE / 4];
+  __shared__ __align__(16) char more[sizeof(Bins) > LIST_BYTES ? sizeof(Bins) : LIST_BYTES];
+  const int b = blockIdx.x;
+  const RowSpace r = space_of(z, b);
+  Group q(m);
+  fill_table(m.table);
+  float span;
+  const Head h = head_of_slices(a, z, b, r, q, span);
+  if (!h.good) {
+    if (threadIdx.x == 0) store(a, b, NO_TOKEN, NAN);
+  } else if (h.t == 0.f) {
+    // the first slice that has the maximum
+    const int t = threadIdx.x;
+    u64 total;
+    const bool has = t < z.count && r.most[t] == h.top;
+    if (q.before(has, total) == 0 && has) m.word2 = t;
+    __syncthreads();
+    Tokens T;
+    load_slice(data, a, z, b, m.word2, T);
+    __syncthreads();
+    store_top(T, q, a, b, h.top);
+  } else if (!by_slices(h) || !join_slices(a, z, b, h, r, span, q, data, more)) {
+    any_row(a, b, h, m, reinterpret_cast<Bins*>(more)->hist);
+  }
 }
 
 }  // namespace
@@ -821,10 +1110,47 @@ void check_sample_params(const SampleParams& p) {
   if (std::isnan(p.top_p) || std::isnan(p.min_p)) fail(ST_OP, "sample: a filter is NaN");
 }
 
-size_t sample_workspace(size_t rows, size_t n) { return 0; }
+// Slices of a row: as many workgroups as fill the chip, of whole quads of all threads. (8 rows of 262144: slices of 8192.)
+static Slices slices_of(size_t rows, size_t n) {
+  constexpr size_t unit = 4 * ST;
+  Slices z{};
+  if (n <= SLICE || n > (size_t)SLICE * MOST_SLICES) return z;
+  const size_t fill = (n * rows / 256 + unit - 1) / unit * unit, least = (n / MOST_SLICES + unit) / unit * unit;
+  z.length = (int)std::min<size_t>(SLICE, std::max({fill, least, 2 * unit}));
+  z.count = (int)((n + z.length - 1) / z.length);
+  z.bytes = (8 * (BINS + 2 * NEAR + (size_t)z.count) + 8 * (size_t)z.count + 4 * ((size_t)z.count + 1) + 8 * (size_t)SEGMENT * z.count + 15) / 16 * 16;
+  return z;
+}
+
+size_t sample_workspace(size_t rows, size_t n) {
+  const Slices z = slices_of(rows, n);
+  return rows * z.bytes;
+}
 
 void launch_sample(const SampleArgs& a, int rows, void* ws, hipStream_t st) {
-  hipLaunchKernelGGL((a.n <= SLICE ? row_kernel : any_kernel), dim3((unsigned)rows), dim3(ST), 0, st, a);
+  Slices z = slices_of((size_t)rows, (size_t)a.n);
+  if (z.count == 0) {
+    hipLaunchKernelGGL(row_kernel, dim3((unsigned)rows), dim3(ST), 0, st, a);
+    return;
+  }
+  z.base = static_cast<char*>(ws);
+  // (a grid's second dimension has 65535 at most)
+  for (int b = 0; b < rows; b += 65535) {
+    const int some = std::min(rows - b, 65535);
+    SampleArgs x = a;
+    x.logits += (size_t)b * a.stride;
+    x.index += b;
+    if (x.prob) x.prob += b;
+    for (const float** p : {&x.temperature, &x.top_p, &x.min_p, &x.r})
+      if (*p) *p += b;
+    if (x.top_k) x.top_k += b;
+    const dim3 grid((unsigned)z.count, (unsigned)some);
+    hipLaunchKernelGGL(slice_most_kernel, grid, dim3(ST), 0, st, x, z);
+    hipLaunchKernelGGL(slice_bins_kernel, grid, dim3(ST), 0, st, x, z);
+    hipLaunchKernelGGL(slice_cut_kernel, grid, dim3(ST), 0, st, x, z);
+    hipLaunchKernelGGL(slice_join_kernel, dim3((unsigned)some), dim3(ST), 0, st, x, z);
+    z.base += (size_t)some * z.bytes;
+  }
 }
 
 }  // namespace iek
