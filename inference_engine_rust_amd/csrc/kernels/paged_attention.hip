@@ -195,7 +195,7 @@ IEK_DEV Ids<F16> ids_of(const Paged& c, const Pages& g, int tile) {
 #pragma unroll
   for (int x = 0; x < (F16 ? 2 : 1); ++x) {
     const int j = tile * tile_of<F16>() + 16 * x;
-    r.id[x] = j < g.end ? scalar(g.list, j >> c.shift) : -1;
+    r.id[x] = uniform(j < g.end ? scalar(g.list, j >> c.shift) : -1);
     if ((unsigned)r.id[x] >= (unsigned)c.n_pages) r.id[x] = -1;
   }
   return r;
@@ -206,61 +206,74 @@ IEK_DEV Ids<F16> ids_of(const Paged& c, const Pages& g, int tile) {
 template <int HD, bool F16>
 IEK_DEV __amdgpu_buffer_rsrc_t rows_rsrc(const Paged& c, const void* pool, int h, int id, int j, int end) {
   const size_t row = (((size_t)max(id, 0) * c.n_kv + h) << c.shift) + (j & ((1 << c.shift) - 1));
-  const int live = id < 0 ? 0 : max(0, min(16, end - j));
+  const int live = uniform(id < 0 ? 0 : max(0, min(16, end - j)));  // (a median of three is a vector instruction)
   const char* base = static_cast<const char*>(pool) + row * (HD * (F16 ? 2 : 4));
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), (short)0, live * HD * (F16 ? 2 : 4), 0x00020000);
 }
 
-// A wave's part of a tile: lane (r = lane & 15, kg = lane >> 4). sum: o[x]'s V^T, of f(v) in v's
-// place, times weights (for the rare tiles with a V that is not finite).
-template <int DIMS, bool F16>
+// A wave's part of a tile: lane (r = lane & 15, kg = lane >> 4). sum: o[x]'s V^T, of 1 in place of every infinity of the sign
+// and NaN and 0 for the rest, times weights (for the rare tiles with a V that is not finite).
+template <int DIMS, bool HALVES>
 struct Tile;
 template <int DIMS>
 struct Tile<DIMS, false> {
   f4_t k[DIMS / 16];     // K[r][16 i + 4 kg + e]
   f4_t v[4][DIMS / 64];  // V[4 kg + i][64 u + 4 r + e]
-  static IEK_DEV bool bad(float x) { return (__float_as_uint(x) & 0x7F800000u) == 0x7F800000u; }
+  template <bool>
   IEK_DEV bool not_finite() const {
-    bool any = false;
+    uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < 4 * (DIMS / 64) * 4; ++i) any |= bad(v[i & 3][i >> 4][i >> 2 & 3]);
-    return any;
+    for (int i = 0; i < 4 * (DIMS / 64) * 4; ++i) top = max(top, __float_as_uint(v[i & 3][i >> 4][i >> 2 & 3]) & 0x7FFFFFFFu);
+    return top >= 0x7F800000u;
   }
+  template <bool>
   IEK_DEV void drop() {
 #pragma unroll
-    for (int i = 0; i < 4 * (DIMS / 64) * 4; ++i)
-      if (bad(v[i & 3][i >> 4][i >> 2 & 3])) v[i & 3][i >> 4][i >> 2 & 3] = 0.f;
+    for (int i = 0; i < 4 * (DIMS / 64) * 4; ++i) {
+      float x = v[i & 3][i >> 4][i >> 2 & 3];
+      asm volatile("" : "+v"(x));
+      v[i & 3][i >> 4][i >> 2 & 3] = (__float_as_uint(x) & 0x7FFFFFFFu) >= 0x7F800000u ? 0.f : x;
+    }
   }
-  template <class F>
-  IEK_DEV f4_t sum(int x, const float (&w)[4], F f) const {
+  template <bool>
+  IEK_DEV f4_t sum(int x, const float (&w)[4], bool minus) const {
     f4_t o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float y = v[i][x >> 2][x & 3];
       asm volatile("" : "+v"(y));  // (nothing of this is to be kept for another column, in registers of the common path)
-      o = mfma(f(y), w[i], o);
+      o = mfma(y == (minus ? -INFINITY : INFINITY) || y != y ? 1.f : 0.f, w[i], o);
     }
     return o;
   }
 };
+// (fp16, or with F16 false bf16)
 template <int DIMS>
 struct Tile<DIMS, true> {
   static constexpr int VW = DIMS / 32;
   u4_t k[2][VW];         // K[16 s + r][32 i + 8 kg + (0 .. 7)]
   uint32_t v[8][VW];     // V[16 (j >> 2) + 4 kg + (j & 3)][DIMS / 16 * r + ...]
-  static IEK_DEV bool bad(uint32_t x) { return (x & 0x7C00u) == 0x7C00u; }
+  template <bool F16>
+  static constexpr uint32_t INF = F16 ? 0x7C00u : 0x7F80u;
+  template <bool F16>
   IEK_DEV bool not_finite() const {
-    bool any = false;
+    uint32_t lo = 0, hi = 0;
 #pragma unroll
-    for (int i = 0; i < 8 * VW; ++i) any |= bad(v[i & 7][i >> 3]) || bad(v[i & 7][i >> 3] >> 16);
-    return any;
+    for (int i = 0; i < 8 * VW; ++i) {
+      lo = max(lo, v[i & 7][i >> 3] & 0x7FFFu);
+      hi = max(hi, v[i & 7][i >> 3] & 0x7FFF0000u);
+    }
+    return lo >= INF<F16> || hi >= INF<F16> << 16;
   }
+  template <bool F16>
   IEK_DEV void drop() {
 #pragma unroll
     for (int i = 0; i < 8 * VW; ++i) {
-      uint32_t& x = v[i & 7][i >> 3];
-      x = bad(x) ? x & 0xFFFF0000u : x;
-      x = bad(x >> 16) ? x & 0x0000FFFFu : x;
+      uint32_t x = v[i & 7][i >> 3];
+      asm volatile("" : "+v"(x));
+      x = (x & 0x7FFFu) >= INF<F16> ? x & 0xFFFF0000u : x;
+      x = (x & 0x7FFF0000u) >= INF<F16> << 16 ? x & 0x0000FFFFu : x;
+      v[i & 7][i >> 3] = x;
     }
   }
   // V^T's operand for the dims 2 w + e
@@ -270,15 +283,18 @@ struct Tile<DIMS, true> {
     for (int j = 0; j < 4; ++j) r[j] = __builtin_amdgcn_perm(v[2 * j + 1][w], v[2 * j][w], e ? 0x07060302u : 0x05040100u);
     return r;
   }
-  template <class F>
-  IEK_DEV f4_t sum(int x, const float (&w)[8], F f) const {
+  template <bool F16>
+  IEK_DEV f4_t sum(int x, const float (&w)[8], bool minus) const {
     u4_t y = operand(x >> 1, x & 1), z;
     asm volatile("" : "+v"(y));  // (nothing of this is to be kept for another column, in registers of the common path)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
+      auto flag = [&](uint32_t half) -> uint32_t {  // 1 in fp16
+        const uint32_t size = half & 0x7FFFu;
+        return size > INF<F16> || (size == INF<F16> && (half >> 15 & 1) == (minus ? 1u : 0u)) ? 0x3C00u : 0u;
+      };
       const uint32_t both = y[j];  // (bit_cast of an element of a vector takes the vector's first)
-      const h2_t p = __builtin_bit_cast(h2_t, both);
-      y[j] = __builtin_bit_cast(uint32_t, h2_t{(_Float16)f((float)p[0]), (_Float16)f((float)p[1])});
+      y[j] = flag(both) | flag(both >> 16) << 16;
       z[j] = __builtin_bit_cast(uint32_t, h2_t{(_Float16)w[2 * j], (_Float16)w[2 * j + 1]});
     }
     return mfma(y, z, f4_t{0.f, 0.f, 0.f, 0.f});
@@ -352,6 +368,29 @@ struct Query<DIMS, true, CG> {
   u4_t hi[CG][DIMS / 32], lo[CG][DIMS / 32];
 };
 
+// A column's scores of a tile, base 2, to shares of its running maximum m; l their sum, o what is scaled along.
+template <bool F16, int NX, int ND>
+IEK_DEV void weigh_tile(float (&s)[NX], float& m, float& l, f4_t (&o)[ND]) {
+  float top = s[0];
+#pragma unroll
+  for (int i = 1; i < NX; ++i) top = fmaxf(top, s[i]);
+  top = groups_max(top);
+  if (__any(top > m + LAG<F16> || (m == -INFINITY && top > m))) {
+    const bool up = top > m + LAG<F16> || m == -INFINITY;
+    const float corr = up && m != -INFINITY ? __builtin_amdgcn_exp2f(m - top) : 1.f;  // (all is 0 before)
+    if (up) m = top;
+    l *= corr;
+#pragma unroll
+    for (int i = 0; i < ND; ++i) o[i] *= corr;
+  }
+  const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+  for (int i = 0; i < NX; ++i) {
+    s[i] = __builtin_amdgcn_exp2f(s[i] - ref);
+    l += s[i];
+  }
+}
+
 // What a job's columns and entries are.
 struct Job {
   int h;
@@ -371,6 +410,33 @@ struct Shared {
   float o[SETS][16][HD];
 };
 
+// Four dims of column cc of the job, or of the output.
+template <int HD>
+IEK_DEV void put_dims(const PagedAttn& a, const Plan& p, const Job& J, int cc, int dim, f4_t y, float sum) {
+  if (J.o) {
+    *reinterpret_cast<f4_t*>(J.o + (size_t)cc * HD + dim) = y;
+  } else {
+    const int col = J.col0 + cc, b = col / p.cols, t = (col - b * p.cols) / p.group, g = col - b * p.cols - t * p.group;
+    float* out = a.out + (((size_t)b * a.n_q + t) * a.n_heads + J.h * p.group + g) * HD + dim;
+    *reinterpret_cast<f4_t*>(out) = sum == 0.f ? f4_t{0.f, 0.f, 0.f, 0.f} : y / sum;
+  }
+}
+IEK_DEV void put_sums(const Job& J, int cc, float m, float l) {
+  if (!J.ml) return;
+  J.ml[2 * cc] = isnan(l) ? l : m;  // (a NaN: the maxima pass it over)
+  J.ml[2 * cc + 1] = l;
+}
+// A lane's part of a column: the wave's DIMS of it from dim0 on.
+template <int HD, int DIMS, bool HALVES, int ND>
+IEK_DEV void put_column(const PagedAttn& a, const Plan& p, const Job& J, int cc, int dim0, int kg, float m, float l, const f4_t (&o)[ND], float scale) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+#pragma unroll
+    for (int i = 0; i < ND; i += 4)
+      put_dims<HD>(a, p, J, cc, dim0 + dim_at<DIMS, HALVES>(i, kg, r), f4_t{o[i][r], o[i + 1][r], o[i + 2][r], o[i + 3][r]} * scale, l);
+  if (dim0 == 0 && kg == 0) put_sums(J, cc, m, l);
+}
+
 template <int HD, bool F16, bool WIDE, int CG>
 IEK_DEV void run_job(const Paged& c, const PagedAttn& a, const Plan& p, const Job& J, Shared<HD, F16>& L) {
   constexpr int DIMS = dims_of(HD), SETS = sets_of(HD), DW = WAVES / SETS, TILE = tile_of<F16>();
@@ -381,9 +447,11 @@ IEK_DEV void run_job(const Paged& c, const PagedAttn& a, const Plan& p, const Jo
   const int col_base = WIDE ? (J.block * SETS + set) * CG * 16 : J.block * CG * 16;
   const float ks = a.scale * 1.44269504088896340736f;
   const int G = p.group;
-  int tile = J.t0 + (WIDE ? 0 : set);
-  Ids<F16> id = ids_of<F16>(c, J.pages, tile < J.t1 ? tile : J.t0), next = id;
-  if (tile + STEP < J.t1) next = ids_of<F16>(c, J.pages, tile + STEP);
+  int tile = uniform(J.t0 + (WIDE ? 0 : set));
+  // Loads are issued without conditions, those past the chunk's last entry of nothing: with a branch around them the
+  // waits for K were ones for V too, which is issued behind it.
+  const Pages pages{J.pages.list, min(J.pages.end, J.t1 * TILE)};
+  Ids<F16> id = ids_of<F16>(c, pages, tile), next = ids_of<F16>(c, pages, tile + STEP);
   Tile<DIMS, F16> T;
   // this lane's columns
   int hi[CG], lo[CG];
@@ -412,10 +480,8 @@ IEK_DEV void run_job(const Paged& c, const PagedAttn& a, const Plan& p, const Jo
       for (int i = 0; i < DIMS / 16; ++i) Q.q[u][i] = *reinterpret_cast<const f4_t*>(rows[u] + 16 * i + 4 * kg);
     }
   }
-  if (tile < J.t1) {
-    load_k<HD>(T, c, J.h, id, tile, J.pages.end, dim0, lane);
-    load_v<HD>(T, c, J.h, id, tile, J.pages.end, dim0, lane);
-  }
+  load_k<HD>(T, c, J.h, id, tile, pages.end, dim0, lane);
+  load_v<HD>(T, c, J.h, id, tile, pages.end, dim0, lane);
   int lo_max = 0, hi_min = INT32_MAX;
 #pragma unroll
   for (int u = 0; u < CG; ++u) {
@@ -464,13 +530,11 @@ IEK_DEV void run_job(const Paged& c, const PagedAttn& a, const Plan& p, const Jo
     for (int i = 0; i < ND; ++i) o[u][i] = f4_t{0.f, 0.f, 0.f, 0.f};
   }
   const int span = J.t1 - J.t0;
-  const int t_end = DW > 1 ? J.t0 + (span + STEP - 1) / STEP * STEP : J.t1;  // (all waves go through the barriers)
-  for (int turn = 0; tile < t_end; tile += STEP, turn ^= 1) {
-    const bool have = DW == 1 || tile < J.t1, more = tile + STEP < J.t1;
+  const int t_end = DW > 1 ? J.t0 + (span + STEP - 1) / STEP * STEP : J.t1;  // (all waves go through the barriers, some with no tile)
+  for (int turn = 0; tile < t_end; tile = uniform(tile + STEP), turn ^= 1) {
     float s[CG][NX];
-    Ids<F16> after = next;
-    if (have) {
-      if (tile + 2 * STEP < J.t1) after = ids_of<F16>(c, J.pages, tile + 2 * STEP);
+    const Ids<F16> after = ids_of<F16>(c, pages, tile + 2 * STEP);
+    {
       f4_t d[CG][NH];
 #pragma unroll
       for (int u = 0; u < CG; ++u)
@@ -494,7 +558,7 @@ IEK_DEV void run_job(const Paged& c, const PagedAttn& a, const Plan& p, const Jo
 #pragma unroll
             for (int u = 0; u < CG; ++u) d[u][0] = mfma(T.k[i][e], Q.q[u][i][e], d[u][0]);
       }
-      if (more) load_k<HD>(T, c, J.h, next, tile + STEP, J.pages.end, dim0, lane);
+      load_k<HD>(T, c, J.h, next, tile + STEP, pages.end, dim0, lane);
 #pragma unroll
       for (int u = 0; u < CG; ++u)
 #pragma unroll
@@ -507,20 +571,17 @@ IEK_DEV void run_job(const Paged& c, const PagedAttn& a, const Plan& p, const Jo
     }
     if constexpr (DW > 1) {
       __syncthreads();
-      if (have) {
 #pragma unroll
-        for (int u = 0; u < CG; ++u)
+      for (int u = 0; u < CG; ++u)
 #pragma unroll
-          for (int x = 0; x < NH; ++x) {
-            f4_t y = L.parts[turn][set * DW][u][x][lane];
+        for (int x = 0; x < NH; ++x) {
+          f4_t y = L.parts[turn][set * DW][u][x][lane];
 #pragma unroll
-            for (int w = 1; w < DW; ++w) y += L.parts[turn][set * DW + w][u][x][lane];  // (the same order in every wave)
+          for (int w = 1; w < DW; ++w) y += L.parts[turn][set * DW + w][u][x][lane];  // (the same order in every wave)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[u][4 * x + i] = y[i];
-          }
-      }
+          for (int i = 0; i < 4; ++i) s[u][4 * x + i] = y[i];
+        }
     }
-    if (!have) continue;
     const bool inner = tile * TILE >= lo_max && (tile + 1) * TILE <= hi_min && id.id[0] >= 0 && id.id[NH - 1] >= 0;
 #pragma unroll
     for (int u = 0; u < CG; ++u) {
@@ -531,26 +592,9 @@ IEK_DEV void run_job(const Paged& c, const PagedAttn& a, const Plan& p, const Jo
           if (j < lo[u] || j >= hi[u] || id.id[i >> 2] < 0) s[u][i] = -INFINITY;
         }
       }
-      float top = s[u][0];
-#pragma unroll
-      for (int i = 1; i < NX; ++i) top = fmaxf(top, s[u][i]);
-      top = groups_max(top);
-      if (__any(top > m[u] + LAG<F16> || (m[u] == -INFINITY && top > m[u]))) {
-        const bool up = top > m[u] + LAG<F16> || m[u] == -INFINITY;
-        const float corr = up && m[u] != -INFINITY ? __builtin_amdgcn_exp2f(m[u] - top) : 1.f;  // (all is 0 before)
-        if (up) m[u] = top;
-        l[u] *= corr;
-#pragma unroll
-        for (int i = 0; i < ND; ++i) o[u][i] *= corr;
-      }
-      const float ref = m[u] == -INFINITY ? 0.f : m[u];
-#pragma unroll
-      for (int i = 0; i < NX; ++i) {
-        s[u][i] = __builtin_amdgcn_exp2f(s[u][i] - ref);
-        l[u] += s[u][i];
-      }
+      weigh_tile<F16>(s[u], m[u], l[u], o[u]);
     }
-    if (!inner && __any(T.not_finite())) {
+    if (!inner && __any(T.template not_finite<F16>())) {
       // V that is not finite, in entries that some columns may not see: taken out of the product (where a weight of 0
       // would make NaN of it), and given as infinities of the same sign (both for NaN) to the columns that do see it
 #pragma unroll
@@ -563,13 +607,12 @@ IEK_DEV void run_job(const Paged& c, const PagedAttn& a, const Plan& p, const Jo
         }
 #pragma unroll
         for (int x = 0; x < ND; ++x) {
-          const f4_t up = T.sum(x, sees, [](float v) { return v == INFINITY || v != v ? 1.f : 0.f; });
-          const f4_t down = T.sum(x, sees, [](float v) { return v == -INFINITY || v != v ? 1.f : 0.f; });
+          const f4_t up = T.template sum<F16>(x, sees, false), down = T.template sum<F16>(x, sees, true);
 #pragma unroll
           for (int r = 0; r < 4; ++r) o[u][x][r] += (up[r] > 0.f ? INFINITY : 0.f) + (down[r] > 0.f ? -INFINITY : 0.f);
         }
       }
-      T.drop();
+      T.template drop<F16>();
     }
     if constexpr (F16) {
       u4_t ph[CG], pl[CG];
@@ -602,36 +645,18 @@ IEK_DEV void run_job(const Paged& c, const PagedAttn& a, const Plan& p, const Jo
 #pragma unroll
           for (int u = 0; u < CG; ++u) o[u][x] = mfma(T.v[i][x >> 2][x & 3], s[u][i], o[u][x]);
     }
-    if (more) load_v<HD>(T, c, J.h, next, tile + STEP, J.pages.end, dim0, lane);
+    load_v<HD>(T, c, J.h, next, tile + STEP, pages.end, dim0, lane);
     id = next;
     next = after;
   }
 
-  auto put = [&](int cc, int dim, f4_t y, float sum) {  // four dims of a column
-    if (J.o) {
-      *reinterpret_cast<f4_t*>(J.o + (size_t)cc * HD + dim) = y;
-    } else {
-      const int col = J.col0 + cc, b = col / p.cols, t = (col - b * p.cols) / G, g = col - b * p.cols - t * G;
-      float* out = a.out + (((size_t)b * a.n_q + t) * a.n_heads + J.h * G + g) * HD + dim;
-      *reinterpret_cast<f4_t*>(out) = sum == 0.f ? f4_t{0.f, 0.f, 0.f, 0.f} : y / sum;
-    }
-  };
   constexpr float DOWN = 1.f / UP<F16>;
   if constexpr (WIDE) {
 #pragma unroll
     for (int u = 0; u < CG; ++u) {
       l[u] = groups_sum(l[u]);
       const int cc = col_base + 16 * u + cl;
-      if (cc >= J.cols) continue;
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int i = 0; i < ND; i += 4)
-          put(cc, dim0 + dim_at<DIMS, F16>(i, kg, r), f4_t{o[u][i][r], o[u][i + 1][r], o[u][i + 2][r], o[u][i + 3][r]} * DOWN, l[u]);
-      if (J.ml && dim0 == 0 && kg == 0) {
-        J.ml[2 * cc] = isnan(l[u]) ? l[u] : m[u];  // (a NaN: the maxima pass it over)
-        J.ml[2 * cc + 1] = l[u];
-      }
+      if (cc < J.cols) put_column<HD, DIMS, F16>(a, p, J, cc, dim0, kg, m[u], l[u], o[u], DOWN);
     }
   } else {
     // the sets' parts: to a common maximum, then summed through LDS
@@ -667,24 +692,385 @@ IEK_DEV void run_job(const Paged& c, const PagedAttn& a, const Plan& p, const Jo
 #pragma unroll
         for (int w = 0; w < SETS; ++w)
           ll += L.l[w][col] * (L.m[w][col] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(L.m[w][col] - mm));
-        put(cc, dim, y, ll);
-        if (J.ml && dim == 0) {
-          J.ml[2 * cc] = isnan(ll) ? ll : mm;
-          J.ml[2 * cc + 1] = ll;
-        }
+        put_dims<HD>(a, p, J, cc, dim, y, ll);
+        if (dim == 0) put_sums(J, cc, mm, ll);
       }
     }
   }
 }
 
-constexpr int WIDE_CG = 2;
+// ---- many columns: tiles in LDS -----------------------------------------------------------------------
+// For rows of up to 128 the four waves split the columns of a job and share its tiles of 32 slots, which they put into
+// LDS in turn, each thread 16-byte pieces of rows, the next tile's in flight in registers meanwhile. Both products are
+// mfma_f32_16x16x32 ones. fp16 pages: 32 columns a wave, K and V one plane, q and P pairs (as above). f32 pages: 16 columns
+// a wave, every operand as three bf16 numbers that sum to it exactly (8 bits each, the first one cut off, the others
+// rounded), six products: of the parts' orders those up to the third; what is left out is below 2^-22 of a product.
+// (mfma_f32_16x16x4_f32, exact, takes 32 cycles for 4 of the 32 terms: 4096 shared entries of 32 sequences of 32 heads took
+// 33 us with it.)
+typedef __bf16 b2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
+IEK_DEV f4_t mfma_b(u4_t a, u4_t b, f4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8_t, a), __builtin_bit_cast(b8_t, b), c, 0, 0, 0);
+}
+// Two numbers as three pairs of bf16.
+IEK_DEV void three(float x, float y, uint32_t& a, uint32_t& b, uint32_t& c) {
+  const uint32_t xa = __float_as_uint(x) & 0xFFFF0000u, ya = __float_as_uint(y) & 0xFFFF0000u;
+  a = __builtin_amdgcn_perm(ya, xa, 0x07060302u);
+  const float xr = x - __uint_as_float(xa), yr = y - __uint_as_float(ya);
+  b = __builtin_bit_cast(uint32_t, b2_t{(__bf16)xr, (__bf16)yr});
+  const float xs = xr - __uint_as_float(b << 16), ys = yr - __uint_as_float(b & 0xFFFF0000u);
+  c = __builtin_bit_cast(uint32_t, b2_t{(__bf16)xs, (__bf16)ys});
+}
+
+template <int HD, bool F16>
+struct Staged {
+  static constexpr int NP = F16 ? 1 : 3, PIECES = HD / 8;  // planes; pieces of eight numbers a row
+  static constexpr int CG = F16 ? 2 : 1;                   // groups of 16 columns a wave
+  static constexpr int RING = F16 ? 4 : 1;                 // tiles
+  struct One {
+    u4_t k[NP][32 * PIECES], v[NP][32 * PIECES];
+  } ring[RING];
+  // K's pieces are permuted within rows, so that 16 rows' pieces of the same dims are in different banks
+  static IEK_DEV int turned(int row) { return HD == 128 ? row & 15 : row >> 1 & 7; }
+  static IEK_DEV int k_at(int row, int piece) { return row * PIECES + (piece ^ turned(row)); }
+};
+
+// 16 bytes a lane from memory to 1024 in a row in LDS, without registers. (The waits are the caller's.)
+IEK_DEV void copy16(const void* lds, const void* from) {
+  const uint32_t at = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)lds;
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(at)), "v"(from) : "memory");
+}
+template <int N>
+IEK_DEV void copies_left() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+// fp16 tiles into LDS. Rows behind the last live one are that one again, and those without a page any row: such a tile is
+// not an inner one, where values out of sight are looked at.
+template <int HD>
+IEK_DEV void copy_tile(typename Staged<HD, true>::One& to, const Paged& c, int h, const Ids<true>& id, int tile, int end) {
+  using S = Staged<HD, true>;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+#pragma unroll
+  for (int i = 0; i < S::PIECES / 8; ++i) {  // (a wave's rows are in one half of the tile)
+    const int piece = (i * WAVES + wave) * 64, half = piece / S::PIECES >> 4, at = piece + lane;
+    const int row = at / S::PIECES, j = 32 * tile + 16 * half, page = half ? id.id[1] : id.id[0];
+    const size_t first = (((size_t)max(page, 0) * c.n_kv + h) << c.shift) + (j & ((1 << c.shift) - 1));
+    const int live = min(row & 15, max(0, min(16, end - j) - 1)), src = at % S::PIECES;
+    const char* k = static_cast<const char*>(c.k) + first * (2 * HD);
+    const char* v = static_cast<const char*>(c.v) + first * (2 * HD);
+    copy16(&to.k[0][piece], k + live * (2 * HD) + 16 * (src ^ S::turned(row)));
+    copy16(&to.v[0][piece], v + live * (2 * HD) + 16 * src);
+  }
+}
+
+// A thread's pieces of a tile on their way: piece t % PIECES of the rows t / PIECES, ...
+template <int HD, bool F16>
+struct Way {
+  static constexpr int PIECES = HD / 8, RPP = 64 * WAVES / PIECES, NPASS = 32 / RPP, N = F16 ? 1 : 2;
+  u4_t k[NPASS][N], v[NPASS][N];
+  IEK_DEV void load(const Paged& c, int h, const Ids<true>& id, int tile, int end) {
+    const int t = threadIdx.x, wave = uniform(t >> 6);
+#pragma unroll
+    for (int p = 0; p < NPASS; ++p) {
+      // (a wave's rows of a pass are in one half of the tile)
+      const int half = (p * RPP + wave * 64 / PIECES) >> 4, row = (p * RPP + t / PIECES) & 15;
+      const int off = (row * HD + 8 * (t % PIECES)) * (F16 ? 2 : 4);
+      const auto rk = rows_rsrc<HD, F16>(c, c.k, h, half ? id.id[1] : id.id[0], 32 * tile + 16 * half, end);
+      const auto rv = rows_rsrc<HD, F16>(c, c.v, h, half ? id.id[1] : id.id[0], 32 * tile + 16 * half, end);
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        k[p][n] = __builtin_amdgcn_raw_buffer_load_b128(rk, off, 16 * n, 0);
+        v[p][n] = __builtin_amdgcn_raw_buffer_load_b128(rv, off, 16 * n, 0);
+      }
+    }
+  }
+  IEK_DEV void store(typename Staged<HD, F16>::One& L) const {
+    const int t = threadIdx.x;
+#pragma unroll
+    for (int p = 0; p < NPASS; ++p) {
+      const int row = p * RPP + t / PIECES, piece = t % PIECES;
+      if constexpr (F16) {
+        L.k[0][Staged<HD, F16>::k_at(row, piece)] = k[p][0];
+        L.v[0][row * PIECES + piece] = v[p][0];
+      } else {
+        u4_t x[3], y[3];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          uint32_t q[3];
+          const u4_t kk = k[p][e >> 1], vv = v[p][e >> 1];
+          three(__uint_as_float(kk[2 * (e & 1)]), __uint_as_float(kk[2 * (e & 1) + 1]), q[0], q[1], q[2]);
+          x[0][e] = q[0], x[1][e] = q[1], x[2][e] = q[2];
+          three(__uint_as_float(vv[2 * (e & 1)]), __uint_as_float(vv[2 * (e & 1) + 1]), q[0], q[1], q[2]);
+          y[0][e] = q[0], y[1][e] = q[1], y[2][e] = q[2];
+        }
+#pragma unroll
+        for (int n = 0; n < 3; ++n) {
+          L.k[n][Staged<HD, F16>::k_at(row, piece)] = x[n];
+          L.v[n][row * PIECES + piece] = y[n];
+        }
+      }
+    }
+  }
+};
+
+template <int HD, bool F16>
+IEK_DEV void run_wide(const Paged& c, const PagedAttn& a, const Plan& p, const Job& J, Staged<HD, F16>& R) {
+  using S = Staged<HD, F16>;
+  constexpr int CG = S::CG, NP = S::NP, PIECES = S::PIECES, KS = HD / 32, ND = HD / 16, TILE = 32, DW2 = HD / 32;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), kg = lane >> 4, cl = lane & 15, G = p.group;
+  const int col_base = (J.block * WAVES + wave) * CG * 16;
+  const bool idle = col_base >= J.cols;  // (such a wave takes part in the staging alone)
+  const Pages pages{J.pages.list, min(J.pages.end, J.t1 * TILE)};
+  // f32: the tile after the present one is under way to registers; fp16: three are to LDS
+  constexpr int AHEAD = S::RING - 1, COPIES = S::PIECES / 4;  // (copies a wave and tile)
+  Ids<true> id[F16 ? AHEAD + 2 : 3];
+#pragma unroll
+  for (int i = 0; i < (F16 ? AHEAD + 2 : 3); ++i) id[i] = ids_of<true>(c, pages, J.t0 + i);
+  Way<HD, false> way;
+  if constexpr (F16) {
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+      if (J.t0 + i < J.t1) copy_tile<HD>(R.ring[i], c, J.h, id[i], J.t0 + i, pages.end);
+  } else {
+    way.load(c, J.h, id[0], J.t0, pages.end);
+  }
+  int hi[CG], lo[CG], lo_max = 0, hi_min = INT32_MAX;
+  float qs[CG], m[CG], l[CG];
+  u4_t q[CG][KS][F16 ? 2 : 3];
+  f4_t o[CG][ND];
+#pragma unroll
+  for (int u = 0; u < CG; ++u) {
+    const int col = J.col0 + min(col_base + 16 * u + cl, J.cols - 1);
+    const int b = col / p.cols, t = (col - b * p.cols) / G, g = col - b * p.cols - t * G;
+    hi[u] = col_hi(a, bounded(a.len[b], a.max_len), t);
+    lo[u] = max(col_lo(a, hi[u]), J.begin);
+    hi[u] = min(hi[u], J.pages.end);
+    lo_max = max(lo_max, lo[u]);
+    hi_min = min(hi_min, hi[u]);
+    const float* row = a.q + ((size_t)b * a.n_q + t) * a.q_stride + (size_t)(J.h * G + g) * HD + 8 * kg;
+    f4_t raw[2 * KS];
+#pragma unroll
+    for (int i = 0; i < KS; ++i) {
+      raw[2 * i] = *reinterpret_cast<const f4_t*>(row + 32 * i);
+      raw[2 * i + 1] = *reinterpret_cast<const f4_t*>(row + 32 * i + 4);
+    }
+    qs[u] = a.scale * 1.44269504088896340736f;
+    float up = 1.f;
+    if constexpr (F16) {  // into [2^13, 2^14) by a power of two (an infinity or NaN, or a row of zeros, stays what it is)
+      float top = 0.f;
+#pragma unroll
+      for (int i = 0; i < 2 * KS; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(raw[i][e]));
+      top = groups_max(top);
+      int ex = (int)(__float_as_uint(top) >> 23) - 127;
+      ex = ex == 128 ? 0 : min(13 - ex, 126);
+      up = __builtin_amdgcn_ldexpf(1.f, ex);
+      qs[u] = __builtin_amdgcn_ldexpf(qs[u], -ex);
+    }
+#pragma unroll
+    for (int i = 0; i < KS; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float y0 = raw[2 * i + (e >> 1)][2 * (e & 1)] * up, y1 = raw[2 * i + (e >> 1)][2 * (e & 1) + 1] * up;
+        if constexpr (F16) {
+          const h2_t w = {(_Float16)y0, (_Float16)y1};
+          const h2_t z = {(_Float16)(y0 - (float)w[0]), (_Float16)(y1 - (float)w[1])};
+          q[u][i][0][e] = __builtin_bit_cast(uint32_t, w);
+          q[u][i][1][e] = __builtin_bit_cast(uint32_t, z);
+        } else {
+          uint32_t x, y, z;
+          three(y0, y1, x, y, z);
+          q[u][i][0][e] = x;
+          q[u][i][1][e] = y;
+          q[u][i][2][e] = z;
+        }
+      }
+    m[u] = -INFINITY;
+    l[u] = 0.f;
+#pragma unroll
+    for (int i = 0; i < ND; ++i) o[u][i] = f4_t{0.f, 0.f, 0.f, 0.f};
+  }
+#pragma unroll
+  for (int x = 1; x < 16; x <<= 1) {
+    lo_max = max(lo_max, __shfl_xor(lo_max, x));
+    hi_min = min(hi_min, __shfl_xor(hi_min, x));
+  }
+  lo_max = uniform(lo_max);
+  hi_min = uniform(hi_min);
+  for (int tile = J.t0; tile < J.t1; tile = uniform(tile + 1)) {
+    const Ids<true> more = ids_of<true>(c, pages, tile + (F16 ? AHEAD + 2 : 3));
+    typename S::One& L = R.ring[F16 ? (tile - J.t0) & AHEAD : 0];
+    if constexpr (F16) {
+      // this tile's copies are there, the wave's by the wait and the others' by the barrier; that also frees the tile before
+      if (tile + 2 < J.t1) copies_left<2 * COPIES>();
+      else if (tile + 1 < J.t1) copies_left<COPIES>();
+      else copies_left<0>();
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      if (tile + AHEAD < J.t1) copy_tile<HD>(R.ring[(tile - J.t0 + AHEAD) & AHEAD], c, J.h, id[AHEAD], tile + AHEAD, pages.end);
+    } else {
+      __syncthreads();  // (all waves have read the tile before)
+      way.store(L);
+      way.load(c, J.h, id[1], tile + 1, pages.end);
+      __syncthreads();
+    }
+    if (!idle) {
+      f4_t d[CG][2];
+#pragma unroll
+      for (int u = 0; u < CG; ++u) d[u][0] = d[u][1] = f4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < KS; ++i)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int at = S::k_at(16 * x + cl, 4 * i + kg);
+          if constexpr (F16) {
+            const u4_t k = L.k[0][at];
+#pragma unroll
+            for (int u = 0; u < CG; ++u) {
+              d[u][x] = mfma(k, q[u][i][1], d[u][x]);
+              d[u][x] = mfma(k, q[u][i][0], d[u][x]);
+            }
+          } else {
+            const u4_t k0 = L.k[0][at], k1 = L.k[1][at], k2 = L.k[2][at];
+#pragma unroll
+            for (int u = 0; u < CG; ++u) {
+              d[u][x] = mfma_b(k2, q[u][i][0], d[u][x]);
+              d[u][x] = mfma_b(k0, q[u][i][2], d[u][x]);
+              d[u][x] = mfma_b(k1, q[u][i][1], d[u][x]);
+              d[u][x] = mfma_b(k1, q[u][i][0], d[u][x]);
+              d[u][x] = mfma_b(k0, q[u][i][1], d[u][x]);
+              d[u][x] = mfma_b(k0, q[u][i][0], d[u][x]);
+            }
+          }
+        }
+      const bool inner = tile * TILE >= lo_max && (tile + 1) * TILE <= hi_min && id[0].id[0] >= 0 && id[0].id[1] >= 0;
+      u4_t w[CG][F16 ? 2 : 3];
+#pragma unroll
+      for (int u = 0; u < CG; ++u) {
+        float s[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[i] = d[u][i >> 2][i & 3] * qs[u];
+        if (!inner) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int j = tile * TILE + 16 * (i >> 2) + 4 * kg + (i & 3);
+            if (j < lo[u] || j >= hi[u] || id[0].id[i >> 2] < 0) s[i] = -INFINITY;
+          }
+        }
+        weigh_tile<F16>(s, m[u], l[u], o[u]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float y0 = s[2 * i] * UP<F16>, y1 = s[2 * i + 1] * UP<F16>;
+          if constexpr (F16) {
+            const h2_t x = {(_Float16)y0, (_Float16)y1};
+            const h2_t z = {(_Float16)(y0 - (float)x[0]), (_Float16)(y1 - (float)x[1])};
+            w[u][0][i] = __builtin_bit_cast(uint32_t, x);
+            w[u][1][i] = __builtin_bit_cast(uint32_t, z);
+          } else {
+            uint32_t x, y, z;
+            three(y0, y1, x, y, z);
+            w[u][0][i] = x;
+            w[u][1][i] = y;
+            w[u][2][i] = z;
+          }
+        }
+      }
+#pragma unroll
+      for (int n = NP - 1; n >= 0; --n) {
+        Tile<HD, true> T;  // (the plane's part of this lane, as fp16 pages' tiles are held)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int row = 16 * (j >> 2) + 4 * kg + (j & 3);
+          if constexpr (HD == 128) {
+            const u4_t x = L.v[n][row * PIECES + cl];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) T.v[j][e] = x[e];
+          } else {
+            const uint2 x = *(reinterpret_cast<const uint2*>(&L.v[n][row * PIECES]) + cl);
+            T.v[j][0] = x.x;
+            T.v[j][1] = x.y;
+          }
+        }
+        if (!inner && __any(T.template not_finite<F16>())) {
+          // (as in run_job; a number that is not finite is so in its first part, and its other parts are dropped too)
+          if (n == 0) {
+#pragma unroll
+            for (int u = 0; u < CG; ++u) {
+              float sees[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const int j = tile * TILE + 16 * (i >> 2) + 4 * kg + (i & 3);
+                sees[i] = j < lo[u] || j >= hi[u] || id[0].id[i >> 2] < 0 ? 0.f : 1.f;
+              }
+#pragma unroll
+              for (int x = 0; x < ND; ++x) {
+                const f4_t plus = T.template sum<F16>(x, sees, false), minus = T.template sum<F16>(x, sees, true);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o[u][x][r] += (plus[r] > 0.f ? INFINITY : 0.f) + (minus[r] > 0.f ? -INFINITY : 0.f);
+              }
+            }
+          }
+          T.template drop<F16>();
+        }
+#pragma unroll
+        for (int y = 0; y < DW2; ++y)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const u4_t v = T.operand(y, e);
+#pragma unroll
+            for (int u = 0; u < CG; ++u) {
+              f4_t& to = o[u][2 * y + e];
+              if constexpr (F16) {
+                to = mfma(v, w[u][1], to);
+                to = mfma(v, w[u][0], to);
+              } else {
+                if (n == 0) to = mfma_b(v, w[u][2], to);
+                if (n <= 1) to = mfma_b(v, w[u][1], to);
+                to = mfma_b(v, w[u][0], to);
+              }
+            }
+          }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i + 1 < (F16 ? AHEAD + 2 : 3); ++i) id[i] = id[i + 1];
+    id[(F16 ? AHEAD + 2 : 3) - 1] = more;
+  }
+#pragma unroll
+  for (int u = 0; u < CG; ++u) {
+    l[u] = groups_sum(l[u]);
+    const int cc = col_base + 16 * u + cl;
+    if (cc < J.cols) put_column<HD, HD, true>(a, p, J, cc, 0, kg, m[u], l[u], o[u], 1.f / UP<F16>);
+  }
+}
+
+// Columns of a workgroup of a job of many, and the slots of its tiles.
+constexpr bool staged(int hd) { return hd <= 128; }
+constexpr int wide_groups(int hd, bool f16) { return f16 ? (staged(hd) ? 2 : 1) : staged(hd) ? 1 : 2; }  // of 16, a wave
+constexpr int wide_columns(int hd, bool f16) { return 16 * sets_of(hd) * wide_groups(hd, f16); }
+constexpr int wide_tile(int hd, bool f16) { return f16 || staged(hd) ? 32 : 16; }
+template <int HD, bool F16>
+union Room {
+  Shared<HD, F16> narrow;
+  Staged<staged(HD) ? HD : 64, F16> wide;
+};
+template <int HD, bool F16, bool WIDE>
+IEK_DEV void run(const Paged& c, const PagedAttn& a, const Plan& p, const Job& J, Room<HD, F16>& L) {
+  if constexpr (!WIDE) run_job<HD, F16, false, 1>(c, a, p, J, L.narrow);
+  else if constexpr (staged(HD)) run_wide<HD, F16>(c, a, p, J, L.wide);
+  else run_job<HD, F16, true, wide_groups(HD, F16)>(c, a, p, J, L.narrow);
+}
+template <int HD, bool F16, bool WIDE>
+constexpr int TILE_OF = WIDE ? wide_tile(HD, F16) : tile_of<F16>();
 
 // Workgroups: first the shared entries' ([chunk][column block][head]), then the own ones'. The chunks that do not
 // exist are the last of their kind.
 template <int HD, bool F16, bool PRE_WIDE, bool OWN_WIDE>
 __global__ __launch_bounds__(64 * WAVES, 2) void part_kernel(Paged c, PagedAttn a, Plan p, int pre_groups) {
-  constexpr int TILE = tile_of<F16>(), SETS = sets_of(HD);
-  __shared__ __align__(16) Shared<HD, F16> L;
+  __shared__ __align__(16) char room[PRE_WIDE ? sizeof(Room<HD, F16>) : sizeof(Shared<HD, F16>)];
+  Room<HD, F16>& L = *reinterpret_cast<Room<HD, F16>*>(room);
   const int shared = shared_entries(a);
   Job J;
   int id = blockIdx.x;
@@ -693,7 +1079,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void part_kernel(Paged c, PagedAttn 
     id /= c.n_kv;
     J.block = id % p.pre_blocks;
     const int x = id / p.pre_blocks;
-    const PreCut pc = pre_cut<TILE>(c, a, p, shared);
+    const PreCut pc = pre_cut<TILE_OF<HD, F16, PRE_WIDE>>(c, a, p, shared);
     if (x >= pc.count) return;
     J.col0 = 0;
     J.cols = p.all;
@@ -704,7 +1090,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void part_kernel(Paged c, PagedAttn 
     const size_t row = ((size_t)x * c.n_kv + J.h) * p.all;
     J.ml = p.pml + 2 * row;
     J.o = p.po + row * HD;
-    run_job<HD, F16, PRE_WIDE, PRE_WIDE ? WIDE_CG : 1>(c, a, p, J, L);
+    run<HD, F16, PRE_WIDE>(c, a, p, J, L);
     return;
   }
   id -= pre_groups;
@@ -712,7 +1098,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void part_kernel(Paged c, PagedAttn 
   id /= c.n_kv;
   J.block = id % p.own_blocks;
   const int x = id / p.own_blocks;
-  const Cut ct = cut<true, TILE, OWN_WIDE ? 1 : SETS>(c, a, p, shared, x, 0);
+  constexpr int TILE = TILE_OF<HD, F16, OWN_WIDE>;
+  const Cut ct = cut<true, TILE, OWN_WIDE ? 1 : sets_of(HD)>(c, a, p, shared, x, 0);
   if (ct.count == 0) return;  // uniform
   J.col0 = ct.b * p.cols;
   J.cols = p.cols;
@@ -725,13 +1112,13 @@ __global__ __launch_bounds__(64 * WAVES, 2) void part_kernel(Paged c, PagedAttn 
   const size_t row = ((size_t)x * c.n_kv + J.h) * p.cols;
   J.ml = p.direct ? nullptr : p.ml + 2 * row;
   J.o = p.direct ? nullptr : p.o + row * HD;
-  run_job<HD, F16, OWN_WIDE, OWN_WIDE ? WIDE_CG : 1>(c, a, p, J, L);
+  run<HD, F16, OWN_WIDE>(c, a, p, J, L);
 }
 
 // The join: 64 dims of a column of a KV head a workgroup, sixteen partial results at a time.
-template <int HD, bool F16>
+template <int HD, bool F16, bool PRE_WIDE, bool OWN_WIDE>
 __global__ __launch_bounds__(256) void join_kernel(Paged c, PagedAttn a, Plan p) {
-  constexpr int TILE = tile_of<F16>(), SETS = sets_of(HD), SD = 64, TPR = SD / 4, GRP = 256 / TPR;
+  constexpr int SD = 64, TPR = SD / 4, GRP = 256 / TPR;
   __shared__ float w[2 * MAX_SPLIT];
   __shared__ float red[2][4];
   __shared__ __align__(16) f4_t acc[GRP][TPR];
@@ -739,8 +1126,8 @@ __global__ __launch_bounds__(256) void join_kernel(Paged c, PagedAttn a, Plan p)
   const int slice = blockIdx.x % (HD / SD), hc = blockIdx.x / (HD / SD), h = hc / p.all, col = hc - h * p.all;
   const int b = col / p.cols, cc = col - b * p.cols;
   const int shared = shared_entries(a);
-  const int pre = p.pre_chunks > 0 ? pre_cut<TILE>(c, a, p, shared).count : 0;
-  const Cut ct = p.own_wide ? cut<false, TILE, 1>(c, a, p, shared, 0, b) : cut<false, TILE, SETS>(c, a, p, shared, 0, b);
+  const int pre = p.pre_chunks > 0 ? pre_cut<TILE_OF<HD, F16, PRE_WIDE>>(c, a, p, shared).count : 0;
+  const Cut ct = cut<false, TILE_OF<HD, F16, OWN_WIDE>, OWN_WIDE ? 1 : sets_of(HD)>(c, a, p, shared, 0, b);
   const int live = pre + ct.count;
   const size_t pstep = (size_t)c.n_kv * p.all, ostep = (size_t)c.n_kv * p.cols;
   const size_t prow = (size_t)h * p.all + col, orow = (size_t)ct.first * ostep + (size_t)h * p.cols + cc;
@@ -791,8 +1178,8 @@ __global__ __launch_bounds__(256) void join_kernel(Paged c, PagedAttn a, Plan p)
 }
 
 size_t up256(size_t x) { return (x + 255) / 256 * 256; }
-int blocks_of(int hd, long long cols, bool wide) {
-  const int per = wide ? sets_of(hd) * WIDE_CG * 16 : 16;
+int blocks_of(const Paged& c, long long cols, bool wide) {
+  const int per = wide ? wide_columns(c.hd, c.f16) : 16;
   return (int)((cols + per - 1) / per);
 }
 
@@ -800,14 +1187,16 @@ int blocks_of(int hd, long long cols, bool wide) {
 // more of them never need less.
 Plan make_plan(const Paged& c, int n_heads, int n_q, int own, int shared, bool edge) {
   Plan p{};
-  const int tile = c.f16 ? 32 : 16, sets = sets_of(c.hd);
+  const int sets = sets_of(c.hd);
   p.group = n_heads / c.n_kv;
   p.cols = p.group * n_q;
   p.all = p.cols * c.batch;
+  auto tile_of_kind = [&](bool wide) { return wide ? wide_tile(c.hd, c.f16) : c.f16 ? 32 : 16; };
   p.own_wide = p.cols > 16;
-  p.pre_wide = p.all > 16;
-  p.own_blocks = blocks_of(c.hd, p.cols, p.own_wide);
-  p.pre_blocks = blocks_of(c.hd, p.all, p.pre_wide);
+  p.pre_wide = p.own_wide || (shared > 0 && p.all > 16);
+  const int tile = tile_of_kind(p.own_wide), pre_tile = tile_of_kind(p.pre_wide);
+  p.own_blocks = blocks_of(c, p.cols, p.own_wide);
+  p.pre_blocks = blocks_of(c, p.all, p.pre_wide);
   constexpr int target = 512;  // workgroups that fill the chip once, two a CU
   const int tiles = (own + tile - 1) / tile + (edge ? 1 : 0);
   const int step = p.own_wide ? 1 : sets;
@@ -827,7 +1216,7 @@ Plan make_plan(const Paged& c, int n_heads, int n_q, int own, int shared, bool e
     p.direct = shared == 0 && p.nsplit == 1;
   }
   if (shared > 0) {
-    const int pt = (shared + tile - 1) / tile;
+    const int pt = (shared + pre_tile - 1) / pre_tile;
     p.pre_tiles = p.pre_wide ? 4 : 2 * sets;
     p.pre_chunks = std::max(1, std::min({MAX_SPLIT, (pt + p.pre_tiles - 1) / p.pre_tiles, target / (c.n_kv * p.pre_blocks)}));
   }
@@ -857,12 +1246,15 @@ Grid grid_of(const Paged& c, const Plan& p) {
 template <int HD, bool F16>
 void launch_hd(const Paged& c, const PagedAttn& a, const Plan& p, hipStream_t st) {
   const Grid g = grid_of(c, p);
+  auto go = [&](auto pre, auto own) {
+    constexpr bool PRE = decltype(pre)::value, OWN = decltype(own)::value;
+    hipLaunchKernelGGL((part_kernel<HD, F16, PRE, OWN>), dim3((unsigned)(g.pre + g.own)), dim3(64 * WAVES), 0, st, c, a, p, g.pre);
+    if (g.join) hipLaunchKernelGGL((join_kernel<HD, F16, PRE, OWN>), dim3((unsigned)g.join), dim3(256), 0, st, c, a, p);
+  };
   // (own_wide: pre_wide, too)
-  auto fn = p.own_wide   ? part_kernel<HD, F16, true, true>
-            : p.pre_wide ? part_kernel<HD, F16, true, false>
-                         : part_kernel<HD, F16, false, false>;
-  hipLaunchKernelGGL(fn, dim3((unsigned)(g.pre + g.own)), dim3(64 * WAVES), 0, st, c, a, p, g.pre);
-  if (g.join) hipLaunchKernelGGL((join_kernel<HD, F16>), dim3((unsigned)g.join), dim3(256), 0, st, c, a, p);
+  if (p.own_wide) go(std::true_type{}, std::true_type{});
+  else if (p.pre_wide) go(std::true_type{}, std::false_type{});
+  else go(std::false_type{}, std::false_type{});
 }
 
 }  // namespace
