@@ -31,6 +31,7 @@ typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
 constexpr int WAVES = 4;
 constexpr int MAX_SPLIT = 256;
 constexpr int SHARED_BATCH = 64;
+constexpr int TURN = 256;
 
 // The running maximum is only a reference: it moves when a tile's is more than 2^LAG above it. For fp16 pages P is held
 // at 2^UP times its share, at most 2^15, so that what fp16 cuts off at its lower end, 2^-25, is 2^-38 of the largest.
@@ -407,7 +408,7 @@ struct Shared {
   static constexpr int SETS = sets_of(HD), DW = WAVES / SETS;
   f4_t parts[DW > 1 ? 2 : 1][DW > 1 ? WAVES : 1][2][F16 ? 2 : 1][64];
   float m[SETS][16], l[SETS][16];
-  float o[SETS][16][HD];
+  float o[SETS][16][HD + 4 * DW];
 };
 
 // Four dims of column cc of the job, or of the output.
@@ -426,15 +427,27 @@ IEK_DEV void put_sums(const Job& J, int cc, float m, float l) {
   J.ml[2 * cc] = isnan(l) ? l : m;  // (a NaN: the maxima pass it over)
   J.ml[2 * cc + 1] = l;
 }
-// A lane's part of a column: the wave's DIMS of it from dim0 on.
+// A wave's 16 columns from cc0 on, DIMS of them from dim0 on: turned through LDS of its own (`room`), since a lane holds
+// pieces of 16 or 32 bytes of a column. (Written as they are held, TODO.)
+constexpr int turn_row(int dims) { return dims + 4; }
 template <int HD, int DIMS, bool HALVES, int ND>
-IEK_DEV void put_column(const PagedAttn& a, const Plan& p, const Job& J, int cc, int dim0, int kg, float m, float l, const f4_t (&o)[ND], float scale) {
+IEK_DEV void put_columns(const PagedAttn& a, const Plan& p, const Job& J, float* room, int cc0, int dim0, float m, float l, const f4_t (&o)[ND], float scale) {
+  constexpr int ROW = turn_row(DIMS), PER = DIMS / 4;
+  const int lane = threadIdx.x & 63, kg = lane >> 4, cl = lane & 15;
 #pragma unroll
   for (int r = 0; r < 4; ++r)
 #pragma unroll
     for (int i = 0; i < ND; i += 4)
-      put_dims<HD>(a, p, J, cc, dim0 + dim_at<DIMS, HALVES>(i, kg, r), f4_t{o[i][r], o[i + 1][r], o[i + 2][r], o[i + 3][r]} * scale, l);
-  if (dim0 == 0 && kg == 0) put_sums(J, cc, m, l);
+      *reinterpret_cast<f4_t*>(room + cl * ROW + dim_at<DIMS, HALVES>(i, kg, r)) = f4_t{o[i][r], o[i + 1][r], o[i + 2][r], o[i + 3][r]} * scale;
+  if (kg == 0) room[cl * ROW + DIMS] = l;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+  for (int i = 0; i < 16 * PER / 64; ++i) {
+    const int at = 64 * i + lane, col = at / PER, dim = 4 * (at % PER);
+    if (cc0 + col < J.cols) put_dims<HD>(a, p, J, cc0 + col, dim0 + dim, *reinterpret_cast<const f4_t*>(room + col * ROW + dim), room[col * ROW + DIMS]);
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  if (dim0 == 0 && kg == 0 && cc0 + cl < J.cols) put_sums(J, cc0 + cl, m, l);
 }
 
 template <int HD, bool F16, bool WIDE, int CG>
@@ -655,8 +668,7 @@ IEK_DEV void run_job(const Paged& c, const PagedAttn& a, const Plan& p, const Jo
 #pragma unroll
     for (int u = 0; u < CG; ++u) {
       l[u] = groups_sum(l[u]);
-      const int cc = col_base + 16 * u + cl;
-      if (cc < J.cols) put_column<HD, DIMS, F16>(a, p, J, cc, dim0, kg, m[u], l[u], o[u], DOWN);
+      put_columns<HD, DIMS, F16>(a, p, J, &L.o[0][0][0] + wave * 16 * turn_row(DIMS), col_base + 16 * u, dim0, m[u], l[u], o[u], DOWN);
     }
   } else {
     // the sets' parts: to a common maximum, then summed through LDS
@@ -1038,11 +1050,13 @@ IEK_DEV void run_wide(const Paged& c, const PagedAttn& a, const Plan& p, const J
     for (int i = 0; i + 1 < (F16 ? AHEAD + 2 : 3); ++i) id[i] = id[i + 1];
     id[(F16 ? AHEAD + 2 : 3) - 1] = more;
   }
+  __syncthreads();  // (all waves have read the last tile)
+  static_assert(sizeof(float) * WAVES * 16 * turn_row(HD) <= sizeof(S), "");
+  float* room = reinterpret_cast<float*>(&R) + wave * 16 * turn_row(HD);
 #pragma unroll
   for (int u = 0; u < CG; ++u) {
     l[u] = groups_sum(l[u]);
-    const int cc = col_base + 16 * u + cl;
-    if (cc < J.cols) put_column<HD, HD, true>(a, p, J, cc, 0, kg, m[u], l[u], o[u], 1.f / UP<F16>);
+    put_columns<HD, HD, true>(a, p, J, room, col_base + 16 * u, 0, m[u], l[u], o[u], 1.f / UP<F16>);
   }
 }
 
@@ -1073,8 +1087,14 @@ __global__ __launch_bounds__(64 * WAVES, 2) void part_kernel(Paged c, PagedAttn 
   Room<HD, F16>& L = *reinterpret_cast<Room<HD, F16>*>(room);
   const int shared = shared_entries(a);
   Job J;
+  // The shared chunks, which the matrix cores bound, and the own ones, which the memory bounds, take turns in runs of one
+  // workgroup a CU, so that most CUs have one of each (all shared ones first: TODO).
+  const int own_groups = gridDim.x - pre_groups, both = min(pre_groups, own_groups) / TURN * TURN;
   int id = blockIdx.x;
-  if (id < pre_groups) {
+  bool pre = id < 2 * both ? id / TURN % 2 == 0 : id < both + pre_groups;
+  if (id < 2 * both) id = id / (2 * TURN) * TURN + id % TURN;
+  else id -= pre ? both : pre_groups;
+  if (pre) {
     J.h = id % c.n_kv;
     id /= c.n_kv;
     J.block = id % p.pre_blocks;
@@ -1093,7 +1113,6 @@ __global__ __launch_bounds__(64 * WAVES, 2) void part_kernel(Paged c, PagedAttn 
     run<HD, F16, PRE_WIDE>(c, a, p, J, L);
     return;
   }
-  id -= pre_groups;
   J.h = id % c.n_kv;
   id /= c.n_kv;
   J.block = id % p.own_blocks;
@@ -1118,7 +1137,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void part_kernel(Paged c, PagedAttn 
 // The join: 64 dims of a column of a KV head a workgroup, sixteen partial results at a time.
 template <int HD, bool F16, bool PRE_WIDE, bool OWN_WIDE>
 __global__ __launch_bounds__(256) void join_kernel(Paged c, PagedAttn a, Plan p) {
-  constexpr int SD = 64, TPR = SD / 4, GRP = 256 / TPR;
+  constexpr int SD = 64, TPR = SD / 4, GRP = 256 / TPR, EARLY = 4;
   __shared__ float w[2 * MAX_SPLIT];
   __shared__ float red[2][4];
   __shared__ __align__(16) f4_t acc[GRP][TPR];
@@ -1131,6 +1150,15 @@ __global__ __launch_bounds__(256) void join_kernel(Paged c, PagedAttn a, Plan p)
   const int live = pre + ct.count;
   const size_t pstep = (size_t)c.n_kv * p.all, ostep = (size_t)c.n_kv * p.cols;
   const size_t prow = (size_t)h * p.all + col, orow = (size_t)ct.first * ostep + (size_t)h * p.cols + cc;
+  const int g = t / TPR, d = slice * SD + 4 * (t % TPR);
+  auto part = [&](int i) {
+    const float* o = i < pre ? p.po + (prow + i * pstep) * HD : p.o + (orow + (i - pre) * ostep) * HD;
+    return *reinterpret_cast<const f4_t*>(o + d);
+  };
+  // the first ones are under way while their weights are made
+  f4_t early[EARLY];
+#pragma unroll
+  for (int i = 0; i < EARLY; ++i) early[i] = g + i * GRP < live ? part(g + i * GRP) : f4_t{0.f, 0.f, 0.f, 0.f};
   float m[2], l[2], top = -INFINITY;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -1159,13 +1187,12 @@ __global__ __launch_bounds__(256) void join_kernel(Paged c, PagedAttn a, Plan p)
   if (lane == 0) red[1][wave] = sum;
   __syncthreads();
   sum = red[1][0] + red[1][1] + red[1][2] + red[1][3];
-  const int g = t / TPR, d = slice * SD + 4 * (t % TPR);
   f4_t y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < EARLY; ++i)
+    if (g + i * GRP < live) y += early[i] * w[g + i * GRP];
 #pragma unroll 4
-  for (int i = g; i < live; i += GRP) {
-    const float* o = i < pre ? p.po + (prow + i * pstep) * HD : p.o + (orow + (i - pre) * ostep) * HD;
-    y += *reinterpret_cast<const f4_t*>(o + d) * w[i];
-  }
+  for (int i = g + EARLY * GRP; i < live; i += GRP) y += part(i) * w[i];
   acc[g][t % TPR] = y;
   __syncthreads();
   if (t < TPR) {
