@@ -32,6 +32,7 @@ constexpr int WAVES = 4;
 constexpr int MAX_SPLIT = 256;
 constexpr int SHARED_BATCH = 64;
 constexpr int TURN = 256;
+constexpr int JOIN_WAVES = 512;
 
 // The running maximum is only a reference: it moves when a tile's is more than 2^LAG above it. For fp16 pages P is held
 // at 2^UP times its share, at most 2^15, so that what fp16 cuts off at its lower end, 2^-25, is 2^-38 of the largest.
@@ -1204,6 +1205,76 @@ __global__ __launch_bounds__(256) void join_kernel(Paged c, PagedAttn a, Plan p)
   }
 }
 
+// The same for many columns: one a wave, and no barrier. A row takes HD / 4 lanes, so a wave sums 256 / HD partial results
+// at a time (a lane has two pieces of a row of 512); 64 of the pairs are read at once and go to the lanes that need them.
+template <int HD, bool F16, bool PRE_WIDE, bool OWN_WIDE>
+__global__ __launch_bounds__(256) void join_columns_kernel(Paged c, PagedAttn a, Plan p) {
+  constexpr int TPR = HD < 256 ? HD / 4 : 64, GRP = 64 / TPR, V = HD / 4 / TPR, EARLY = 4;
+  const int lane = threadIdx.x & 63, hc = uniform(blockIdx.x * 4 + (threadIdx.x >> 6)), h = hc / p.all, col = hc - h * p.all;
+  if (h >= c.n_kv) return;
+  const int b = col / p.cols, cc = col - b * p.cols;
+  const int shared = shared_entries(a);
+  const int pre = p.pre_chunks > 0 ? pre_cut<TILE_OF<HD, F16, PRE_WIDE>>(c, a, p, shared).count : 0;
+  const Cut ct = cut<false, TILE_OF<HD, F16, OWN_WIDE>, OWN_WIDE ? 1 : sets_of(HD)>(c, a, p, shared, 0, b);
+  const int live = uniform(pre + ct.count);
+  const size_t pstep = (size_t)c.n_kv * p.all, ostep = (size_t)c.n_kv * p.cols;
+  const size_t prow = (size_t)h * p.all + col, orow = (size_t)ct.first * ostep + (size_t)h * p.cols + cc;
+  const int g = lane / TPR, d = 4 * (lane % TPR);
+  f4_t y[V];
+  float top = -INFINITY, sum = 0.f;
+#pragma unroll
+  for (int v = 0; v < V; ++v) y[v] = f4_t{0.f, 0.f, 0.f, 0.f};
+  for (int first = 0; first < live; first += 64) {
+    const int n = min(64, live - first);
+    float m = -INFINITY, l = 0.f;
+    if (lane < n) {
+      const int k = first + lane;
+      const float* ml = k < pre ? p.pml + 2 * (prow + k * pstep) : p.ml + 2 * (orow + (k - pre) * ostep);
+      m = ml[0];
+      l = ml[1];
+    }
+    auto part = [&](int i, int v) {
+      const int k = first + min(i, n - 1);
+      const float* o = k < pre ? p.po + (prow + k * pstep) * HD : p.o + (orow + (k - pre) * ostep) * HD;
+      return *reinterpret_cast<const f4_t*>(o + d + 256 * v);
+    };
+    f4_t x[EARLY][V];  // (under way while the weights are made)
+#pragma unroll
+    for (int i = 0; i < EARLY; ++i)
+#pragma unroll
+      for (int v = 0; v < V; ++v) x[i][v] = part(i * GRP + g, v);
+    const float old = top;
+    top = fmaxf(top, wave_max(m));
+    const float down = old == top ? 1.f : __builtin_amdgcn_exp2f(old - top);
+    const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+    sum = sum * down + wave_sum(l * f);
+#pragma unroll
+    for (int v = 0; v < V; ++v) y[v] *= down;
+    for (int i = 0; i < n; i += EARLY * GRP) {
+#pragma unroll
+      for (int e = 0; e < EARLY; ++e) {
+        const int at = i + e * GRP + g;
+        const float w = __shfl(f, min(at, 63));
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          if (at < n) y[v] += x[e][v] * w;
+          x[e][v] = part(at + EARLY * GRP, v);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int s = TPR; s < 64; s <<= 1)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) y[0][r] += __shfl_xor(y[0][r], s);
+  if (g == 0) {
+    const int tq = cc / p.group;
+    float* out = a.out + (((size_t)b * a.n_q + tq) * a.n_heads + h * p.group + cc - tq * p.group) * HD + d;
+#pragma unroll
+    for (int v = 0; v < V; ++v) *reinterpret_cast<f4_t*>(out + 256 * v) = sum == 0.f ? f4_t{0.f, 0.f, 0.f, 0.f} : y[v] / sum;
+  }
+}
+
 size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 int blocks_of(const Paged& c, long long cols, bool wide) {
   const int per = wide ? wide_columns(c.hd, c.f16) : 16;
@@ -1227,8 +1298,13 @@ Plan make_plan(const Paged& c, int n_heads, int n_q, int own, int shared, bool e
   constexpr int target = 512;  // workgroups that fill the chip once, two a CU
   const int tiles = (own + tile - 1) / tile + (edge ? 1 : 0);
   const int step = p.own_wide ? 1 : sets;
-  p.tiles = p.own_wide ? 4 : 2 * step;
-  p.direct = shared == 0 && tiles <= p.tiles;
+  // Up to so many tiles a sequence is one chunk and has no join, a launch of 4 us: a further tile of each set takes 0.7 to
+  // 1.2 us (one sequence of 250 f32 entries, 32 heads of 128: one chunk 11.2 us, two 12.9; 500 fp16 ones 9.8 and 12.2).
+  // Where there is a join anyway, chunks are as small as they come as long as the chip is not full: 531 entries of one
+  // sequence 7.2 us, with two tiles a set 8.5; a window of 512 over 64 columns of 256 dims 13.4, with four tiles 20.
+  const int whole = p.own_wide ? 4 : 4 * step;
+  p.direct = shared == 0 && tiles <= whole;
+  p.tiles = p.direct ? whole : p.own_wide && staged(c.hd) ? 2 : step;
   if (c.batch <= SHARED_BATCH) {
     p.share = std::max(1, target / (c.n_kv * p.own_blocks));
     p.nsplit = 0;
@@ -1244,7 +1320,7 @@ Plan make_plan(const Paged& c, int n_heads, int n_q, int own, int shared, bool e
   }
   if (shared > 0) {
     const int pt = (shared + pre_tile - 1) / pre_tile;
-    p.pre_tiles = p.pre_wide ? 4 : 2 * sets;
+    p.pre_tiles = !p.pre_wide ? sets : staged(c.hd) ? 2 : 1;
     p.pre_chunks = std::max(1, std::min({MAX_SPLIT, (pt + p.pre_tiles - 1) / p.pre_tiles, target / (c.n_kv * p.pre_blocks)}));
   }
   return p;
@@ -1276,7 +1352,10 @@ void launch_hd(const Paged& c, const PagedAttn& a, const Plan& p, hipStream_t st
   auto go = [&](auto pre, auto own) {
     constexpr bool PRE = decltype(pre)::value, OWN = decltype(own)::value;
     hipLaunchKernelGGL((part_kernel<HD, F16, PRE, OWN>), dim3((unsigned)(g.pre + g.own)), dim3(64 * WAVES), 0, st, c, a, p, g.pre);
-    if (g.join) hipLaunchKernelGGL((join_kernel<HD, F16, PRE, OWN>), dim3((unsigned)g.join), dim3(256), 0, st, c, a, p);
+    if (g.join == 0) return;
+    const int columns = c.n_kv * p.all;
+    if (columns < JOIN_WAVES) hipLaunchKernelGGL((join_kernel<HD, F16, PRE, OWN>), dim3((unsigned)g.join), dim3(256), 0, st, c, a, p);
+    else hipLaunchKernelGGL((join_columns_kernel<HD, F16, PRE, OWN>), dim3((unsigned)(columns + 3) / 4), dim3(256), 0, st, c, a, p);
   };
   // (own_wide: pre_wide, too)
   if (p.own_wide) go(std::true_type{}, std::true_type{});
