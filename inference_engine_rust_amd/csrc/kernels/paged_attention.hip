@@ -31,8 +31,8 @@ typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
 constexpr int WAVES = 4;
 constexpr int MAX_SPLIT = 256;
 constexpr int SHARED_BATCH = 64;
-constexpr int TURN = 256;
-constexpr int JOIN_WAVES = 512;
+constexpr int TURN = 256;        // workgroups: one a CU
+constexpr int JOIN_WAVES = 512;  // columns from which the join gives each to one wave
 
 // The running maximum is only a reference: it moves when a tile's is more than 2^LAG above it. For fp16 pages P is held
 // at 2^UP times its share, at most 2^15, so that what fp16 cuts off at its lower end, 2^-25, is 2^-38 of the largest.
@@ -429,7 +429,7 @@ IEK_DEV void put_sums(const Job& J, int cc, float m, float l) {
   J.ml[2 * cc + 1] = l;
 }
 // A wave's 16 columns from cc0 on, DIMS of them from dim0 on: turned through LDS of its own (`room`), since a lane holds
-// pieces of 16 or 32 bytes of a column. (Written as they are held, TODO.)
+// pieces of 16 or 32 bytes of a column. (64 sequences over 16384 shared fp16 entries: 77 us, written as they are held 86.)
 constexpr int turn_row(int dims) { return dims + 4; }
 template <int HD, int DIMS, bool HALVES, int ND>
 IEK_DEV void put_columns(const PagedAttn& a, const Plan& p, const Job& J, float* room, int cc0, int dim0, float m, float l, const f4_t (&o)[ND], float scale) {
@@ -713,13 +713,15 @@ IEK_DEV void run_job(const Paged& c, const PagedAttn& a, const Plan& p, const Jo
 }
 
 // ---- many columns: tiles in LDS -----------------------------------------------------------------------
-// For rows of up to 128 the four waves split the columns of a job and share its tiles of 32 slots, which they put into
-// LDS in turn, each thread 16-byte pieces of rows, the next tile's in flight in registers meanwhile. Both products are
-// mfma_f32_16x16x32 ones. fp16 pages: 32 columns a wave, K and V one plane, q and P pairs (as above). f32 pages: 16 columns
-// a wave, every operand as three bf16 numbers that sum to it exactly (8 bits each, the first one cut off, the others
-// rounded), six products: of the parts' orders those up to the third; what is left out is below 2^-22 of a product.
-// (mfma_f32_16x16x4_f32, exact, takes 32 cycles for 4 of the 32 terms: 4096 shared entries of 32 sequences of 32 heads took
-// 33 us with it.)
+// For rows of up to 128 the four waves split the columns of a job and share its tiles of 32 slots, which lie in LDS. Both
+// products are mfma_f32_16x16x32 ones. fp16 pages: a ring of four tiles, filled by copies without registers three tiles
+// ahead; 32 columns a wave, K and V one plane, q and P pairs (as above). f32 pages: one tile, each thread 16-byte pieces of
+// rows, the next tile's in flight in registers meanwhile; 16 columns a wave, every operand as three bf16 numbers that sum
+// to it exactly (8 bits each, the first one cut off, the others rounded), six products: of the parts' orders those up to the
+// third; what is left out is below 2^-22 of a product. (mfma_f32_16x16x4_f32, exact, takes 32 cycles for 4 of the 32 terms.)
+// 32 heads of 128, part launch: 16384 shared fp16 entries, 64 sequences 65 us (with each wave's tiles in its registers 113),
+// 4096 f32 ones, 32 sequences 28 us (42). The matrix cores are busy for 14 and 10 us of these: a SIMD's two waves leave each
+// other waiting for the softmax's vector work, and the first tile, the results and the own chunks' one turn take 15 to 20.
 typedef __bf16 b2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
 IEK_DEV f4_t mfma_b(u4_t a, u4_t b, f4_t c) {
@@ -749,32 +751,42 @@ struct Staged {
 };
 
 // 16 bytes a lane from memory to 1024 in a row in LDS, without registers. (The waits are the caller's.)
-IEK_DEV void copy16(const void* lds, const void* from) {
+IEK_DEV void copy16(const void* lds, const char* from, uint32_t offset) {
   const uint32_t at = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)lds;
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(at)), "v"(from) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(at)), "v"(offset), "s"(from) : "memory");
 }
 template <int N>
 IEK_DEV void copies_left() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
-// fp16 tiles into LDS. Rows behind the last live one are that one again, and those without a page any row: such a tile is
-// not an inner one, where values out of sight are looked at.
+// fp16 tiles into LDS, 64 pieces a copy. Rows behind the last live one are that one again, and
+// those without a page any row: such a tile is not an inner one, where values out of sight are looked at.
 template <int HD>
-IEK_DEV void copy_tile(typename Staged<HD, true>::One& to, const Paged& c, int h, const Ids<true>& id, int tile, int end) {
+struct Copies {
   using S = Staged<HD, true>;
-  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-#pragma unroll
-  for (int i = 0; i < S::PIECES / 8; ++i) {  // (a wave's rows are in one half of the tile)
-    const int piece = (i * WAVES + wave) * 64, half = piece / S::PIECES >> 4, at = piece + lane;
-    const int row = at / S::PIECES, j = 32 * tile + 16 * half, page = half ? id.id[1] : id.id[0];
-    const size_t first = (((size_t)max(page, 0) * c.n_kv + h) << c.shift) + (j & ((1 << c.shift) - 1));
-    const int live = min(row & 15, max(0, min(16, end - j) - 1)), src = at % S::PIECES;
-    const char* k = static_cast<const char*>(c.k) + first * (2 * HD);
-    const char* v = static_cast<const char*>(c.v) + first * (2 * HD);
-    copy16(&to.k[0][piece], k + live * (2 * HD) + 16 * (src ^ S::turned(row)));
-    copy16(&to.v[0][piece], v + live * (2 * HD) + 16 * src);
+  static constexpr int N = S::PIECES / 8;  // copies of K, and of V, a wave and tile
+  uint32_t row, k_at, v_at;  // this lane's of 16 rows, and its pieces' places
+  IEK_DEV Copies() {
+    const int at = (threadIdx.x & 63) + 64 * (int)(threadIdx.x >> 6);
+    row = at / S::PIECES & 15;
+    k_at = 16 * (at % S::PIECES ^ S::turned(at / S::PIECES));
+    v_at = 16 * (at % S::PIECES);
   }
-}
+  IEK_DEV void tile(typename S::One& to, const Paged& c, int h, const Ids<true>& id, int tile, int end) const {
+    const int wave = uniform(threadIdx.x >> 6);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int piece = (i * WAVES + wave) * 64, half = N == 2 ? i : wave >> 1, j = 32 * tile + 16 * half;
+      const int page = max(half ? id.id[1] : id.id[0], 0);
+      const size_t first = ((((size_t)(uint32_t)page * (uint32_t)c.n_kv + h) << c.shift) + (j & ((1 << c.shift) - 1))) * (2 * HD);
+      uint32_t from = row;
+      if (end - j < 16) from = min(from, (uint32_t)max(0, end - j - 1));  // (uniform)
+      from *= 2 * HD;
+      copy16(&to.k[0][piece], static_cast<const char*>(c.k) + first, from + k_at);
+      copy16(&to.v[0][piece], static_cast<const char*>(c.v) + first, from + v_at);
+    }
+  }
+};
 
 // A thread's pieces of a tile on their way: piece t % PIECES of the rows t / PIECES, ...
 template <int HD, bool F16>
@@ -840,10 +852,11 @@ IEK_DEV void run_wide(const Paged& c, const PagedAttn& a, const Plan& p, const J
 #pragma unroll
   for (int i = 0; i < (F16 ? AHEAD + 2 : 3); ++i) id[i] = ids_of<true>(c, pages, J.t0 + i);
   Way<HD, false> way;
+  const Copies<HD> copies;
   if constexpr (F16) {
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i)
-      if (J.t0 + i < J.t1) copy_tile<HD>(R.ring[i], c, J.h, id[i], J.t0 + i, pages.end);
+      if (J.t0 + i < J.t1) copies.tile(R.ring[i], c, J.h, id[i], J.t0 + i, pages.end);
   } else {
     way.load(c, J.h, id[0], J.t0, pages.end);
   }
@@ -922,7 +935,7 @@ IEK_DEV void run_wide(const Paged& c, const PagedAttn& a, const Plan& p, const J
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
-      if (tile + AHEAD < J.t1) copy_tile<HD>(R.ring[(tile - J.t0 + AHEAD) & AHEAD], c, J.h, id[AHEAD], tile + AHEAD, pages.end);
+      if (tile + AHEAD < J.t1) copies.tile(R.ring[(tile - J.t0 + AHEAD) & AHEAD], c, J.h, id[AHEAD], tile + AHEAD, pages.end);
     } else {
       __syncthreads();  // (all waves have read the tile before)
       way.store(L);
@@ -941,10 +954,9 @@ IEK_DEV void run_wide(const Paged& c, const PagedAttn& a, const Plan& p, const J
           if constexpr (F16) {
             const u4_t k = L.k[0][at];
 #pragma unroll
-            for (int u = 0; u < CG; ++u) {
-              d[u][x] = mfma(k, q[u][i][1], d[u][x]);
-              d[u][x] = mfma(k, q[u][i][0], d[u][x]);
-            }
+            for (int z = 1; z >= 0; --z)
+#pragma unroll
+              for (int u = 0; u < CG; ++u) d[u][x] = mfma(k, q[u][i][z], d[u][x]);
           } else {
             const u4_t k0 = L.k[0][at], k1 = L.k[1][at], k2 = L.k[2][at];
 #pragma unroll
@@ -1032,13 +1044,17 @@ IEK_DEV void run_wide(const Paged& c, const PagedAttn& a, const Plan& p, const J
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const u4_t v = T.operand(y, e);
+            if constexpr (F16) {
+#pragma unroll
+              for (int z = 1; z >= 0; --z)
+#pragma unroll
+                for (int u = 0; u < CG; ++u) o[u][2 * y + e] = mfma(v, w[u][z], o[u][2 * y + e]);
+              continue;
+            }
 #pragma unroll
             for (int u = 0; u < CG; ++u) {
               f4_t& to = o[u][2 * y + e];
-              if constexpr (F16) {
-                to = mfma(v, w[u][1], to);
-                to = mfma(v, w[u][0], to);
-              } else {
+              if constexpr (!F16) {
                 if (n == 0) to = mfma_b(v, w[u][2], to);
                 if (n <= 1) to = mfma_b(v, w[u][1], to);
                 to = mfma_b(v, w[u][0], to);
@@ -1089,7 +1105,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void part_kernel(Paged c, PagedAttn 
   const int shared = shared_entries(a);
   Job J;
   // The shared chunks, which the matrix cores bound, and the own ones, which the memory bounds, take turns in runs of one
-  // workgroup a CU, so that most CUs have one of each (all shared ones first: TODO).
+  // workgroup a CU, so that most CUs have one of each (32 sequences, 4096 shared f32 entries and up to 714 own ones: 49 us, with
+  // the shared ones first 52).
   const int own_groups = gridDim.x - pre_groups, both = min(pre_groups, own_groups) / TURN * TURN;
   int id = blockIdx.x;
   bool pre = id < 2 * both ? id / TURN % 2 == 0 : id < both + pre_groups;
@@ -1205,7 +1222,8 @@ __global__ __launch_bounds__(256) void join_kernel(Paged c, PagedAttn a, Plan p)
   }
 }
 
-// The same for many columns: one a wave, and no barrier. A row takes HD / 4 lanes, so a wave sums 256 / HD partial results
+// The same for many columns (2048 of 128 dims with one or two partial results 4.3 us, above 10; 512 of two or three 4.8 and
+// 5.2; 256 of 64 5.0 and 4.8; 32 of 64 7.8 and 4.8): one a wave, and no barrier. A row takes HD / 4 lanes, so a wave sums 256 / HD partial results
 // at a time (a lane has two pieces of a row of 512); 64 of the pairs are read at once and go to the lanes that need them.
 template <int HD, bool F16, bool PRE_WIDE, bool OWN_WIDE>
 __global__ __launch_bounds__(256) void join_columns_kernel(Paged c, PagedAttn a, Plan p) {
@@ -1276,6 +1294,7 @@ __global__ __launch_bounds__(256) void join_columns_kernel(Paged c, PagedAttn a,
 }
 
 size_t up256(size_t x) { return (x + 255) / 256 * 256; }
+int tile_of_kind(const Paged& c, bool wide) { return wide ? wide_tile(c.hd, c.f16) : c.f16 ? 32 : 16; }
 int blocks_of(const Paged& c, long long cols, bool wide) {
   const int per = wide ? wide_columns(c.hd, c.f16) : 16;
   return (int)((cols + per - 1) / per);
@@ -1289,10 +1308,9 @@ Plan make_plan(const Paged& c, int n_heads, int n_q, int own, int shared, bool e
   p.group = n_heads / c.n_kv;
   p.cols = p.group * n_q;
   p.all = p.cols * c.batch;
-  auto tile_of_kind = [&](bool wide) { return wide ? wide_tile(c.hd, c.f16) : c.f16 ? 32 : 16; };
   p.own_wide = p.cols > 16;
   p.pre_wide = p.own_wide || (shared > 0 && p.all > 16);
-  const int tile = tile_of_kind(p.own_wide), pre_tile = tile_of_kind(p.pre_wide);
+  const int tile = tile_of_kind(c, p.own_wide), pre_tile = tile_of_kind(c, p.pre_wide);
   p.own_blocks = blocks_of(c, p.cols, p.own_wide);
   p.pre_blocks = blocks_of(c, p.all, p.pre_wide);
   constexpr int target = 512;  // workgroups that fill the chip once, two a CU
@@ -1377,6 +1395,15 @@ void launch_paged_attention(const Paged& c, const PagedAttn& a, void* ws, hipStr
   const long long span = a.window > 0 ? std::min<long long>(a.max_len, (long long)a.window + a.n_q - 1) : a.max_len;
   Plan p = make_plan(c, a.n_heads, a.n_q, (int)span, a.max_shared, span < a.max_len);
   const Sizes z = sizes(c, p);
+  if (p.pre_wide && !p.own_wide) {
+    // Two workgroups a CU read the shared entries; if the own ones are twice their tiles or more, and so the longer work,
+    // one does, and own ones take the other place: half the partial results. (Part and join, one and two: 4096 shared f32
+    // entries and up to 714 own ones of 32 sequences 47 and 55 us, fp16 33 and 41; 16384 shared fp16 entries of 64 sequences
+    // with up to 2616 own ones 111 and 132, with up to 616, on the other side of the rule, 91 and 85.)
+    const long long mine = a.window > 0 ? span : std::max(0, a.max_len - a.max_shared);
+    const long long own = c.batch * (mine / tile_of_kind(c, false)), shared = p.pre_blocks * (a.max_shared / tile_of_kind(c, true));
+    if (own >= 2 * shared) p.pre_chunks = std::min(p.pre_chunks, std::max(1, 256 / (c.n_kv * p.pre_blocks)));
+  }
   char* base = static_cast<char*>(ws);
   p.ml = reinterpret_cast<float*>(base);
   p.o = reinterpret_cast<float*>(base + z.ml);
