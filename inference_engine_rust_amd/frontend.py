@@ -199,11 +199,14 @@ class ChatPromptStyle(Enum):
 
 def generate(model: "E.LoadedModel", tokenizer: Tokenizer, prompt: str, new_tokens: int = 20,
              chat: ChatPromptStyle = ChatPromptStyle.RAW, temperature: float = 0.0, rng=None,
-             session: "E.InferenceSession | None" = None) -> tuple[str, list[int]]:
+             session: "E.InferenceSession | None" = None, top_k: int = 0, top_p: float = 1.0,
+             min_p: float = 0.0) -> tuple[str, list[int]]:
     """The CLI's loop: wrap the prompt for its style, encode with the model's BOS/EOS rule,
     prefill, then up to `new_tokens` x { next id (greedy on the device, or sample_temperature on
     the device when temperature > 0, drawing r from `rng`); stop at EOS; stop at a Gemma structure
-    marker; decode it }. Returns (visible continuation, generated ids)."""
+    marker; decode it }. Returns (visible continuation, generated ids). With top_k > 0, top_p < 1 or
+    min_p > 0 the draw is from what these leave (include/iek.h, iek_sample); greedy needs none of them."""
+    filters = top_k > 0 or not top_p >= 1.0 or not min_p <= 0.0  # (a NaN goes on, to be refused)
     text = chat.wrap(prompt)
     cfg = TokenizerPromptConfig.from_model(model)
     ids = tokenizer.encode_with_prompt_config(text, cfg)
@@ -212,7 +215,10 @@ def generate(model: "E.LoadedModel", tokenizer: Tokenizer, prompt: str, new_toke
     s.prefill(ids)
     generated: list[int] = []
     for _ in range(new_tokens):
-        if temperature > 0.0:
+        if temperature > 0.0 and filters:
+            r = min(float(rng.random()), 1.0 - 2.0 ** -24)  # (the largest f32 below 1)
+            nxt = E.sample_next_token(s, temperature, r, top_k, top_p, min_p)
+        elif temperature > 0.0:
             nxt = E.sample_temperature_next_token(s, temperature, float(rng.random()))
         else:
             nxt = E.greedy_next_token(s)
@@ -241,6 +247,11 @@ def main(argv=None) -> int:
     ap.add_argument("--chat", default="raw", help="prompt style: raw | mistral-instruct | gemma4-e2b")
     ap.add_argument("--temperature", type=float, default=0.0,
                     help="> 0: sample_temperature on the device instead of greedy (not in the reference CLI)")
+    ap.add_argument("--top-k", type=int, default=0, help="> 0: sample from the top-k tokens alone")
+    ap.add_argument("--top-p", type=float, default=1.0,
+                    help="< 1: from the likeliest tokens that together have this share")
+    ap.add_argument("--min-p", type=float, default=0.0,
+                    help="> 0: from the tokens with this share of the likeliest one's probability or more")
     ap.add_argument("--seed", type=int, default=0, help="seed of the uniform draws when sampling")
     ap.add_argument("prompt", nargs="?", default=None, help="prompt text; one line of stdin when omitted")
     a = ap.parse_args(argv)
@@ -261,7 +272,8 @@ def main(argv=None) -> int:
         model = E.LoadedModel.load(a.model)
         tok = Tokenizer.load_from_file(a.tokenizer)
         import random
-        text, _ = generate(model, tok, prompt, a.new_tokens, style, a.temperature, random.Random(a.seed))
+        text, _ = generate(model, tok, prompt, a.new_tokens, style, a.temperature, random.Random(a.seed),
+                           top_k=a.top_k, top_p=a.top_p, min_p=a.min_p)
     except (E.EngineError, TokenizerError) as e:
         print(f"error: {e}", file=sys.stderr)
         return 1
