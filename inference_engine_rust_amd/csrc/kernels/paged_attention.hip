@@ -565,12 +565,21 @@ IEK_DEV void run_job(const Paged& c, const PagedAttn& a, const Plan& p, const Jo
               d[u][x] = mfma(T.k[x][i], Q.lo[u][i], d[u][x]);
             }
       } else {
+        // (several sums of a quarter or half of the dims: one of all of them rounds up to 128 times in a row)
+        constexpr int N = 4 / CG;
+        f4_t z[CG][N];
+#pragma unroll
+        for (int u = 0; u < CG; ++u)
+#pragma unroll
+          for (int x = 0; x < N; ++x) z[u][x] = f4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < DIMS / 16; ++i)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
 #pragma unroll
-            for (int u = 0; u < CG; ++u) d[u][0] = mfma(T.k[i][e], Q.q[u][i][e], d[u][0]);
+            for (int u = 0; u < CG; ++u) z[u][e % N] = mfma(T.k[i][e], Q.q[u][i][e], z[u][e % N]);
+#pragma unroll
+        for (int u = 0; u < CG; ++u) d[u][0] = N == 4 ? (z[u][0] + z[u][1]) + (z[u][2 % N] + z[u][3 % N]) : z[u][0] + z[u][1 % N];
       }
       load_k<HD>(T, c, J.h, next, tile + STEP, pages.end, dim0, lane);
 #pragma unroll
