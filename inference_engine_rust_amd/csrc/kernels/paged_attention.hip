@@ -1410,7 +1410,8 @@ void launch_paged_attention(const Paged& c, const PagedAttn& a, void* ws, hipStr
     // entries and up to 714 own ones of 32 sequences 47 and 55 us, fp16 33 and 41; 16384 shared fp16 entries of 64 sequences
     // with up to 2616 own ones 111 and 132, with up to 616, on the other side of the rule, 91 and 85.)
     const long long mine = a.window > 0 ? span : std::max(0, a.max_len - a.max_shared);
-    const long long own = c.batch * (mine / tile_of_kind(c, false)), shared = p.pre_blocks * (a.max_shared / tile_of_kind(c, true));
+    const long long own = (long long)c.batch * (mine / tile_of_kind(c, false));
+    const long long shared = (long long)p.pre_blocks * (a.max_shared / tile_of_kind(c, true));
     if (own >= 2 * shared) p.pre_chunks = std::min(p.pre_chunks, std::max(1, 256 / (c.n_kv * p.pre_blocks)));
   }
   char* base = static_cast<char*>(ws);
