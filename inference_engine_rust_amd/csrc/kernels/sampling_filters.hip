@@ -864,13 +864,20 @@ __host__ IEK_DEV RowSpace space_of(const Slices& z, int b) {
 IEK_DEV bool by_list(const Head& h) { return h.k > 0 && h.k <= ST; }
 IEK_DEV bool by_slices(const Head& h) { return h.good && h.t > 0.f && h.r > 0.f && h.k <= ST; }
 
-// The row's head from its slices' maxima, and the span of the threads' maxima.
-IEK_DEV Head head_of_slices(const SampleArgs& a, const Slices& z, int b, const RowSpace& r, Group& q, float& span) {
-  const SampleParams o = params_of(a, b);
+// What a workgroup takes of the row's part first, all of it at once and ahead of its logits; from these the row's head and
+// the span of the threads' maxima.
+struct Early {
+  SampleParams o;
+  float most, least;
+};
+IEK_DEV Early early_of(const SampleArgs& a, const Slices& z, int b, const RowSpace& r) {
   const int t = threadIdx.x;
-  const float top = q.most(t < z.count ? r.most[t] : -INFINITY);
-  span = q.most(t < z.count ? top - r.least[t] : 0.f);
-  return head_of(o, a.n, top);
+  return Early{params_of(a, b), t < z.count ? r.most[t] : -INFINITY, t < z.count ? r.least[t] : INFINITY};
+}
+IEK_DEV Head head_of_slices(const SampleArgs& a, const Slices& z, const Early& e, Group& q, float& span) {
+  const float top = q.most(e.most);
+  span = q.most((int)threadIdx.x < z.count ? top - e.least : 0.f);
+  return head_of(e.o, a.n, top);
 }
 IEK_DEV float load_slice(float4* to, const SampleArgs& a, const Slices& z, int b, int s, Tokens& T) {
   const int first = s * z.length, n = min(z.length, a.n - first);
@@ -903,12 +910,13 @@ __global__ __launch_bounds__(ST) void slice_bins_kernel(SampleArgs a, Slices z) 
   __shared__ u64 hist[BINS];
   const int b = blockIdx.y, s = blockIdx.x, t = threadIdx.x;
   const RowSpace r = space_of(z, b);
+  const Early e = early_of(a, z, b, r);
   Group q(m);
   Tokens T;
   const float most = load_slice(data, a, z, b, s, T);
   fill_table(m.table);
   float span;
-  const Head h = head_of_slices(a, z, b, r, q, span);
+  const Head h = head_of_slices(a, z, e, q, span);
   if (!by_slices(h)) return;
   const Weigh weigh = weigh_of(h, a.n, m.table);
   if (!by_list(h) && !(h.p < 1.f)) {
@@ -928,10 +936,16 @@ __global__ __launch_bounds__(ST) void slice_bins_kernel(SampleArgs a, Slices z) 
     if (hist[i]) atomicAdd(&r.hist[i], hist[i]);
 }
 
-// The bin of the row's histogram that the border is in; into m.hist's copy.
-IEK_DEV int cross_row(const Head& h, const RowSpace& r, Group& q, u64* hist, u64& above, u64& total) {
+// The bin of the row's histogram (`bins`: the thread's of it) that the border is in; into m.hist's copy.
+constexpr int PER = BINS / ST;
+IEK_DEV void bins_of(const RowSpace& r, u64 (&bins)[PER]) {
+#pragma unroll
+  for (int i = 0; i < PER; ++i) bins[i] = r.hist[threadIdx.x + i * ST];
+}
+IEK_DEV int cross_row(const Head& h, const u64 (&bins)[PER], Group& q, u64* hist, u64& above, u64& total) {
   clear_bins(q.m, hist);
-  for (int i = threadIdx.x; i < BINS; i += ST) hist[i] = r.hist[i];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) hist[threadIdx.x + i * ST] = bins[i];
   __syncthreads();
   const bool list = by_list(h);
   return cross(q, hist, [&](u64 v, u64 all) { return list ? v < (u64)h.k : v == 0 || (double)v < (double)h.p * (double)all; }, above, total);
@@ -944,15 +958,18 @@ __global__ __launch_bounds__(ST) void slice_cut_kernel(SampleArgs a, Slices z) {
   __shared__ Bins bins;
   const int b = blockIdx.y, s = blockIdx.x, t = threadIdx.x;
   const RowSpace r = space_of(z, b);
+  const Early e = early_of(a, z, b, r);
+  u64 row[PER];
+  bins_of(r, row);
   Group q(m);
   Tokens T;
   load_slice(data, a, z, b, s, T);
   fill_table(m.table);
   float span;
-  const Head h = head_of_slices(a, z, b, r, q, span);
+  const Head h = head_of_slices(a, z, e, q, span);
   if (!by_slices(h) || (!by_list(h) && !(h.p < 1.f))) return;
   u64 above, total;
-  const int bin = cross_row(h, r, q, bins.hist, above, total);
+  const int bin = cross_row(h, row, q, bins.hist, above, total);
   if (by_list(h)) {
     const float scale = list_scale(span), far = bin < 0 ? INFINITY : (float)(bin + 1);
     float* x = r.x + (size_t)s * SEGMENT;
@@ -985,7 +1002,11 @@ __global__ __launch_bounds__(ST) void slice_cut_kernel(SampleArgs a, Slices z) {
 }
 
 // The token of a row of slices. False: it is left to any_row.
-IEK_DEV bool join_slices(const SampleArgs& a, const Slices& z, int b, const Head& h, const RowSpace& r, float span, Group& q, float4* data, char* more) {
+struct Joined {
+  u64 bins[PER], near, near_w, sum;  // (near: of a row that has them; the thread's sum is its slice's)
+  int found, border;
+};
+IEK_DEV bool join_slices(const SampleArgs& a, const Slices& z, int b, const Head& h, const RowSpace& r, const Joined& e, Group& q, float4* data, char* more) {
   const int t = threadIdx.x;
   Smem& m = q.m;
   Bins& bins = *reinterpret_cast<Bins*>(more);
@@ -993,7 +1014,7 @@ IEK_DEV bool join_slices(const SampleArgs& a, const Slices& z, int b, const Head
   if (by_list(h)) {
     const List list{reinterpret_cast<float4*>(more), reinterpret_cast<uint32_t*>(more + 16 * ST)};
     Bins& room = *reinterpret_cast<Bins*>(data);
-    const int mine = t < z.count ? r.found[t] : 0;
+    const int mine = t < z.count ? e.found : 0;
     u64 total, most;
     const int at = (int)q.before(mine, total);
     q.before(mine > SEGMENT, most);
@@ -1019,16 +1040,16 @@ IEK_DEV bool join_slices(const SampleArgs& a, const Slices& z, int b, const Head
     return true;
   }
   Cut cut{-INFINITY, 0};
-  u64 mine = t < z.count ? r.sum[t] : 0;
+  u64 mine = t < z.count ? e.sum : 0;
   const float least = fminf(h.m, 1.f);
   if (h.p < 1.f) {
     u64 above, total;
-    cross_row(h, r, q, bins.hist, above, total);
-    const int n = r.found[z.count];
+    cross_row(h, e.bins, q, bins.hist, above, total);
+    const int n = e.border;
     if (n > NEAR) return false;
     if (t < n) {
-      bins.near[t] = r.near[t];
-      bins.near_w[t] = r.near_w[t];
+      bins.near[t] = e.near;
+      bins.near_w[t] = e.near_w;
     }
     u64* add = bins.hist;  // (of each slice, the kept ones of these)
     __syncthreads();
@@ -1056,8 +1077,8 @@ IEK_DEV bool join_slices(const SampleArgs& a, const Slices& z, int b, const Head
   const u64 from = m.word;
   const int s = m.word2;
   if (cut.ties > 0) {  // the kept ties before it
-    const uint32_t index = t < r.found[z.count] ? ~(uint32_t)bins.near[t] : 0xFFFFFFFFu;
-    const bool tie = t < r.found[z.count] && value_of((uint32_t)(bins.near[t] >> 32)) == cut.over && index < (uint32_t)(s * z.length);
+    const uint32_t index = t < e.border ? ~(uint32_t)bins.near[t] : 0xFFFFFFFFu;
+    const bool tie = t < e.border && value_of((uint32_t)(bins.near[t] >> 32)) == cut.over && index < (uint32_t)(s * z.length);
     cut.ties = max(0, cut.ties - (int)q.sum(tie));
   }
   Tokens T;
@@ -1079,24 +1100,33 @@ __global__ __launch_bounds__(ST) void slice_join_kernel(SampleArgs a, Slices z) 
   __shared__ __align__(16) char more[sizeof(Bins) > LIST_BYTES ? sizeof(Bins) : LIST_BYTES];
   const int b = blockIdx.x;
   const RowSpace r = space_of(z, b);
+  // (what a row has no use for, or what nobody wrote, is not looked at)
+  const int t = threadIdx.x, c = min(t, z.count - 1), near = min(t, NEAR - 1);
+  const Early first = early_of(a, z, b, r);
+  Joined e;
+  bins_of(r, e.bins);
+  e.near = r.near[near];
+  e.near_w = r.near_w[near];
+  e.sum = r.sum[c];
+  e.found = r.found[c];
+  e.border = r.found[z.count];
   Group q(m);
   fill_table(m.table);
   float span;
-  const Head h = head_of_slices(a, z, b, r, q, span);
+  const Head h = head_of_slices(a, z, first, q, span);
   if (!h.good) {
     if (threadIdx.x == 0) store(a, b, NO_TOKEN, NAN);
   } else if (h.t == 0.f) {
     // the first slice that has the maximum
-    const int t = threadIdx.x;
     u64 total;
-    const bool has = t < z.count && r.most[t] == h.top;
+    const bool has = t < z.count && first.most == h.top;
     if (q.before(has, total) == 0 && has) m.word2 = t;
     __syncthreads();
     Tokens T;
     load_slice(data, a, z, b, m.word2, T);
     __syncthreads();
     store_top(T, q, a, b, h.top);
-  } else if (!by_slices(h) || !join_slices(a, z, b, h, r, span, q, data, more)) {
+  } else if (!by_slices(h) || !join_slices(a, z, b, h, r, e, q, data, more)) {
     any_row(a, b, h, m, reinterpret_cast<Bins*>(more)->hist);
   }
 }
