@@ -516,12 +516,13 @@ IEK_DEV void rank(const Bins& s, int n, To to) {
 }
 
 // The border among n <= NEAR tokens of a bin: keeps(the sum before a token). m.border, m.ties: the last value that stays
-// and how many of it; m.word: the sum up to it; m.word2: whether it is the last of them.
-template <class Keeps>
-IEK_DEV void rank_near(Smem& m, const Bins& s, int n, u64 above, Keeps keeps) {
+// and how many of it; m.word: the sum up to it; m.word2: whether it is the last of them. kept(token), for those that stay.
+template <class Keeps, class Kept>
+IEK_DEV void rank_near(Smem& m, const Bins& s, int n, u64 above, Keeps keeps, Kept kept) {
   rank(s, n, [&](int i, u64 sum, int count, int equal) {
     const u64 own = s.near_w[i];
     sum += above;
+    if (keeps(sum)) kept(i);
     const bool last = count == n - 1;
     if (keeps(sum) && (last || !keeps(sum + own))) {
       m.border = value_of((uint32_t)(s.near[i] >> 32));
@@ -582,7 +583,7 @@ IEK_DEV bool cut_at(const Tokens& T, Group& q, Bins& s, const Weigh& weigh, bool
     m.word = above;
   }
   __syncthreads();
-  rank_near(m, s, n, above, [&](u64 v) { return keeps(v, total); });
+  rank_near(m, s, n, above, [&](u64 v) { return keeps(v, total); }, [](int) {});
   // all of the bin's, and some of the value that was the last one before
   const u64 sum = m.word;
   if (m.word2 && bin == tie_bin && keeps(sum, total)) {
@@ -1019,12 +1020,15 @@ IEK_DEV bool join_slices(const SampleArgs& a, const Slices& z, int b, const Head
     const int at = (int)q.before(mine, total);
     q.before(mine > SEGMENT, most);
     if (most > 0 || total > LIST) return false;
-    // each segment by its thread's wave: (place, count) from the lane that has them
-    for (int i = 0; i < 64; ++i) {
-      const int n = __builtin_amdgcn_readlane(mine, i), to = __builtin_amdgcn_readlane(at, i);
-      const size_t from = (size_t)((t & ~63) + i) * SEGMENT;
-      for (int j = t & 63; j < n; j += 64) list.put(to + j, r.x[from + j], r.index[from + j]);
+    // the waves take the segments in turn: their places and counts through LDS
+    int2* seg = reinterpret_cast<int2*>(data);
+    if (t < z.count) seg[t] = int2{at, mine};
+    __syncthreads();
+    for (int i = t >> 6; i < z.count; i += NW) {
+      const int2 g = seg[i];
+      for (int j = t & 63; j < g.y; j += 64) list.put(g.x + j, r.x[(size_t)i * SEGMENT + j], r.index[(size_t)i * SEGMENT + j]);
     }
+    __syncthreads();
     const int n = (int)total;
     const Tokens L = list.tokens(n);
     if (n <= NEAR) {
@@ -1055,14 +1059,11 @@ IEK_DEV bool join_slices(const SampleArgs& a, const Slices& z, int b, const Head
     __syncthreads();
     add[t] = 0;
     __syncthreads();
-    rank_near(m, bins, n, above, [&](u64 v) { return v == 0 || (double)v < (double)h.p * (double)total; });
-    cut = Cut{m.border, m.ties};
-    rank(bins, n, [&](int i, u64, int, int equal) {
-      const float x = value_of((uint32_t)(bins.near[i] >> 32));
-      if ((x > cut.over || (x == cut.over && equal < cut.ties)) && weigh.real(x) >= least)
+    rank_near(m, bins, n, above, [&](u64 v) { return v == 0 || (double)v < (double)h.p * (double)total; }, [&](int i) {
+      if (weigh.real(value_of((uint32_t)(bins.near[i] >> 32))) >= least)
         atomicAdd(&add[~(uint32_t)bins.near[i] / (uint32_t)z.length], bins.near_w[i]);
     });
-    __syncthreads();
+    cut = Cut{m.border, m.ties};
     mine += add[t];
   }
   // the slice that has the token
