@@ -1317,7 +1317,10 @@ Plan make_plan(const Paged& c, int n_heads, int n_q, int own, int shared, bool e
   p.group = n_heads / c.n_kv;
   p.cols = p.group * n_q;
   p.all = p.cols * c.batch;
-  p.own_wide = p.cols > 16;
+  // Up to 32 columns a sequence take one or two workgroups, each with its tiles in registers. (Part launch, 16 sequences up to
+  // 2048 of 8 KV heads of 128, 20 columns: fp16 21.5 us, as many columns 30; f32 43.5 and 42.5; one sequence of 500 10.7 us
+  // without a join, as many columns 11.0 and one. With 64 columns in four workgroups f32 takes 80 us, as many columns 48.)
+  p.own_wide = p.cols > 32;
   p.pre_wide = p.own_wide || (shared > 0 && p.all > 16);
   const int tile = tile_of_kind(c, p.own_wide), pre_tile = tile_of_kind(c, p.pre_wide);
   p.own_blocks = blocks_of(c, p.cols, p.own_wide);
@@ -1410,7 +1413,7 @@ void launch_paged_attention(const Paged& c, const PagedAttn& a, void* ws, hipStr
     // entries and up to 714 own ones of 32 sequences 47 and 55 us, fp16 33 and 41; 16384 shared fp16 entries of 64 sequences
     // with up to 2616 own ones 111 and 132, with up to 616, on the other side of the rule, 91 and 85.)
     const long long mine = a.window > 0 ? span : std::max(0, a.max_len - a.max_shared);
-    const long long own = (long long)c.batch * (mine / tile_of_kind(c, false));
+    const long long own = (long long)c.batch * p.own_blocks * (mine / tile_of_kind(c, false));
     const long long shared = (long long)p.pre_blocks * (a.max_shared / tile_of_kind(c, true));
     if (own >= 2 * shared) p.pre_chunks = std::min(p.pre_chunks, std::max(1, 256 / (c.n_kv * p.pre_blocks)));
   }

@@ -27,3 +27,11 @@ def test_lengths_at_one_chunks_limits(gpu, dtype, hd, group, n_q, around):
     for lens in ([around - 1], [around], [around + 1], [around, 0, around - 1]):
         check_attention(around, dtype, 2, group, hd, n_q, lens, page=32)
     check_attention(around, dtype, 2, group, hd, n_q, [around + 300, around + 17], page=32, window=around)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+@pytest.mark.parametrize("group,n_q", [(8, 2), (1, 17), (4, 8), (3, 11), (8, 8), (5, 13)])
+@pytest.mark.parametrize("shared,window", [(0, 0), (130, 0), (0, 100)])
+def test_columns_of_a_sequence(gpu, dtype, hd, group, n_q, shared, window):
+    check_attention(hd + n_q, dtype, 1, group, hd, n_q, [shared + 700, shared + 3, shared + 129, 0], page=32, shared=shared, window=window)
