@@ -1351,7 +1351,7 @@ Plan make_plan(const Paged& c, int n_heads, int n_q, int own, int shared, bool e
   if (shared > 0) {
     const int pt = (shared + pre_tile - 1) / pre_tile;
     p.pre_tiles = !p.pre_wide ? sets : staged(c.hd) ? 2 : 1;
-    p.pre_chunks = std::max(1, std::min({MAX_SPLIT, (pt + p.pre_tiles - 1) / p.pre_tiles, target / (c.n_kv * p.pre_blocks)}));
+    p.pre_chunks = std::max(1, std::min({MAX_SPLIT, (pt + p.pre_tiles - 1) / p.pre_tiles, (int)(target / ((long long)c.n_kv * p.pre_blocks))}));
   }
   return p;
 }
@@ -1415,7 +1415,7 @@ void launch_paged_attention(const Paged& c, const PagedAttn& a, void* ws, hipStr
     const long long mine = a.window > 0 ? span : std::max(0, a.max_len - a.max_shared);
     const long long own = (long long)c.batch * p.own_blocks * (mine / tile_of_kind(c, false));
     const long long shared = (long long)p.pre_blocks * (a.max_shared / tile_of_kind(c, true));
-    if (own >= 2 * shared) p.pre_chunks = std::min(p.pre_chunks, std::max(1, 256 / (c.n_kv * p.pre_blocks)));
+    if (own >= 2 * shared) p.pre_chunks = std::min(p.pre_chunks, std::max(1, (int)(256 / ((long long)c.n_kv * p.pre_blocks))));
   }
   char* base = static_cast<char*>(ws);
   p.ml = reinterpret_cast<float*>(base);

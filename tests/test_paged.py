@@ -169,3 +169,11 @@ def test_the_reference_of_attention_by_hand():
     assert np.allclose(out[0], 17 / 2) and np.allclose(out[1], 15 / 2)
     out, _ = c.attention(np.ones((2, 2, 1, 64), np.float32), [18, 0], 4, 1.0)
     assert np.allclose(out[0, 0], (13 + 14 + 15 + 16) / 4) and np.allclose(out[0, 1], (14 + 15 + 16 + 17) / 4) and (out[1] == 0).all()
+
+
+@pytest.mark.parametrize("hd", [64, 512])
+@pytest.mark.parametrize("dtype", [E.F32, E.F16])
+@pytest.mark.parametrize("kv,batch,n_q", [(4096, 65535, 64), (4096, 32768, 64), (2048, 65535, 1), (4096, 8192, 8)])
+def test_more_columns_than_a_launch_can_have(hd, dtype, kv, batch, n_q):
+    c = cache(dtype=dtype, kv=kv, hd=hd, batch=batch)
+    refused("Op", "too large", E.paged_attention_workspace, c, 8 * kv, n_q, 80, 40)
