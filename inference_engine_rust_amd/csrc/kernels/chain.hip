@@ -57,22 +57,24 @@ typedef const __attribute__((address_space(4))) ChainPhase* CPhase;
 // before a slot is read, an lgkmcnt wait before a slot is refilled), and without the clobber the
 // compiler keeps the phase fields in scalar registers across copies.
 // The LDS offset is wave-uniform by construction; readfirstlane puts it in a scalar register even
-// where the compiler cannot prove that.
+// where the compiler cannot prove that. The copy takes it from m0, which the compiler writes, as an
+// operand; an instruction has to lie between that write and the copy, and the compiler puts none
+// into inline assembly.
 IEK_DEV void dma16(uint32_t lds_off, const void* g) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds_off)),
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"{m0}"(__builtin_amdgcn_readfirstlane(lds_off)),
                "v"(g));
 }
 // sc1: device-coherent (bypasses the non-coherent per-XCD L2 copy), for data other workgroups
 // wrote in this launch
 IEK_DEV void dma16_coh(uint32_t lds_off, const void* g) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off sc1" ::"s"(__builtin_amdgcn_readfirstlane(lds_off)),
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, off sc1" ::"{m0}"(__builtin_amdgcn_readfirstlane(lds_off)),
                "v"(g)
                : "memory");
 }
 // 4-byte copy per lane into LDS, used to touch one 128-byte line per lane so a later copy of the
 // item finds it in L2
 IEK_DEV void dma4(uint32_t lds_off, const void* g) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds_off)),
+  asm volatile("s_nop 0\n\tglobal_load_lds_dword %1, off" ::"{m0}"(__builtin_amdgcn_readfirstlane(lds_off)),
                "v"(g));
 }
 template <int N>

@@ -759,10 +759,11 @@ struct Staged {
   static IEK_DEV int k_at(int row, int piece) { return row * PIECES + (piece ^ turned(row)); }
 };
 
-// 16 bytes a lane from memory to 1024 in a row in LDS, without registers. (The waits are the caller's.)
+// 16 bytes a lane from memory to 1024 in a row in LDS, without registers. (The waits for it are the caller's; the one between
+// the write of m0, where LDS is written, and the copy is here: the compiler puts none into inline assembly.)
 IEK_DEV void copy16(const void* lds, const char* from, uint32_t offset) {
   const uint32_t at = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)lds;
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(at)), "v"(offset), "s"(from) : "memory");
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"{m0}"(__builtin_amdgcn_readfirstlane(at)), "v"(offset), "s"(from) : "memory");
 }
 template <int N>
 IEK_DEV void copies_left() {
