@@ -458,6 +458,12 @@ IEK_DEV float load_tokens(float4* to, const float* p, int n) {
 
 IEK_DEV float steps(float x, float top, float scale) { return fminf((top - x) * scale, (float)(BINS - 1)); }
 IEK_DEV int bin_of(float x, float top, float scale) { return (int)steps(x, top, scale); }
+// Whether a token is less than `far` steps below the top. Where the span is beyond f32, the scale is 0 and the steps of a
+// token as far down are NaN: bin_of counts it in the last bin, so it is within every bound.
+IEK_DEV bool within(float x, float top, float scale, float far) {
+  const float s = (top - x) * scale;
+  return x > -INFINITY && (!(s >= far) || far == INFINITY);
+}
 
 IEK_DEV void clear_bins(Smem& m, u64* hist) {
 #pragma unroll
@@ -784,7 +790,7 @@ IEK_DEV bool one_row(const SampleArgs& a, int b, const Head& h, Group& q, float4
     far = -logf(fminf(h.m, 1.f)) * h.t * 1.0001f + 1e-6f * fabsf(h.top) + 1e-30f;
   }
   if (far >= 0.f) {
-    const int n = compact(T, q, LIST, [&](float v) { return v > -INFINITY && fminf((h.top - v) * scale, 1e30f) < far; }, put);
+    const int n = compact(T, q, LIST, [&](float v) { return within(v, h.top, scale, far); }, put);
     if (n <= LIST) {
       const Tokens L = list.tokens(n);
       if (n <= NEAR) {
@@ -979,7 +985,7 @@ __global__ __launch_bounds__(ST) void slice_cut_kernel(SampleArgs a, Slices z) {
     const float scale = list_scale(span), far = bin < 0 ? INFINITY : (float)(bin + 1);
     float* x = r.x + (size_t)s * SEGMENT;
     uint32_t* index = r.index + (size_t)s * SEGMENT;
-    const int n = compact(T, q, SEGMENT, [&](float v) { return v > -INFINITY && fminf((h.top - v) * scale, 1e30f) < far; },
+    const int n = compact(T, q, SEGMENT, [&](float v) { return within(v, h.top, scale, far); },
                           [&](int at, float v, uint32_t i) {
                             x[at] = v;
                             index[at] = i;

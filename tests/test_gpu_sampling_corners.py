@@ -1,0 +1,42 @@
+"""Sampling at the ends of its arguments' ranges, against tests/paged_ref.py in 64 bits with the bars of test_gpu_sampling."""
+import numpy as np
+import pytest
+
+from test_gpu_sampling import check
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+
+def far_apart(rng, n, high, low):
+    """-inf but for `high` logits next to 3e38 and `low` next to -3e38, whose distance f32 cannot hold."""
+    x = np.full(n, -np.inf, np.float32)
+    at = rng.permutation(n)[:high + low]
+    x[at[:high]] = np.float32(3e38) * (1 - rng.integers(0, 3, high) / 64)
+    x[at[high:]] = np.float32(-3e38) * (1 - rng.integers(0, 5, low) / 64)
+    return x
+
+
+def test_top_k_of_logits_further_apart_than_f32(gpu):
+    x = np.full((1, 2048), -3e38, np.float32)
+    x[0, :100] = 3e38
+    check(x, [1e38], np.float32([0.9999]), [200])
+
+
+@pytest.mark.parametrize("n", [500, 2048, 9000, 32768, 40000, 262144])
+def test_filters_of_logits_further_apart_than_f32(gpu, n):
+    rng = np.random.default_rng(n)
+    high, low, k, p, m = zip(*[(100, 150, 200, 1.0, 0.0), (3, 200, 30, 1.0, 0.0), (100, 390, 101, 0.99, 0.0), (1, 400, 300, 1.0, 0.002),
+                               (100, 150, 0, 0.995, 0.0), (100, 150, 0, 1.0, 0.0026), (5, 9, 14, 1.0, 0.0), (200, 290, 450, 0.9999, 1e-4)])
+    x = np.stack([far_apart(rng, n, *c) for c in zip(high, low)])
+    for t in (1e38, 3e38):
+        for r in (0.9999, 0.999, 0.5):
+            check(x, [t] * len(x), np.full(len(x), r, np.float32), k, p, m)
+
+
+@pytest.mark.parametrize("n", [6000, 50000])
+def test_top_k_of_many_logits_further_apart_than_f32(gpu, n):
+    rng = np.random.default_rng(n)
+    x = np.stack([far_apart(rng, n, 1500, 4000), far_apart(rng, n, 400, 4000), far_apart(rng, n, 40, 2000)])
+    check(x, [1e38] * 3, np.float32([0.99995, 0.998, 0.9]), [5000, 1024, 900])
