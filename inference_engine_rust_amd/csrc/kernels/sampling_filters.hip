@@ -299,8 +299,10 @@ IEK_DEV void any_row(const SampleArgs& a, int b, const Head& h, Smem& m, u64* hi
   auto weight = [&](float x, bool tie_kept, bool any) -> u64 {
     const uint32_t key = key_of(x);
     if (!(key > kept.key || (tie_kept && key == kept.key))) return 0;
-    const double w = weigh.real(x);
-    return !(w >= least) ? 0 : any ? exp(((double)x - weigh.top) / (double)h.t) > 0 : weigh.whole(w);
+    double w = weigh.real(x);
+    if (!any) return w >= least ? weigh.whole(w) : 0;
+    if (w < 0x1p-60) w = exp(((double)x - weigh.top) / (double)h.t);  // (min_p may be below all that is told apart above)
+    return w > 0 && w >= least;
   };
   // one pass over the run, group by group: f(weights of the lane's four, their index)
   auto walk = [&](bool any, auto f) {

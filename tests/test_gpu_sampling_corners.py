@@ -40,3 +40,21 @@ def test_top_k_of_many_logits_further_apart_than_f32(gpu, n):
     rng = np.random.default_rng(n)
     x = np.stack([far_apart(rng, n, 1500, 4000), far_apart(rng, n, 400, 4000), far_apart(rng, n, 40, 2000)])
     check(x, [1e38] * 3, np.float32([0.99995, 0.998, 0.9]), [5000, 1024, 900])
+
+
+@pytest.mark.parametrize("n", [2, 4000, 32768, 70001])
+@pytest.mark.parametrize("m", [1e-20, 1e-25, 1e-40])
+def test_min_p_below_the_weights_that_sums_hold(gpu, n, m):
+    """A draw of exactly 0 takes the first token of any weight: of those not below min_p, however small that is."""
+    x = np.full((6, n), -np.inf, np.float32)
+    x[:, n - 1] = 0
+    x[0, 0] = -60  # (a weight of 9e-27)
+    x[1, 0] = -46  # 1e-20: 1.05e-20
+    x[2, 0] = -100  # 4e-44, between the smallest numbers of f32
+    x[3, 0], x[3, n // 2] = -120, -40
+    x[4, 0] = -92.2  # 9e-41, just below 1e-40
+    x[5, 0] = -45.9
+    zero = np.zeros(6, np.float32)
+    check(x, [1.0] * 6, zero, None, None, [m] * 6)
+    check(x, [0.5] * 6, zero, None, None, [m] * 6)
+    check(x, [1.0] * 6, zero, [2] * 6, [0.9] * 6, [m] * 6)
