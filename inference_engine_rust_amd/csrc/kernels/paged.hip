@@ -44,14 +44,14 @@ __global__ __launch_bounds__(AT) void append_kernel(Paged c, PagedAppend a) {
   const int pos = start + i, page = c.table[(size_t)b * c.max_pages + (pos >> c.shift)];
   const bool there = (unsigned)page < (unsigned)c.n_pages;  // (rows without a page are dropped)
   const int d = 4 * (t % QUADS);
-  const bool turned = d < 2 * a.pairs;
+  const bool turned = d < 2 * a.pairs, both = d + 2 < 2 * a.pairs;  // (of an odd number of pairs the last one is alone)
   pf4_t cs = {1.f, 0.f, 1.f, 0.f};
   if (turned) {
     const float* e = a.rope + ((size_t)pos * a.pairs + d / 2) * 2;
-    // (with an odd number of pairs the second one here may be past the row's, and its rows may be 8-byte aligned)
+    // (rows may be 8-byte aligned)
     cs[0] = e[0];
     cs[1] = e[1];
-    if (d + 2 < 2 * a.pairs) {
+    if (both) {
       cs[2] = e[2];
       cs[3] = e[3];
     }
@@ -74,7 +74,11 @@ __global__ __launch_bounds__(AT) void append_kernel(Paged c, PagedAppend a) {
       const int h = h0 + u * (AT / QUADS);
       if (h >= heads) break;
       const bool value = h >= nq + c.n_kv;
-      const pf4_t y = turned && !value ? turn(x[u], cs) : x[u];
+      pf4_t y = x[u];
+      if (turned && !value) {
+        y = turn(x[u], cs);
+        if (!both) y = pf4_t{y[0], y[1], x[u][2], x[u][3]};
+      }
       if (h < nq) {
         *reinterpret_cast<pf4_t*>(qo + (size_t)h * HD + d) = y;
       } else if (there) {
