@@ -835,7 +835,9 @@ struct Way {
           const u4_t kk = k[p][e >> 1], vv = v[p][e >> 1];
           three(__uint_as_float(kk[2 * (e & 1)]), __uint_as_float(kk[2 * (e & 1) + 1]), q[0], q[1], q[2]);
           x[0][e] = q[0], x[1][e] = q[1], x[2][e] = q[2];
-          three(__uint_as_float(vv[2 * (e & 1)]), __uint_as_float(vv[2 * (e & 1) + 1]), q[0], q[1], q[2]);
+          // (a signalling NaN made a quiet one: the first part, cut off, may be an infinity otherwise)
+          three(__builtin_canonicalizef(__uint_as_float(vv[2 * (e & 1)])), __builtin_canonicalizef(__uint_as_float(vv[2 * (e & 1) + 1])), q[0], q[1],
+                q[2]);
           y[0][e] = q[0], y[1][e] = q[1], y[2][e] = q[2];
         }
 #pragma unroll
