@@ -7,9 +7,9 @@
 // The pick is the first token in index order up to which the kept weights sum to more than r times their total.
 //
 // Weights are summed as integers, w 2^S rounded, with S as large as n of them allow in 64 bits and at most 50: sums do
-// not depend on their order, so atomics on histograms and any split give the same token every time, and a weight is
-// off by about 2^-S of the largest (2^-49 at 32000 tokens), where f32 sums would move the borders of tokens by 1e-7
-// of the total.
+// not depend on their order, so atomics on histograms and any split give the same token every time. A weight is off by
+// 2^-(S + 1) of the largest (2^-50 at 32000 tokens) and 2^-48.4 of itself at most, where f32 sums would move the borders of
+// tokens by 1e-7 of the total.
 //
 // A row of up to 32768 logits stays in the LDS of one workgroup. A border (top-k, top-p) is found by one histogram over
 // the distance to the maximum, of counts or of weights, in 2048 bins; the few tokens of the bin that the border is in
@@ -42,7 +42,9 @@ IEK_DEV uint32_t key_of(float x) {
 IEK_DEV float value_of(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k); }
 
 // Weights of a row: w 2^S as an integer. 2^(y / 64), y = i + f, is a table's entry of 64 (in LDS) times a polynomial in
-// f of degree 4, which leaves out (f ln 2 / 64)^5 / 120 < 2^-44; the additions of 1.5 2^52 round to integers.
+// f of degree 4: the exponential's first terms, and in place of z^5 / 120 (z = f L, L = ln 2 / 64, |z| <= L / 2) the cubic nearest to
+// it, (L / 2)^2 z^3 / 96 - (L / 2)^4 z / 384 (Chebyshev: 16 x^5 = 20 x^3 - 5 x + T_5(x)), which leaves out (L / 2)^5 / 1920 <
+// 2^-48.5; without the cubic it were 2^-44.5. The additions of 1.5 2^52 round to integers.
 struct Weigh {
   double top, rate;  // 64 log2 e / T
   double one;        // 2^S
@@ -51,9 +53,9 @@ struct Weigh {
     const double y = fmax(((double)x - top) * rate, -4096.0), n = y + 0x1.8p52, f = y - (n - 0x1.8p52);
     constexpr double L = 0.693147180559945309417232 / 64;
     double e = L * L * L * L / 24;
-    e = fma(e, f, L * L * L / 6);
+    e = fma(e, f, L * L * L / 6 * (1 + L * L / 64));
     e = fma(e, f, L * L / 2);
-    e = fma(e, f, L);
+    e = fma(e, f, L * (1 - L * L * L * L / 6144));
     e = fma(e, f, 1.0);
     const int i = (int)__double_as_longlong(n);
     e *= table[i & 63];

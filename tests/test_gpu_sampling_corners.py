@@ -58,3 +58,13 @@ def test_min_p_below_the_weights_that_sums_hold(gpu, n, m):
     check(x, [1.0] * 6, zero, None, None, [m] * 6)
     check(x, [0.5] * 6, zero, None, None, [m] * 6)
     check(x, [1.0] * 6, zero, [2] * 6, [0.9] * 6, [m] * 6)
+
+
+@pytest.mark.parametrize("l,t,r", [(-0.005526490043848753, 1.0212681293487549, 0.501352846622467), (-0.005455499980598688, 1.0065972805023193, 0.5013549327850342),
+                                   (-0.005429748445749283, 1.0016255378723145, 0.5013552308082581)])
+def test_weights_are_within_two_to_the_minus_44(gpu, l, t, r):
+    """Draws that are 1.07 to 1.14 times 2^-44 of the larger weight away from the border of two tokens, of 2^19: a sum that is
+    2^-44 off finds the same token as the definition. (In 64 bits the border is off by 2^-52.)"""
+    x = np.full((1, 2 ** 19), -np.inf, np.float32)
+    x[0, :2] = 0, l
+    check(x, [t], np.float32([r]))
