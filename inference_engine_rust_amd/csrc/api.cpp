@@ -996,16 +996,11 @@ iek_status iek_dev_paged_attention(const iek_paged_kv* cache, const float* q, si
 }
 
 // ---- sampling of a batch ----
-static void sample_shape(size_t rows, size_t n) {
-  if (n == 0) fail(ST_SAMPLING, "logits slice is empty");
-  if (n > (1u << 25) || rows > (1u << 21)) fail(ST_OP, "sample: dims too large");
-}
-
 iek_status iek_sample_workspace(size_t rows, size_t n, size_t* bytes) {
   IEK_API_TRY({
-    sample_shape(rows, n);
+    const size_t need = sample_workspace(rows, n);
     if (!bytes) fail(ST_OP, "null argument");
-    *bytes = sample_workspace(rows, n);
+    *bytes = need;
   })
 }
 
@@ -1014,7 +1009,7 @@ iek_status iek_dev_sample(const float* logits, size_t rows, size_t n, size_t row
                           uint32_t* out_index, float* out_prob, void* workspace, size_t workspace_bytes, void* stream) {
   IEK_API_TRY({
     constexpr const char* op = "sample";
-    sample_shape(rows, n);
+    const size_t need = sample_workspace(rows, n);
     if (row_stride < n) fail(ST_OP, "sample: row_stride must be at least a row");
     if (row_stride > (1u << 30)) fail(ST_OP, "sample: dims too large");
     if (rows == 0) return IEK_OK;
@@ -1026,8 +1021,8 @@ iek_status iek_dev_sample(const float* logits, size_t rows, size_t n, size_t row
     aligned(r, 4, "r", op);
     aligned(out_index, 4, "out_index", op);
     optional_aligned(out_prob, 4, "out_prob", op);
-    if (workspace_bytes < sample_workspace(rows, n)) fail(ST_OP, "sample: the workspace is too small");
-    if (sample_workspace(rows, n)) aligned(workspace, 16, "workspace", op);
+    if (workspace_bytes < need) fail(ST_OP, "sample: the workspace is too small");
+    if (need) aligned(workspace, 16, "workspace", op);
     OnDeviceOf on(as_stream(stream));
     const SampleArgs a{logits, (int)n, row_stride, temperature, top_k, top_p, min_p, r, out_index, out_prob, {}};
     launch_sample(a, (int)rows, workspace, as_stream(stream));
@@ -1226,10 +1221,9 @@ iek_status iek_sample_temperature(const float* logits, size_t n, float temperatu
 iek_status iek_sample(const float* logits, size_t n, float temperature, int32_t top_k, float top_p, float min_p, float r,
                       uint32_t* out_index, float* out_prob) {
   IEK_API_TRY({
-    sample_shape(1, n);
+    const size_t ws = sample_workspace(1, n);
     const SampleParams one{temperature, top_p, min_p, r, top_k};
     check_sample_params(one);
-    const size_t ws = sample_workspace(1, n);
     HostCall hc({n * 4, 8, ws});
     const float* dl = hc.up<float>(0, logits, n * 4);
     uint32_t* word = hc.ptr<uint32_t>(1);

@@ -24,6 +24,7 @@ struct SampleArgs {
   float* prob;  // or null
   SampleParams one;
 };
+// Throws for what launch_sample cannot take.
 size_t sample_workspace(size_t rows, size_t n);
 void launch_sample(const SampleArgs& a, int rows, void* ws, hipStream_t st);
 

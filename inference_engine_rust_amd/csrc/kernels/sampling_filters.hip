@@ -1159,7 +1159,7 @@ void check_sample_params(const SampleParams& p) {
 static Slices slices_of(size_t rows, size_t n) {
   constexpr size_t unit = 4 * ST;
   Slices z{};
-  if (n <= SLICE || n > (size_t)SLICE * MOST_SLICES) return z;
+  if (n <= SLICE) return z;
   const size_t fill = (n * rows / 256 + unit - 1) / unit * unit, least = (n / MOST_SLICES + unit) / unit * unit;
   z.length = (int)std::min<size_t>(SLICE, std::max({fill, least, 2 * unit}));
   z.count = (int)((n + z.length - 1) / z.length);
@@ -1168,6 +1168,8 @@ static Slices slices_of(size_t rows, size_t n) {
 }
 
 size_t sample_workspace(size_t rows, size_t n) {
+  if (n == 0) fail(ST_SAMPLING, "logits slice is empty");
+  if (n > (size_t)SLICE * MOST_SLICES || rows > (1u << 21)) fail(ST_OP, "sample: dims too large");
   const Slices z = slices_of(rows, n);
   return rows * z.bytes;
 }

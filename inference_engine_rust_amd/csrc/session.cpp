@@ -1550,10 +1550,9 @@ uint32_t Session::sample_temperature(float temperature, float r) {
 
 uint32_t Session::sample(const SampleParams& p) {
   check_state();
-  if (m_->cfg.vocab == 0) fail(ST_SAMPLING, "logits slice is empty");
+  const size_t vocab = (size_t)m_->cfg.vocab, bytes = sample_workspace(1, vocab);
   check_sample_params(p);
-  const size_t vocab = (size_t)m_->cfg.vocab;
-  if (!sample_ws_) sample_ws_ = dev_alloc<char>(sample_workspace(1, vocab) + 16);
+  if (!sample_ws_) sample_ws_ = dev_alloc<char>(bytes + 16);
   logits_body(false);
   launch_sample({logits_, (int)vocab, vocab, nullptr, nullptr, nullptr, nullptr, nullptr, d_tok_, nullptr, p}, 1, sample_ws_, st_);
   uint32_t tok = 0;
