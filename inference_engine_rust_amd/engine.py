@@ -378,12 +378,21 @@ def sample_temperature_next_token(session: InferenceSession, temperature: float,
     return v.value
 
 
+def _sample_draw(r: float) -> float:
+    """A draw in [0, 1) as the entries take it: what f32 would round to 1 is the largest f32 below."""
+    return 1.0 - 2.0 ** -24 if 1.0 - 2.0 ** -25 <= r < 1.0 else r
+
+
+def _sample_top_k(k: int) -> int:
+    return max(0, min(int(k), 2 ** 31 - 1))
+
+
 def sample_next_token(session: InferenceSession, temperature: float, r: float, top_k: int = 0, top_p: float = 1.0,
                       min_p: float = 0.0) -> int:
     """A token of the session's last-token logits by temperature, top-k, top-p and min-p (include/iek.h, iek_sample) on
     the device; r is a uniform draw in [0, 1)."""
     v = ctypes.c_uint32()
-    _check(lib().iek_session_sample(session._h, temperature, top_k, top_p, min_p, r, ctypes.byref(v)))
+    _check(lib().iek_session_sample(session._h, temperature, _sample_top_k(top_k), top_p, min_p, _sample_draw(r), ctypes.byref(v)))
     return v.value
 
 
@@ -486,7 +495,8 @@ def host_sample(logits, temperature: float, r: float, top_k: int = 0, top_p: flo
     """iek_sample: the token of one row of logits and its probability."""
     x = _f32(logits)
     v, p = ctypes.c_uint32(), ctypes.c_float()
-    _check(lib().iek_sample(_np_ptr(x), x.size, temperature, top_k, top_p, min_p, r, ctypes.byref(v), ctypes.byref(p)))
+    _check(lib().iek_sample(_np_ptr(x), x.size, temperature, _sample_top_k(top_k), top_p, min_p, _sample_draw(r), ctypes.byref(v),
+                            ctypes.byref(p)))
     return v.value, p.value
 
 

@@ -216,8 +216,7 @@ def generate(model: "E.LoadedModel", tokenizer: Tokenizer, prompt: str, new_toke
     generated: list[int] = []
     for _ in range(new_tokens):
         if temperature > 0.0 and filters:
-            r = min(float(rng.random()), 1.0 - 2.0 ** -24)  # (the largest f32 below 1)
-            nxt = E.sample_next_token(s, temperature, r, top_k, top_p, min_p)
+            nxt = E.sample_next_token(s, temperature, float(rng.random()), top_k, top_p, min_p)
         elif temperature > 0.0:
             nxt = E.sample_temperature_next_token(s, temperature, float(rng.random()))
         else:
