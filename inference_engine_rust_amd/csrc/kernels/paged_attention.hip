@@ -798,53 +798,49 @@ struct Copies {
   }
 };
 
-// A thread's pieces of a tile on their way: piece t % PIECES of the rows t / PIECES, ...
-template <int HD, bool F16>
+// A thread's pieces of an f32 tile on their way: piece t % PIECES of the rows t / PIECES, ...
+template <int HD>
 struct Way {
-  static constexpr int PIECES = HD / 8, RPP = 64 * WAVES / PIECES, NPASS = 32 / RPP, N = F16 ? 1 : 2;
-  u4_t k[NPASS][N], v[NPASS][N];
+  using S = Staged<HD, false>;
+  static constexpr int PIECES = HD / 8, RPP = 64 * WAVES / PIECES, NPASS = 32 / RPP;
+  u4_t k[NPASS][2], v[NPASS][2];
   IEK_DEV void load(const Paged& c, int h, const Ids<true>& id, int tile, int end) {
     const int t = threadIdx.x, wave = uniform(t >> 6);
 #pragma unroll
     for (int p = 0; p < NPASS; ++p) {
       // (a wave's rows of a pass are in one half of the tile)
       const int half = (p * RPP + wave * 64 / PIECES) >> 4, row = (p * RPP + t / PIECES) & 15;
-      const int off = (row * HD + 8 * (t % PIECES)) * (F16 ? 2 : 4);
-      const auto rk = rows_rsrc<HD, F16>(c, c.k, h, half ? id.id[1] : id.id[0], 32 * tile + 16 * half, end);
-      const auto rv = rows_rsrc<HD, F16>(c, c.v, h, half ? id.id[1] : id.id[0], 32 * tile + 16 * half, end);
+      const int off = (row * HD + 8 * (t % PIECES)) * 4;
+      const auto rk = rows_rsrc<HD, false>(c, c.k, h, half ? id.id[1] : id.id[0], 32 * tile + 16 * half, end);
+      const auto rv = rows_rsrc<HD, false>(c, c.v, h, half ? id.id[1] : id.id[0], 32 * tile + 16 * half, end);
 #pragma unroll
-      for (int n = 0; n < N; ++n) {
+      for (int n = 0; n < 2; ++n) {
         k[p][n] = __builtin_amdgcn_raw_buffer_load_b128(rk, off, 16 * n, 0);
         v[p][n] = __builtin_amdgcn_raw_buffer_load_b128(rv, off, 16 * n, 0);
       }
     }
   }
-  IEK_DEV void store(typename Staged<HD, F16>::One& L) const {
+  IEK_DEV void store(typename S::One& L) const {
     const int t = threadIdx.x;
 #pragma unroll
     for (int p = 0; p < NPASS; ++p) {
       const int row = p * RPP + t / PIECES, piece = t % PIECES;
-      if constexpr (F16) {
-        L.k[0][Staged<HD, F16>::k_at(row, piece)] = k[p][0];
-        L.v[0][row * PIECES + piece] = v[p][0];
-      } else {
-        u4_t x[3], y[3];
+      u4_t x[3], y[3];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          uint32_t q[3];
-          const u4_t kk = k[p][e >> 1], vv = v[p][e >> 1];
-          three(__uint_as_float(kk[2 * (e & 1)]), __uint_as_float(kk[2 * (e & 1) + 1]), q[0], q[1], q[2]);
-          x[0][e] = q[0], x[1][e] = q[1], x[2][e] = q[2];
-          // (a signalling NaN made a quiet one: the first part, cut off, may be an infinity otherwise)
-          three(__builtin_canonicalizef(__uint_as_float(vv[2 * (e & 1)])), __builtin_canonicalizef(__uint_as_float(vv[2 * (e & 1) + 1])), q[0], q[1],
-                q[2]);
-          y[0][e] = q[0], y[1][e] = q[1], y[2][e] = q[2];
-        }
+      for (int e = 0; e < 4; ++e) {
+        uint32_t q[3];
+        const u4_t kk = k[p][e >> 1], vv = v[p][e >> 1];
+        three(__uint_as_float(kk[2 * (e & 1)]), __uint_as_float(kk[2 * (e & 1) + 1]), q[0], q[1], q[2]);
+        x[0][e] = q[0], x[1][e] = q[1], x[2][e] = q[2];
+        // (a signalling NaN made a quiet one: the first part, cut off, may be an infinity otherwise)
+        three(__builtin_canonicalizef(__uint_as_float(vv[2 * (e & 1)])), __builtin_canonicalizef(__uint_as_float(vv[2 * (e & 1) + 1])), q[0], q[1],
+              q[2]);
+        y[0][e] = q[0], y[1][e] = q[1], y[2][e] = q[2];
+      }
 #pragma unroll
-        for (int n = 0; n < 3; ++n) {
-          L.k[n][Staged<HD, F16>::k_at(row, piece)] = x[n];
-          L.v[n][row * PIECES + piece] = y[n];
-        }
+      for (int n = 0; n < 3; ++n) {
+        L.k[n][S::k_at(row, piece)] = x[n];
+        L.v[n][row * PIECES + piece] = y[n];
       }
     }
   }
@@ -863,7 +859,7 @@ IEK_DEV void run_wide(const Paged& c, const PagedAttn& a, const Plan& p, const J
   Ids<true> id[F16 ? AHEAD + 2 : 3];
 #pragma unroll
   for (int i = 0; i < (F16 ? AHEAD + 2 : 3); ++i) id[i] = ids_of<true>(c, pages, J.t0 + i);
-  Way<HD, false> way;
+  Way<HD> way;
   const Copies<HD> copies;
   if constexpr (F16) {
 #pragma unroll

@@ -743,7 +743,7 @@ IEK_DEV void pick_of_few(const Tokens& T, int n, Group& q, Bins& s, const Sample
   __syncthreads();
   const u64 above = live ? s.hist[t] : 0;
   const bool first = live && (h.k <= 0 || (int)s.hist[NEAR + t] < h.k);
-  bool kept = first && (t >= n || real >= fminf(h.m, 1.f));
+  bool kept = first && real >= fminf(h.m, 1.f);
   if (h.p < 1.f) {
     const u64 all = q.sum(first ? w : 0);
     kept &= above == 0 || (double)above < (double)h.p * (double)all;
@@ -860,7 +860,7 @@ struct RowSpace {
   float* x;                          // [slices][SEGMENT] candidates
   uint32_t* index;
 };
-__host__ IEK_DEV RowSpace space_of(const Slices& z, int b) {
+IEK_DEV RowSpace space_of(const Slices& z, int b) {
   char* p = z.base + (size_t)b * z.bytes;
   const size_t n = (size_t)z.count;
   RowSpace r;
