@@ -430,13 +430,14 @@ iek_status iek_dev_paged_append(const iek_paged_kv* cache, const float* q, const
  * hi = len[b] - (n_q - 1 - t), lo = hi - sliding_window if that is positive and there is a window (0: none). out[b][t][h]
  * = softmax(scale * q . K[j]) . V[j] over them, h's KV head being h / (n_heads / n_kv_heads); zeros where there are none.
  * Entries that no query sees may hold anything. An infinity or NaN reaches the queries that see it alone, as NaN or (of
- * an infinity in V) as an infinity.
+ * an infinity in V) as an infinity; an infinity in K whose score is -inf may also have no weight.
  * The first *shared entries of every sequence (a word in HBM, at most max_shared <= max_len, which sizes the launch) are
  * the same ones, in the pages shared_pages[j / page_size] (ceil(max_shared / page_size) numbers): they are read from
  * there, once for the whole batch, whatever the tables say, and the answer is that of tables that begin with them. *shared
  * need not be a multiple of page_size. max_shared 0 (both NULL): nothing is shared. Sums are f32, of shares relative to a
  * maximum that may lag by 2^8: the entries times the largest |V| must stay below 2^119. Of fp16 caches, products are
- * those of 22 bits of q and of the weights. workspace: iek_paged_attention_workspace bytes for the same arguments, its
+ * those of 22 bits of q and of the weights; of f32 caches they may leave out 2^-22 of a product. Chunks follow the
+ * lengths for up to 64 sequences; more of them are cut by max_len. workspace: iek_paged_attention_workspace bytes for the same arguments, its
  * contents of no matter. */
 iek_status iek_paged_attention_workspace(const iek_paged_kv* cache, size_t n_heads, size_t n_q, size_t max_len,
                                          size_t max_shared, size_t* bytes);

@@ -462,8 +462,9 @@ IEK_DEV void run_job(const Paged& c, const PagedAttn& a, const Plan& p, const Jo
   const float ks = a.scale * 1.44269504088896340736f;
   const int G = p.group;
   int tile = uniform(J.t0 + (WIDE ? 0 : set));
-  // Loads are issued without conditions, those past the chunk's last entry of nothing: with a branch around them the
-  // waits for K were ones for V too, which is issued behind it.
+  // Loads are issued without conditions, those past the chunk's last entry of nothing. (The compiler moves the first ones behind
+  // q's conversion, V before K for fp16, so its wait at the loop's head, for both ways into it, is one for all loads in
+  // flight: a tile's K products wait for its V too.)
   const Pages pages{J.pages.list, min(J.pages.end, J.t1 * TILE)};
   Ids<F16> id = ids_of<F16>(c, pages, tile), next = ids_of<F16>(c, pages, tile + STEP);
   Tile<DIMS, F16> T;
@@ -724,13 +725,15 @@ IEK_DEV void run_job(const Paged& c, const PagedAttn& a, const Plan& p, const Jo
 // ---- many columns: tiles in LDS -----------------------------------------------------------------------
 // For rows of up to 128 the four waves split the columns of a job and share its tiles of 32 slots, which lie in LDS. Both
 // products are mfma_f32_16x16x32 ones. fp16 pages: a ring of four tiles, filled by copies without registers three tiles
-// ahead; 32 columns a wave, K and V one plane, q and P pairs (as above). f32 pages: one tile, each thread 16-byte pieces of
+// ahead (of head_dim 128 one tile's time ahead: the 13 or 26 registers that spill are read back in the block for values that are not
+// finite, and for these the compiler waits at every tile for all that is in flight, the copies just issued among them);
+// 32 columns a wave, K and V one plane, q and P pairs (as above). f32 pages: one tile, each thread 16-byte pieces of
 // rows, the next tile's in flight in registers meanwhile; 16 columns a wave, every operand as three bf16 numbers that sum
 // to it exactly (8 bits each, the first one cut off, the others rounded), six products: of the parts' orders those up to the
 // third; what is left out is below 2^-22 of a product. (mfma_f32_16x16x4_f32, exact, takes 32 cycles for 4 of the 32 terms.)
 // 32 heads of 128, part launch: 16384 shared fp16 entries, 64 sequences 65 us (with each wave's tiles in its registers 113),
-// 4096 f32 ones, 32 sequences 28 us (42). The matrix cores are busy for 14 and 10 us of these: a SIMD's two waves leave each
-// other waiting for the softmax's vector work, and the first tile, the results and the own chunks' one turn take 15 to 20.
+// 4096 f32 ones, 32 sequences 28 us (42). The matrix cores are busy for 14 and 10 us of these, a SIMD issues for half of the time: it waits for copies and for
+// its two waves' softmax, and the first tile, the results and the own chunks' one turn take 15 to 20.
 typedef __bf16 b2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
 IEK_DEV f4_t mfma_b(u4_t a, u4_t b, f4_t c) {
@@ -854,7 +857,7 @@ IEK_DEV void run_wide(const Paged& c, const PagedAttn& a, const Plan& p, const J
   const int col_base = (J.block * WAVES + wave) * CG * 16;
   const bool idle = col_base >= J.cols;  // (such a wave takes part in the staging alone)
   const Pages pages{J.pages.list, min(J.pages.end, J.t1 * TILE)};
-  // f32: the tile after the present one is under way to registers; fp16: three are to LDS
+  // f32: the tile after the present one is under way to registers; fp16: up to three are to LDS
   constexpr int AHEAD = S::RING - 1, COPIES = S::PIECES / 4;  // (copies a wave and tile)
   Ids<true> id[F16 ? AHEAD + 2 : 3];
 #pragma unroll

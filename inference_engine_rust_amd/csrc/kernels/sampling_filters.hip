@@ -15,14 +15,20 @@
 // the distance to the maximum, of counts or of weights, in 2048 bins; the few tokens of the bin that the border is in
 // are ranked against each other. For a top-k of up to 1024 the threads' own maxima come first: the k-th largest of them
 // is no larger than the k-th logit, so what lies below it (all but about k tokens) is out, and the rest goes on as a
-// list; so do the tokens that top-p or min-p leave. A list of up to 512 is ranked as a whole. Rows that the bins do not
-// suit (thousands of equal logits at a border, a larger top-k, a draw of exactly 0) take any_row: a radix selection on
-// the logits' bits as ordered integers, 11, 11 and 10 bits at a time, from memory.
+// list; so do the tokens that top-p or min-p leave. A list of up to 512 is ranked as a whole.
 // Larger rows are cut into slices over several workgroups, in four launches: the maxima; the row's histogram; the slices'
 // candidates and sums; the border and the slice that has the token.
+// Rows that the bins do not suit take any_row: a radix selection on the logits' bits as ordered integers, 11, 11 and 10 bits
+// at a time, from memory, by one workgroup. These are
+//   rows with more than NEAR tokens in the bin that a border is in: thousands of equal logits; top-k where masks of f32's lowest value
+//     stretch the bins; and of large rows ordinary ones, since top-p's bins are 1/64 of an octave of weight (8 rows of 262144
+//     normal logits: at a temperature of 1 and a p of 0.9 36 us, of 0.98 545; at 1.3 and 0.9 557);
+//   rows of several slices with a top-k above 1024 (8 rows of 262144: 1000 27 us, 5000 403), or with more than SEGMENT of its
+//     candidates in one slice (256 rows of 40000, whose slices are 32768 long: 100 51 us, 500 124);
+//   draws of exactly 0.
 // Bound by the latency of one workgroup's phases, and by the exponentials where every token needs one. 32000 logits, one
 // row: 4.8 us greedy, 10.4 with top-k 50, 19 with top-p, 24 with a top-k of 5000; 256 rows of mixed filters 32 (their bytes
-// take 5). 8 rows of 262144 with top-p 4 + 10 + 10 + 15 us, by one workgroup a row 550.
+// take 5). 8 rows of 262144 with top-p of 0.9 at a temperature of 1: 4 + 10 + 10 + 15 us.
 #include "common.cuh"
 #include "sampling.h"
 
