@@ -437,8 +437,8 @@ iek_status iek_dev_paged_append(const iek_paged_kv* cache, const float* q, const
  * need not be a multiple of page_size. max_shared 0 (both NULL): nothing is shared. Sums are f32, of shares relative to a
  * maximum that may lag by 2^8: the entries times the largest |V| must stay below 2^119. Of fp16 caches, products are
  * those of 22 bits of q and of the weights; of f32 caches they may leave out 2^-22 of a product. Chunks follow the
- * lengths for up to 64 sequences; more of them are cut by max_len. workspace: iek_paged_attention_workspace bytes for the same arguments, its
- * contents of no matter. */
+ * lengths for up to 64 sequences; more of them are cut by max_len. workspace: iek_paged_attention_workspace bytes for
+ * the same arguments, its contents of no matter. */
 iek_status iek_paged_attention_workspace(const iek_paged_kv* cache, size_t n_heads, size_t n_q, size_t max_len,
                                          size_t max_shared, size_t* bytes);
 iek_status iek_dev_paged_attention(const iek_paged_kv* cache, const float* q, size_t n_heads, size_t n_q, size_t q_stride,
